@@ -46,7 +46,8 @@ typedef enum {
     QMM_ETIMEOUT = 5      /* a bounded device-side wait gave up */
 } qmm_status;
 
-typedef enum { QMM_BF16 = 0, QMM_F16 = 1 } qmm_dtype;
+/* QMM_F32: only where an entry says so (values to and from the MX formats). */
+typedef enum { QMM_BF16 = 0, QMM_F16 = 1, QMM_F32 = 2 } qmm_dtype;
 
 /* Human-readable text of a status, and of the last error recorded on the
  * calling thread (empty string when none). */
@@ -324,6 +325,67 @@ QMM_API int qmm_dequantize(const uint32_t* w, const void* scales, const void* bi
  */
 QMM_API int qmm_quantize(const float* w, uint32_t* wq, void* scales, void* biases, int64_t N, int64_t K, int group_size,
                  int bits, int dtype, void* stream);
+
+/*
+ * Microscaled (MX) formats: blocks of 32 values along the last axis, each
+ * block's codes times one power of two (OCP Microscaling Formats v1.0).
+ *   scales  uint8 [.., K/32]   byte b stands for 2^(b - 127), 255 for NaN
+ *   mxfp4   uint32 [.., K/8]   e2m1 codes, low bits first  (bits = 4)
+ *   mxfp8   uint32 [.., K/4]   e4m3 codes, low bits first  (bits = 8)
+ * These are the layouts of mx.quantize with mode="mxfp4" / "mxfp8"; the
+ * reference itself quantises in affine mode only (mlxturbo/rebit.py:103-121).
+ * K is a multiple of 32.  All pointers are 16-byte aligned, scales excepted.
+ *
+ * qmm_mx_quantize: v [rows, K] (QMM_BF16, QMM_F16 or QMM_F32) to words and
+ * scales.  Scale exponent floor(log2(max|v|)) - emax (emax 2 for mxfp4, 8 for
+ * mxfp8) clamped to [-127, 127]; codes rounded to nearest even and saturated.
+ * A block holding an infinity or a NaN becomes NaN (scale byte 255).
+ * qmm_mx_dequantize: the values, rounded once to `dtype` (any of the three).
+ */
+QMM_API int qmm_mx_quantize(const void* v, uint32_t* words, uint8_t* scales, int64_t rows, int64_t K, int bits,
+                            int dtype, void* stream);
+QMM_API int qmm_mx_dequantize(const uint32_t* words, const uint8_t* scales, void* out, int64_t rows, int64_t K,
+                              int bits, int dtype, void* stream);
+
+/*
+ * Residual addition, root-mean-square norm and mxfp8 rows in one launch (no
+ * counterpart in the reference, which leaves norms to MLX):
+ *   s = x + residual (fp32; s = x when residual is NULL)
+ *   h = s rounded to dtype (written when residual is given)
+ *   (xq, x_scales) = mxfp8 of s / sqrt(mean(s^2) + eps) * weight
+ * x, residual, h [rows, K] and weight [K] of dtype; sums in fp32.  h may be
+ * x or residual itself.
+ */
+QMM_API int qmm_mx_rms_norm(const void* x, const void* residual, const void* weight, void* h, uint32_t* xq,
+                            uint8_t* x_scales, int64_t rows, int64_t K, float eps, int dtype, void* stream);
+
+/*
+ * y[M, N] (dtype) = x @ dequant(w)^T with mxfp4 weights w [N, K/8], scales
+ * [N, K/32] and fp32 accumulation (mx.quantized_matmul with mode="mxfp4").
+ * x is [M, K] of dtype when x_scales is NULL, else mxfp8: words [M, K/4] and
+ * x_scales [M, K/32].
+ * workspace: qmm_mx_matmul_workspace_size bytes of device scratch, 256-byte
+ * aligned (NULL when that is 0), with no requirement on its content.
+ */
+QMM_API size_t qmm_mx_matmul_workspace_size(int64_t M, int64_t N, int64_t K, int dtype, int x_is_mx);
+QMM_API int qmm_mx_matmul(const void* x, const uint8_t* x_scales, const uint32_t* w, const uint8_t* scales, void* y,
+                          int64_t M, int64_t N, int64_t K, int dtype, void* workspace, size_t workspace_bytes,
+                          void* stream);
+
+/*
+ * The same product grouped by expert (mx.gather_qmm with mode="mxfp4"):
+ * y[r] = x[lhs[r]] @ dequant(w[rhs[r]])^T for r in [0, rows), w [E, N, K/8],
+ * scales [E, N, K/32], x of x_rows rows, lhs int32 [rows] or NULL (row r).
+ * sorted != 0 promises that rhs is non-decreasing; otherwise rows are sorted
+ * by expert on the device first.  Rows whose expert is outside [0, E) become
+ * zero.  rows, x_rows <= 2^30, E <= 16384.
+ */
+QMM_API size_t qmm_mx_gather_workspace_size(int64_t rows, int64_t E, int64_t N, int64_t K, int dtype, int x_is_mx,
+                                            int sorted);
+QMM_API int qmm_mx_gather(const void* x, const uint8_t* x_scales, const uint32_t* w, const uint8_t* scales,
+                          const int32_t* lhs, const int32_t* rhs, void* y, int64_t rows, int64_t x_rows, int64_t E,
+                          int64_t N, int64_t K, int dtype, int sorted, void* workspace, size_t workspace_bytes,
+                          void* stream);
 
 /*
  * Kernel fire counters (mirrors mlxturbo/kernels/_fire.py:1-32): how many

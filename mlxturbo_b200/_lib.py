@@ -16,12 +16,13 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libmlxturbo_b200.so")
 
 QMM_OK, QMM_EUNSUPPORTED, QMM_EINVAL, QMM_ECUDA, QMM_ENCCL, QMM_ETIMEOUT = range(6)
-QMM_BF16, QMM_F16 = 0, 1
+QMM_BF16, QMM_F16, QMM_F32 = 0, 1, 2
 
 _p = ctypes.c_void_p
 _i64 = ctypes.c_int64
 _i = ctypes.c_int
 _sz = ctypes.c_size_t
+_f = ctypes.c_float
 
 # name -> (restype, argtypes); must match include/mlxturbo_b200.h
 SIGNATURES = {
@@ -56,6 +57,13 @@ SIGNATURES = {
     "qmm_device_error": (_i, [_i]),
     "qmm_stream_read": (_i, [_p, _sz, _i, _p, _p]),
     "qmm_copy_kernel": (_i, [_p, _p, _sz, _p]),
+    "qmm_mx_quantize": (_i, [_p, _p, _p, _i64, _i64, _i, _i, _p]),
+    "qmm_mx_dequantize": (_i, [_p, _p, _p, _i64, _i64, _i, _i, _p]),
+    "qmm_mx_rms_norm": (_i, [_p, _p, _p, _p, _p, _p, _i64, _i64, _f, _i, _p]),
+    "qmm_mx_matmul_workspace_size": (_sz, [_i64, _i64, _i64, _i, _i]),
+    "qmm_mx_matmul": (_i, [_p, _p, _p, _p, _p, _i64, _i64, _i64, _i, _p, _sz, _p]),
+    "qmm_mx_gather_workspace_size": (_sz, [_i64, _i64, _i64, _i64, _i, _i, _i]),
+    "qmm_mx_gather": (_i, [_p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i, _i, _p, _sz, _p]),
     "qmm_gather_tables": (_i, [_p, _i64, _i64, _p, _sz, _p]),
     "qmm_moe_route": (_i, [_p, _i64, _i64, _i, _p, _p, _p, _p, _p, _sz, _p]),
     "qmm_ep_pack": (_i, [_p, _i64, _i64, _i64, _i, _p, _i64, _p, _i64, _p, _p]),

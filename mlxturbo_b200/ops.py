@@ -8,6 +8,11 @@ mlxturbo/kernels/dispatch.py:317-327, fused.py:3105-3116) call them unchanged:
     gather_qmm(x, w, scales, biases, lhs_indices=None, rhs_indices=None, transpose=True,
                group_size=64, bits=4, mode="affine", sorted_indices=False)
 
+mode="mxfp4" (group_size=32, bits=4, no biases) selects the microscaled format:
+blocks of 32 e2m1 codes with one power-of-two scale byte each.  ``quantize`` and
+``dequantize`` also know mode="mxfp8" (e4m3 codes, bits=8), the type of the
+activations that ``rms_norm_quantize`` writes and ``mx_matmul`` multiplies.
+
 Tensors live on a CUDA device; weights are uint32 (MLX packing).  torch has no
 uint32 arithmetic on CUDA, so int32 tensors holding the same bits are accepted
 as well.  Every call goes through libmlxturbo_b200.so on the current stream;
@@ -55,6 +60,34 @@ def _contig(t: torch.Tensor) -> torch.Tensor:
         if t.data_ptr() % 16:
             t = t.clone()
     return t
+
+
+_MX_BITS = {"mxfp4": 4, "mxfp8": 8}
+
+
+def _check_mx(mode: str, group_size: int, bits: int, biases=None) -> None:
+    if mode not in _MX_BITS:
+        raise NotImplementedError(f"mode={mode!r}: affine, mxfp4 and mxfp8 are implemented")
+    if group_size != 32 or bits != _MX_BITS[mode]:
+        raise NotImplementedError(f"mode={mode!r} has group_size=32 and bits={_MX_BITS[mode]}, "
+                                  f"got group_size={group_size} bits={bits}")
+    if biases is not None:
+        raise ValueError(f"mode={mode!r} has no biases")
+
+
+def _mx_ops():
+    ops = _lib.torch_ops()
+    if ops is None:
+        raise ImportError(f"{_lib.TORCH_OPS_PATH} is not built; run `python -m mlxturbo_b200.build`")
+    return ops
+
+
+def _check_mx_weight(mode: str, group_size: int, bits: int, biases, transpose: bool) -> None:
+    _check_mx(mode, group_size, bits, biases)
+    if mode != "mxfp4":
+        raise NotImplementedError(f"mode={mode!r}: products take mxfp4 weights")
+    if not transpose:
+        raise NotImplementedError("transpose=False is not on the hot path (the reference only uses transpose=True)")
 
 
 def _check_mode(mode: str, transpose: bool) -> None:
@@ -129,7 +162,19 @@ def quantized_matmul(x: torch.Tensor, w: torch.Tensor, scales: torch.Tensor, bia
     microseconds of host time) when libmlxturbo_b200_torch.so is built, else
     through the ctypes binding with the same checks in Python; both call the
     same C ABI entry and raise the same exception types.
+
+    mode="mxfp4" (group_size=32, bits=4, biases=None): w holds e2m1 codes and
+    scales uint8 [N, K/32].  bf16 activations enter without rounding, fp16 ones
+    too, as long as a value is no more than 2^14 below the largest of its 32
+    (below that to 2^-21 of that largest value); sums are in fp32.  A row with
+    an infinity or a NaN gives NaN where the product does not depend on it
+    alone.
     """
+    if mode != "affine" and mode in _MX_BITS:
+        _check_mx_weight(mode, group_size, bits, biases, transpose)
+        if out is None:
+            return _mx_ops().mx_matmul(x, None, w, scales, x.dtype)
+        return _mx_ops().mx_matmul_out(x, None, w, scales, out=out)
     if mode != "affine" or not transpose:
         _check_mode(mode, transpose)
     if biases is None:
@@ -291,8 +336,14 @@ def gather_qmm(x: torch.Tensor, w: torch.Tensor, scales: torch.Tensor, biases: t
     rhs_indices (rows,) and an output (rows, 1, N).  Here, as in MLX, the
     output shape is index_shape + (M, N) where x is (..., M, K) with batch
     dims broadcast against the indices; lhs_indices select x batches.
+    mode="mxfp4" takes the microscaled banks of ``quantize`` (scales uint8
+    [E, N, K/32], biases None); rows whose index is outside [0, E) become zero.
     """
-    _check_mode(mode, transpose)
+    mx = mode in _MX_BITS
+    if mx:
+        _check_mx_weight(mode, group_size, bits, biases, transpose)
+    else:
+        _check_mode(mode, transpose)
     if rhs_indices is None:
         raise NotImplementedError("gather_qmm without rhs_indices is quantized_matmul")
     _check_cuda(x, w, scales, biases, rhs_indices)
@@ -300,7 +351,8 @@ def gather_qmm(x: torch.Tensor, w: torch.Tensor, scales: torch.Tensor, biases: t
         raise ValueError("w must be [E, N, K*bits/32]")
     E, N = w.shape[0], w.shape[1]
     K = x.shape[-1]
-    if w.shape[2] * 32 != K * bits or scales.shape != (E, N, K // group_size) or biases.shape != scales.shape:
+    if w.shape[2] * 32 != K * bits or scales.shape != (E, N, K // group_size) or (
+            not mx and biases.shape != scales.shape):
         raise ValueError("w/scales/biases do not match x's K, bits and group_size")
     dt = _dtype_code(x)
     Mx = x.shape[-2] if x.dim() >= 2 else 1
@@ -331,6 +383,10 @@ def gather_qmm(x: torch.Tensor, w: torch.Tensor, scales: torch.Tensor, biases: t
         lhs_rows = (base[:, None] + torch.arange(Mx, device=x.device)[None, :]).reshape(-1)
         rhs_rows = rhs[:, None].expand(n_idx, Mx).reshape(-1)
     rows = rhs_rows.numel()
+    if mx:
+        y = _mx_ops().mx_gather(x_rows2, None, w, scales, None if lhs_rows is None else lhs_rows.to(torch.int32),
+                                rhs_rows.to(torch.int32), x.dtype, bool(sorted_indices))
+        return y.reshape(*idx_shape, Mx, N)
     rhs32 = _contig(rhs_rows.to(torch.int32))
     lhs32 = None if lhs_rows is None else _contig(lhs_rows.to(torch.int32))
     out = torch.empty((rows, N), dtype=x.dtype, device=x.device)
@@ -350,9 +406,16 @@ def gather_qmm(x: torch.Tensor, w: torch.Tensor, scales: torch.Tensor, biases: t
 # --------------------------------------------------------------------------
 
 def dequantize(w: torch.Tensor, scales: torch.Tensor, biases: torch.Tensor, group_size: int = 64, bits: int = 4,
-               mode: str = "affine") -> torch.Tensor:
-    """mx.dequantize: T [N, K] from the packed layout (scales' dtype)."""
+               mode: str = "affine", *, dtype: torch.dtype | None = None) -> torch.Tensor:
+    """mx.dequantize: T [N, K] from the packed layout (scales' dtype).
+
+    mode="mxfp4" / "mxfp8": values [..., K] of `dtype` (default bfloat16)."""
+    if mode in _MX_BITS:
+        _check_mx(mode, group_size, bits, biases)
+        return _mx_ops().mx_dequantize(w, scales, bits, dtype or torch.bfloat16)
     _check_mode(mode, True)
+    if dtype not in (None, scales.dtype):
+        raise NotImplementedError("affine dequantize returns the scales' dtype")
     _check_cuda(w, scales, biases)
     N = w.shape[0]
     K = w.shape[1] * 32 // bits
@@ -369,7 +432,18 @@ def quantize(w: torch.Tensor, group_size: int = 64, bits: int = 4, mode: str = "
     """mx.quantize (affine): (w_q uint32-bits-in-int32 [N, K*bits/32], scales, biases).
 
     Scales and biases take `dtype` (default: w's dtype if 16-bit, else bf16).
+
+    mode="mxfp4" (group_size=32, bits=4) and "mxfp8" (32, 8) take values
+    [..., K] of bf16, fp16 or fp32 and return (w_q int32 [..., K*bits/32],
+    scales uint8 [..., K/32]): per block of 32 the scale 2^e with
+    e = floor(log2(max|v|)) - 2 (mxfp4) or - 8 (mxfp8), codes rounded to nearest
+    even and saturated at 6 or 448; a block with an infinity or a NaN becomes NaN.
     """
+    if mode in _MX_BITS:
+        _check_mx(mode, group_size, bits)
+        if dtype is not None:
+            raise ValueError(f"mode={mode!r} has uint8 scales; dtype does not apply")
+        return _mx_ops().mx_quantize(w, bits)
     _check_mode(mode, True)
     _check_cuda(w)
     if w.dim() != 2:
@@ -385,6 +459,54 @@ def quantize(w: torch.Tensor, group_size: int = 64, bits: int = 4, mode: str = "
                                   bits, _DTYPE[dtype], _stream(w.device))
     _lib.check(rc, "quantize")
     return wq, sc, bi
+
+
+# --------------------------------------------------------------------------
+# 8-bit activations
+# --------------------------------------------------------------------------
+
+def rms_norm_quantize(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, *,
+                      residual: torch.Tensor | None = None
+                      ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor | None]:
+    """Residual addition, root-mean-square norm and mxfp8 rows in one launch.
+
+    Returns ``(xq, x_scales, h)``: with s = x + residual in fp32, h is s in x's
+    dtype (None without a residual) and xq int32 [..., K/4], x_scales uint8
+    [..., K/32] hold s / sqrt(mean(s^2) + eps) * weight in the mxfp8 format of
+    ``quantize``, computed in fp32 from s before its rounding.
+    """
+    xq, xs, h = _mx_ops().mx_rms_norm(x, residual, weight, eps)
+    return xq, xs, h if residual is not None else None
+
+
+def mx_matmul(xq: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor, scales: torch.Tensor, *,
+              dtype: torch.dtype = torch.bfloat16, lhs_indices: torch.Tensor | None = None,
+              rhs_indices: torch.Tensor | None = None, sorted_indices: bool = False,
+              out: torch.Tensor | None = None) -> torch.Tensor:
+    """y = dequant(xq) @ dequant(w)^T: mxfp8 activations times mxfp4 weights, fp32 sums.
+
+    xq int32 [..., K/4] and x_scales uint8 [..., K/32] as ``quantize`` (mode
+    "mxfp8") or ``rms_norm_quantize`` make them, w int32 [N, K/8] and scales
+    uint8 [N, K/32] of mode "mxfp4"; the result [..., N] has `dtype`.
+
+    With rhs_indices [rows] the weights are a bank [E, N, K/8] and row r of the
+    result [rows, N] is row lhs_indices[r] (r without lhs_indices) of the
+    flattened activations times expert rhs_indices[r]; sorted_indices promises
+    that rhs_indices do not decrease.
+    """
+    if rhs_indices is None:
+        if lhs_indices is not None or sorted_indices:
+            raise ValueError("lhs_indices and sorted_indices go with rhs_indices")
+        if out is None:
+            return _mx_ops().mx_matmul(xq, x_scales, w, scales, dtype)
+        if out.dtype != dtype:
+            raise ValueError(f"out has dtype {out.dtype}, expected {dtype}")
+        return _mx_ops().mx_matmul_out(xq, x_scales, w, scales, out=out)
+    if out is not None:
+        raise NotImplementedError("out is not supported with rhs_indices")
+    flat = [t if t is None else t.to(torch.int32) for t in (lhs_indices, rhs_indices)]
+    return _mx_ops().mx_gather(xq.reshape(-1, xq.shape[-1]), x_scales.reshape(-1, x_scales.shape[-1]), w, scales,
+                               flat[0], flat[1], dtype, bool(sorted_indices))
 
 
 def copy_(dst: torch.Tensor, src: torch.Tensor) -> torch.Tensor:
