@@ -162,6 +162,14 @@ struct MxMatmul {
 };
 int launch_mx_warp(const MxMatmul& a, const int4* items, const int32_t* n_items, long long items_max, int item_rows);
 int mx_warp_item_rows(long long rows, long long E);  // rows of one expert that a block takes
+// The tensor-core kernel (K % 128 == 0 and aligned weights), its rows per item
+// and its workspace behind the row tables.
+bool mx_tc_takes(const void* x, const uint8_t* xs, const uint32_t* w, const uint8_t* ws, long long rows, long long E,
+                 long long N, long long K);
+int mx_tc_item_rows(long long rows, long long E, bool mx, bool f16);
+size_t mx_tc_workspace(long long rows, long long E, long long N, long long K, bool mx, bool f16, bool grouped);
+int launch_mx_tc(const MxMatmul& a, const int4* items, const int32_t* n_items, const int32_t* ids, int bt, void* ws);
+int mx_device_error(int reset);
 // Items (expert, first sorted row, rows) of at most ir rows from ascending ids,
 // and their number; ids outside [0, E) have no item.
 int launch_mx_items(const int32_t* ids_sorted, long long rows, int E, int ir, int32_t* row_start, int4* items,

@@ -185,7 +185,10 @@ int qmm_mx_rms_norm(const void* x, const void* residual, const void* weight, voi
                               static_cast<cudaStream_t>(stream));
 }
 
-size_t qmm_mx_matmul_workspace_size(int64_t M, int64_t N, int64_t K, int dtype, int x_is_mx) { return 0; }
+size_t qmm_mx_matmul_workspace_size(int64_t M, int64_t N, int64_t K, int dtype, int x_is_mx) {
+    if (M <= 0 || N <= 0 || K <= 0 || K % 128) return 0;
+    return mx_tc_workspace(M, 1, N, K, x_is_mx, dtype == QMM_F16, false);
+}
 
 int qmm_mx_matmul(const void* x, const uint8_t* x_scales, const uint32_t* w, const uint8_t* scales, void* y,
                   int64_t M, int64_t N, int64_t K, int dtype, void* workspace, size_t workspace_bytes, void* stream) {
@@ -214,13 +217,21 @@ int qmm_mx_matmul(const void* x, const uint8_t* x_scales, const uint32_t* w, con
     a.f16 = dtype == QMM_F16;
     a.st = static_cast<cudaStream_t>(stream);
     fire("mx_matmul");
+    if (mx_tc_takes(x, x_scales, w, scales, M, 1, N, K))
+        return launch_mx_tc(a, nullptr, nullptr, nullptr, mx_tc_item_rows(M, 1, x_scales, a.f16), workspace);
     return launch_mx_warp(a, nullptr, nullptr, 0, mx_warp_item_rows(M, 1));
 }
 
 size_t qmm_mx_gather_workspace_size(int64_t rows, int64_t E, int64_t N, int64_t K, int dtype, int x_is_mx,
                                     int sorted) {
     if (rows <= 0 || E <= 0) return 0;
-    return gather_tables(nullptr, rows, E, sorted, mx_warp_item_rows(rows, E)).bytes;
+    // the kernel depends on the pointers' alignment too: room for either
+    const size_t warp = gather_tables(nullptr, rows, E, sorted, mx_warp_item_rows(rows, E)).bytes;
+    if (K <= 0 || K % 128) return warp;
+    const bool f16 = dtype == QMM_F16;
+    const size_t tc = gather_tables(nullptr, rows, E, sorted, mx_tc_item_rows(rows, E, x_is_mx, f16)).bytes +
+                      mx_tc_workspace(rows, E, N, K, x_is_mx, f16, true);
+    return tc > warp ? tc : warp;
 }
 
 int qmm_mx_gather(const void* x, const uint8_t* x_scales, const uint32_t* w, const uint8_t* scales,
@@ -248,7 +259,10 @@ int qmm_mx_gather(const void* x, const uint8_t* x_scales, const uint32_t* w, con
                               qmm_mx_gather_workspace_size(rows, E, N, K, dtype, x_scales != nullptr, sorted))))
         return rc;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    const GatherTables t = gather_tables(workspace, rows, E, sorted, mx_warp_item_rows(rows, E));
+    const bool f16 = dtype == QMM_F16, tc = mx_tc_takes(x, x_scales, w, scales, rows, E, N, K);
+    const GatherTables t =
+        gather_tables(workspace, rows, E, sorted,
+                      tc ? mx_tc_item_rows(rows, E, x_scales, f16) : mx_warp_item_rows(rows, E));
     MxMatmul a{};
     a.x = x;
     a.xs = x_scales;
@@ -260,7 +274,7 @@ int qmm_mx_gather(const void* x, const uint8_t* x_scales, const uint32_t* w, con
     a.E = E;
     a.N = N;
     a.K = K;
-    a.f16 = dtype == QMM_F16;
+    a.f16 = f16;
     a.st = st;
     const int32_t* n_items = t.n_items;
     if (sorted) {
@@ -284,9 +298,10 @@ int qmm_mx_gather(const void* x, const uint8_t* x_scales, const uint32_t* w, con
             a.src = t.row_src;
         }
     }
-    if (!rc) rc = launch_mx_zero_rows(rhs, rows, (int)E, y, N, st);
     if (rc) return rc;
     fire("mx_gather");
+    if (tc) return launch_mx_tc(a, t.items, n_items, rhs, t.item_rows, static_cast<char*>(workspace) + t.bytes);
+    if ((rc = launch_mx_zero_rows(rhs, rows, (int)E, y, N, st))) return rc;
     return launch_mx_warp(a, t.items, n_items, t.items_max, t.item_rows);
 }
 
