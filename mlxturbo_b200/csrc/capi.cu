@@ -81,7 +81,7 @@ int launch_ep_pack(const int32_t* ids, int n, int e_local, int world, int top_k,
                    int hidden, uint16_t* send, int row_stride, int32_t* slot_of, cudaStream_t st);
 int launch_moe_route(const uint32_t* ids, int M, int E, int top_k, int ir, uint32_t* order, uint32_t* idx_s,
                      uint32_t* row_src, uint32_t* inv, int32_t* row_start, int32_t* item_prefix, int4* item_info,
-                     cudaStream_t st);
+                     cudaStream_t st, const int32_t* lhs = nullptr);
 int launch_sort_rows(const uint32_t* ids, int M, int E, int top_k, uint32_t* order, uint32_t* idx_s,
                      uint32_t* row_src, uint32_t* inv, void* ws, size_t ws_bytes, cudaStream_t st);
 int launch_moe_combine(const uint16_t* out_sorted, long long src_rows, const uint32_t* inv, const float* w,

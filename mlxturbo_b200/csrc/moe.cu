@@ -255,8 +255,9 @@ constexpr int kRouteWarps = kRouteThreads / 32;
 constexpr int kRouteMaxRows = 16384;
 constexpr int kRouteMaxExperts = 1024;
 
+// lhs (null in qmm_moe_route): row_src = lhs[order] instead.
 __global__ void __launch_bounds__(kRouteThreads) moe_route_kernel(const uint32_t* ids, int M, int E, int top_k, int ir,
-                                                                  uint32_t* order, uint32_t* idx_s, uint32_t* row_src,
+                                                                  const int32_t* lhs, uint32_t* order, uint32_t* idx_s, uint32_t* row_src,
                                                                   uint32_t* inv, int32_t* row_start,
                                                                   int32_t* item_prefix, int4* item_info) {
     extern __shared__ int32_t sm[];
@@ -338,7 +339,7 @@ __global__ void __launch_bounds__(kRouteThreads) moe_route_kernel(const uint32_t
         if (valid) {
             order[pos] = (uint32_t)i;
             idx_s[pos] = e;
-            row_src[pos] = (uint32_t)i / (uint32_t)top_k;
+            row_src[pos] = lhs ? (uint32_t)lhs[i] : (uint32_t)i / (uint32_t)top_k;
             inv[i] = (uint32_t)pos;
         }
     }
@@ -569,7 +570,7 @@ size_t route_smem(long long M, long long E) {
 
 int launch_moe_route(const uint32_t* ids, int M, int E, int top_k, int ir, uint32_t* order, uint32_t* idx_s,
                      uint32_t* row_src, uint32_t* inv, int32_t* row_start, int32_t* item_prefix, int4* item_info,
-                     cudaStream_t st) {
+                     cudaStream_t st, const int32_t* lhs) {
     const size_t smem = route_smem(M, E);
     if (!smem) {
         set_error("moe_route: M=%d E=%d outside the one-CTA route (M <= %d, E <= %d)", M, E, qmm::kRouteMaxRows,
@@ -582,7 +583,7 @@ int launch_moe_route(const uint32_t* ids, int M, int E, int top_k, int ir, uint3
     }
     // a plain launch: the ids may come from work this library does not own
     // (a router kernel, or a collective's cross-stream join)
-    qmm::moe_route_kernel<<<1, qmm::kRouteThreads, smem, st>>>(ids, M, E, top_k, ir, order, idx_s, row_src, inv,
+    qmm::moe_route_kernel<<<1, qmm::kRouteThreads, smem, st>>>(ids, M, E, top_k, ir, lhs, order, idx_s, row_src, inv,
                                                                 row_start, item_prefix, item_info);
     return cuda_status(cudaGetLastError(), "moe_route launch");
 }

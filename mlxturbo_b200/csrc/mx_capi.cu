@@ -10,7 +10,7 @@ size_t sort_workspace(long long M, long long E);
 size_t route_smem(long long M, long long E);
 int launch_moe_route(const uint32_t* ids, int M, int E, int top_k, int ir, uint32_t* order, uint32_t* idx_s,
                      uint32_t* row_src, uint32_t* inv, int32_t* row_start, int32_t* item_prefix, int4* item_info,
-                     cudaStream_t st);
+                     cudaStream_t st, const int32_t* lhs = nullptr);
 int launch_sort_rows(const uint32_t* ids, int M, int E, int top_k, uint32_t* order, uint32_t* idx_s,
                      uint32_t* row_src, uint32_t* inv, void* ws, size_t ws_bytes, cudaStream_t st);
 int launch_compose(const int32_t* lhs, const uint32_t* order, uint32_t* out, long long n, cudaStream_t st);
@@ -186,7 +186,9 @@ int qmm_mx_rms_norm(const void* x, const void* residual, const void* weight, voi
 }
 
 size_t qmm_mx_matmul_workspace_size(int64_t M, int64_t N, int64_t K, int dtype, int x_is_mx) {
-    if (M <= 0 || N <= 0 || K <= 0 || K % 128) return 0;
+    if (M <= 0 || N <= 0 || K <= 0 || K % 32) return 0;
+    if (mx_f4_takes(M, 1, N, K)) return mx_f4_workspace(M, K, mx_f4_item_rows(M, 1, false));
+    if (K % 128) return 0;
     return mx_tc_workspace(M, 1, N, K, x_is_mx, dtype == QMM_F16, false);
 }
 
@@ -217,6 +219,8 @@ int qmm_mx_matmul(const void* x, const uint8_t* x_scales, const uint32_t* w, con
     a.f16 = dtype == QMM_F16;
     a.st = static_cast<cudaStream_t>(stream);
     fire("mx_matmul");
+    if (mx_f4_takes(M, 1, N, K))
+        return launch_mx_f4(a, nullptr, nullptr, nullptr, mx_f4_item_rows(M, 1, false), workspace);
     if (mx_tc_takes(x, x_scales, w, scales, M, 1, N, K))
         return launch_mx_tc(a, nullptr, nullptr, nullptr, mx_tc_item_rows(M, 1, x_scales, a.f16), workspace);
     return launch_mx_warp(a, nullptr, nullptr, 0, mx_warp_item_rows(M, 1));
@@ -225,13 +229,20 @@ int qmm_mx_matmul(const void* x, const uint8_t* x_scales, const uint32_t* w, con
 size_t qmm_mx_gather_workspace_size(int64_t rows, int64_t E, int64_t N, int64_t K, int dtype, int x_is_mx,
                                     int sorted) {
     if (rows <= 0 || E <= 0) return 0;
-    // the kernel depends on the pointers' alignment too: room for either
-    const size_t warp = gather_tables(nullptr, rows, E, sorted, mx_warp_item_rows(rows, E)).bytes;
-    if (K <= 0 || K % 128) return warp;
+    if (K <= 0 || K % 32) return 0;
+    // the kernel depends on alignment and limits too: room for any that may run
     const bool f16 = dtype == QMM_F16;
-    const size_t tc = gather_tables(nullptr, rows, E, sorted, mx_tc_item_rows(rows, E, x_is_mx, f16)).bytes +
-                      mx_tc_workspace(rows, E, N, K, x_is_mx, f16, true);
-    return tc > warp ? tc : warp;
+    size_t need = gather_tables(nullptr, rows, E, sorted, mx_warp_item_rows(rows, E)).bytes;
+    auto also = [&](int item_rows, size_t more) {
+        const size_t n = gather_tables(nullptr, rows, E, sorted, item_rows).bytes + more;
+        need = n > need ? n : need;
+    };
+    if (mx_f4_takes(rows, E, N, K)) {
+        const int bt = mx_f4_item_rows(rows, E, true);
+        also(bt, mx_f4_workspace(rows, K, bt));
+    } else if (K % 128 == 0)
+        also(mx_tc_item_rows(rows, E, x_is_mx, f16), mx_tc_workspace(rows, E, N, K, x_is_mx, f16, true));
+    return need;
 }
 
 int qmm_mx_gather(const void* x, const uint8_t* x_scales, const uint32_t* w, const uint8_t* scales,
@@ -259,10 +270,11 @@ int qmm_mx_gather(const void* x, const uint8_t* x_scales, const uint32_t* w, con
                               qmm_mx_gather_workspace_size(rows, E, N, K, dtype, x_scales != nullptr, sorted))))
         return rc;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    const bool f16 = dtype == QMM_F16, tc = mx_tc_takes(x, x_scales, w, scales, rows, E, N, K);
-    const GatherTables t =
-        gather_tables(workspace, rows, E, sorted,
-                      tc ? mx_tc_item_rows(rows, E, x_scales, f16) : mx_warp_item_rows(rows, E));
+    const bool f16 = dtype == QMM_F16;
+    const int f4 = mx_f4_takes(rows, E, N, K) ? mx_f4_item_rows(rows, E, true) : 0;
+    const bool tc = !f4 && mx_tc_takes(x, x_scales, w, scales, rows, E, N, K);
+    const int item_rows = f4 ? f4 : tc ? mx_tc_item_rows(rows, E, x_scales, f16) : mx_warp_item_rows(rows, E);
+    const GatherTables t = gather_tables(workspace, rows, E, sorted, item_rows);
     MxMatmul a{};
     a.x = x;
     a.xs = x_scales;
@@ -277,13 +289,18 @@ int qmm_mx_gather(const void* x, const uint8_t* x_scales, const uint32_t* w, con
     a.f16 = f16;
     a.st = st;
     const int32_t* n_items = t.n_items;
+    if (f4 && mx_f4_direct(rows, E, true)) {
+        fire("mx_gather");
+        a.lhs = lhs;
+        return launch_mx_f4(a, nullptr, nullptr, rhs, f4, nullptr);
+    }
     if (sorted) {
         rc = launch_mx_items(rhs, rows, (int)E, t.item_rows, t.row_start, t.items, t.items_max, t.n_items, st);
         a.src = reinterpret_cast<const uint32_t*>(lhs);
     } else {
-        if (route_smem(rows, E)) {  // a decode batch: sort and tables in one launch
+        if (route_smem(rows, E)) {  // a decode batch: sort, tables and x rows in one launch
             rc = launch_moe_route(reinterpret_cast<const uint32_t*>(rhs), (int)rows, (int)E, 1, t.item_rows, t.order,
-                                  t.idx_s, t.row_src, t.inv, t.row_start, t.item_prefix, t.items, st);
+                                  t.idx_s, t.row_src, t.inv, t.row_start, t.item_prefix, t.items, st, lhs);
             n_items = t.item_prefix + E;
         } else {
             rc = launch_sort_rows(reinterpret_cast<const uint32_t*>(rhs), (int)rows, (int)E, 1, t.order, t.idx_s,
@@ -291,15 +308,14 @@ int qmm_mx_gather(const void* x, const uint8_t* x_scales, const uint32_t* w, con
             if (!rc)
                 rc = launch_mx_items(reinterpret_cast<const int32_t*>(t.idx_s), rows, (int)E, t.item_rows, t.row_start,
                                      t.items, t.items_max, t.n_items, st);
+            if (!rc && lhs) rc = launch_compose(lhs, t.order, t.row_src, rows, st);
         }
-        a.src = a.dst = t.order;
-        if (!rc && lhs) {
-            rc = launch_compose(lhs, t.order, t.row_src, rows, st);
-            a.src = t.row_src;
-        }
+        a.dst = t.order;
+        a.src = t.row_src;
     }
     if (rc) return rc;
     fire("mx_gather");
+    if (f4) return launch_mx_f4(a, t.items, n_items, rhs, f4, static_cast<char*>(workspace) + t.bytes);
     if (tc) return launch_mx_tc(a, t.items, n_items, rhs, t.item_rows, static_cast<char*>(workspace) + t.bytes);
     if ((rc = launch_mx_zero_rows(rhs, rows, (int)E, y, N, st))) return rc;
     return launch_mx_warp(a, t.items, n_items, t.items_max, t.item_rows);

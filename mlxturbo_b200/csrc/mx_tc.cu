@@ -29,54 +29,11 @@
 // over the blocks, a tile shared by several is joined by the last of them to
 // finish, in the order of k, so results do not depend on timing.
 
-#include "mx.cuh"
-#include "tc.cuh"
-#include "tma.cuh"
+#include "mx_mma.cuh"
 
 namespace qmm {
 
-__device__ int g_mx_error;
-
-constexpr int MT_ROWS = 128;  // weight rows of a tile
 constexpr int MT_BK = 128;    // K of a stage
-
-// Bounded wait; false once it gave up, with the error flag set to `where` (the
-// first wait of the kernel to give up).
-QMM_DEVINL bool mt_wait(uint32_t bar, uint32_t parity, volatile int* abort, int where) {
-    for (uint32_t i = 0; i < (1u << 22); ++i) {
-        uint32_t ok;
-        asm volatile(
-            "{\n\t.reg .pred p;\n\t"
-            "mbarrier.test_wait.parity.acquire.cta.shared::cta.b64 p, [%1], %2;\n\t"
-            "selp.u32 %0, 1, 0, p;\n\t}"
-            : "=r"(ok)
-            : "r"(bar), "r"(parity)
-            : "memory");
-        if (ok) return true;
-        if ((i & 255u) == 255u && *abort) return false;
-        asm volatile(
-            "{\n\t.reg .pred p;\n\t"
-            "mbarrier.try_wait.parity.acquire.cta.shared::cta.b64 p, [%1], %2, %3;\n\t"
-            "selp.u32 %0, 1, 0, p;\n\t}"
-            : "=r"(ok)
-            : "r"(bar), "r"(parity), "r"(20u)
-            : "memory");
-        if (ok) return true;
-    }
-    *abort = 1;
-    atomicCAS(&g_mx_error, 0, where);
-    return false;
-}
-
-// Scale bytes for one operand block of up to 128 rows x 4 blocks of 32 (512
-// bytes): row r, block j at (r % 32) * 16 + (r / 32) * 4 + j.  Copied as 32
-// lanes x 16 bytes to every lane quarter of four TMEM columns.
-QMM_DEVINL void mt_copy_scales(uint32_t taddr, uint32_t saddr) {
-    uint64_t d = (uint64_t)((saddr & 0x3FFFFu) >> 4);
-    d |= (uint64_t)(128u >> 4) << 32;  // 8-row groups of 16-byte rows are 128 bytes apart
-    d |= (uint64_t)1 << 46;
-    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(d) : "memory");
-}
 
 QMM_DEVINL void mt_mma(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t sfa, uint32_t sfb,
                        uint32_t accumulate) {
@@ -96,18 +53,6 @@ QMM_DEVINL constexpr uint32_t mt_idesc(int N, uint32_t id) {
            (id << 29);
 }
 
-struct MxTcParams {
-    const uint8_t* sfw;       // [E * N, K/32]
-    const uint8_t* sfb;       // [P * R, K/32]
-    uint16_t* y;
-    const int4* items;        // grouped: (expert, first row, rows); dense: null
-    const int32_t* n_items;
-    const uint32_t* dst;      // y row of each row, or null
-    float* partial;           // [2 * gridDim.x][BT][128]
-    uint32_t* counters;       // four per tile (one per 32 rows), zero
-    int rows, R, N, KB, n_tiles, split;
-};
-
 // PCOL: the planes are columns of one MMA (BT * P wide; weights cross shared
 // memory once); else they are further K of the same accumulator.
 template <bool F16_, int P_, bool PCOL_, int BT_, int STAGES_>
@@ -120,12 +65,13 @@ struct MxTc {
     static constexpr int A_BYTES = MT_ROWS * MT_BK;
     static constexpr int A_TX = A_BYTES / 2;  // what a copy of packed codes counts on its barrier: the codes
     static constexpr int B_BYTES = PK * NB * MT_BK;
-    static constexpr int S_BYTES = 512 * (1 + PK * SFB);
+    static constexpr int S_BYTES = 512 * (1 + PK * SFB);  // scales of a k-block
+    static constexpr int SG = 3;                          // ring of scale groups (four k-blocks each)
     static constexpr int A_OFF = 0;
     static constexpr int B_OFF = A_OFF + STAGES * A_BYTES;
     static constexpr int S_OFF = B_OFF + STAGES * B_BYTES;
-    static constexpr int BAR_OFF = S_OFF + STAGES * S_BYTES;
-    static constexpr int BARS = 3 * STAGES + 4;
+    static constexpr int BAR_OFF = S_OFF + SG * 4 * S_BYTES;
+    static constexpr int BARS = 2 * STAGES + 2 * SG + 4;
     static constexpr int SMEM = BAR_OFF + BARS * 8 + 32 + 1024;
     static constexpr int S_COLS = 4 * (1 + PK * SFB);  // TMEM columns of a stage's scales
     static constexpr int ACCS = 2 * NB + STAGES * S_COLS <= 512 ? 2 : 1;
@@ -136,65 +82,6 @@ struct MxTc {
     static_assert(SMEM <= 227 * 1024, "shared memory");
     static_assert(NB % 16 == 0 && NB <= 256 && BT % 8 == 0, "MMA width");
 };
-
-// The stretches of k-blocks of one tile that a block works on, in order.
-struct MxWalk {
-    long long u, end;
-    int kb, step;  // step: whole tiles, every step-th
-    // split: block b of g has the k-blocks [all * b / g, all * (b + 1) / g), at least one
-    static QMM_DEVINL long long sharers(long long all) { return all < gridDim.x ? all : gridDim.x; }
-    QMM_DEVINL MxWalk(const MxTcParams& p, long long tiles) : kb(p.KB) {
-        if (p.split) {
-            const long long all = tiles * p.KB, g = sharers(all);
-            step = 0;
-            u = end = 0;
-            if (blockIdx.x < g) {
-                u = all * blockIdx.x / g;
-                end = all * (blockIdx.x + 1) / g;
-            }
-        } else {
-            step = gridDim.x;
-            u = blockIdx.x;
-            end = tiles;
-        }
-    }
-    QMM_DEVINL bool next(long long& tile, int& k0, int& k1) {
-        if (u >= end) return false;
-        if (step) {
-            tile = u;
-            k0 = 0;
-            k1 = kb;
-            u += step;
-        } else {
-            tile = u / kb;
-            k0 = (int)(u - tile * kb);
-            const long long left = end - u;
-            k1 = left < kb - k0 ? k0 + (int)left : kb;
-            u += k1 - k0;
-        }
-        return true;
-    }
-};
-
-struct MxTile {
-    int expert, row0, rows, n0;
-};
-QMM_DEVINL MxTile mt_tile(const MxTcParams& p, long long tile, int bt) {
-    MxTile t;
-    const int item = (int)(tile / p.n_tiles);
-    t.n0 = (int)(tile - (long long)item * p.n_tiles) * MT_ROWS;
-    if (p.items) {
-        const int4 it = ld_dep(p.items + item);
-        t.expert = it.x;
-        t.row0 = it.y;
-        t.rows = it.z;
-    } else {
-        t.expert = 0;
-        t.row0 = item * bt;
-        t.rows = min(bt, p.rows - t.row0);
-    }
-    return t;
-}
 
 template <int CH>
 QMM_DEVINL void mt_tmem_ld(uint32_t taddr, uint32_t (&v)[CH]) {
@@ -212,10 +99,11 @@ __global__ void __launch_bounds__(C::THREADS, 1)
     uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     const uint32_t sbase = smem_u32(smem), bars = sbase + C::BAR_OFF;
     auto full = [&](int s) { return bars + 8 * s; };
-    auto scaled = [&](int s) { return bars + 8 * (STAGES + s); };
-    auto empty = [&](int s) { return bars + 8 * (2 * STAGES + s); };
-    auto acc_full = [&](int b) { return bars + 8 * (3 * STAGES + b); };
-    auto acc_empty = [&](int b) { return bars + 8 * (3 * STAGES + 2 + b); };
+    auto empty = [&](int s) { return bars + 8 * (STAGES + s); };
+    auto scaled = [&](int g) { return bars + 8 * (2 * STAGES + g); };
+    auto s_empty = [&](int g) { return bars + 8 * (2 * STAGES + C::SG + g); };
+    auto acc_full = [&](int b) { return bars + 8 * (2 * STAGES + 2 * C::SG + b); };
+    auto acc_empty = [&](int b) { return bars + 8 * (2 * STAGES + 2 * C::SG + 2 + b); };
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::BAR_OFF + C::BARS * 8);
     volatile int* abort = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
@@ -224,8 +112,11 @@ __global__ void __launch_bounds__(C::THREADS, 1)
         *abort = 0;
         for (int s = 0; s < STAGES; ++s) {
             mbar_init(full(s), 1);
-            mbar_init(scaled(s), 4);
             mbar_init(empty(s), 1);
+        }
+        for (int g = 0; g < C::SG; ++g) {
+            mbar_init(scaled(g), 4);
+            mbar_init(s_empty(g), 1);
         }
         for (int b = 0; b < 2; ++b) {
             mbar_init(acc_full(b), 1);
@@ -251,10 +142,10 @@ __global__ void __launch_bounds__(C::THREADS, 1)
     // before this one, so the other warps wait for it here, and the TMA warp
     // once the weights of its first ring are on the way.
     if (warp != 0 || p.items) pdl_wait();
-    const long long tiles =
-        (long long)p.n_tiles * (p.items ? ld_dep(p.n_items) : (p.rows + C::BT - 1) / C::BT);
+    const uint32_t tiles =
+        (uint32_t)p.n_tiles * (uint32_t)(p.items ? ld_dep(p.n_items) : (p.rows + C::BT - 1) / C::BT);
     MxWalk walk(p, tiles);
-    long long tile;
+    uint32_t tile;
     int k0, k1;
 
     if (warp == 0) {
@@ -267,7 +158,7 @@ __global__ void __launch_bounds__(C::THREADS, 1)
 #pragma unroll
             for (int q = 0; q < C::P; ++q)
                 tma_load_2d(sbase + C::B_OFF + s * C::B_BYTES + q * C::BT * MT_BK, &tmap_b, full(s), kb * MT_BK,
-                            q * p.R + t.row0);
+                            q * p.rows + t.row0);
         };
         int i = 0, early = 0;
         if (!p.items) {
@@ -295,7 +186,7 @@ __global__ void __launch_bounds__(C::THREADS, 1)
     } else if (warp == 1) {
         // ---------------- scale copies and MMAs ----------------
         const uint64_t adesc0 = umma_desc_sw128(sbase + C::A_OFF), bdesc0 = umma_desc_sw128(sbase + C::B_OFF);
-        int i = 0, seg = 0;
+        int i = 0, seg = 0, g = -1;  // k-blocks, stretches and scale groups so far
         while (walk.next(tile, k0, k1) && !*abort) {
             const int b = seg % C::ACCS;
             const uint32_t acc = tmem + b * C::NB;
@@ -303,11 +194,15 @@ __global__ void __launch_bounds__(C::THREADS, 1)
             ++seg;
             for (int kb = k0; kb < k1; ++kb, ++i) {
                 const int s = i % STAGES;
-                const uint32_t ph = (uint32_t)(i / STAGES) & 1u;
-                if (!mt_wait(full(s), ph, abort, 4) || !mt_wait(scaled(s), ph, abort, 8)) break;
+                if (kb == k0 || (kb & 3) == 0) {
+                    ++g;
+                    if (!mt_wait(scaled(g % C::SG), (uint32_t)(g / C::SG) & 1u, abort, 8)) break;
+                }
+                if (!mt_wait(full(s), (uint32_t)(i / STAGES) & 1u, abort, 4)) break;
                 tc_fence_after();
                 if (elect_one()) {
-                    const uint32_t sfa = sf_cols + s * C::S_COLS, ssm = sbase + C::S_OFF + s * C::S_BYTES;
+                    const uint32_t sfa = sf_cols + s * C::S_COLS;
+                    const uint32_t ssm = sbase + C::S_OFF + ((g % C::SG) * 4 + (kb & 3)) * C::S_BYTES;
 #pragma unroll
                     for (int q = 0; q < 1 + C::PK * C::SFB; ++q) mt_copy_scales(sfa + 4 * q, ssm + 512 * q);
                     const uint64_t ad = adesc0 + ((uint32_t)(s * C::A_BYTES) >> 4);
@@ -320,6 +215,7 @@ __global__ void __launch_bounds__(C::THREADS, 1)
                                    mt_idesc(C::NB, (uint32_t)j), sfa, sfa + 4 * (1 + q * C::SFB),
                                    kb != k0 || q || j);
                     umma_commit(empty(s));
+                    if ((kb & 3) == 3 || kb + 1 == k1) umma_commit(s_empty(g % C::SG));
                 }
                 __syncwarp();
             }
@@ -328,46 +224,53 @@ __global__ void __launch_bounds__(C::THREADS, 1)
         }
     } else if (warp < 6) {
         // ---------------- scales ----------------
-        constexpr int NL = 1 + C::PK * C::SFB;  // words of this thread per k-block
-        constexpr int AHEAD = 4;                // k-blocks whose loads are in flight
+        // Thread r owns row r of the weight tile and of each block of 128 MMA
+        // columns; a row's words of four k-blocks are one 16-byte load where
+        // rows are that aligned.  Loads run three groups ahead.
+        constexpr int NL = 1 + C::PK * C::SFB;
+        constexpr int AHEAD = 3;
         const int r = (warp - 2) * 32 + lane;
-        const long long kw = p.KB;              // words (four blocks of 32) per row
         const uint32_t sdst = sbase + C::S_OFF + (r & 31) * 16 + (r >> 5) * 4;
-        int i = 0;
+        int g = 0;
         while (walk.next(tile, k0, k1) && !*abort) {
             const MxTile t = mt_tile(p, tile, C::BT);
-            const uint32_t* src[NL];
-            const int n = min(t.n0 + r, p.N - 1);
-            src[0] = reinterpret_cast<const uint32_t*>(p.sfw) + ((long long)t.expert * p.N + n) * kw;
+            const uint8_t* src[NL];
+            const int n_sf = p.KB * 4;
+            src[0] = p.sfw + ((long long)t.expert * p.N + min(t.n0 + r, p.N - 1)) * n_sf;
 #pragma unroll
             for (int q = 0; q < C::PK * C::SFB; ++q) {
                 const int c = min((q % C::SFB) * 128 + r, C::NB - 1);  // column of the MMA
                 const int plane = C::PCOL ? c / C::BT : q / C::SFB, tok = C::PCOL ? c % C::BT : c;
-                src[1 + q] = reinterpret_cast<const uint32_t*>(p.sfb) +
-                             ((long long)plane * p.R + min(t.row0 + tok, p.R - 1)) * kw;
+                src[1 + q] = p.sfb + ((long long)plane * p.rows + min(t.row0 + tok, p.rows - 1)) * n_sf;
             }
-            uint32_t v[AHEAD][NL];
+            const int last = (k1 - 1) >> 2;
+            auto load = [&](int q, int grp) {
+                return mt_scale_bytes(src[q], 16 * grp, n_sf, p.vec);
+            };
+            uint4 v[AHEAD][NL];
 #pragma unroll
             for (int a = 0; a < AHEAD; ++a)
 #pragma unroll
-                for (int q = 0; q < NL; ++q) v[a][q] = ld_dep(src[q] + min(k0 + a, k1 - 1));
-            for (int kb = k0; kb < k1; kb += AHEAD) {
+                for (int q = 0; q < NL; ++q) v[a][q] = load(q, min((k0 >> 2) + a, last));
+            for (int base = k0 >> 2; base <= last; base += AHEAD) {
 #pragma unroll
                 for (int a = 0; a < AHEAD; ++a) {
-                    if (kb + a >= k1) break;
-                    const int s = i % STAGES;
-                    const bool ok = mt_wait(empty(s), ((uint32_t)(i / STAGES) & 1u) ^ 1u, abort, 16);
-                    if (!ok) break;
-                    ++i;
+                    if (base + a > last) break;
+                    if (!mt_wait(s_empty(g % C::SG), ((uint32_t)(g / C::SG) & 1u) ^ 1u, abort, 16)) break;
+                    const uint32_t to = sdst + (g % C::SG) * 4 * C::S_BYTES;
+                    ++g;
 #pragma unroll
                     for (int q = 0; q < NL; ++q) {
-                        asm volatile("st.shared.u32 [%0], %1;" ::"r"(sdst + s * C::S_BYTES + 512 * q), "r"(v[a][q])
-                                     : "memory");
-                        v[a][q] = ld_dep(src[q] + min(kb + a + AHEAD, k1 - 1));
+                        const uint32_t w[4] = {v[a][q].x, v[a][q].y, v[a][q].z, v[a][q].w};
+#pragma unroll
+                        for (int c = 0; c < 4; ++c)
+                            asm volatile("st.shared.u32 [%0], %1;" ::"r"(to + c * C::S_BYTES + 512 * q), "r"(w[c])
+                                         : "memory");
+                        v[a][q] = load(q, min(base + a + AHEAD, last));
                     }
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                     __syncwarp();
-                    if (lane == 0) mbar_arrive(scaled(s));
+                    if (lane == 0) mbar_arrive(scaled((g - 1) % C::SG));
                 }
             }
         }
@@ -413,34 +316,15 @@ __global__ void __launch_bounds__(C::THREADS, 1)
             __syncwarp();
             if (lane == 0) mbar_arrive(acc_empty(b));
             if (whole) continue;
-            // Join: blocks first .. final share the tile; of each quarter of its
-            // rows the last warp to arrive adds the parts in the order of k.
-            const long long all = tiles * p.KB, g = MxWalk::sharers(all), a0 = tile * p.KB, a1 = a0 + p.KB;
-            auto block_of = [&](long long unit) {  // the block whose range holds this k-block
-                long long c = unit * g / all;
-                while (all * (c + 1) / g <= unit) ++c;
-                while (all * c / g > unit) --c;
-                return (int)c;
-            };
-            const int first = block_of(a0), final_ = block_of(a1 - 1);
-            __threadfence();
-            __syncwarp();
-            uint32_t before = 0;
-            if (lane == 0) before = atomicAdd(p.counters + tile * 4 + (warp & 3), 1u);
-            if (__shfl_sync(0xffffffffu, before, 0) != (uint32_t)(final_ - first)) continue;
-            __threadfence();
+            int first, final_;
+            if (!mt_last_of(p, walk, tile, first, final_)) continue;
             for (int c0 = 0; c0 < t.rows; c0 += 8) {
-                float f[8] = {};
-                for (int c = first; c <= final_; ++c) {
-                    const bool head = all * c / g <= a0;  // its stretch begins with the tile
-                    const float* q = p.partial + (long long)(2 * c + head) * (C::BT * MT_ROWS) + row;
-#pragma unroll
-                    for (int j = 0; j < 8; ++j)
-                        if (c0 + j < t.rows) f[j] += __ldcg(q + (c0 + j) * MT_ROWS);
-                }
+                float f[8];
+                const int nj = min(8, t.rows - c0);
+                mt_join8(p, first, final_, C::BT, c0, nj, row, f);
 #pragma unroll
                 for (int j = 0; j < 8; ++j)
-                    if (c0 + j < t.rows && n < p.N) store_y(c0 + j, f[j]);
+                    if (j < nj && n < p.N) store_y(c0 + j, f[j]);
             }
         }
     }
@@ -533,21 +417,6 @@ namespace qmm_host {
 
 namespace {
 
-size_t al256(size_t b) { return (b + 255) & ~(size_t)255; }
-
-constexpr int kMaxBlocks = 148;
-
-int sm_count() {
-    static int n = 0;
-    if (!n) {
-        int dev = 0, v = 0;
-        if (cudaGetDevice(&dev) == cudaSuccess &&
-            cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess && v > 0)
-            n = v < kMaxBlocks ? v : kMaxBlocks;
-    }
-    return n ? n : kMaxBlocks;
-}
-
 // Workspace of a tensor-core product behind the row tables.
 struct TcLayout {
     size_t planes, scales, counters, partial, bytes;
@@ -564,7 +433,7 @@ long long tiles_max(long long rows, long long E, long long N, int bt, bool group
 // Whether the k-blocks of the tiles are divided over the blocks: with fewer
 // whole tiles than about eight for each block the last round of tiles would
 // leave many blocks without one.
-bool tc_split(long long tiles, int bt) { return bt <= 64 ? tiles < 8 * kMaxBlocks : tiles < kMaxBlocks; }
+bool tc_split(long long tiles, int bt) { return bt <= 64 ? tiles < 8 * kMxMaxBlocks : tiles < kMxMaxBlocks; }
 
 TcLayout tc_layout(long long rows, long long E, long long N, long long K, bool mx, bool f16, bool grouped, int bt) {
     TcLayout l{};
@@ -575,13 +444,13 @@ TcLayout tc_layout(long long rows, long long E, long long N, long long K, bool m
     size_t at = 0;
     auto take = [&](size_t n) {
         const size_t o = at;
-        at += al256(n);
+        at += mx_al256(n);
         return o;
     };
     l.planes = take(l.prep ? (size_t)P * rows * K : 0);
     l.scales = take(l.prep ? (size_t)P * rows * (K / 32) : 0);
     l.counters = take(split ? (size_t)tiles * 16 : 0);
-    l.partial = take(split ? (size_t)2 * kMaxBlocks * bt * 128 * 4 : 0);
+    l.partial = take(split ? (size_t)2 * kMxMaxBlocks * bt * 128 * 4 : 0);
     l.bytes = at;
     return l;
 }
@@ -662,14 +531,19 @@ int launch_mx_tc(const MxMatmul& a, const int4* items, const int32_t* n_items, c
     p.dst = a.dst;
     p.partial = reinterpret_cast<float*>(base + l.partial);
     p.counters = counters;
-    p.rows = p.R = (int)a.rows;
+    p.rows = (int)a.rows;
+    p.K = (int)a.K;
     p.N = (int)a.N;
     p.KB = (int)(a.K / 128);
     p.n_tiles = (int)((a.N + 127) / 128);
+    p.vec = mx_scale_vec(a.K, p.sfw, p.sfb);
     const long long units = tiles * p.KB;
-    const int sms = sm_count();
+    const int sms = mx_sm_count();
     int blocks = (int)(tiles < sms ? tiles : sms);
-    if (p.split) blocks = (int)(units < sms ? units : sms);
+    if (p.split) {  // at least four k-blocks each: a join reads every sharer's part
+        const long long most = (units + 3) / 4;
+        blocks = (int)(most < sms ? most : sms);
+    }
 
     const bool prep = l.prep || p.split;
     if (prep) {
@@ -701,14 +575,6 @@ int launch_mx_tc(const MxMatmul& a, const int4* items, const int32_t* n_items, c
                  : launch_tc_bt<false, 2>(a, mw, mb, p, blocks, prep, bt);
 }
 
-int mx_device_error(int reset) {
-    int v = 0;
-    if (cudaMemcpyFromSymbol(&v, qmm::g_mx_error, sizeof(int)) != cudaSuccess) return -1;
-    if (reset && v) {
-        const int z = 0;
-        cudaMemcpyToSymbol(qmm::g_mx_error, &z, sizeof(int));
-    }
-    return v;
-}
+int mx_tc_device_error(int reset) { return mx_error_flag(reset); }
 
 }  // namespace qmm_host

@@ -375,6 +375,42 @@ def test_gather_many_rows(ops):
     check_grouped(y, host(x), ids, np.arange(rows), wv, False)
 
 
+@pytest.mark.parametrize("rows,E,N,K", [(100, 60, 2048, 512), (60, 40, 1920, 256), (90, 30, 1536, 768),
+                                        (20, 100, 2048, 2560)])
+def test_gather_many_tiles(ops, rows, E, N, K):
+    """Several tiles and several experts to a block."""
+    rng = np.random.default_rng(rows)
+    w = rng.integers(0, 1 << 32, size=(E, N, K // 8), dtype=np.uint64).astype(np.uint32).view(np.int32)
+    s = rng.integers(115, 125, size=(E, N, K // 32)).astype(np.uint8)
+    ids = np.minimum(rng.zipf(1.3, size=rows) - 1, E + 1).astype(np.int32)
+    rng.shuffle(ids)
+    x = activations(rng, rows, K, "bf16")
+    wt, st = dev(w), dev(s)
+    y = ops.gather_qmm(x.reshape(rows, 1, K), wt, st, None, rhs_indices=dev(ids), group_size=32, bits=4, mode="mxfp4")
+    used = np.unique(ids[ids < E])
+    wv = {int(e): _mx.values(w[e], s[e], 4) for e in used}
+    for e in np.unique(ids):
+        at = np.flatnonzero(ids == e)
+        rows_e = y[torch.from_numpy(at).cuda(), 0]
+        if e >= E:
+            assert (rows_e == 0).all()
+        else:
+            check_product(rows_e, host(x)[at], wv[int(e)], False, f"expert {e}")
+    assert ops.device_error() == 0
+
+
+@pytest.mark.parametrize("M", [1, 2, 3, 8, 12, 32])
+@pytest.mark.parametrize("N,K", [(40000, 256), (30000, 544)])
+def test_wide_products(ops, M, N, K):
+    """Many tiles to a block, K within one ring of k-blocks and past a whole number of them."""
+    rng = np.random.default_rng(M + K)
+    w, s, wv = _mx.random_weights(rng, (N, K))
+    x = activations(rng, M, K, "bf16")
+    y = ops.quantized_matmul(x, dev(w), dev(s), None, group_size=32, bits=4, mode="mxfp4")
+    check_product(y, host(x), wv, False)
+    assert ops.device_error() == 0
+
+
 def test_gather_promise_broken_is_contained(ops):
     """Ids that are not ascending after all: wrong rows, but nothing out of range, and later calls are right."""
     rng = np.random.default_rng(10)
