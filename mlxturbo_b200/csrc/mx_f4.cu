@@ -156,12 +156,6 @@ QMM_DEVINL void f4_digits(const F4Group& g, uint32_t (&plane)[8]) {
 // 24; a NaN stays in plane 0, the others' codes are zero).
 QMM_DEVINL uint32_t f4_plane_scale(uint32_t four, int q) { return four - 0x03030303u * (uint32_t)q; }
 
-QMM_DEVINL uint32_t cluster_rank() {
-    uint32_t r;
-    asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-    return r;
-}
-
 struct F4Params {
     MxTcParams c;
     const void* x;            // activations [x_rows, K] (values or e4m3 codes)
@@ -204,18 +198,6 @@ struct MxF4 {
     static_assert(SMEM <= 227 * 1024, "shared memory");
     static_assert(NB % 16 == 0 && NB <= 256 && (!OWN || BT <= 8), "MMA width");
 };
-
-QMM_DEVINL uint32_t f4_remote(uint32_t addr, uint32_t rank) {
-    uint32_t r;
-    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
-    return r;
-}
-QMM_DEVINL void f4_remote_arrive(uint32_t bar) {
-    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
-}
-QMM_DEVINL void f4_remote_store(uint32_t addr, float f) {
-    asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(f) : "memory");
-}
 
 // A cluster's tiles (a run, so that neighbours share an expert) and this
 // block's k-blocks of each.
@@ -302,7 +284,7 @@ __global__ void __launch_bounds__(C::THREADS, 1)
     volatile int* reached = abort + 1;  // k-blocks the MMA warp has begun
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const uint32_t S = (uint32_t)p.cluster, rank = cluster_rank();
+    const uint32_t S = (uint32_t)p.cluster, rank = mt_cluster_rank();
     if (threadIdx.x == 0) {
         *abort = 0;
         *reached = 0;
@@ -342,7 +324,7 @@ __global__ void __launch_bounds__(C::THREADS, 1)
         __syncthreads();
         tc_fence_after();
         // the other blocks' barriers are touched from the first join on
-        if (S > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+        if (S > 1) mt_cluster_arrive();
         tmem = *tmem_slot;
     };
 
@@ -534,9 +516,9 @@ __global__ void __launch_bounds__(C::THREADS, 1)
             for (int r = blockIdx.x * 4 + warp - 6; r < p.c.rows; r += gridDim.x * 4)
                 if ((uint32_t)ld_dep(p.ids + r) >= (uint32_t)p.E)
                     for (int n = lane; n < p.c.N; n += 32) p.c.y[(long long)r * p.c.N + n] = 0;
-        if (S > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+        if (S > 1) mt_cluster_wait();
         const uint32_t j_row = sbase + C::J_OFF + row * 4;
-        const uint32_t to = S > 1 && rank ? f4_remote(j_row + (rank - 1) * (C::BT * MT_ROWS * 4), 0) : 0;
+        const uint32_t to = S > 1 && rank ? mt_remote(j_row + (rank - 1) * (C::BT * MT_ROWS * 4), 0) : 0;
         constexpr int PER = C::BT < 4 ? C::BT : 4;  // rows of a TMEM load
         int seg = 0;
         for (F4Tiles tiles(p, walk, C::BT); tiles.more() && !*abort; tiles.next(p, C::BT)) {
@@ -569,7 +551,7 @@ __global__ void __launch_bounds__(C::THREADS, 1)
 #pragma unroll
                     for (int q = 6; q >= 0; --q) f += __uint_as_float(u[8 * d + q]);
                     if (rank != 0) {
-                        f4_remote_store(to + j * (MT_ROWS * 4), f);
+                        mt_remote_store(to + j * (MT_ROWS * 4), f);
                         continue;
                     }
                     for (uint32_t o = 0; o + 1 < S; ++o) {
@@ -587,9 +569,9 @@ __global__ void __launch_bounds__(C::THREADS, 1)
             __syncwarp();
             if (lane == 0) {
                 mbar_arrive(acc_empty(b));
-                if (rank != 0) f4_remote_arrive(f4_remote(join_full(quarter), 0));
+                if (rank != 0) mt_remote_arrive(mt_remote(join_full(quarter), 0));
                 else
-                    for (uint32_t o = 1; o < S; ++o) f4_remote_arrive(f4_remote(join_empty(quarter), o));
+                    for (uint32_t o = 1; o < S; ++o) mt_remote_arrive(mt_remote(join_empty(quarter), o));
             }
         }
     } else if constexpr (C::OWN) {
@@ -746,10 +728,10 @@ __global__ void __launch_bounds__(C::THREADS, 1)
         // every thread arrives twice and waits twice; a block's shared memory
         // outlives the others' last access to it
         __syncwarp();
-        if (warp < 6 || warp >= 10) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+        if (warp < 6 || warp >= 10) mt_cluster_wait();
         __syncwarp();
-        asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-        asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+        mt_cluster_arrive();
+        mt_cluster_wait();
     }
     tc_fence_before();
     __syncthreads();

@@ -53,14 +53,44 @@ QMM_DEVINL bool mt_wait(uint32_t bar, uint32_t parity, volatile int* abort, int 
     return false;
 }
 
+QMM_DEVINL uint32_t mt_cluster_rank() {
+    uint32_t r;
+    asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+// The address of another block's shared memory, an arrival there, a store.
+QMM_DEVINL uint32_t mt_remote(uint32_t addr, uint32_t rank) {
+    uint32_t r;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+    return r;
+}
+QMM_DEVINL void mt_remote_arrive(uint32_t bar) {
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+// The same without ordering other blocks' memory: what it announces is in this
+// block's own shared memory, behind a proxy fence.  (The cluster-wide release
+// costs about a microsecond.)
+QMM_DEVINL void mt_pair_arrive(uint32_t bar) {
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+QMM_DEVINL void mt_remote_store(uint32_t addr, float f) {
+    asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(f) : "memory");
+}
+QMM_DEVINL void mt_cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+QMM_DEVINL void mt_cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+
 // Scale bytes for one operand block of up to 128 rows x 4 blocks of 32 (512
 // bytes): row r, block j at (r % 32) * 16 + (r / 32) * 4 + j.  Copied as 32
 // lanes x 16 bytes to every lane quarter of four TMEM columns.
+template <int CTAS = 1>
 QMM_DEVINL void mt_copy_scales(uint32_t taddr, uint32_t saddr) {
     uint64_t d = (uint64_t)((saddr & 0x3FFFFu) >> 4);
     d |= (uint64_t)(128u >> 4) << 32;  // 8-row groups of 16-byte rows are 128 bytes apart
     d |= (uint64_t)1 << 46;
-    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(d) : "memory");
+    if constexpr (CTAS == 1)
+        asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(d) : "memory");
+    else
+        asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(d) : "memory");
 }
 
 struct MxTcParams {
@@ -70,36 +100,36 @@ struct MxTcParams {
     const int4* items;        // grouped: (expert, first row, rows); dense: null
     const int32_t* n_items;
     const uint32_t* dst;      // y row of each row, or null
-    float* partial;           // split: [2 * gridDim.x][rows of a tile][128]
-    uint32_t* counters;       // split: four per tile (one per 32 weight rows), zero
+    float* partial;           // split: parts of tiles
+    uint32_t* counters;       // split: one per tile and 32 weight rows, zero
     int rows, N, K, KB;       // KB: k-blocks
     int n_tiles, split;
     int vec;                  // bytes that one load of scale bytes may take: 16, 4 or 1
 };
 
-// The stretches of k-blocks of one tile that a block works on, in order.
-// Whole tiles: every gridDim.x-th.  Split: of g blocks the first `more` have
-// base + 1 k-blocks and the others base, consecutive.  32-bit arithmetic: the
+// The stretches of k-blocks of one tile that worker `me` of `count` (a pair of
+// blocks) has, in order.  Whole tiles: every count-th.  Split: of g workers the
+// first `more` have base + 1 k-blocks and the others base, consecutive.  32-bit arithmetic: the
 // host keeps tiles * KB below 2^31.
 struct MxWalk {
     uint32_t u, end, kb, step;
     uint32_t base, more;
-    QMM_DEVINL MxWalk(const MxTcParams& p, uint32_t tiles) : kb((uint32_t)p.KB) {
+    QMM_DEVINL MxWalk(const MxTcParams& p, uint32_t tiles, uint32_t me, uint32_t count) : kb((uint32_t)p.KB) {
         if (p.split) {
-            const uint32_t all = tiles * kb, g = min(all, gridDim.x);  // a block with no k-block shares nothing
+            const uint32_t all = tiles * kb, g = min(all, count);  // a worker with no k-block shares nothing
             step = base = more = u = end = 0;
             if (g) {
                 base = all / g;
                 more = all - base * g;
             }
-            if (blockIdx.x < g) {
-                u = start_of(blockIdx.x);
-                end = start_of(blockIdx.x + 1);
+            if (me < g) {
+                u = start_of(me);
+                end = start_of(me + 1);
             }
         } else {
             base = more = 0;
-            step = gridDim.x;
-            u = blockIdx.x;
+            step = count;
+            u = me;
             end = tiles;
         }
     }
@@ -128,10 +158,10 @@ struct MxWalk {
 struct MxTile {
     int expert, row0, rows, n0;
 };
-QMM_DEVINL MxTile mt_tile(const MxTcParams& p, uint32_t tile, int bt) {
+QMM_DEVINL MxTile mt_tile(const MxTcParams& p, uint32_t tile, int bt, int weight_rows) {
     MxTile t;
     const int item = (int)(tile / (uint32_t)p.n_tiles);
-    t.n0 = ((int)tile - item * p.n_tiles) * MT_ROWS;
+    t.n0 = ((int)tile - item * p.n_tiles) * weight_rows;
     if (p.items) {
         const int4 it = ld_dep(p.items + item);
         t.expert = it.x;
@@ -161,31 +191,30 @@ QMM_DEVINL uint4 mt_scale_bytes(const uint8_t* row, int at, int n, int vec) {
     return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// A block that computed a part of a tile stored it in its slot of p.partial;
-// true for the warp that has to join the parts (of its 32 weight rows): the
-// last of the blocks first .. final that share the tile.
-QMM_DEVINL bool mt_last_of(const MxTcParams& p, const MxWalk& w, uint32_t tile, int& first, int& final_) {
+// A worker that computed a part of a tile stored it in its slot; true for the
+// warp that has to join the parts (of its 32 weight rows, with a counter of
+// their own): the last of the workers first .. final that share the tile.
+QMM_DEVINL bool mt_last_of(const MxWalk& w, uint32_t tile, uint32_t* counter, int& first, int& final_) {
     first = (int)w.block_of(tile * w.kb);
     final_ = (int)w.block_of(tile * w.kb + w.kb - 1);
     __threadfence();
     __syncwarp();
     uint32_t before = 0;
-    if ((threadIdx.x & 31) == 0) before = atomicAdd(p.counters + tile * 4 + ((threadIdx.x >> 5) & 3), 1u);
+    if ((threadIdx.x & 31) == 0) before = atomicAdd(counter, 1u);
     if (__shfl_sync(0xffffffffu, before, 0) != (uint32_t)(final_ - first)) return false;
     __threadfence();
     return true;
 }
 
-// Slot of a block's part: 0 for a stretch that begins inside a tile (its
-// first), 1 for one that begins with the tile and ends inside it (its last).
-// The parts of columns c0 .. c0 + 7 at `row`, added in the order of k.
-QMM_DEVINL void mt_join8(const MxTcParams& p, int first, int final_, int bt, int c0, int nj, int row, float (&f)[8]) {
-    const long long slot = (long long)bt * MT_ROWS;
-    const float* base = p.partial + c0 * MT_ROWS + row;
+// The parts of eight columns (128 rows each, from `base` of the first worker's
+// slots), added in the order of k.  Slot 0 of a worker is a stretch that begins
+// inside a tile (its first), slot 1 one that begins with the tile and ends
+// inside it (its last).
+QMM_DEVINL void mt_join8(const float* base, long long slot, int first, int final_, int nj, float (&f)[8]) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) f[j] = 0.0f;
     for (int c = first; c <= final_; c += 4) {
-        float v[4][8];  // loads of four blocks in flight
+        float v[4][8];  // loads of four workers in flight
 #pragma unroll
         for (int d = 0; d < 4; ++d) {
             const float* from = base + (2 * (c + d) + (c + d == first)) * slot;

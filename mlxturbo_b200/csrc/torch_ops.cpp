@@ -360,7 +360,7 @@ at::Tensor mx_gather(const at::Tensor& x_in, const std::optional<at::Tensor>& xs
     const int64_t rows = rhs.size(0);
     at::Tensor y = at::empty({rows, N}, x.options().dtype(dtype));
     if (rows == 0) return y;
-    const size_t need = qmm_mx_gather_workspace_size(rows, E, N, K, dt, mx, sorted);
+    const size_t need = qmm_mx_gather_workspace_size(rows, x.size(0), E, N, K, dt, mx, sorted);
     const at::Tensor ws = mx_scratch(x, need);
     check(qmm_mx_gather(x.data_ptr(), mx ? static_cast<const uint8_t*>(xs.data_ptr()) : nullptr,
                         static_cast<const uint32_t*>(w.data_ptr()), static_cast<const uint8_t*>(s.data_ptr()),
