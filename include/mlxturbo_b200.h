@@ -380,8 +380,8 @@ QMM_API int qmm_mx_matmul(const void* x, const uint8_t* x_scales, const uint32_t
  * by expert on the device first.  Rows whose expert is outside [0, E) become
  * zero.  rows, x_rows <= 2^30, E <= 16384.
  */
-QMM_API size_t qmm_mx_gather_workspace_size(int64_t rows, int64_t x_rows, int64_t E, int64_t N, int64_t K, int dtype,
-                                            int x_is_mx, int sorted);
+QMM_API size_t qmm_mx_gather_workspace_size(int64_t rows, int64_t E, int64_t N, int64_t K, int dtype, int x_is_mx,
+                                            int sorted);
 QMM_API int qmm_mx_gather(const void* x, const uint8_t* x_scales, const uint32_t* w, const uint8_t* scales,
                           const int32_t* lhs, const int32_t* rhs, void* y, int64_t rows, int64_t x_rows, int64_t E,
                           int64_t N, int64_t K, int dtype, int sorted, void* workspace, size_t workspace_bytes,

@@ -62,7 +62,7 @@ SIGNATURES = {
     "qmm_mx_rms_norm": (_i, [_p, _p, _p, _p, _p, _p, _i64, _i64, _f, _i, _p]),
     "qmm_mx_matmul_workspace_size": (_sz, [_i64, _i64, _i64, _i, _i]),
     "qmm_mx_matmul": (_i, [_p, _p, _p, _p, _p, _i64, _i64, _i64, _i, _p, _sz, _p]),
-    "qmm_mx_gather_workspace_size": (_sz, [_i64, _i64, _i64, _i64, _i64, _i, _i, _i]),
+    "qmm_mx_gather_workspace_size": (_sz, [_i64, _i64, _i64, _i64, _i, _i, _i]),
     "qmm_mx_gather": (_i, [_p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i, _i, _p, _sz, _p]),
     "qmm_gather_tables": (_i, [_p, _i64, _i64, _p, _sz, _p]),
     "qmm_moe_route": (_i, [_p, _i64, _i64, _i, _p, _p, _p, _p, _p, _sz, _p]),

@@ -185,11 +185,9 @@ int launch_mx_warp(const MxMatmul& a, const int4* items, const int32_t* n_items,
 int mx_warp_item_rows(long long rows, long long E);  // rows of one expert that a block takes
 // The kernel for many rows (K % 128 == 0 and aligned scales), its rows per item
 // and its workspace behind the row tables.
-bool mx_tc_takes(const uint8_t* xs, const uint8_t* ws, long long rows, long long x_rows, long long E, long long N,
-                 long long K);
+bool mx_tc_takes(const uint8_t* xs, const uint8_t* ws, long long rows, long long E, long long N, long long K);
 int mx_tc_item_rows();
-size_t mx_tc_workspace(long long rows, long long x_rows, long long E, long long N, long long K, bool mx, bool f16,
-                       bool grouped);
+size_t mx_tc_workspace(long long rows, long long E, long long N, long long K, bool mx, bool f16, bool grouped);
 int launch_mx_tc(const MxMatmul& a, const int4* items, const int32_t* n_items, const int32_t* ids, void* ws);
 // The kernel for a few rows of an expert (any K % 32 == 0); item_rows 0 where
 // it is not for this size.  items == nullptr in a grouped call (`ids` given):

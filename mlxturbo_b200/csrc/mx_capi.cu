@@ -189,7 +189,7 @@ size_t qmm_mx_matmul_workspace_size(int64_t M, int64_t N, int64_t K, int dtype, 
     if (M <= 0 || N <= 0 || K <= 0 || K % 32) return 0;
     if (mx_f4_takes(M, 1, N, K)) return mx_f4_workspace(M, K, mx_f4_item_rows(M, 1, false));
     if (K % 128) return 0;
-    return mx_tc_workspace(M, M, 1, N, K, x_is_mx, dtype == QMM_F16, false);
+    return mx_tc_workspace(M, 1, N, K, x_is_mx, dtype == QMM_F16, false);
 }
 
 int qmm_mx_matmul(const void* x, const uint8_t* x_scales, const uint32_t* w, const uint8_t* scales, void* y,
@@ -221,13 +221,13 @@ int qmm_mx_matmul(const void* x, const uint8_t* x_scales, const uint32_t* w, con
     fire("mx_matmul");
     if (mx_f4_takes(M, 1, N, K))
         return launch_mx_f4(a, nullptr, nullptr, nullptr, mx_f4_item_rows(M, 1, false), workspace);
-    if (mx_tc_takes(x_scales, scales, M, M, 1, N, K))
+    if (mx_tc_takes(x_scales, scales, M, 1, N, K))
         return launch_mx_tc(a, nullptr, nullptr, nullptr, workspace);
     return launch_mx_warp(a, nullptr, nullptr, 0, mx_warp_item_rows(M, 1));
 }
 
-size_t qmm_mx_gather_workspace_size(int64_t rows, int64_t x_rows, int64_t E, int64_t N, int64_t K, int dtype,
-                                    int x_is_mx, int sorted) {
+size_t qmm_mx_gather_workspace_size(int64_t rows, int64_t E, int64_t N, int64_t K, int dtype, int x_is_mx,
+                                    int sorted) {
     if (rows <= 0 || E <= 0) return 0;
     if (K <= 0 || K % 32) return 0;
     // the kernel depends on alignment and limits too: room for any that may run
@@ -241,7 +241,7 @@ size_t qmm_mx_gather_workspace_size(int64_t rows, int64_t x_rows, int64_t E, int
         const int bt = mx_f4_item_rows(rows, E, true);
         also(bt, mx_f4_workspace(rows, K, bt));
     } else if (K % 128 == 0)
-        also(mx_tc_item_rows(), mx_tc_workspace(rows, x_rows, E, N, K, x_is_mx, f16, true));
+        also(mx_tc_item_rows(), mx_tc_workspace(rows, E, N, K, x_is_mx, f16, true));
     return need;
 }
 
@@ -267,13 +267,12 @@ int qmm_mx_gather(const void* x, const uint8_t* x_scales, const uint32_t* w, con
         return QMM_EINVAL;
     }
     if ((rc = check_workspace("mx_gather", workspace, workspace_bytes,
-                              qmm_mx_gather_workspace_size(rows, x_rows, E, N, K, dtype, x_scales != nullptr,
-                                                           sorted))))
+                              qmm_mx_gather_workspace_size(rows, E, N, K, dtype, x_scales != nullptr, sorted))))
         return rc;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     const bool f16 = dtype == QMM_F16;
     const int f4 = mx_f4_takes(rows, E, N, K) ? mx_f4_item_rows(rows, E, true) : 0;
-    const bool tc = !f4 && mx_tc_takes(x_scales, scales, rows, x_rows, E, N, K);
+    const bool tc = !f4 && mx_tc_takes(x_scales, scales, rows, E, N, K);
     const int item_rows = f4 ? f4 : tc ? mx_tc_item_rows() : mx_warp_item_rows(rows, E);
     const GatherTables t = gather_tables(workspace, rows, E, sorted, item_rows);
     MxMatmul a{};

@@ -65,15 +65,6 @@ QMM_DEVINL void mt_commit2(uint32_t bar) {
         "h"((uint16_t)3)
         : "memory");
 }
-// Four rows of a matrix by their indexes.
-QMM_DEVINL void mt_gather4(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, const int (&r)[4]) {
-    asm volatile(
-        "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes [%0], "
-        "[%1, {%3, %4, %5, %6, %7}], [%2];" ::"r"(dst),
-        "l"(map), "r"(bar), "r"(c0), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3])
-        : "memory");
-}
-
 // Instruction descriptor: A e2m1 (5), B e4m3 (0), both K-major, ue8m0 scales,
 // 256 x N, scale byte `id` of the four in a TMEM column for both operands.
 QMM_DEVINL uint32_t mt_idesc2(int N, uint32_t id) {
@@ -82,9 +73,8 @@ QMM_DEVINL uint32_t mt_idesc2(int N, uint32_t id) {
 
 struct MtParams {
     MxTcParams c;
-    const uint32_t* src;  // row -> plane row, or null
     const int32_t* ids;   // grouped: expert of each y row
-    int R, E;             // rows of a plane, experts
+    int E;                // experts
 };
 
 template <bool F16_, int P_, int STAGES_>
@@ -199,15 +189,6 @@ __global__ void __launch_bounds__(C::THREADS, 1)
         while (walk.next(tile, k0, k1) && !*abort) {
             const MxTile t = mt_tile(p.c, tile, MT_BT, MT_W);
             const int half = cols(t) / 2, mine = t.row0 + (int)rank * half;
-            int r[4];
-            if (p.src) {
-#pragma unroll
-                for (int d = 0; d < 4; ++d) {
-                    const int at = min((int)rank * half + lane * 4 + d, t.rows - 1);
-                    const uint32_t row = ld_dep(p.src + t.row0 + at);
-                    r[d] = row < (uint32_t)p.R ? (int)row : p.R - 1;
-                }
-            }
             for (int kb = k0; kb < k1; ++kb, ++i) {
                 if (kb == k0 || (kb & 1) == 0) {
                     const int w = pack % C::PACKS;
@@ -222,20 +203,10 @@ __global__ void __launch_bounds__(C::THREADS, 1)
                 if (!mt_wait(empty(s), ((uint32_t)(i / STAGES) & 1u) ^ 1u, abort, 1)) break;
                 const uint32_t b = sbase + C::B_OFF + s * C::B_BYTES;
                 if (elect_one()) {
-                    mbar_expect_tx(full_b(s), p.src ? C::P * half * MT_BK : C::B_BYTES);
-                    if (!p.src) {
+                    mbar_expect_tx(full_b(s), C::B_BYTES);
 #pragma unroll
-                        for (int q = 0; q < C::P; ++q)
-                            tma_load_2d(b + q * C::PLANE, &tmap_b, full_b(s), kb * MT_BK, q * p.R + mine);
-                    }
-                }
-                __syncwarp();
-                if (p.src && lane * 4 < half) {
-#pragma unroll
-                    for (int q = 0; q < C::P; ++q) {
-                        const int rq[4] = {r[0] + q * p.R, r[1] + q * p.R, r[2] + q * p.R, r[3] + q * p.R};
-                        mt_gather4(b + q * C::PLANE + lane * 4 * MT_BK, &tmap_b, full_b(s), kb * MT_BK, rq);
-                    }
+                    for (int q = 0; q < C::P; ++q)
+                        tma_load_2d(b + q * C::PLANE, &tmap_b, full_b(s), kb * MT_BK, q * p.c.rows + mine);
                 }
                 __syncwarp();
             }
@@ -289,13 +260,9 @@ __global__ void __launch_bounds__(C::THREADS, 1)
             src[0] = p.c.sfw + ((long long)t.expert * p.c.N + min(t.n0 + (int)rank * MT_ROWS + r, p.c.N - 1)) * n_sf;
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                int row = t.row0 + min(h * 128 + r, t.rows - 1);
-                if (p.src) {
-                    const uint32_t from = ld_dep(p.src + row);
-                    row = from < (uint32_t)p.R ? (int)from : p.R - 1;
-                }
+                const int row = t.row0 + min(h * 128 + r, t.rows - 1);
 #pragma unroll
-                for (int q = 0; q < C::P; ++q) src[1 + 2 * q + h] = p.c.sfb + ((long long)q * p.R + row) * n_sf;
+                for (int q = 0; q < C::P; ++q) src[1 + 2 * q + h] = p.c.sfb + ((long long)q * p.c.rows + row) * n_sf;
             }
             const int last = (k1 - 1) >> 2;
             auto load = [&](uint4 (&v)[NL], int grp) {
@@ -329,6 +296,9 @@ __global__ void __launch_bounds__(C::THREADS, 1)
                                          : "r"(from + (((4 * set + d) ^ (r & 7)) << 4))
                                          : "memory");
                     }
+                    // the reads above come before TMA's next write to the buffer (an
+                    // arrive alone does not wait for them)
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                     __syncwarp();
                     if (lane == 0) mbar_arrive(empty_w(w));
                     if (!in) continue;
@@ -431,10 +401,12 @@ __global__ void __launch_bounds__(C::THREADS, 1)
     }
 }
 
-// Activations to P e4m3 planes [P][R][K] with scales [P][R][K/32]; four lanes
-// hold a block.  Also clears the counters of the product that follows.
+// Activations to P e4m3 planes [P][R][K] with scales [P][R][K/32], rows taken
+// through src; four lanes hold a block.  P = 1 copies mxfp8 rows.  Also clears
+// the counters of the product that follows.
 template <int T, int P>
-__global__ void __launch_bounds__(256) mx_planes_kernel(const void* x, uint8_t* planes, uint8_t* scales, int R, int K,
+__global__ void __launch_bounds__(256) mx_planes_kernel(const void* x, const uint8_t* xs, uint8_t* planes,
+                                                        uint8_t* scales, const uint32_t* src, int x_rows, int R, int K,
                                                         uint32_t* counters, int n_counters) {
     pdl_launch_dependents();
     const int tid = blockIdx.y * gridDim.x + blockIdx.x;
@@ -446,8 +418,20 @@ __global__ void __launch_bounds__(256) mx_planes_kernel(const void* x, uint8_t* 
     const long long plane = (long long)R * g;
     for (int r = blockIdx.y; r < R; r += gridDim.y) {
         const long long i = (long long)r * g + c;
+        long long from = r;
+        if (src) {
+            from = ld_dep(src + r);
+            from = from < x_rows ? from : x_rows - 1;
+        }
+        if constexpr (P == 1) {
+            if (!in) continue;
+            reinterpret_cast<uint2*>(planes)[i] =
+                ld_dep(reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(x) + from * K) + c);
+            if ((c & 3) == 0) scales[i >> 2] = ld_dep(xs + from * (K / 32) + (c >> 2));
+            continue;
+        }
         float v[8] = {};
-        if (in) load8<T>(static_cast<const uint16_t*>(x) + i * 8, v);
+        if (in) load8<T>(static_cast<const uint16_t*>(x) + from * K + c * 8, v);
         uint32_t m = 0;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
@@ -513,8 +497,9 @@ long long tc_tiles_max(long long rows, long long E, long long N, bool grouped) {
 // last round.
 bool tc_split(long long tiles) { return tiles < 2 * kPairs; }
 
-TcLayout tc_layout(long long rows, long long x_rows, long long E, long long N, long long K, bool mx, bool f16,
-                   bool grouped) {
+// planes: of every row of the product; mxfp8 rows that are taken in order are
+// read where they are
+TcLayout tc_layout(long long rows, long long E, long long N, long long K, bool mx, bool f16, bool grouped) {
     TcLayout l{};
     const long long tiles = tc_tiles_max(rows, E, N, grouped);
     const bool split = tc_split(tiles);
@@ -525,8 +510,8 @@ TcLayout tc_layout(long long rows, long long x_rows, long long E, long long N, l
         at += mx_al256(n);
         return o;
     };
-    l.planes = take(mx ? 0 : (size_t)P * x_rows * K);
-    l.scales = take(mx ? 0 : (size_t)P * x_rows * (K / 32));
+    l.planes = take(mx && !grouped ? 0 : (size_t)P * rows * K);
+    l.scales = take(mx && !grouped ? 0 : (size_t)P * rows * (K / 32));
     l.counters = take(split ? (size_t)tiles * 32 : 0);
     l.partial = take(split ? (size_t)4 * kPairs * qmm::MT_BT * 128 * 4 : 0);
     l.bytes = at;
@@ -560,22 +545,20 @@ int launch_tc(const MxMatmul& a, const CUtensorMap& mw, const CUtensorMap& mb, c
 int mx_tc_item_rows() { return qmm::MT_BT; }
 
 // Rows of packed weights are whole 16-byte runs and k-blocks whole.
-bool mx_tc_takes(const uint8_t* xs, const uint8_t* ws, long long rows, long long x_rows, long long E, long long N,
-                 long long K) {
+bool mx_tc_takes(const uint8_t* xs, const uint8_t* ws, long long rows, long long E, long long N, long long K) {
     return K % 128 == 0 && ((uintptr_t)ws & 3u) == 0 && ((uintptr_t)xs & 3u) == 0 && E * N <= (1LL << 31) - 512 &&
-           3 * x_rows <= (1LL << 31) - 512 && rows <= (1LL << 31) - 512 &&
+           3 * rows <= (1LL << 31) - 512 &&
            tc_tiles_max(rows, E, N, true) * (K / 128) < (1LL << 31);
 }
 
-size_t mx_tc_workspace(long long rows, long long x_rows, long long E, long long N, long long K, bool mx, bool f16,
-                       bool grouped) {
-    return tc_layout(rows, x_rows, E, N, K, mx, f16, grouped).bytes;
+size_t mx_tc_workspace(long long rows, long long E, long long N, long long K, bool mx, bool f16, bool grouped) {
+    return tc_layout(rows, E, N, K, mx, f16, grouped).bytes;
 }
 
 int launch_mx_tc(const MxMatmul& a, const int4* items, const int32_t* n_items, const int32_t* ids, void* ws) {
-    const bool mx = a.xs != nullptr, grouped = items != nullptr;
+    const bool mx = a.xs != nullptr, grouped = items != nullptr, in_place = mx && !a.src;
     const int P = planes_of(mx, a.f16);
-    const TcLayout l = tc_layout(a.rows, a.x_rows, a.E, a.N, a.K, mx, a.f16, grouped);
+    const TcLayout l = tc_layout(a.rows, a.E, a.N, a.K, mx, a.f16, grouped);
     char* const base = static_cast<char*>(ws);
     const long long tiles = tc_tiles_max(a.rows, a.E, a.N, grouped);
     uint8_t* planes = reinterpret_cast<uint8_t*>(base + l.planes);
@@ -583,7 +566,7 @@ int launch_mx_tc(const MxMatmul& a, const int4* items, const int32_t* n_items, c
     qmm::MtParams p{};
     p.c.split = tc_split(tiles);
     p.c.sfw = a.ws;
-    p.c.sfb = mx ? a.xs : scales;
+    p.c.sfb = in_place ? a.xs : scales;
     p.c.y = static_cast<uint16_t*>(a.y);
     p.c.items = items;
     p.c.n_items = n_items;
@@ -596,9 +579,7 @@ int launch_mx_tc(const MxMatmul& a, const int4* items, const int32_t* n_items, c
     p.c.KB = (int)(a.K / 128);
     p.c.n_tiles = (int)((a.N + qmm::MT_W - 1) / qmm::MT_W);
     p.c.vec = mx_scale_vec(a.K, p.c.sfw, p.c.sfb);
-    p.src = a.src;
     p.ids = ids;
-    p.R = (int)a.x_rows;
     p.E = (int)a.E;
     const int most = mx_sm_count() / 2;
     long long pairs = tiles;
@@ -607,13 +588,14 @@ int launch_mx_tc(const MxMatmul& a, const int4* items, const int32_t* n_items, c
 
     const size_t n_counters = p.c.split ? (size_t)tiles * 8 : 0;
     int rc = QMM_OK;
-    if (!mx) {
+    if (!in_place) {
         const int g = (int)(a.K / 8);
-        const dim3 grid((unsigned)((g + 255) / 256), (unsigned)(a.x_rows < 32768 ? a.x_rows : 32768));
+        const dim3 grid((unsigned)((g + 255) / 256), (unsigned)(a.rows < 32768 ? a.rows : 32768));
 #define QMM_PLANES(T, PP)                                                                                         \
-    qmm::mx_planes_kernel<T, PP><<<grid, 256, 0, a.st>>>(a.x, planes, scales, (int)a.x_rows, (int)a.K,             \
-                                                         p.c.counters, (int)n_counters)
-        if (a.f16) QMM_PLANES(qmm::MX_F16, 3);
+    qmm::mx_planes_kernel<T, PP><<<grid, 256, 0, a.st>>>(a.x, a.xs, planes, scales, a.src, (int)a.x_rows,          \
+                                                         (int)a.rows, (int)a.K, p.c.counters, (int)n_counters)
+        if (mx) QMM_PLANES(qmm::MX_BF16, 1);
+        else if (a.f16) QMM_PLANES(qmm::MX_F16, 3);
         else QMM_PLANES(qmm::MX_BF16, 2);
 #undef QMM_PLANES
         rc = cuda_status(cudaGetLastError(), "mx_planes launch");
@@ -625,13 +607,12 @@ int launch_mx_tc(const MxMatmul& a, const int4* items, const int32_t* n_items, c
     rc = tensor_map_2d(&mw, CU_TENSOR_MAP_DATA_TYPE_UINT8, a.w, (uint64_t)a.K / 2, (uint64_t)(a.E * a.N),
                        (uint64_t)a.K / 2, 128, 128, CU_TENSOR_MAP_SWIZZLE_128B);
     if (rc) return rc;
-    rc = tensor_map_2d(&mb, CU_TENSOR_MAP_DATA_TYPE_UINT8, mx ? a.x : planes, (uint64_t)a.K,
-                       (uint64_t)(P * a.x_rows), (uint64_t)a.K, 128, a.src ? 1 : qmm::MT_HALF,
-                       CU_TENSOR_MAP_SWIZZLE_128B);
+    rc = tensor_map_2d(&mb, CU_TENSOR_MAP_DATA_TYPE_UINT8, in_place ? a.x : planes, (uint64_t)a.K,
+                       (uint64_t)(P * a.rows), (uint64_t)a.K, 128, qmm::MT_HALF, CU_TENSOR_MAP_SWIZZLE_128B);
     if (rc) return rc;
     using namespace qmm;
-    if (mx) return a.f16 ? launch_tc<MxTc<true, 1, 6>>(a, mw, mb, p, (int)pairs, false)
-                         : launch_tc<MxTc<false, 1, 6>>(a, mw, mb, p, (int)pairs, false);
+    if (mx) return a.f16 ? launch_tc<MxTc<true, 1, 6>>(a, mw, mb, p, (int)pairs, !in_place)
+                         : launch_tc<MxTc<false, 1, 6>>(a, mw, mb, p, (int)pairs, !in_place);
     return a.f16 ? launch_tc<MxTc<true, 3, 3>>(a, mw, mb, p, (int)pairs, true)
                  : launch_tc<MxTc<false, 2, 4>>(a, mw, mb, p, (int)pairs, true);
 }

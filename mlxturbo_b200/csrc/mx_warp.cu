@@ -164,11 +164,24 @@ __global__ void __launch_bounds__(1024) mx_items_kernel(const int32_t* ids, int 
                                                         int32_t* row_start, int4* items, int items_max,
                                                         int32_t* n_items) {
     __shared__ int wsum[32];
-    auto bucket = [&](int i) { return i < 0 ? -1 : i >= rows ? E : max(-1, min(E, ld_dep(ids + i))); };
-    // row_start[e] = first row with id >= e, for e in [0, E]
-    for (int i = threadIdx.x; i <= rows; i += blockDim.x) {
-        const int lo = bucket(i - 1), hi = i == rows ? E : bucket(i);
-        for (int e = lo + 1; e <= hi; ++e) row_start[e] = i;
+    auto bucket = [&](int id) { return max(-1, min(E, id)); };
+    // row_start[e] = first row with id >= e, for e in [0, E]; 16 rows a thread at
+    // a time, so that a few rounds of loads cover a long batch
+    constexpr int RUN = 16;
+    for (int i0 = threadIdx.x * RUN; i0 <= rows; i0 += blockDim.x * RUN) {
+        int id[RUN + 1];  // of row i0 - 1 first
+#pragma unroll
+        for (int j = 0; j <= RUN; ++j) {
+            const int i = i0 + j - 1;
+            id[j] = i >= 0 && i < rows ? ld_dep(ids + i) : 0;
+        }
+#pragma unroll
+        for (int j = 0; j < RUN; ++j) {
+            const int i = i0 + j;
+            if (i > rows) break;
+            const int lo = i == 0 ? -1 : bucket(id[j]), hi = i == rows ? E : bucket(id[j + 1]);
+            for (int e = lo + 1; e <= hi; ++e) row_start[e] = i;
+        }
     }
     __syncthreads();  // orders the block's own global writes and reads
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;

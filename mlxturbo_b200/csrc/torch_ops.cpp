@@ -193,12 +193,11 @@ int64_t mx_check_words(const char* what, const char* name, const at::Tensor& w, 
     if (w.element_size() != 4 || w.is_floating_point() || w.dim() < 1)
         fail(Err::kValue, "%s: %s must hold packed 32-bit words", what, name);
     if (s.scalar_type() != at::kByte) fail(Err::kValue, "%s: the scales of %s must be uint8", what, name);
-    const int64_t K = w.size(-1) * 32 / bits;
-    std::vector<int64_t> want(w.sizes().begin(), w.sizes().end());
-    want.back() = K / 32;
-    if (K % 32 || s.sizes() != at::IntArrayRef(want))
-        fail(Err::kValue, "%s: the scales of %s have shape %s, expected %s", what, name, dims(s.sizes()).c_str(),
-             dims(at::IntArrayRef(want)).c_str());
+    const int64_t K = w.size(-1) * 32 / bits, lead = w.dim() - 1;
+    if (K % 32 || s.dim() != w.dim() || s.size(-1) != K / 32 ||
+        s.sizes().slice(0, lead) != w.sizes().slice(0, lead))
+        fail(Err::kValue, "%s: the scales of %s have shape %s for words of shape %s", what, name,
+             dims(s.sizes()).c_str(), dims(w.sizes()).c_str());
     return K;
 }
 
@@ -336,7 +335,7 @@ at::Tensor& mx_matmul_out(const at::Tensor& x, const std::optional<at::Tensor>& 
     return out;
 }
 
-// x [x_rows, K] (or mxfp8 words [x_rows, K/4]), w [E, N, K/8]; lhs / rhs int32 [rows]; y [rows, N].
+// x [x_rows, K] or [x_rows, 1, K] (or mxfp8 words), w [E, N, K/8]; lhs / rhs int32 [rows]; y [rows, (1,) N].
 at::Tensor mx_gather(const at::Tensor& x_in, const std::optional<at::Tensor>& xs_in, const at::Tensor& w_in,
                      const at::Tensor& s_in, const std::optional<at::Tensor>& lhs_in, const at::Tensor& rhs_in,
                      at::ScalarType dtype, bool sorted) {
@@ -345,8 +344,9 @@ at::Tensor mx_gather(const at::Tensor& x_in, const std::optional<at::Tensor>& xs
     const int dt = mx_half_code(dtype);
     if (w_in.dim() != 3) fail(Err::kValue, "w must be [E, N, K/8]");
     const int64_t K = mx_check_words("mx_gather", "w", w_in, s_in, 4), E = w_in.size(0), N = w_in.size(1);
-    if (x_in.dim() != 2) fail(Err::kValue, "mx_gather: x must have two dimensions");
-    int64_t Kx = x_in.size(1);
+    const bool one = x_in.dim() == 3 && x_in.size(1) == 1;  // [x_rows, 1, K]: y is [rows, 1, N]
+    if (x_in.dim() != 2 && !one) fail(Err::kValue, "mx_gather: x must have shape [rows, K] or [rows, 1, K]");
+    int64_t Kx = x_in.size(-1);
     if (mx) Kx = mx_check_words("mx_gather", "x", x_in, *xs_in, 8);
     else if (x_in.scalar_type() != dtype) fail(Err::kValue, "mx_gather: x must have the output's dtype");
     if (Kx != K || K == 0 || N == 0 || E == 0)
@@ -358,9 +358,9 @@ at::Tensor mx_gather(const at::Tensor& x_in, const std::optional<at::Tensor>& xs
     const at::Tensor x = contiguous16(x_in), w = contiguous16(w_in), s = s_in.contiguous(), rhs = rhs_in.contiguous();
     const at::Tensor xs = mx ? xs_in->contiguous() : at::Tensor(), l = lhs ? lhs_in->contiguous() : at::Tensor();
     const int64_t rows = rhs.size(0);
-    at::Tensor y = at::empty({rows, N}, x.options().dtype(dtype));
+    at::Tensor y = one ? at::empty({rows, 1, N}, x.options().dtype(dtype)) : at::empty({rows, N}, x.options().dtype(dtype));
     if (rows == 0) return y;
-    const size_t need = qmm_mx_gather_workspace_size(rows, x.size(0), E, N, K, dt, mx, sorted);
+    const size_t need = qmm_mx_gather_workspace_size(rows, E, N, K, dt, mx, sorted);
     const at::Tensor ws = mx_scratch(x, need);
     check(qmm_mx_gather(x.data_ptr(), mx ? static_cast<const uint8_t*>(xs.data_ptr()) : nullptr,
                         static_cast<const uint32_t*>(w.data_ptr()), static_cast<const uint8_t*>(s.data_ptr()),

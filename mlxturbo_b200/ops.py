@@ -75,11 +75,29 @@ def _check_mx(mode: str, group_size: int, bits: int, biases=None) -> None:
         raise ValueError(f"mode={mode!r} has no biases")
 
 
-def _mx_ops():
-    ops = _lib.torch_ops()
-    if ops is None:
-        raise ImportError(f"{_lib.TORCH_OPS_PATH} is not built; run `python -m mlxturbo_b200.build`")
-    return ops
+class _MxOps:
+    """The MX operators' overloads, looked up once (a look-up by name costs a microsecond a call)."""
+
+    def __init__(self):
+        ops = _lib.torch_ops()
+        if ops is None:
+            raise ImportError(f"{_lib.TORCH_OPS_PATH} is not built; run `python -m mlxturbo_b200.build`")
+        self.quantize = ops.mx_quantize.default
+        self.dequantize = ops.mx_dequantize.default
+        self.rms_norm = ops.mx_rms_norm.default
+        self.matmul = ops.mx_matmul.default
+        self.matmul_out = ops.mx_matmul_out.default
+        self.gather = ops.mx_gather.default
+
+
+_MX: _MxOps | None = None
+
+
+def _mx_ops() -> _MxOps:
+    global _MX
+    if _MX is None:
+        _MX = _MxOps()
+    return _MX
 
 
 def _check_mx_weight(mode: str, group_size: int, bits: int, biases, transpose: bool) -> None:
@@ -173,8 +191,8 @@ def quantized_matmul(x: torch.Tensor, w: torch.Tensor, scales: torch.Tensor, bia
     if mode != "affine" and mode in _MX_BITS:
         _check_mx_weight(mode, group_size, bits, biases, transpose)
         if out is None:
-            return _mx_ops().mx_matmul(x, None, w, scales, x.dtype)
-        return _mx_ops().mx_matmul_out(x, None, w, scales, out=out)
+            return _mx_ops().matmul(x, None, w, scales, x.dtype)
+        return _mx_ops().matmul_out(x, None, w, scales, out=out)
     if mode != "affine" or not transpose:
         _check_mode(mode, transpose)
     if biases is None:
@@ -346,6 +364,11 @@ def gather_qmm(x: torch.Tensor, w: torch.Tensor, scales: torch.Tensor, biases: t
         _check_mode(mode, transpose)
     if rhs_indices is None:
         raise NotImplementedError("gather_qmm without rhs_indices is quantized_matmul")
+    if mx and x.dim() == 3 and x.shape[1] == 1 and rhs_indices.dim() == 1 and rhs_indices.dtype == torch.int32 and (
+            x.shape[0] == rhs_indices.shape[0] if lhs_indices is None
+            else lhs_indices.dtype == torch.int32 and lhs_indices.shape == rhs_indices.shape):
+        # one row to an index, the form of a routed batch: as it is
+        return _mx_ops().gather(x, None, w, scales, lhs_indices, rhs_indices, x.dtype, sorted_indices)
     _check_cuda(x, w, scales, biases, rhs_indices)
     if w.dim() != 3:
         raise ValueError("w must be [E, N, K*bits/32]")
@@ -384,7 +407,7 @@ def gather_qmm(x: torch.Tensor, w: torch.Tensor, scales: torch.Tensor, biases: t
         rhs_rows = rhs[:, None].expand(n_idx, Mx).reshape(-1)
     rows = rhs_rows.numel()
     if mx:
-        y = _mx_ops().mx_gather(x_rows2, None, w, scales, None if lhs_rows is None else lhs_rows.to(torch.int32),
+        y = _mx_ops().gather(x_rows2, None, w, scales, None if lhs_rows is None else lhs_rows.to(torch.int32),
                                 rhs_rows.to(torch.int32), x.dtype, bool(sorted_indices))
         return y.reshape(*idx_shape, Mx, N)
     rhs32 = _contig(rhs_rows.to(torch.int32))
@@ -412,7 +435,7 @@ def dequantize(w: torch.Tensor, scales: torch.Tensor, biases: torch.Tensor, grou
     mode="mxfp4" / "mxfp8": values [..., K] of `dtype` (default bfloat16)."""
     if mode in _MX_BITS:
         _check_mx(mode, group_size, bits, biases)
-        return _mx_ops().mx_dequantize(w, scales, bits, dtype or torch.bfloat16)
+        return _mx_ops().dequantize(w, scales, bits, dtype or torch.bfloat16)
     _check_mode(mode, True)
     if dtype not in (None, scales.dtype):
         raise NotImplementedError("affine dequantize returns the scales' dtype")
@@ -443,7 +466,7 @@ def quantize(w: torch.Tensor, group_size: int = 64, bits: int = 4, mode: str = "
         _check_mx(mode, group_size, bits)
         if dtype is not None:
             raise ValueError(f"mode={mode!r} has uint8 scales; dtype does not apply")
-        return _mx_ops().mx_quantize(w, bits)
+        return _mx_ops().quantize(w, bits)
     _check_mode(mode, True)
     _check_cuda(w)
     if w.dim() != 2:
@@ -475,7 +498,7 @@ def rms_norm_quantize(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, 
     [..., K/32] hold s / sqrt(mean(s^2) + eps) * weight in the mxfp8 format of
     ``quantize``, computed in fp32 from s before its rounding.
     """
-    xq, xs, h = _mx_ops().mx_rms_norm(x, residual, weight, eps)
+    xq, xs, h = _mx_ops().rms_norm(x, residual, weight, eps)
     return xq, xs, h if residual is not None else None
 
 
@@ -498,14 +521,14 @@ def mx_matmul(xq: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor, scales:
         if lhs_indices is not None or sorted_indices:
             raise ValueError("lhs_indices and sorted_indices go with rhs_indices")
         if out is None:
-            return _mx_ops().mx_matmul(xq, x_scales, w, scales, dtype)
+            return _mx_ops().matmul(xq, x_scales, w, scales, dtype)
         if out.dtype != dtype:
             raise ValueError(f"out has dtype {out.dtype}, expected {dtype}")
-        return _mx_ops().mx_matmul_out(xq, x_scales, w, scales, out=out)
+        return _mx_ops().matmul_out(xq, x_scales, w, scales, out=out)
     if out is not None:
         raise NotImplementedError("out is not supported with rhs_indices")
     flat = [t if t is None else t.to(torch.int32) for t in (lhs_indices, rhs_indices)]
-    return _mx_ops().mx_gather(xq.reshape(-1, xq.shape[-1]), x_scales.reshape(-1, x_scales.shape[-1]), w, scales,
+    return _mx_ops().gather(xq.reshape(-1, xq.shape[-1]), x_scales.reshape(-1, x_scales.shape[-1]), w, scales,
                                flat[0], flat[1], dtype, bool(sorted_indices))
 
 

@@ -263,6 +263,23 @@ def test_product_forms(ops):
     check_product(ops.quantized_matmul(x[:, ::2], view, dev(s), None, **kw), host(x[:, ::2]), wv, False)
 
 
+@pytest.mark.parametrize("M,N,K", [(130, 512, 1664), (300, 1024, 1152), (64, 640, 2048), (5, 1000, 640), (20, 512, 2048)])
+def test_products_repeat(ops, M, N, K):
+    """Equal bits on every call: no sum, hand-over or buffer depends on timing."""
+    rng = np.random.default_rng(M)
+    w, s, _ = _mx.random_weights(rng, (N, K))
+    xq, xs, _ = _mx.random_weights(rng, (M, K), 8, 1.0)
+    w, s, xq, xs = dev(w), dev(s), dev(xq), dev(xs)
+    x = {dt: activations(rng, M, K, dt) for dt in ("bf16", "f16")}
+    calls = [lambda: ops.mx_matmul(xq, xs, w, s)] + [
+        lambda v=v: ops.quantized_matmul(v, w, s, None, group_size=32, bits=4, mode="mxfp4") for v in x.values()]
+    for call in calls:
+        first = call()
+        same = torch.stack([(call() == first).all() for _ in range(400)])
+        assert same.all()
+    assert ops.device_error() == 0
+
+
 def test_products_on_another_stream(ops):
     rng = np.random.default_rng(7)
     w, s, wv = _mx.random_weights(rng, (512, 1024))
