@@ -29,9 +29,9 @@
 //   warp 0      TMA: packed weights and planes
 //   warp 1      tensor memory; in the first block scale copies and MMAs
 //   warps 2..9  two sets of four, a k-block each in turn: spread the weights'
-//               codes, 8 to 16 bytes as the instruction reads them; scale bytes
-//               into the instruction's layout
-//   warps 10..13 epilogue: TMEM -> y, or a partial sum
+//               codes, 8 to 16 bytes as the instruction reads them
+//   warps 10..13 scale bytes into the instruction's layout
+//   warps 14..17 epilogue: TMEM -> y, or a partial sum
 // TMA could spread the codes itself, but at 8 packed bytes a clock and SM: 1024
 // clocks for 128 x 128, which the MMAs of one plane need 384 for.
 //
@@ -85,19 +85,20 @@ struct MxTc {
     static constexpr int A_BYTES = MT_ROWS * MT_BK;     // spread
     static constexpr int PLANE = MT_HALF * MT_BK;
     static constexpr int B_BYTES = P * PLANE;
-    static constexpr int S_BYTES = 512 * (1 + 2 * P);   // weights, then two blocks of columns per plane
+    static constexpr int S_BYTES = 512 * (1 + 2 * P);   // of a k-block: weights, then two blocks of columns per plane
     static constexpr int W_BYTES = MT_ROWS * MT_BK;     // packed, two k-blocks
     static constexpr int A_OFF = 0;
     static constexpr int B_OFF = A_OFF + STAGES * A_BYTES;
     static constexpr int W_OFF = B_OFF + STAGES * B_BYTES;
+    static constexpr int SG = 2;                        // ring of scale groups, four k-blocks each
     static constexpr int S_OFF = W_OFF + PACKS * W_BYTES;
-    static constexpr int BAR_OFF = S_OFF + STAGES * S_BYTES;
-    static constexpr int BARS = 3 * STAGES + 2 * PACKS + 4;
+    static constexpr int BAR_OFF = S_OFF + SG * 4 * S_BYTES;
+    static constexpr int BARS = 3 * STAGES + 2 * PACKS + 2 * SG + 4;
     static constexpr int SMEM = BAR_OFF + BARS * 8 + 32 + 1024;
     static constexpr int S_COLS = 4 * (1 + 2 * P);
     static constexpr int USED = 2 * MT_BT + STAGES * S_COLS;
     static constexpr int COLS = 512;
-    static constexpr int THREADS = 448;
+    static constexpr int THREADS = 576;
     static_assert(USED <= 512, "tensor memory");
     static_assert(SMEM <= 227 * 1024, "shared memory");
 };
@@ -116,8 +117,10 @@ __global__ void __launch_bounds__(C::THREADS, 1)
     auto ready = [&](int s) { return bars + 8 * (2 * STAGES + s); };  // of the first block
     auto full_w = [&](int w) { return bars + 8 * (3 * STAGES + w); };
     auto empty_w = [&](int w) { return bars + 8 * (3 * STAGES + C::PACKS + w); };
-    auto acc_full = [&](int b) { return bars + 8 * (3 * STAGES + 2 * C::PACKS + b); };
-    auto acc_empty = [&](int b) { return bars + 8 * (3 * STAGES + 2 * C::PACKS + 2 + b); };  // of the first block
+    auto scaled = [&](int g) { return bars + 8 * (3 * STAGES + 2 * C::PACKS + g); };  // of the first block
+    auto s_empty = [&](int g) { return bars + 8 * (3 * STAGES + 2 * C::PACKS + C::SG + g); };
+    auto acc_full = [&](int b) { return bars + 8 * (3 * STAGES + 2 * C::PACKS + 2 * C::SG + b); };
+    auto acc_empty = [&](int b) { return bars + 8 * (3 * STAGES + 2 * C::PACKS + 2 * C::SG + 2 + b); };  // of the first
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::BAR_OFF + C::BARS * 8);
     volatile int* abort = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
@@ -133,6 +136,10 @@ __global__ void __launch_bounds__(C::THREADS, 1)
         for (int w = 0; w < C::PACKS; ++w) {
             mbar_init(full_w(w), 1);
             mbar_init(empty_w(w), 8);
+        }
+        for (int g = 0; g < C::SG; ++g) {
+            mbar_init(scaled(g), 8);
+            mbar_init(s_empty(g), 1);
         }
         for (int b = 0; b < 2; ++b) {
             mbar_init(acc_full(b), 1);
@@ -214,7 +221,7 @@ __global__ void __launch_bounds__(C::THREADS, 1)
     } else if (warp == 1) {
         // ---------------- scale copies and MMAs (first block) ----------------
         const uint64_t adesc0 = umma_desc_sw128(sbase + C::A_OFF), bdesc0 = umma_desc_sw128(sbase + C::B_OFF);
-        int i = 0, seg = 0;
+        int i = 0, seg = 0, g = -1;
         while (rank == 0 && walk.next(tile, k0, k1) && !*abort) {
             const int nb = cols(mt_tile(p.c, tile, MT_BT, MT_W)), b = seg & 1;
             const uint32_t acc = tmem + b * MT_BT;
@@ -222,10 +229,15 @@ __global__ void __launch_bounds__(C::THREADS, 1)
             ++seg;
             for (int kb = k0; kb < k1; ++kb, ++i) {
                 const int s = i % STAGES;
+                if (kb == k0 || (kb & 3) == 0) {
+                    ++g;
+                    if (!mt_wait(scaled(g % C::SG), (uint32_t)(g / C::SG) & 1u, abort, 256)) break;
+                }
                 if (!mt_wait(ready(s), (uint32_t)(i / STAGES) & 1u, abort, 4)) break;
                 tc_fence_after();
                 if (elect_one()) {
-                    const uint32_t sfa = sf_cols + s * C::S_COLS, ssm = sbase + C::S_OFF + s * C::S_BYTES;
+                    const uint32_t sfa = sf_cols + s * C::S_COLS;
+                    const uint32_t ssm = sbase + C::S_OFF + ((g % C::SG) * 4 + (kb & 3)) * C::S_BYTES;
 #pragma unroll
                     for (int q = 0; q < 1 + 2 * C::P; ++q) mt_copy_scales<2>(sfa + 4 * q, ssm + 512 * q);
                     const uint64_t ad = adesc0 + ((uint32_t)(s * C::A_BYTES) >> 4);
@@ -237,6 +249,7 @@ __global__ void __launch_bounds__(C::THREADS, 1)
                             mt_mma2(acc, ad + 2 * j, bd + ((q * C::PLANE) >> 4) + 2 * j, mt_idesc2(nb, (uint32_t)j), sfa,
                                     sfa + 4 * (1 + 2 * q), kb != k0 || q || j);
                     mt_commit2(empty(s));
+                    if ((kb & 3) == 3 || kb + 1 == k1) mt_commit2(s_empty(g % C::SG));
                 }
                 __syncwarp();
             }
@@ -244,19 +257,68 @@ __global__ void __launch_bounds__(C::THREADS, 1)
             __syncwarp();
         }
     } else if (warp < 10) {
-        // ---------------- codes and scales ----------------
-        // Thread r of a set has row r of this block's weights, and columns r and
-        // r + 128 of the tile; set 0 takes the even k-blocks, set 1 the odd.  A
-        // row's scale words of four k-blocks are one 16-byte load where rows are
-        // that aligned; two such groups are in flight.
-        constexpr int NL = 1 + 2 * C::P;
-        const int set = (warp - 2) >> 2, r = ((warp - 2) & 3) * 32 + lane, n_sf = p.c.KB * 4;
-        const uint32_t sdst = sbase + C::S_OFF + (r & 31) * 16 + (r >> 5) * 4;
+        // ---------------- codes ----------------
+        // Thread r of a set has row r of this block's weights; set 0 takes the
+        // even k-blocks, set 1 the odd.
+        const int set = (warp - 2) >> 2, r = ((warp - 2) & 3) * 32 + lane;
         const uint32_t ready0 = mt_remote(ready(0), 0);
         int i0 = 0, pack = 0;  // k-blocks before this stretch, pairs so far
         while (walk.next(tile, k0, k1) && !*abort) {
+            for (int j = k0 >> 1; j <= (k1 - 1) >> 1; ++j, ++pack) {
+                const int kb = 2 * j + set, w = pack % C::PACKS;
+                const bool in = kb >= k0 && kb < k1;
+                uint32_t c[4][4];
+                if (!mt_wait(full_w(w), (uint32_t)(pack / C::PACKS) & 1u, abort, 8)) break;
+                if (in) {
+                    const uint32_t from = sbase + C::W_OFF + w * C::W_BYTES + r * 128;
+#pragma unroll
+                    for (int d = 0; d < 4; ++d)  // 128-byte swizzle: chunk ^ row
+                        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                                     : "=r"(c[d][0]), "=r"(c[d][1]), "=r"(c[d][2]), "=r"(c[d][3])
+                                     : "r"(from + (((4 * set + d) ^ (r & 7)) << 4))
+                                     : "memory");
+                }
+                // the reads above come before TMA's next write to the buffer (an
+                // arrive alone does not wait for them)
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) mbar_arrive(empty_w(w));
+                if (!in) continue;
+                const int i = i0 + kb - k0, s = i % STAGES;
+                const uint32_t ph = (uint32_t)(i / STAGES) & 1u;
+                if (!mt_wait(empty(s), ph ^ 1u, abort, 128)) break;
+                const uint32_t to = sbase + C::A_OFF + s * C::A_BYTES + r * 128;
+#pragma unroll
+                for (int d = 0; d < 4; ++d)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e)  // 16 codes of 8 bytes to 16 bytes
+                        asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(to + (((2 * d + e) ^ (r & 7)) << 4)),
+                                     "r"(c[d][2 * e]), "r"(c[d][2 * e + 1])
+                                     : "memory");
+                if (!mt_wait(full_b(s), ph, abort, 16)) break;
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) mt_pair_arrive(ready0 + 8 * s);
+            }
+            i0 += k1 - k0;
+        }
+    } else if (warp < 14) {
+        // ---------------- scales ----------------
+        // Thread r has row r of this block's weights, and columns r and r + 128
+        // of the tile.  A group is 16 bytes of a row (four k-blocks); loads run
+        // AHEAD groups ahead, across tiles.
+        constexpr int NL = 1 + 2 * C::P;
+        constexpr int AHEAD = C::P == 3 ? 2 : 3;
+        const int r = (warp - 10) * 32 + lane, n_sf = p.c.KB * 4;
+        const uint32_t sdst = sbase + C::S_OFF + (r & 31) * 16 + (r >> 5) * 4;
+        const uint32_t scaled0 = mt_remote(scaled(0), 0);
+        const uint8_t* src[NL];
+        int grp = 0, last = -1;
+        bool more = true;
+        auto enter = [&]() {  // the next stretch
+            more = walk.next(tile, k0, k1);
+            if (!more) return;
             const MxTile t = mt_tile(p.c, tile, MT_BT, MT_W);
-            const uint8_t* src[NL];
             src[0] = p.c.sfw + ((long long)t.expert * p.c.N + min(t.n0 + (int)rank * MT_ROWS + r, p.c.N - 1)) * n_sf;
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
@@ -264,85 +326,58 @@ __global__ void __launch_bounds__(C::THREADS, 1)
 #pragma unroll
                 for (int q = 0; q < C::P; ++q) src[1 + 2 * q + h] = p.c.sfb + ((long long)q * p.c.rows + row) * n_sf;
             }
-            const int last = (k1 - 1) >> 2;
-            auto load = [&](uint4 (&v)[NL], int grp) {
-                grp = min(grp, last);
-                if (p.c.vec == 16) {
-                    v[0] = ldg_v4(src[0] + 16 * grp);
+            grp = k0 >> 2;
+            last = (k1 - 1) >> 2;
+        };
+        auto load = [&](uint4 (&v)[NL]) {  // false past the end
+            if (!more) return false;
+            if (p.c.vec == 16) {
+                v[0] = ldg_v4(src[0] + 16 * grp);
 #pragma unroll
-                    for (int q = 1; q < NL; ++q) v[q] = ld_v4(src[q] + 16 * grp);
-                } else {
+                for (int q = 1; q < NL; ++q) v[q] = ld_v4(src[q] + 16 * grp);
+            } else {
 #pragma unroll
-                    for (int q = 0; q < NL; ++q) v[q] = mt_scale_bytes(src[q], 16 * grp, n_sf, p.c.vec);
-                }
-            };
-            auto blocks = [&](const uint4 (&v)[NL], int grp) {  // up to two pairs of k-blocks
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const int kb = 4 * grp + 2 * h + set;
-                    if ((kb | 1) < k0 || (kb & ~1) >= k1) continue;  // no k-block of the pair
-                    const int w = pack % C::PACKS;
-                    const uint32_t pph = (uint32_t)(pack / C::PACKS) & 1u;
-                    ++pack;
-                    const bool in = kb >= k0 && kb < k1;
-                    uint32_t c[4][4];
-                    if (!mt_wait(full_w(w), pph, abort, 8)) return;
-                    if (in) {
-                        const uint32_t from = sbase + C::W_OFF + w * C::W_BYTES + r * 128;
-#pragma unroll
-                        for (int d = 0; d < 4; ++d)  // 128-byte swizzle: chunk ^ row
-                            asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
-                                         : "=r"(c[d][0]), "=r"(c[d][1]), "=r"(c[d][2]), "=r"(c[d][3])
-                                         : "r"(from + (((4 * set + d) ^ (r & 7)) << 4))
-                                         : "memory");
-                    }
-                    // the reads above come before TMA's next write to the buffer (an
-                    // arrive alone does not wait for them)
-                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(empty_w(w));
-                    if (!in) continue;
-                    const int i = i0 + kb - k0, s = i % STAGES;
-                    const uint32_t ph = (uint32_t)(i / STAGES) & 1u;
-                    if (!mt_wait(empty(s), ph ^ 1u, abort, 128)) return;
-                    const uint32_t to = sbase + C::A_OFF + s * C::A_BYTES + r * 128;
-#pragma unroll
-                    for (int d = 0; d < 4; ++d)
-#pragma unroll
-                        for (int e = 0; e < 2; ++e)  // 16 codes of 8 bytes to 16 bytes
-                            asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(to + (((2 * d + e) ^ (r & 7)) << 4)),
-                                         "r"(c[d][2 * e]), "r"(c[d][2 * e + 1])
-                                         : "memory");
-#pragma unroll
-                    for (int q = 0; q < NL; ++q) {
-                        const uint32_t word = h == 0 ? (set ? v[q].y : v[q].x) : (set ? v[q].w : v[q].z);
-                        asm volatile("st.shared.u32 [%0], %1;" ::"r"(sdst + s * C::S_BYTES + 512 * q), "r"(word)
-                                     : "memory");
-                    }
-                    if (!mt_wait(full_b(s), ph, abort, 16)) return;
-                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                    __syncwarp();
-                    if (lane == 0) mt_pair_arrive(ready0 + 8 * s);
-                }
-            };
-            uint4 u[NL], v[NL];
-            load(u, k0 >> 2);
-            load(v, (k0 >> 2) + 1);
-            for (int grp = k0 >> 2; grp <= last; grp += 2) {
-                blocks(u, grp);
-                load(u, grp + 2);
-                if (grp + 1 > last) break;
-                blocks(v, grp + 1);
-                load(v, grp + 3);
+                for (int q = 0; q < NL; ++q) v[q] = mt_scale_bytes(src[q], 16 * grp, n_sf, p.c.vec);
             }
-            i0 += k1 - k0;
+            if (++grp > last) enter();
+            return true;
+        };
+        uint4 v[AHEAD][NL];
+        bool have[AHEAD];
+        enter();
+#pragma unroll
+        for (int a = 0; a < AHEAD; ++a) have[a] = load(v[a]);
+        int g = 0;
+        while (have[0] && !*abort) {
+#pragma unroll
+            for (int a = 0; a < AHEAD; ++a) {
+                if (!have[a]) {
+                    have[0] = false;
+                    break;
+                }
+                if (!mt_wait(s_empty(g % C::SG), ((uint32_t)(g / C::SG) & 1u) ^ 1u, abort, 512)) break;
+                const uint32_t to = sdst + (g % C::SG) * 4 * C::S_BYTES;
+#pragma unroll
+                for (int q = 0; q < NL; ++q) {
+                    const uint32_t w[4] = {v[a][q].x, v[a][q].y, v[a][q].z, v[a][q].w};
+#pragma unroll
+                    for (int c = 0; c < 4; ++c)
+                        asm volatile("st.shared.u32 [%0], %1;" ::"r"(to + c * C::S_BYTES + 512 * q), "r"(w[c])
+                                     : "memory");
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) mt_pair_arrive(scaled0 + 8 * (g % C::SG));
+                ++g;
+                have[a] = load(v[a]);
+            }
         }
     } else {
         // ---------------- epilogue ----------------
         const int quarter = warp & 3, row = quarter * 32 + lane;  // weight row of the block = TMEM lane
         const uint32_t t_lane = tmem + ((uint32_t)(quarter * 32) << 16);
         if (p.ids)  // y rows whose id has no expert
-            for (int q = blockIdx.x * 4 + warp - 10; q < p.c.rows; q += gridDim.x * 4)
+            for (int q = blockIdx.x * 4 + warp - 14; q < p.c.rows; q += gridDim.x * 4)
                 if ((uint32_t)ld_dep(p.ids + q) >= (uint32_t)p.E)
                     for (int n = lane; n < p.c.N; n += 32) p.c.y[(long long)q * p.c.N + n] = 0;
         constexpr long long SLOT = (long long)MT_BT * MT_ROWS;
