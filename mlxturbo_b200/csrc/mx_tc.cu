@@ -397,16 +397,35 @@ __global__ void __launch_bounds__(C::THREADS, 1)
                 const long long out = p.c.dst ? (long long)ld_dep(p.c.dst + t.row0 + j) : t.row0 + j;
                 if (n < p.c.N) p.c.y[out * p.c.N + n] = H::from_f32(f);
             };
+            // Two lanes exchange halves, so that each stores two neighbouring
+            // outputs at once: the even lane for even rows, the odd for odd.
+            const bool pairs = whole && (p.c.N & 1) == 0;
+            const int n2 = n & ~1;
 #pragma unroll 1
-            for (int c0 = 0; c0 < t.rows; c0 += 16) {
-                uint32_t u[16];
-                tmem_ld16(t_lane + b * MT_BT + c0, u);
+            for (int c0 = 0; c0 < t.rows; c0 += 32) {
+                uint32_t u[32];
+                tmem_ld32(t_lane + b * MT_BT + c0, u);
+                int out_l = t.row0 + c0 + lane;  // y row of column c0 + lane
+                if (p.c.dst && c0 + lane < t.rows) out_l = (int)ld_dep(p.c.dst + out_l);
                 tmem_wait_ld();
+                if (pairs) {
 #pragma unroll
-                for (int j = 0; j < 16; ++j) {
-                    if (c0 + j >= t.rows) continue;
-                    if (!whole) part[(c0 + j) * MT_ROWS] = __uint_as_float(u[j]);
-                    else store_y(c0 + j, __uint_as_float(u[j]));
+                    for (int j = 0; j < 32; j += 2) {
+                        const uint32_t mine = lane & 1 ? u[j + 1] : u[j], give = lane & 1 ? u[j] : u[j + 1];
+                        const uint32_t got = __shfl_xor_sync(0xffffffffu, give, 1);
+                        const uint32_t lo = lane & 1 ? got : mine, hi = lane & 1 ? mine : got;
+                        const int out = __shfl_sync(0xffffffffu, out_l, j + (lane & 1));
+                        if (c0 + j + (lane & 1) < t.rows && n2 < p.c.N)
+                            *reinterpret_cast<uint32_t*>(p.c.y + (long long)out * p.c.N + n2) =
+                                H::pack2(__uint_as_float(lo), __uint_as_float(hi));
+                    }
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) {
+                        if (c0 + j >= t.rows) continue;
+                        if (!whole) part[(c0 + j) * MT_ROWS] = __uint_as_float(u[j]);
+                        else store_y(c0 + j, __uint_as_float(u[j]));
+                    }
                 }
             }
             tc_fence_before();
@@ -451,55 +470,81 @@ __global__ void __launch_bounds__(256) mx_planes_kernel(const void* x, const uin
     const int g = K / 8, c = blockIdx.x * blockDim.x + threadIdx.x;
     const bool in = c < g;  // whole blocks of 32 are in or out
     const long long plane = (long long)R * g;
-    for (int r = blockIdx.y; r < R; r += gridDim.y) {
-        const long long i = (long long)r * g + c;
-        long long from = r;
-        if (src) {
-            from = ld_dep(src + r);
-            from = from < x_rows ? from : x_rows - 1;
+    constexpr int RUN = 4;  // rows whose loads are in flight together
+    for (int r0 = blockIdx.y * RUN; r0 < R; r0 += gridDim.y * RUN) {
+        long long from[RUN];
+#pragma unroll
+        for (int k = 0; k < RUN; ++k) {
+            const int r = min(r0 + k, R - 1);
+            from[k] = r;
+            if (src) {
+                from[k] = ld_dep(src + r);
+                from[k] = from[k] < x_rows ? from[k] : x_rows - 1;
+            }
         }
         if constexpr (P == 1) {
             if (!in) continue;
-            reinterpret_cast<uint2*>(planes)[i] =
-                ld_dep(reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(x) + from * K) + c);
-            if ((c & 3) == 0) scales[i >> 2] = ld_dep(xs + from * (K / 32) + (c >> 2));
+            uint2 w[RUN];
+            uint8_t e[RUN];
+#pragma unroll
+            for (int k = 0; k < RUN; ++k) {
+                w[k] = ld_dep(reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(x) + from[k] * K) + c);
+                e[k] = (c & 3) == 0 ? ld_dep(xs + from[k] * (K / 32) + (c >> 2)) : 0;
+            }
+#pragma unroll
+            for (int k = 0; k < RUN; ++k) {
+                if (r0 + k >= R) break;
+                const long long i = (long long)(r0 + k) * g + c;
+                reinterpret_cast<uint2*>(planes)[i] = w[k];
+                if ((c & 3) == 0) scales[i >> 2] = e[k];
+            }
             continue;
         }
-        float v[8] = {};
-        if (in) load8<T>(static_cast<const uint16_t*>(x) + from * K + c * 8, v);
-        uint32_t m = 0;
+        uint4 raw[RUN];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const uint32_t a = abs_bits(v[j]);
-            if (a < 0x7F800000u) m = max(m, a);
-            else v[j] = __uint_as_float(0x7FC00000u);  // an infinity has no code: NaN
-        }
-        m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
-        m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
-        float inv;
-        // 128 <= largest < 256 on the grid: rounding cannot reach 448
-        uint32_t byte = mx_scale_byte<7>(m, inv);
+        for (int k = 0; k < RUN; ++k)
+            raw[k] = in ? ld_v4(static_cast<const uint16_t*>(x) + from[k] * K + c * 8) : make_uint4(0, 0, 0, 0);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] *= inv;
+        for (int k = 0; k < RUN; ++k) {
+            const long long i = (long long)(r0 + k) * g + c;
+            const bool live = in && r0 + k < R;
+            using H = Half<T == MX_F16>;
+            float v[8] = {H::lo_f32(raw[k].x), H::hi_f32(raw[k].x), H::lo_f32(raw[k].y), H::hi_f32(raw[k].y),
+                          H::lo_f32(raw[k].z), H::hi_f32(raw[k].z), H::lo_f32(raw[k].w), H::hi_f32(raw[k].w)};
+            uint32_t m = 0;
 #pragma unroll
-        for (int q = 0; q < P; ++q) {
-            uint32_t h[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) h[j] = cvt2_e4m3(v[2 * j], v[2 * j + 1]);
-            if (in) {
-                const long long o = q * plane + i;
-                reinterpret_cast<uint2*>(planes)[o] = make_uint2(h[0] | (h[1] << 16), h[2] | (h[3] << 16));
-                if ((c & 3) == 0) scales[o >> 2] = (uint8_t)byte;
+            for (int j = 0; j < 8; ++j) {
+                const uint32_t a = abs_bits(v[j]);
+                if (a < 0x7F800000u) m = max(m, a);
+                else v[j] = __uint_as_float(0x7FC00000u);  // an infinity has no code: NaN
             }
-            if (q + 1 < P) {
-                const uint32_t next = byte > 4 ? byte - 4 : 0;  // the remainder, up to 16 times larger
-                const float up = __uint_as_float((127u + byte - next) << 23);
-                byte = next;
+            m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
+            m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
+            float inv;
+            // 128 <= largest < 256 on the grid: rounding cannot reach 448
+            uint32_t byte = mx_scale_byte<7>(m, inv);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const uint32_t f = e4m3x2_f16x2(h[j]);
-                    v[2 * j] = (v[2 * j] - Half<true>::lo_f32(f)) * up;
-                    v[2 * j + 1] = (v[2 * j + 1] - Half<true>::hi_f32(f)) * up;
+            for (int j = 0; j < 8; ++j) v[j] *= inv;
+#pragma unroll
+            for (int q = 0; q < P; ++q) {
+                uint32_t h[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) h[j] = cvt2_e4m3(v[2 * j], v[2 * j + 1]);
+                if (live) {
+                    const long long o = q * plane + i;
+                    reinterpret_cast<uint2*>(planes)[o] = make_uint2(h[0] | (h[1] << 16), h[2] | (h[3] << 16));
+                    if ((c & 3) == 0) scales[o >> 2] = (uint8_t)byte;
+                }
+                if (q + 1 < P) {
+                    const uint32_t next = byte > 4 ? byte - 4 : 0;  // the remainder, up to 16 times larger
+                    const float up = __uint_as_float((127u + byte - next) << 23);
+                    byte = next;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const uint32_t f = e4m3x2_f16x2(h[j]);
+                        v[2 * j] = (v[2 * j] - Half<true>::lo_f32(f)) * up;
+                        v[2 * j + 1] = (v[2 * j + 1] - Half<true>::hi_f32(f)) * up;
+                    }
                 }
             }
         }
@@ -625,7 +670,8 @@ int launch_mx_tc(const MxMatmul& a, const int4* items, const int32_t* n_items, c
     int rc = QMM_OK;
     if (!in_place) {
         const int g = (int)(a.K / 8);
-        const dim3 grid((unsigned)((g + 255) / 256), (unsigned)(a.rows < 32768 ? a.rows : 32768));
+        const long long runs = (a.rows + 3) / 4;
+        const dim3 grid((unsigned)((g + 255) / 256), (unsigned)(runs < 32768 ? runs : 32768));
 #define QMM_PLANES(T, PP)                                                                                         \
     qmm::mx_planes_kernel<T, PP><<<grid, 256, 0, a.st>>>(a.x, a.xs, planes, scales, a.src, (int)a.x_rows,          \
                                                          (int)a.rows, (int)a.K, p.c.counters, (int)n_counters)

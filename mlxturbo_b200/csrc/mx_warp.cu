@@ -156,34 +156,22 @@ __global__ void __launch_bounds__(256) mx_warp_kernel(const void* x, const uint8
         }
 }
 
-// Ascending ids -> first row of each expert, then items of at most ir rows.
-// One block: a row whose id differs from its predecessor's starts every expert
-// between the two; the experts' item counts are then prefix-summed.  Ids that
-// are not ascending give wrong rows, never a row or an item out of range.
-__global__ void __launch_bounds__(1024) mx_items_kernel(const int32_t* ids, int rows, int E, int ir,
-                                                        int32_t* row_start, int4* items, int items_max,
-                                                        int32_t* n_items) {
+// Ascending ids -> first row of each expert: a row whose id differs from its
+// predecessor's starts every expert between the two.
+__global__ void __launch_bounds__(256) mx_row_start_kernel(const int32_t* ids, int rows, int E, int32_t* row_start) {
+    const int i = blockIdx.x * blockDim.x + threadIdx.x;
+    if (i > rows) return;
+    const int lo = i == 0 ? -1 : max(-1, min(E, ld_dep(ids + i - 1)));
+    const int hi = i == rows ? E : max(-1, min(E, ld_dep(ids + i)));
+    for (int e = lo + 1; e <= hi; ++e) row_start[e] = i;
+}
+
+// Items of at most ir rows from the experts' first rows: their numbers per
+// expert, prefix-summed over one block.  Ids that were not ascending give wrong
+// rows, never a row or an item out of range.
+__global__ void __launch_bounds__(1024) mx_items_kernel(const int32_t* row_start, int E, int ir, int4* items,
+                                                        int items_max, int32_t* n_items) {
     __shared__ int wsum[32];
-    auto bucket = [&](int id) { return max(-1, min(E, id)); };
-    // row_start[e] = first row with id >= e, for e in [0, E]; 16 rows a thread at
-    // a time, so that a few rounds of loads cover a long batch
-    constexpr int RUN = 16;
-    for (int i0 = threadIdx.x * RUN; i0 <= rows; i0 += blockDim.x * RUN) {
-        int id[RUN + 1];  // of row i0 - 1 first
-#pragma unroll
-        for (int j = 0; j <= RUN; ++j) {
-            const int i = i0 + j - 1;
-            id[j] = i >= 0 && i < rows ? ld_dep(ids + i) : 0;
-        }
-#pragma unroll
-        for (int j = 0; j < RUN; ++j) {
-            const int i = i0 + j;
-            if (i > rows) break;
-            const int lo = i == 0 ? -1 : bucket(id[j]), hi = i == rows ? E : bucket(id[j + 1]);
-            for (int e = lo + 1; e <= hi; ++e) row_start[e] = i;
-        }
-    }
-    __syncthreads();  // orders the block's own global writes and reads
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int per = (E + (int)blockDim.x - 1) / (int)blockDim.x;
     const int e0 = min(E, (int)threadIdx.x * per), e1 = min(E, e0 + per);
@@ -266,7 +254,10 @@ int launch_mx_warp(const MxMatmul& a, const int4* items, const int32_t* n_items,
 
 int launch_mx_items(const int32_t* ids_sorted, long long rows, int E, int ir, int32_t* row_start, int4* items,
                     long long items_max, int32_t* n_items, cudaStream_t st) {
-    qmm::mx_items_kernel<<<1, 1024, 0, st>>>(ids_sorted, (int)rows, E, ir, row_start, items, (int)items_max, n_items);
+    qmm::mx_row_start_kernel<<<(unsigned)(rows / 256 + 1), 256, 0, st>>>(ids_sorted, (int)rows, E, row_start);
+    const int rc = cuda_status(cudaGetLastError(), "mx_row_start launch");
+    if (rc) return rc;
+    qmm::mx_items_kernel<<<1, 1024, 0, st>>>(row_start, E, ir, items, (int)items_max, n_items);
     return cuda_status(cudaGetLastError(), "mx_items launch");
 }
 
