@@ -353,8 +353,8 @@ QMM_API int qmm_mx_dequantize(const uint32_t* words, const uint8_t* scales, void
  *   s = x + residual (fp32; s = x when residual is NULL)
  *   h = s rounded to dtype (written when residual is given)
  *   (xq, x_scales) = mxfp8 of s / sqrt(mean(s^2) + eps) * weight
- * x, residual, h [rows, K] and weight [K] of dtype; sums in fp32.  h may be
- * x or residual itself.
+ * x, residual, h [rows, K] and weight [K] of dtype; sums in fp32, in an order
+ * that depends on K only.  h must not overlap x or residual.
  */
 QMM_API int qmm_mx_rms_norm(const void* x, const void* residual, const void* weight, void* h, uint32_t* xq,
                             uint8_t* x_scales, int64_t rows, int64_t K, float eps, int dtype, void* stream);

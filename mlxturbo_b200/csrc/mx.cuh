@@ -134,6 +134,21 @@ QMM_DEVINL uint32_t round8_e2m1(const float (&v)[8], uint32_t (&h)[4]) {
     return r;
 }
 
+// Largest of the magnitudes of eight packed 16-bit floats, as one 16-bit
+// pattern (patterns without the sign order like the magnitudes they stand for,
+// infinity and then NaN above all), in both halves of the result's low bits.
+QMM_DEVINL uint32_t max_abs8(const uint4& a) {
+    const uint32_t M = 0x7FFF7FFFu;
+    return __vmaxu2(__vmaxu2(a.x & M, a.y & M), __vmaxu2(a.z & M, a.w & M));
+}
+// The fp32 bits of the larger half.
+template <bool F16>
+QMM_DEVINL uint32_t max_abs_f32(uint32_t two) {
+    const uint32_t m = max(two & 0xFFFFu, two >> 16);
+    if constexpr (F16) return __float_as_uint(Half<true>::to_f32((uint16_t)m));
+    else return m << 16;
+}
+
 // Four lanes of a warp hold a block, eight values each: quantise and store the
 // words and (the first of the four) the scale byte.  `o8` counts groups of
 // eight values; lanes with `in` false only take part in the shuffles.

@@ -176,8 +176,8 @@ int qmm_mx_rms_norm(const void* x, const void* residual, const void* weight, voi
     if (rows == 0) return QMM_OK;
     if ((rc = check_aligned("mx_rms_norm", {x, weight, xq}))) return rc;
     if (residual && (rc = check_aligned("mx_rms_norm", {residual, h}))) return rc;
-    if (!x_scales) {
-        set_error("mx_rms_norm: null pointer");
+    if (!x_scales || (residual && (h == x || h == residual))) {
+        set_error("mx_rms_norm: null pointer, or h is x or residual");
         return QMM_EINVAL;
     }
     fire("mx_rms_norm");

@@ -11,11 +11,11 @@
 //
 //   x = 2^e0 c0 + 2^(e0-4) c1 (+ 2^(e0-8) c2),  e0 = floor(log2 max|block|) - 7
 //
-// A code holds four significant bits and the remainder of rounding to nearest
-// has one bit less than the half unit it is bounded by, so two planes hold the
-// 8 significant bits of bf16 and three the 11 of fp16, exactly, for values down
-// to 2^-14 of the largest in their block of 32; below that the smallest code of
-// the last plane leaves 2^-21 (bf16) or 2^-25 (fp16) of that largest value.
+// A code holds four significant bits, a plane four more than the one before, so
+// two planes hold the 8 significant bits of bf16 and three the 11 of fp16,
+// exactly, for values down to 2^-14 of the largest in their block of 32; below
+// that the smallest code of the last plane leaves 2^-21 (bf16) or 2^-25 (fp16)
+// of that largest value.
 // The planes are further K of the same fp32 accumulator in TMEM.
 //
 // Bound by the tensor cores: 2 P M N K operations at the 8-bit rate, so a
@@ -455,11 +455,95 @@ __global__ void __launch_bounds__(C::THREADS, 1)
     }
 }
 
+// The two planes of bf16 rows, sixteen values to a thread, two at a time in
+// bf16, where a power of two, the cut after four bits and the remainder are
+// exact.  False (for the warp) where a block holds a value below the smallest
+// normal code or one that is not finite.
+QMM_DEVINL bool mt_planes_bf16(const uint4 (&raw)[2], bool live, uint4 (&out)[2], uint32_t& byte) {
+    const uint32_t u[8] = {raw[0].x, raw[0].y, raw[0].z, raw[0].w, raw[1].x, raw[1].y, raw[1].z, raw[1].w};
+    uint32_t m = max_abs_f32<false>(__vmaxu2(max_abs8(raw[0]), max_abs8(raw[1])));
+    m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
+    float inv;
+    byte = mx_scale_byte<7>(m, inv);
+    const uint32_t inv2 = (__float_as_uint(inv) >> 16) * 0x10001u;
+    uint32_t v2[8], least = 0xFFFFFFFFu;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(v2[j]) : "r"(u[j]), "r"(inv2));
+        least = __vminu2(least, v2[j] & 0x7FFF7FFFu);
+    }
+    const bool plain = byte >= 4 && m < 0x7F800000u && (least & 0xFFFFu) >= 0x3C80u && (least >> 16) >= 0x3C80u;  // 2^-6
+    if (!__all_sync(0xffffffffu, plain || !live)) return false;
+    uint32_t hi[8], lo[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const uint32_t top = v2[j] & 0xFFF0FFF0u;
+        uint32_t minus, rest;  // 16 (v - top)
+        asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(minus) : "r"(top), "r"(0xC180C180u));
+        asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(rest) : "r"(v2[j]), "r"(0x41804180u), "r"(minus));
+        hi[j] = cvt2_e4m3(Half<false>::lo_f32(top), Half<false>::hi_f32(top));
+        lo[j] = cvt2_e4m3(Half<false>::lo_f32(rest), Half<false>::hi_f32(rest));
+    }
+    out[0] = make_uint4(hi[0] | (hi[1] << 16), hi[2] | (hi[3] << 16), hi[4] | (hi[5] << 16), hi[6] | (hi[7] << 16));
+    out[1] = make_uint4(lo[0] | (lo[1] << 16), lo[2] | (lo[3] << 16), lo[4] | (lo[5] << 16), lo[6] | (lo[7] << 16));
+    return true;
+}
+
+// Eight values of either 16-bit type to P planes, given their block's largest
+// finite magnitude.
+template <int T, int P>
+QMM_DEVINL void mt_planes8(const uint4& raw, uint32_t block_max, uint2 (&out)[P], uint32_t (&bytes)[P]) {
+    using H = Half<T == MX_F16>;
+    float v[8] = {H::lo_f32(raw.x), H::hi_f32(raw.x), H::lo_f32(raw.y), H::hi_f32(raw.y),
+                  H::lo_f32(raw.z), H::hi_f32(raw.z), H::lo_f32(raw.w), H::hi_f32(raw.w)};
+    float inv;
+    // 128 <= largest < 256 on the grid: rounding cannot reach 448
+    uint32_t byte = mx_scale_byte<7>(block_max, inv);
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+        v[j] = abs_bits(v[j]) < 0x7F800000u ? v[j] * inv : __uint_as_float(0x7FC00000u);  // an infinity has no code
+#pragma unroll
+    for (int q = 0; q < P; ++q) {
+        // what this plane's code holds: the first four significant bits, or
+        // whole units of 2^-9 below the smallest normal code
+        float code[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const float four = __uint_as_float(__float_as_uint(v[j]) & 0xFFF00000u);
+            const float unit = __fsub_rn(__fadd_rn(v[j], 24576.0f), 24576.0f);
+            code[j] = q + 1 == P ? v[j] : fabsf(v[j]) < 0x1p-6f ? unit : four;
+        }
+        uint32_t h[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) h[j] = cvt2_e4m3(code[2 * j], code[2 * j + 1]);
+        out[q] = make_uint2(h[0] | (h[1] << 16), h[2] | (h[3] << 16));
+        bytes[q] = byte;
+        const uint32_t next = byte > 4 ? byte - 4 : 0;  // the remainder, up to 16 times larger
+        const float up = __uint_as_float((127u + byte - next) << 23);
+        byte = next;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = (v[j] - code[j]) * up;
+    }
+}
+// Largest finite magnitude of eight values, as fp32 bits.
+template <bool F16>
+QMM_DEVINL uint32_t mt_max_finite(const uint4& raw) {
+    const uint32_t u[4] = {raw.x, raw.y, raw.z, raw.w};
+    constexpr uint32_t INF = F16 ? 0x7C00u : 0x7F80u;
+    uint32_t m = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const uint32_t a = u[j] & 0x7FFFu, b = (u[j] >> 16) & 0x7FFFu;
+        m = max(m, max(a < INF ? a : 0u, b < INF ? b : 0u));
+    }
+    return max_abs_f32<F16>(m);
+}
+
 // Activations to P e4m3 planes [P][R][K] with scales [P][R][K/32], rows taken
-// through src; four lanes hold a block.  P = 1 copies mxfp8 rows.  Also clears
+// through src; two lanes hold a block.  P = 1 copies mxfp8 rows.  Also clears
 // the counters of the product that follows.
 template <int T, int P>
-__global__ void __launch_bounds__(256) mx_planes_kernel(const void* x, const uint8_t* xs, uint8_t* planes,
+__global__ void __launch_bounds__(128) mx_planes_kernel(const void* x, const uint8_t* xs, uint8_t* planes,
                                                         uint8_t* scales, const uint32_t* src, int x_rows, int R, int K,
                                                         uint32_t* counters, int n_counters) {
     pdl_launch_dependents();
@@ -467,10 +551,11 @@ __global__ void __launch_bounds__(256) mx_planes_kernel(const void* x, const uin
     for (long long i = (long long)tid * blockDim.x + threadIdx.x; i < n_counters;
          i += (long long)gridDim.x * gridDim.y * blockDim.x)
         counters[i] = 0;
-    const int g = K / 8, c = blockIdx.x * blockDim.x + threadIdx.x;
+    // sixteen values (half a block) of RUN rows to a thread, their loads together
+    constexpr int RUN = 4;
+    const int g = K / 16, c = blockIdx.x * blockDim.x + threadIdx.x;
     const bool in = c < g;  // whole blocks of 32 are in or out
     const long long plane = (long long)R * g;
-    constexpr int RUN = 4;  // rows whose loads are in flight together
     for (int r0 = blockIdx.y * RUN; r0 < R; r0 += gridDim.y * RUN) {
         long long from[RUN];
 #pragma unroll
@@ -482,69 +567,51 @@ __global__ void __launch_bounds__(256) mx_planes_kernel(const void* x, const uin
                 from[k] = from[k] < x_rows ? from[k] : x_rows - 1;
             }
         }
-        if constexpr (P == 1) {
-            if (!in) continue;
-            uint2 w[RUN];
-            uint8_t e[RUN];
+        constexpr int NV = P == 1 ? 1 : 2;
+        uint4 raw[RUN][2];
+        uint32_t e[RUN];
 #pragma unroll
-            for (int k = 0; k < RUN; ++k) {
-                w[k] = ld_dep(reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(x) + from[k] * K) + c);
-                e[k] = (c & 3) == 0 ? ld_dep(xs + from[k] * (K / 32) + (c >> 2)) : 0;
-            }
+        for (int k = 0; k < RUN; ++k) {
 #pragma unroll
-            for (int k = 0; k < RUN; ++k) {
-                if (r0 + k >= R) break;
-                const long long i = (long long)(r0 + k) * g + c;
-                reinterpret_cast<uint2*>(planes)[i] = w[k];
-                if ((c & 3) == 0) scales[i >> 2] = e[k];
-            }
-            continue;
+            for (int d = 0; d < NV; ++d)
+                raw[k][d] = in ? ld_v4(static_cast<const uint4*>(x) + (from[k] * g + c) * NV + d) : make_uint4(0, 0, 0, 0);
+            if constexpr (P == 1) e[k] = in && (c & 1) == 0 ? ld_dep(xs + from[k] * (K / 32) + (c >> 1)) : 0;
         }
-        uint4 raw[RUN];
-#pragma unroll
-        for (int k = 0; k < RUN; ++k)
-            raw[k] = in ? ld_v4(static_cast<const uint16_t*>(x) + from[k] * K + c * 8) : make_uint4(0, 0, 0, 0);
 #pragma unroll
         for (int k = 0; k < RUN; ++k) {
             const long long i = (long long)(r0 + k) * g + c;
             const bool live = in && r0 + k < R;
-            using H = Half<T == MX_F16>;
-            float v[8] = {H::lo_f32(raw[k].x), H::hi_f32(raw[k].x), H::lo_f32(raw[k].y), H::hi_f32(raw[k].y),
-                          H::lo_f32(raw[k].z), H::hi_f32(raw[k].z), H::lo_f32(raw[k].w), H::hi_f32(raw[k].w)};
-            uint32_t m = 0;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const uint32_t a = abs_bits(v[j]);
-                if (a < 0x7F800000u) m = max(m, a);
-                else v[j] = __uint_as_float(0x7FC00000u);  // an infinity has no code: NaN
-            }
-            m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
-            m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
-            float inv;
-            // 128 <= largest < 256 on the grid: rounding cannot reach 448
-            uint32_t byte = mx_scale_byte<7>(m, inv);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] *= inv;
-#pragma unroll
-            for (int q = 0; q < P; ++q) {
-                uint32_t h[4];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) h[j] = cvt2_e4m3(v[2 * j], v[2 * j + 1]);
-                if (live) {
-                    const long long o = q * plane + i;
-                    reinterpret_cast<uint2*>(planes)[o] = make_uint2(h[0] | (h[1] << 16), h[2] | (h[3] << 16));
-                    if ((c & 3) == 0) scales[o >> 2] = (uint8_t)byte;
-                }
-                if (q + 1 < P) {
-                    const uint32_t next = byte > 4 ? byte - 4 : 0;  // the remainder, up to 16 times larger
-                    const float up = __uint_as_float((127u + byte - next) << 23);
-                    byte = next;
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const uint32_t f = e4m3x2_f16x2(h[j]);
-                        v[2 * j] = (v[2 * j] - Half<true>::lo_f32(f)) * up;
-                        v[2 * j + 1] = (v[2 * j + 1] - Half<true>::hi_f32(f)) * up;
+            uint4* out = reinterpret_cast<uint4*>(planes) + i;
+            if constexpr (P == 1) {
+                if (!live) continue;
+                out[0] = raw[k][0];
+                if ((c & 1) == 0) scales[i >> 1] = (uint8_t)e[k];
+            } else {
+                if constexpr (T == MX_BF16) {
+                    uint4 two[2];
+                    uint32_t byte;
+                    if (mt_planes_bf16(raw[k], live, two, byte)) {
+                        if (!live) continue;
+                        out[0] = two[0];
+                        out[plane] = two[1];
+                        if ((c & 1) == 0) {
+                            scales[i >> 1] = (uint8_t)byte;
+                            scales[(plane + i) >> 1] = (uint8_t)(byte - 4);
+                        }
+                        continue;
                     }
+                }
+                uint32_t m = max(mt_max_finite<T == MX_F16>(raw[k][0]), mt_max_finite<T == MX_F16>(raw[k][1]));
+                m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
+                uint2 lo[P], hi[P];
+                uint32_t bytes[P];
+                mt_planes8<T, P>(raw[k][0], m, lo, bytes);
+                mt_planes8<T, P>(raw[k][1], m, hi, bytes);
+                if (!live) continue;
+#pragma unroll
+                for (int q = 0; q < P; ++q) {
+                    out[q * plane] = make_uint4(lo[q].x, lo[q].y, hi[q].x, hi[q].y);
+                    if ((c & 1) == 0) scales[(q * plane + i) >> 1] = (uint8_t)bytes[q];
                 }
             }
         }
@@ -669,11 +736,11 @@ int launch_mx_tc(const MxMatmul& a, const int4* items, const int32_t* n_items, c
     const size_t n_counters = p.c.split ? (size_t)tiles * 8 : 0;
     int rc = QMM_OK;
     if (!in_place) {
-        const int g = (int)(a.K / 8);
+        const int g = (int)(a.K / 16);
         const long long runs = (a.rows + 3) / 4;
-        const dim3 grid((unsigned)((g + 255) / 256), (unsigned)(runs < 32768 ? runs : 32768));
+        const dim3 grid((unsigned)((g + 127) / 128), (unsigned)(runs < 32768 ? runs : 32768));
 #define QMM_PLANES(T, PP)                                                                                         \
-    qmm::mx_planes_kernel<T, PP><<<grid, 256, 0, a.st>>>(a.x, a.xs, planes, scales, a.src, (int)a.x_rows,          \
+    qmm::mx_planes_kernel<T, PP><<<grid, 128, 0, a.st>>>(a.x, a.xs, planes, scales, a.src, (int)a.x_rows,          \
                                                          (int)a.rows, (int)a.K, p.c.counters, (int)n_counters)
         if (mx) QMM_PLANES(qmm::MX_BF16, 1);
         else if (a.f16) QMM_PLANES(qmm::MX_F16, 3);
