@@ -134,49 +134,61 @@ class QuantConfig:
             return self.group_size, self.bits
         return int(o.get("group_size", self.group_size)), int(o.get("bits", self.bits))
 
+    def mode_for_layer(self, prefix: str) -> str:
+        return self.overrides.get(prefix, {}).get("mode", self.mode)
+
 
 def quantized_prefixes(tensors: dict[str, torch.Tensor]) -> list[str]:
-    """Prefixes that carry a (weight, scales, biases) triple."""
+    """Prefixes that carry a (weight, scales, biases) triple, or (mxfp4) weight and scales."""
     return sorted(n[: -len(".scales")] for n in tensors
                   if n.endswith(".scales") and n[: -len(".scales")] + ".weight" in tensors)
 
 
-def _check(prefix: str, w: torch.Tensor, s: torch.Tensor, b: torch.Tensor, group_size: int, bits: int) -> int:
+def _check(prefix: str, w: torch.Tensor, s: torch.Tensor, b: torch.Tensor | None, group_size: int, bits: int,
+           mode: str) -> int:
     K = w.shape[-1] * 32 // bits
-    if w.shape[-1] * 32 != K * bits or K % group_size or s.shape[-1] != K // group_size or b.shape != s.shape:
+    if (b is None) != (mode != "affine"):
+        raise ValueError(f"{prefix}: mode {mode!r} {'needs' if b is None else 'has no'} biases")
+    if w.shape[-1] * 32 != K * bits or K % group_size or s.shape[-1] != K // group_size or (
+            b is not None and b.shape != s.shape):
         raise ValueError(f"{prefix}: weight {tuple(w.shape)} / scales {tuple(s.shape)} do not match "
                          f"bits={bits} group_size={group_size}")
     return K
 
 
 def load_quantized_linear(tensors: dict[str, torch.Tensor], prefix: str, group_size: int = 64, bits: int = 4,
-                          device=None) -> QuantizedLinear:
-    """A QuantizedLinear from `<prefix>.weight/.scales/.biases` (+ `.bias` if present)."""
-    w, s, b = tensors[f"{prefix}.weight"], tensors[f"{prefix}.scales"], tensors[f"{prefix}.biases"]
-    K = _check(prefix, w, s, b, group_size, bits)
+                          device=None, mode: str = "affine", dtype=torch.bfloat16) -> QuantizedLinear:
+    """A QuantizedLinear from `<prefix>.weight/.scales/.biases` (+ `.bias` if present).
+
+    `dtype` is the activations' of an mxfp4 layer; an affine one's is its scales'."""
+    w, s, b = tensors[f"{prefix}.weight"], tensors[f"{prefix}.scales"], tensors.get(f"{prefix}.biases")
+    K = _check(prefix, w, s, b, group_size, bits, mode)
     dev = device if device is not None else w.device
     bias = tensors.get(f"{prefix}.bias")
-    layer = QuantizedLinear(K, w.shape[0], bias is not None, group_size, bits, dtype=s.dtype, device=dev)
+    layer = QuantizedLinear(K, w.shape[0], bias is not None, group_size, bits, mode,
+                            dtype=s.dtype if mode == "affine" else dtype, device=dev)
     layer.weight.copy_(w.view(torch.int32))
     layer.scales.copy_(s)
-    layer.biases.copy_(b)
+    if b is not None:
+        layer.biases.copy_(b)
     if bias is not None:
         layer.bias.data.copy_(bias)
     return layer
 
 
 def load_switch_linear(tensors: dict[str, torch.Tensor], prefix: str, group_size: int = 64, bits: int = 4,
-                       device=None) -> QuantizedSwitchLinear:
-    """A QuantizedSwitchLinear (expert bank, leading E axis) from its three tensors."""
-    w, s, b = tensors[f"{prefix}.weight"], tensors[f"{prefix}.scales"], tensors[f"{prefix}.biases"]
-    K = _check(prefix, w, s, b, group_size, bits)
+                       device=None, mode: str = "affine", dtype=torch.bfloat16) -> QuantizedSwitchLinear:
+    """A QuantizedSwitchLinear (expert bank, leading E axis) from its tensors."""
+    w, s, b = tensors[f"{prefix}.weight"], tensors[f"{prefix}.scales"], tensors.get(f"{prefix}.biases")
+    K = _check(prefix, w, s, b, group_size, bits, mode)
     dev = device if device is not None else w.device
     bias = tensors.get(f"{prefix}.bias")
-    layer = QuantizedSwitchLinear(K, w.shape[1], w.shape[0], bias is not None, group_size, bits, dtype=s.dtype,
-                                  device=dev)
+    layer = QuantizedSwitchLinear(K, w.shape[1], w.shape[0], bias is not None, group_size, bits, mode,
+                                  dtype=s.dtype if mode == "affine" else dtype, device=dev)
     layer.weight.copy_(w.view(torch.int32))
     layer.scales.copy_(s)
-    layer.biases.copy_(b)
+    if b is not None:
+        layer.biases.copy_(b)
     if bias is not None:
         layer.bias.data.copy_(bias)
     return layer
@@ -197,7 +209,7 @@ def load_model_dir(model_dir: str, device=None) -> tuple[dict[str, torch.nn.Modu
         for prefix in quantized_prefixes(t):
             gs, bits = qc.for_layer(prefix)
             load = load_switch_linear if t[f"{prefix}.weight"].dim() == 3 else load_quantized_linear
-            layers[prefix] = load(t, prefix, gs, bits, device=device)
+            layers[prefix] = load(t, prefix, gs, bits, device=device, mode=qc.mode_for_layer(prefix))
     return layers, qc
 
 

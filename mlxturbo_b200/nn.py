@@ -1,7 +1,11 @@
 """torch modules over the quantized ops: the layer types the reference's
 callers hold (mlx.nn.QuantizedLinear and mlx-lm's QuantizedSwitchLinear /
 SwitchGLU), with MLX's parameter names (weight, scales, biases, bias) and
-call semantics, so model code ported from MLX keeps its shape contracts."""
+call semantics, so model code ported from MLX keeps its shape contracts.
+
+mode="mxfp4" (group_size=32, bits=4) gives them microscaled weights: uint8
+scales, no biases (``biases`` is None); ``dtype`` is then that of activations
+and outputs."""
 
 from __future__ import annotations
 
@@ -9,6 +13,20 @@ import torch
 from torch import nn
 
 from . import ops
+
+
+def _quantized_buffers(module: nn.Module, lead: tuple, input_dims: int, dtype, device) -> None:
+    """weight, scales and (affine) biases of shape lead + (..,)."""
+    bits, group_size = module.bits, module.group_size
+    if module.mode != "affine" and (module.mode, group_size, bits) != ("mxfp4", 32, 4):
+        raise NotImplementedError(f"mode={module.mode!r} with group_size={group_size} bits={bits}: layers have affine "
+                                  "weights, or mxfp4 ones with group_size=32 and bits=4")
+    affine = module.mode == "affine"
+    module.dtype = dtype
+    module.register_buffer("weight", torch.zeros((*lead, input_dims * bits // 32), dtype=torch.int32, device=device))
+    module.register_buffer("scales", torch.zeros((*lead, input_dims // group_size),
+                                                 dtype=dtype if affine else torch.uint8, device=device))
+    module.register_buffer("biases", torch.zeros_like(module.scales) if affine else None)
 
 
 class QuantizedLinear(nn.Module):
@@ -19,23 +37,20 @@ class QuantizedLinear(nn.Module):
         super().__init__()
         self.group_size, self.bits, self.mode = group_size, bits, mode
         self.input_dims, self.output_dims = input_dims, output_dims
-        self.register_buffer("weight", torch.zeros((output_dims, input_dims * bits // 32), dtype=torch.int32,
-                                                   device=device))
-        self.register_buffer("scales", torch.zeros((output_dims, input_dims // group_size), dtype=dtype,
-                                                   device=device))
-        self.register_buffer("biases", torch.zeros_like(self.scales))
+        _quantized_buffers(self, (output_dims,), input_dims, dtype, device)
         self.bias = nn.Parameter(torch.zeros(output_dims, dtype=dtype, device=device)) if bias else None
 
     @classmethod
     def from_float(cls, w: torch.Tensor, bias: torch.Tensor | None = None, group_size: int = 64, bits: int = 4,
-                   dtype=torch.bfloat16):
-        """Quantise a float weight [N, K] (mx.quantize, affine) into a new layer."""
+                   dtype=torch.bfloat16, mode: str = "affine"):
+        """Quantise a float weight [N, K] (mx.quantize) into a new layer."""
         N, K = w.shape
-        layer = cls(K, N, bias is not None, group_size, bits, dtype=dtype, device=w.device)
-        wq, s, b = ops.quantize(w, group_size, bits, dtype=dtype)
+        layer = cls(K, N, bias is not None, group_size, bits, mode, dtype=dtype, device=w.device)
+        wq, s, *b = ops.quantize(w, group_size, bits, mode, **({"dtype": dtype} if mode == "affine" else {}))
         layer.weight.copy_(wq)
         layer.scales.copy_(s)
-        layer.biases.copy_(b)
+        if b:
+            layer.biases.copy_(b[0])
         if bias is not None:
             layer.bias.data.copy_(bias.to(dtype))
         return layer
@@ -45,6 +60,26 @@ class QuantizedLinear(nn.Module):
                                  bits=self.bits, mode=self.mode)
         return y if self.bias is None else y + self.bias
 
+    def forward_mx(self, xq, x_scales):
+        """The same of mxfp8 activations (``ops.rms_norm_quantize``, ``ops.quantize``); mode="mxfp4"."""
+        if self.mode != "mxfp4":
+            raise NotImplementedError(f"mode={self.mode!r}: mxfp8 activations go with mxfp4 weights")
+        y = ops.mx_matmul(xq, x_scales, self.weight, self.scales, dtype=self.dtype)
+        return y if self.bias is None else y + self.bias
+
+
+class RMSNormQuantized(nn.Module):
+    """Residual addition and root-mean-square norm with an mxfp8 result (``ops.rms_norm_quantize``)."""
+
+    def __init__(self, dims: int, eps: float = 1e-6, dtype=torch.bfloat16, device=None):
+        super().__init__()
+        self.eps = eps
+        self.weight = nn.Parameter(torch.ones(dims, dtype=dtype, device=device), requires_grad=False)
+
+    def forward(self, x, residual=None):
+        """(xq, x_scales, h): mxfp8 of the normalised x + residual, and that sum (None without a residual)."""
+        return ops.rms_norm_quantize(x, self.weight, self.eps, residual=residual)
+
 
 class QuantizedSwitchLinear(nn.Module):
     """Expert bank: weight [E, N, K*bits/32]; forward(x, indices, sorted_indices)."""
@@ -53,11 +88,7 @@ class QuantizedSwitchLinear(nn.Module):
                  group_size: int = 64, bits: int = 4, mode: str = "affine", dtype=torch.bfloat16, device=None):
         super().__init__()
         self.group_size, self.bits, self.mode = group_size, bits, mode
-        self.register_buffer("weight", torch.zeros((num_experts, output_dims, input_dims * bits // 32),
-                                                   dtype=torch.int32, device=device))
-        self.register_buffer("scales", torch.zeros((num_experts, output_dims, input_dims // group_size),
-                                                   dtype=dtype, device=device))
-        self.register_buffer("biases", torch.zeros_like(self.scales))
+        _quantized_buffers(self, (num_experts, output_dims), input_dims, dtype, device)
         self.bias = nn.Parameter(torch.zeros(num_experts, output_dims, dtype=dtype, device=device)) if bias else None
 
     @property
@@ -68,10 +99,11 @@ class QuantizedSwitchLinear(nn.Module):
         """A new layer holding experts [start, stop) of this one (expert parallelism)."""
         E, N, kw = self.weight.shape
         out = QuantizedSwitchLinear(kw * 32 // self.bits, N, stop - start, self.bias is not None, self.group_size,
-                                    self.bits, self.mode, dtype=self.scales.dtype, device=self.weight.device)
+                                    self.bits, self.mode, dtype=self.dtype, device=self.weight.device)
         out.weight.copy_(self.weight[start:stop])
         out.scales.copy_(self.scales[start:stop])
-        out.biases.copy_(self.biases[start:stop])
+        if self.biases is not None:
+            out.biases.copy_(self.biases[start:stop])
         if self.bias is not None:
             out.bias.data.copy_(self.bias[start:stop])
         return out
@@ -95,13 +127,13 @@ class SwitchGLU(nn.Module):
     """mlx-lm SwitchGLU over quantized experts (gate/up/down projections)."""
 
     def __init__(self, input_dims: int, hidden_dims: int, num_experts: int, group_size: int = 64, bits: int = 4,
-                 dtype=torch.bfloat16, device=None):
+                 dtype=torch.bfloat16, device=None, mode: str = "affine"):
         super().__init__()
-        self.gate_proj = QuantizedSwitchLinear(input_dims, hidden_dims, num_experts, False, group_size, bits,
+        self.gate_proj = QuantizedSwitchLinear(input_dims, hidden_dims, num_experts, False, group_size, bits, mode,
                                                dtype=dtype, device=device)
-        self.up_proj = QuantizedSwitchLinear(input_dims, hidden_dims, num_experts, False, group_size, bits,
+        self.up_proj = QuantizedSwitchLinear(input_dims, hidden_dims, num_experts, False, group_size, bits, mode,
                                              dtype=dtype, device=device)
-        self.down_proj = QuantizedSwitchLinear(hidden_dims, input_dims, num_experts, False, group_size, bits,
+        self.down_proj = QuantizedSwitchLinear(hidden_dims, input_dims, num_experts, False, group_size, bits, mode,
                                                dtype=dtype, device=device)
         self.activation = swiglu
         self._fused = None
@@ -113,6 +145,8 @@ class SwitchGLU(nn.Module):
         call ``refresh_fused()`` after changing the weights in place."""
         if self._fused is None:
             g, u = self.gate_proj, self.up_proj
+            if g.mode != "affine" or u.mode != "affine":
+                raise NotImplementedError("fused gate/up takes affine banks")
             E, I = g.weight.shape[0], g.weight.shape[1]
             if I % 8 or u.weight.shape != g.weight.shape or g.group_size != u.group_size or g.bits != u.bits:
                 raise NotImplementedError("fused gate/up needs matching banks with intermediate size % 8 == 0")
