@@ -302,7 +302,7 @@ __global__ void __launch_bounds__(C::THREADS, 1)
             mbar_init(acc_empty(b), 4);
         }
         for (int q = 0; q < 4; ++q) {
-            mbar_init(join_full(q), S > 1 ? S - 1 : 1);
+            mbar_init(join_full(q), 1);
             mbar_init(join_empty(q), 1);
         }
         mbar_init(started, 1);
@@ -316,8 +316,9 @@ __global__ void __launch_bounds__(C::THREADS, 1)
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
-    // Barriers and tensor memory are ready after this; each role comes here
-    // once its first loads are on the way.
+    // Barriers and tensor memory are ready after this; each role comes here once
+    // its first lines are asked for (a load would hold the barrier up until its
+    // data came).
     uint32_t tmem = 0;
     auto ready = [&]() {
         tc_fence_before();
@@ -479,10 +480,14 @@ __global__ void __launch_bounds__(C::THREADS, 1)
             }
         };
         uint4 v[AHEAD][NL];
-        if (tiles.more()) rows_of();
+        if (tiles.more()) {
+            rows_of();
+#pragma unroll
+            for (int q = 0; q < NL; ++q) mt_prefetch(src[q] + 16 * grp);
+        }
+        ready();
 #pragma unroll
         for (int a = 0; a < AHEAD; ++a) load(v[a]);
-        ready();
         const int total = (int)(walk.end - walk.tile) * (g1 - g0 + 1);
         for (int base = 0; base < total && !*abort; base += AHEAD) {
 #pragma unroll
@@ -517,9 +522,11 @@ __global__ void __launch_bounds__(C::THREADS, 1)
                 if ((uint32_t)ld_dep(p.ids + r) >= (uint32_t)p.E)
                     for (int n = lane; n < p.c.N; n += 32) p.c.y[(long long)r * p.c.N + n] = 0;
         if (S > 1) mt_cluster_wait();
-        const uint32_t j_row = sbase + C::J_OFF + row * 4;
-        const uint32_t to = S > 1 && rank ? mt_remote(j_row + (rank - 1) * (C::BT * MT_ROWS * 4), 0) : 0;
+        // a block's sums: [rows / PER][128 weight rows][PER]
         constexpr int PER = C::BT < 4 ? C::BT : 4;  // rows of a TMEM load
+        const uint32_t j_row = sbase + C::J_OFF + row * (PER * 4);
+        const uint32_t to = S > 1 && rank ? mt_remote(j_row + (rank - 1) * (C::BT * MT_ROWS * 4), 0) : 0;
+        const uint32_t to_full = S > 1 && rank ? mt_remote(join_full(quarter), 0) : 0;
         int seg = 0;
         for (F4Tiles tiles(p, walk, C::BT); tiles.more() && !*abort; tiles.next(p, C::BT)) {
             const MxTile& t = tiles.t;
@@ -527,9 +534,11 @@ __global__ void __launch_bounds__(C::THREADS, 1)
             if (p.c.dst && lane < t.rows) out_l = (int)ld_dep(p.c.dst + t.row0 + lane);
             const int b = seg % C::ACCS;
             const uint32_t j_ph = (uint32_t)seg & 1u;
+            if (S > 1 && rank == 0 && lane == 0)  // the other blocks' sums of these 32 weight rows
+                mbar_expect_tx(join_full(quarter), (S - 1) * (uint32_t)((t.rows + PER - 1) / PER * PER) * 128);
             if (!mt_wait(acc_full(b), (uint32_t)(seg / C::ACCS) & 1u, abort, 32)) break;
             if (S > 1) {
-                if (rank ? !mt_wait<true>(join_empty(quarter), j_ph ^ 1u, abort, 128)
+                if (rank ? !mt_wait(join_empty(quarter), j_ph ^ 1u, abort, 128)
                          : !mt_wait<true>(join_full(quarter), j_ph, abort, 256))
                     break;
             }
@@ -542,36 +551,45 @@ __global__ void __launch_bounds__(C::THREADS, 1)
                 if constexpr (PER == 4) tmem_ld32(t_lane + b * C::NB + j0 * F4_PLANES, u);
                 else tmem_ld16(t_lane + b * C::NB + j0 * F4_PLANES, u);
                 tmem_wait_ld();
+                float f[PER];
 #pragma unroll
                 for (int d = 0; d < PER; ++d) {
-                    const int j = j0 + d;
-                    const long long out = __shfl_sync(0xffffffffu, out_l, j & 31);
-                    if (j >= t.rows) continue;
-                    float f = __uint_as_float(u[8 * d + 7]);  // small to large
+                    f[d] = __uint_as_float(u[8 * d + 7]);  // small to large
 #pragma unroll
-                    for (int q = 6; q >= 0; --q) f += __uint_as_float(u[8 * d + q]);
-                    if (rank != 0) {
-                        mt_remote_store(to + j * (MT_ROWS * 4), f);
-                        continue;
-                    }
-                    for (uint32_t o = 0; o + 1 < S; ++o) {
-                        float part;
-                        asm volatile("ld.shared.f32 %0, [%1];"
-                                     : "=f"(part)
-                                     : "r"(j_row + (o * C::BT + j) * (MT_ROWS * 4))
+                    for (int q = 6; q >= 0; --q) f[d] += __uint_as_float(u[8 * d + q]);
+                }
+                if (rank != 0) {
+                    mt_remote_store(to + j0 * (MT_ROWS * 4), f, to_full);
+                    continue;
+                }
+                for (uint32_t o = 0; o + 1 < S; ++o) {
+                    const uint32_t from = j_row + (o * C::BT + j0) * (MT_ROWS * 4);
+                    float part[4] = {};
+                    if constexpr (PER == 4)
+                        asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
+                                     : "=f"(part[0]), "=f"(part[1]), "=f"(part[2]), "=f"(part[3])
+                                     : "r"(from)
                                      : "memory");
-                        f += part;
-                    }
-                    if (n < p.c.N) p.c.y[out * p.c.N + n] = H::from_f32(f);
+                    else
+                        asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];"
+                                     : "=f"(part[0]), "=f"(part[1])
+                                     : "r"(from)
+                                     : "memory");
+#pragma unroll
+                    for (int d = 0; d < PER; ++d) f[d] += part[d];
+                }
+#pragma unroll
+                for (int d = 0; d < PER; ++d) {
+                    const long long out = __shfl_sync(0xffffffffu, out_l, (j0 + d) & 31);
+                    if (j0 + d < t.rows && n < p.c.N) p.c.y[out * p.c.N + n] = H::from_f32(f[d]);
                 }
             }
             tc_fence_before();
             __syncwarp();
             if (lane == 0) {
                 mbar_arrive(acc_empty(b));
-                if (rank != 0) mt_remote_arrive(mt_remote(join_full(quarter), 0));
-                else
-                    for (uint32_t o = 1; o < S; ++o) mt_remote_arrive(mt_remote(join_empty(quarter), o));
+                if (rank == 0 && tiles.tile + 1 < tiles.end)
+                    for (uint32_t o = 1; o < S; ++o) mt_pair_arrive(mt_remote(join_empty(quarter), o));
             }
         }
     } else if constexpr (C::OWN) {
@@ -660,16 +678,15 @@ __global__ void __launch_bounds__(C::THREADS, 1)
                 enter();
             }
         };
-        auto begin = [&]() {
-            enter();
-#pragma unroll
-            for (int a = 0; a < AHEAD; ++a) load(st[a]);
-        };
-        if (tiles.more()) row_of();
-        const bool at_once = part < par;  // a warp without a row in the first tile looks for one later
-        if (at_once) begin();
+        if (tiles.more()) {
+            row_of();
+            const int k = min((k0 + part) * F4_BK + lane * 8, p.c.K - 8);
+            if (xrow) mt_prefetch(xrow + (C::X == F4_MX8 ? k : 2 * k));
+        }
         ready();
-        if (!at_once) begin();
+        enter();
+#pragma unroll
+        for (int a = 0; a < AHEAD; ++a) load(st[a]);
         int seen = -1;  // last k-block whose slot this warp waited for
 #pragma unroll 1
         while (st[0].i >= 0 && !*abort) {

@@ -58,25 +58,38 @@ QMM_DEVINL uint32_t mt_cluster_rank() {
     asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
     return r;
 }
-// The address of another block's shared memory, an arrival there, a store.
+// The address of another block's shared memory.
 QMM_DEVINL uint32_t mt_remote(uint32_t addr, uint32_t rank) {
     uint32_t r;
     asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
     return r;
 }
-QMM_DEVINL void mt_remote_arrive(uint32_t bar) {
-    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
-}
-// The same without ordering other blocks' memory: what it announces is in this
-// block's own shared memory, behind a proxy fence.  (The cluster-wide release
-// costs about a microsecond.)
+// An arrival there.  It orders this block's own memory only: what it announces
+// is in its own shared memory behind a proxy fence, or is that it has read
+// something.  (A cluster-wide release waits for every earlier store and costs
+// about a microsecond.)
 QMM_DEVINL void mt_pair_arrive(uint32_t bar) {
     asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
-QMM_DEVINL void mt_remote_store(uint32_t addr, float f) {
-    asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(f) : "memory");
+// N floats stored there, counted on a barrier of the same block.
+template <int N>
+QMM_DEVINL void mt_remote_store(uint32_t addr, const float (&f)[N], uint32_t bar) {
+    static_assert(N == 2 || N == 4, "one transaction");
+    if constexpr (N == 4)
+        asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v4.b32 [%0], {%1, %2, %3, %4}, [%5];" ::"r"(
+                         addr),
+                     "r"(__float_as_uint(f[0])), "r"(__float_as_uint(f[1])), "r"(__float_as_uint(f[2])),
+                     "r"(__float_as_uint(f[3])), "r"(bar)
+                     : "memory");
+    else
+        asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v2.b32 [%0], {%1, %2}, [%3];" ::"r"(
+                         addr),
+                     "r"(__float_as_uint(f[0])), "r"(__float_as_uint(f[1])), "r"(bar)
+                     : "memory");
 }
-QMM_DEVINL void mt_cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+// All threads of the cluster; no memory is ordered by it (barriers are made
+// visible by mbar_fence_init, everything else by mbarriers).
+QMM_DEVINL void mt_cluster_arrive() { asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory"); }
 QMM_DEVINL void mt_cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 
 // Scale bytes for one operand block of up to 128 rows x 4 blocks of 32 (512
@@ -174,6 +187,8 @@ QMM_DEVINL MxTile mt_tile(const MxTcParams& p, uint32_t tile, int bt, int weight
     }
     return t;
 }
+
+QMM_DEVINL void mt_prefetch(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
 
 // 16 scale bytes of a row from `at`, bytes at or past `n` zero.
 QMM_DEVINL uint4 mt_scale_bytes(const uint8_t* row, int at, int n, int vec) {
