@@ -208,8 +208,8 @@ int launch_mx_tc(const MxMatmul& a, const int4* items, const int32_t* n_items, c
 // it is not for this size.  items == nullptr in a grouped call (`ids` given):
 // every row is an item of its own.
 bool mx_f4_direct(long long rows, long long E, bool grouped);
-bool mx_f4_takes(long long rows, long long E, long long N, long long K);
-int mx_f4_item_rows(long long rows, long long E, bool grouped);
+bool mx_f4_takes(long long rows, long long E, long long N, long long K, bool grouped);
+int mx_f4_item_rows(long long rows, long long E, long long N, long long K, bool grouped);
 size_t mx_f4_workspace(long long rows, long long K, int bt);
 int launch_mx_f4(const MxMatmul& a, const int4* items, const int32_t* n_items, const int32_t* ids, int bt, void* ws);
 // Items (expert, first sorted row, rows) of at most ir rows from ascending ids,

@@ -187,7 +187,7 @@ int qmm_mx_rms_norm(const void* x, const void* residual, const void* weight, voi
 
 size_t qmm_mx_matmul_workspace_size(int64_t M, int64_t N, int64_t K, int dtype, int x_is_mx) {
     if (M <= 0 || N <= 0 || K <= 0 || K % 32) return 0;
-    if (mx_f4_takes(M, 1, N, K)) return mx_f4_workspace(M, K, mx_f4_item_rows(M, 1, false));
+    if (mx_f4_takes(M, 1, N, K, false)) return mx_f4_workspace(M, K, mx_f4_item_rows(M, 1, N, K, false));
     if (K % 128) return 0;
     return mx_tc_workspace(M, 1, N, K, x_is_mx, dtype == QMM_F16, false);
 }
@@ -219,8 +219,8 @@ int qmm_mx_matmul(const void* x, const uint8_t* x_scales, const uint32_t* w, con
     a.f16 = dtype == QMM_F16;
     a.st = static_cast<cudaStream_t>(stream);
     fire("mx_matmul");
-    if (mx_f4_takes(M, 1, N, K))
-        return launch_mx_f4(a, nullptr, nullptr, nullptr, mx_f4_item_rows(M, 1, false), workspace);
+    if (mx_f4_takes(M, 1, N, K, false))
+        return launch_mx_f4(a, nullptr, nullptr, nullptr, mx_f4_item_rows(M, 1, N, K, false), workspace);
     if (mx_tc_takes(x_scales, scales, M, 1, N, K))
         return launch_mx_tc(a, nullptr, nullptr, nullptr, workspace);
     return launch_mx_warp(a, nullptr, nullptr, 0, mx_warp_item_rows(M, 1));
@@ -237,8 +237,8 @@ size_t qmm_mx_gather_workspace_size(int64_t rows, int64_t E, int64_t N, int64_t 
         const size_t n = gather_tables(nullptr, rows, E, sorted, item_rows).bytes + more;
         need = n > need ? n : need;
     };
-    if (mx_f4_takes(rows, E, N, K)) {
-        const int bt = mx_f4_item_rows(rows, E, true);
+    if (mx_f4_takes(rows, E, N, K, true)) {
+        const int bt = mx_f4_item_rows(rows, E, N, K, true);
         also(bt, mx_f4_workspace(rows, K, bt));
     } else if (K % 128 == 0)
         also(mx_tc_item_rows(), mx_tc_workspace(rows, E, N, K, x_is_mx, f16, true));
@@ -271,7 +271,7 @@ int qmm_mx_gather(const void* x, const uint8_t* x_scales, const uint32_t* w, con
         return rc;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     const bool f16 = dtype == QMM_F16;
-    const int f4 = mx_f4_takes(rows, E, N, K) ? mx_f4_item_rows(rows, E, true) : 0;
+    const int f4 = mx_f4_takes(rows, E, N, K, true) ? mx_f4_item_rows(rows, E, N, K, true) : 0;
     const bool tc = !f4 && mx_tc_takes(x_scales, scales, rows, E, N, K);
     const int item_rows = f4 ? f4 : tc ? mx_tc_item_rows() : mx_warp_item_rows(rows, E);
     const GatherTables t = gather_tables(workspace, rows, E, sorted, item_rows);

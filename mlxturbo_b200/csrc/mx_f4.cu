@@ -26,7 +26,7 @@
 //   warp 1        tensor memory, scale copies, MMAs
 //   warps 2..5    weight scale bytes into the instruction's layout
 //   warps 6..9    epilogue
-//   warps 10..25  up to eight rows: activations to digits, straight into the
+//   warps 10..25  up to two rows: activations to digits, straight into the
 //                 operand's layout in shared memory
 // S blocks of a cluster share a tile, each with its part of K; the first adds
 // the others' sums from its shared memory in the order of k.  Clusters are
@@ -165,6 +165,7 @@ struct F4Params {
     const int32_t* ids;       // grouped: expert of each y row
     int x_rows, E, cluster;
     int direct;               // grouped: every row is an item of its own
+    int b_bytes;              // of a copy of planes
     uint32_t base, more;      // without items: tiles of a cluster, clusters with one more
     int k_base, k_more;       // k-blocks of a block, blocks of a cluster with one more
 };
@@ -179,7 +180,7 @@ struct MxF4 {
     static constexpr int A_BYTES = MT_ROWS * F4_BK / 2;
     static constexpr int B_BYTES = NB * F4_BK / 2;
     static constexpr int SG = 3;                  // ring of weight-scale groups (two k-blocks each)
-    static constexpr int JOIN = BT <= 2 ? 7 : BT <= 8 ? 7 : BT <= 16 ? 3 : 1;  // most other blocks of a cluster
+    static constexpr int JOIN = BT <= 2 ? 7 : BT <= 16 ? 3 : 1;  // most other blocks of a cluster
     static constexpr int A_OFF = 0;
     static constexpr int B_OFF = A_OFF + STAGES * A_BYTES;
     static constexpr int SA_OFF = B_OFF + STAGES * B_BYTES;         // [SG][4][512]
@@ -196,7 +197,7 @@ struct MxF4 {
     static constexpr int THREADS = OWN ? 832 : 320;
     static_assert(USED <= 512, "tensor memory");
     static_assert(SMEM <= 227 * 1024, "shared memory");
-    static_assert(NB % 16 == 0 && NB <= 256 && (!OWN || BT <= 8), "MMA width");
+    static_assert(NB % 16 == 0 && NB <= 256 && (!OWN || BT <= 2), "MMA width");
 };
 
 // A cluster's tiles (a run, so that neighbours share an expert) and this
@@ -345,7 +346,7 @@ __global__ void __launch_bounds__(C::THREADS, 1)
     if (warp == 0) {
         // ---------------- TMA ----------------
         auto load_w = [&](const MxTile& t, int kb, int s) {
-            mbar_expect_tx(full(s), C::A_BYTES + (C::OWN ? 0 : C::B_BYTES));
+            mbar_expect_tx(full(s), C::A_BYTES + (C::OWN ? 0 : (uint32_t)p.b_bytes));
             tma_load_2d(sbase + C::A_OFF + s * C::A_BYTES, &tmap_w, full(s), kb * (F4_BK / 2),
                         t.expert * p.c.N + t.n0);
         };
@@ -758,10 +759,10 @@ __global__ void __launch_bounds__(C::THREADS, 1)
     }
 }
 
-// The planes of more than eight rows: [R][8][K/2] with scales [R][8][K/32],
+// The planes, where another kernel makes them: [R][8][K/2] with scales [R][8][K/32],
 // rows taken through src and lhs; four lanes hold a block.
 template <int X>
-__global__ void __launch_bounds__(128) mx_f4_planes_kernel(const void* x, const uint8_t* xs, uint32_t* planes,
+__global__ void __launch_bounds__(64) mx_f4_planes_kernel(const void* x, const uint8_t* xs, uint32_t* planes,
                                                            uint8_t* scales, const uint32_t* src, const int32_t* lhs,
                                                            int x_rows, int R, int K) {
     pdl_launch_dependents();
@@ -876,41 +877,48 @@ int launch_f4_bt(const MxMatmul& a, const CUtensorMap& mw, const CUtensorMap& mb
                  int bt) {
     using namespace qmm;
     if (bt == 2) return launch_f4<MxF4<F16, X, 2, 10>>(a, mw, mb, p, tiles);
-    if (bt == 8) return launch_f4<MxF4<F16, X, 8, 7>>(a, mw, mb, p, tiles);
     if (bt == 16) return launch_f4<MxF4<F16, F4_PLANED, 16, 5>>(a, mw, mb, p, tiles);
     return launch_f4<MxF4<F16, F4_PLANED, 32, 3>>(a, mw, mb, p, tiles);
 }
 
 }  // namespace
 
-// Rows of a tile, 0 where the kernel is not for this size.  An expert's rows
-// beyond one tile read its weights again, so a grouped call leaves room for
-// twice the mean.
-int mx_f4_item_rows(long long rows, long long E, bool grouped) {
-    const long long mean = (rows + E - 1) / E;
-    if (mean > 32) return 0;
-    const long long want = grouped ? 2 * mean : mean;
-    return rows <= 2 || mx_f4_direct(rows, E, grouped) ? 2 : want <= 8 ? 8 : want <= 16 ? 16 : 32;
-}
-
 // A few rows over many experts: hardly any two meet, so each is an item of its
 // own and nothing is sorted.
 bool mx_f4_direct(long long rows, long long E, bool grouped) { return grouped && rows <= 32 && 4 * rows <= E; }
 
-bool mx_f4_takes(long long rows, long long E, long long N, long long K) {
-    const int bt = mx_f4_item_rows(rows, E, E > 1);
+// Rows of a tile, 0 where the kernel is not for this size.
+int mx_f4_item_rows(long long rows, long long E, long long N, long long K, bool grouped) {
+    const long long mean = (rows + E - 1) / E;
+    // The kernel of mx_tc.cu does the same work in half the matrix instructions,
+    // on tiles that leave blocks idle when there are few: 64 rows of 17408x5120
+    // take 27 us here and 38 there, 96 rows of 1024x5120 F4A and F4B, 128 rows of
+    // 17408x5120 F4C and 51.
+    if (grouped ? mean > 32 : mean > 64 && (mean > 256 || (mean + 31) / 32 * ((N + 127) / 128) > kMxMaxBlocks)) return 0;
+    if (mx_f4_direct(rows, E, grouped)) return 2;
+    // One launch for a product that is about as short as a launch; with planes
+    // made by a kernel before it the weight stream itself is faster (one row of
+    // 1024x5120: 6.7 us against 6.9, of 17408x5120: 14.2 against 13.2).
+    if (!grouped && rows <= 2 && N * K <= 1LL << 24) return 2;
+    // An expert's rows beyond one tile read its weights again: room for twice
+    // the mean.
+    return (grouped ? 2 * mean : mean) <= 16 ? 16 : 32;
+}
+
+bool mx_f4_takes(long long rows, long long E, long long N, long long K, bool grouped) {
+    const int bt = mx_f4_item_rows(rows, E, N, K, grouped);
     return bt && E * N <= (1LL << 31) - 256 && rows * qmm::F4_PLANES <= (1LL << 31) - 256 &&
            f4_items_max(rows, E, bt, true) * ((N + 127) / 128) * ((K + 255) / 256) < (1LL << 31);
 }
 
 size_t mx_f4_workspace(long long rows, long long K, int bt) {
-    return bt <= 8 ? 0
+    return bt == 2 ? 0
                    : mx_al256((size_t)qmm::F4_PLANES * rows * (K / 2)) +
                          mx_al256((size_t)qmm::F4_PLANES * rows * (K / 32));
 }
 
 int launch_mx_f4(const MxMatmul& a, const int4* items, const int32_t* n_items, const int32_t* ids, int bt, void* ws) {
-    const bool grouped = ids != nullptr, own = bt <= 8;
+    const bool grouped = ids != nullptr, own = bt == 2;
     uint32_t* planes = static_cast<uint32_t*>(ws);
     uint8_t* scales = static_cast<uint8_t*>(ws) + mx_al256((size_t)qmm::F4_PLANES * a.rows * (a.K / 2));
     qmm::F4Params p{};
@@ -951,13 +959,17 @@ int launch_mx_f4(const MxMatmul& a, const int4* items, const int32_t* n_items, c
     if (rc) return rc;
     mb = mw;
     if (!own) {
+        // no taller than the batch: a copy mostly out of range is slower (5 rows of
+        // 17408x5120: 16.7 us with a box for 16, 15.0 with one for 5)
+        const int box = (int)(a.rows < bt ? a.rows : bt) * qmm::F4_PLANES;
+        p.b_bytes = box * (qmm::F4_BK / 2);
         rc = tensor_map_2d(&mb, CU_TENSOR_MAP_DATA_TYPE_UINT8, planes, row, (uint64_t)a.rows * qmm::F4_PLANES, row,
-                           128, (uint32_t)(bt * qmm::F4_PLANES), CU_TENSOR_MAP_SWIZZLE_128B);
+                           128, (uint32_t)box, CU_TENSOR_MAP_SWIZZLE_128B);
         if (rc) return rc;
-        const long long want = (a.rows * (a.K / 8) + 127) / 128;
-        const unsigned g = (unsigned)(want < 148 * 16 ? want : 148 * 16);
+        const long long want = (a.rows * (a.K / 8) + 63) / 64;
+        const unsigned g = (unsigned)(want < 148 * 32 ? want : 148 * 32);
 #define QMM_PLANES(X)                                                                                                \
-    qmm::mx_f4_planes_kernel<X><<<g, 128, 0, a.st>>>(a.x, a.xs, planes, scales, a.src, a.lhs, (int)a.x_rows,          \
+    qmm::mx_f4_planes_kernel<X><<<g, 64, 0, a.st>>>(a.x, a.xs, planes, scales, a.src, a.lhs, (int)a.x_rows,          \
                                                      (int)a.rows, (int)a.K)
         if (a.xs) QMM_PLANES(qmm::F4_MX8);
         else if (a.f16) QMM_PLANES(qmm::F4_FP16);
