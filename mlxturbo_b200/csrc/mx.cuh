@@ -114,26 +114,6 @@ QMM_DEVINL void store8(void* p, const float (&v)[8]) {
     }
 }
 
-// cvt8_e2m1, and the rounded values as f16 pairs.  One asm block: unpacking a
-// word that was packed by another block in the same function lost its upper
-// two codes (CUDA 12.9).
-QMM_DEVINL uint32_t round8_e2m1(const float (&v)[8], uint32_t (&h)[4]) {
-    uint32_t r;
-    asm("{\n\t.reg .b8 a, b, c, d;\n\t"
-        "cvt.rn.satfinite.e2m1x2.f32 a, %6, %5;\n\t"
-        "cvt.rn.satfinite.e2m1x2.f32 b, %8, %7;\n\t"
-        "cvt.rn.satfinite.e2m1x2.f32 c, %10, %9;\n\t"
-        "cvt.rn.satfinite.e2m1x2.f32 d, %12, %11;\n\t"
-        "cvt.rn.f16x2.e2m1x2 %1, a;\n\t"
-        "cvt.rn.f16x2.e2m1x2 %2, b;\n\t"
-        "cvt.rn.f16x2.e2m1x2 %3, c;\n\t"
-        "cvt.rn.f16x2.e2m1x2 %4, d;\n\t"
-        "mov.b32 %0, {a, b, c, d};\n\t}"
-        : "=&r"(r), "=&r"(h[0]), "=&r"(h[1]), "=&r"(h[2]), "=&r"(h[3])
-        : "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]));
-    return r;
-}
-
 // Largest of the magnitudes of eight packed 16-bit floats, as one 16-bit
 // pattern (patterns without the sign order like the magnitudes they stand for,
 // infinity and then NaN above all), in both halves of the result's low bits.
@@ -196,28 +176,24 @@ struct MxMatmul {
     const int32_t* lhs;       // with it, x row lhs[src[s]] (the kernel of mx_f4.cu only)
     cudaStream_t st;
 };
-int launch_mx_warp(const MxMatmul& a, const int4* items, const int32_t* n_items, long long items_max, int item_rows);
-int mx_warp_item_rows(long long rows, long long E);  // rows of one expert that a block takes
-// The kernel for many rows (K % 128 == 0 and aligned scales), its rows per item
-// and its workspace behind the row tables.
-bool mx_tc_takes(const uint8_t* xs, const uint8_t* ws, long long rows, long long E, long long N, long long K);
+// The kernel for many rows, its rows per item and its workspace behind the row
+// tables.
+bool mx_tc_takes(long long rows, long long E, long long N, long long K);
 int mx_tc_item_rows();
-size_t mx_tc_workspace(long long rows, long long E, long long N, long long K, bool mx, bool f16, bool grouped);
+size_t mx_tc_workspace(long long rows, long long N, long long K, bool mx, bool f16, bool grouped);
 int launch_mx_tc(const MxMatmul& a, const int4* items, const int32_t* n_items, const int32_t* ids, void* ws);
-// The kernel for a few rows of an expert (any K % 32 == 0); item_rows 0 where
-// it is not for this size.  items == nullptr in a grouped call (`ids` given):
+// The kernel for a few rows of an expert; item_rows 0 where it is not for this
+// size.  items == nullptr in a grouped call (`ids` given):
 // every row is an item of its own.
 bool mx_f4_direct(long long rows, long long E, bool grouped);
-bool mx_f4_takes(long long rows, long long E, long long N, long long K, bool grouped);
-int mx_f4_item_rows(long long rows, long long E, long long N, long long K, bool grouped);
+bool mx_f4_takes(long long rows, long long E, long long N, long long K, bool mx, bool grouped);
+int mx_f4_item_rows(long long rows, long long E, long long N, long long K, bool mx, bool grouped);
 size_t mx_f4_workspace(long long rows, long long K, int bt);
 int launch_mx_f4(const MxMatmul& a, const int4* items, const int32_t* n_items, const int32_t* ids, int bt, void* ws);
 // Items (expert, first sorted row, rows) of at most ir rows from ascending ids,
 // and their number; ids outside [0, E) have no item.
 int launch_mx_items(const int32_t* ids_sorted, long long rows, int E, int ir, int32_t* row_start, int4* items,
                     long long items_max, int32_t* n_items, cudaStream_t st);
-// y rows whose id is outside [0, E) become zero.
-int launch_mx_zero_rows(const int32_t* ids, long long rows, int E, void* y, long long N, cudaStream_t st);
 int launch_mx_quantize(const void* v, uint32_t* words, uint8_t* scales, long long n, int bits, int dtype,
                        cudaStream_t st);
 int launch_mx_dequantize(const uint32_t* words, const uint8_t* scales, void* out, long long n, int bits, int dtype,

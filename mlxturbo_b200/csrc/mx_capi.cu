@@ -80,6 +80,14 @@ int check_product(const char* what, int64_t M, int64_t N, int64_t K, int dtype) 
     return QMM_OK;
 }
 
+// What the kernel for many rows can index.
+int check_limits(const char* what, int64_t rows, int64_t E, int64_t N, int64_t K) {
+    if (mx_tc_takes(rows, E, N, K)) return QMM_OK;
+    set_error("%s: rows=%lld E=%lld N=%lld K=%lld beyond limits", what, (long long)rows, (long long)E, (long long)N,
+              (long long)K);
+    return QMM_EUNSUPPORTED;
+}
+
 int check_workspace(const char* what, const void* ws, size_t have, size_t need) {
     if (need && (!ws || ((uintptr_t)ws & 255u) || have < need)) {
         set_error("%s: workspace must be 256-byte aligned and hold %zu bytes (%zu given)", what, need, have);
@@ -187,9 +195,9 @@ int qmm_mx_rms_norm(const void* x, const void* residual, const void* weight, voi
 
 size_t qmm_mx_matmul_workspace_size(int64_t M, int64_t N, int64_t K, int dtype, int x_is_mx) {
     if (M <= 0 || N <= 0 || K <= 0 || K % 32) return 0;
-    if (mx_f4_takes(M, 1, N, K, false)) return mx_f4_workspace(M, K, mx_f4_item_rows(M, 1, N, K, false));
-    if (K % 128) return 0;
-    return mx_tc_workspace(M, 1, N, K, x_is_mx, dtype == QMM_F16, false);
+    const int f4 = mx_f4_takes(M, 1, N, K, x_is_mx, false) ? mx_f4_item_rows(M, 1, N, K, x_is_mx, false) : 0;
+    if (f4) return mx_f4_workspace(M, K, f4);
+    return mx_tc_workspace(M, N, K, x_is_mx, dtype == QMM_F16, false);
 }
 
 int qmm_mx_matmul(const void* x, const uint8_t* x_scales, const uint32_t* w, const uint8_t* scales, void* y,
@@ -197,6 +205,9 @@ int qmm_mx_matmul(const void* x, const uint8_t* x_scales, const uint32_t* w, con
     clear_error();
     int rc = check_product("mx_matmul", M, N, K, dtype);
     if (rc) return rc;
+    const bool mx = x_scales != nullptr;
+    const int f4 = mx_f4_takes(M, 1, N, K, mx, false) ? mx_f4_item_rows(M, 1, N, K, mx, false) : 0;
+    if (!f4 && (rc = check_limits("mx_matmul", M, 1, N, K))) return rc;
     if (M == 0) return QMM_OK;
     if ((rc = check_aligned("mx_matmul", {x, w, y}))) return rc;
     if (!scales) {
@@ -219,30 +230,18 @@ int qmm_mx_matmul(const void* x, const uint8_t* x_scales, const uint32_t* w, con
     a.f16 = dtype == QMM_F16;
     a.st = static_cast<cudaStream_t>(stream);
     fire("mx_matmul");
-    if (mx_f4_takes(M, 1, N, K, false))
-        return launch_mx_f4(a, nullptr, nullptr, nullptr, mx_f4_item_rows(M, 1, N, K, false), workspace);
-    if (mx_tc_takes(x_scales, scales, M, 1, N, K))
-        return launch_mx_tc(a, nullptr, nullptr, nullptr, workspace);
-    return launch_mx_warp(a, nullptr, nullptr, 0, mx_warp_item_rows(M, 1));
+    if (f4) return launch_mx_f4(a, nullptr, nullptr, nullptr, f4, workspace);
+    return launch_mx_tc(a, nullptr, nullptr, nullptr, workspace);
 }
 
 size_t qmm_mx_gather_workspace_size(int64_t rows, int64_t E, int64_t N, int64_t K, int dtype, int x_is_mx,
                                     int sorted) {
     if (rows <= 0 || E <= 0) return 0;
     if (K <= 0 || K % 32) return 0;
-    // the kernel depends on alignment and limits too: room for any that may run
-    const bool f16 = dtype == QMM_F16;
-    size_t need = gather_tables(nullptr, rows, E, sorted, mx_warp_item_rows(rows, E)).bytes;
-    auto also = [&](int item_rows, size_t more) {
-        const size_t n = gather_tables(nullptr, rows, E, sorted, item_rows).bytes + more;
-        need = n > need ? n : need;
-    };
-    if (mx_f4_takes(rows, E, N, K, true)) {
-        const int bt = mx_f4_item_rows(rows, E, N, K, true);
-        also(bt, mx_f4_workspace(rows, K, bt));
-    } else if (K % 128 == 0)
-        also(mx_tc_item_rows(), mx_tc_workspace(rows, E, N, K, x_is_mx, f16, true));
-    return need;
+    const int f4 = mx_f4_takes(rows, E, N, K, x_is_mx, true) ? mx_f4_item_rows(rows, E, N, K, x_is_mx, true) : 0;
+    if (f4) return gather_tables(nullptr, rows, E, sorted, f4).bytes + mx_f4_workspace(rows, K, f4);
+    return gather_tables(nullptr, rows, E, sorted, mx_tc_item_rows()).bytes +
+           mx_tc_workspace(rows, N, K, x_is_mx, dtype == QMM_F16, true);
 }
 
 int qmm_mx_gather(const void* x, const uint8_t* x_scales, const uint32_t* w, const uint8_t* scales,
@@ -260,6 +259,9 @@ int qmm_mx_gather(const void* x, const uint8_t* x_scales, const uint32_t* w, con
         set_error("mx_gather: E=%lld x_rows=%lld beyond limits", (long long)E, (long long)x_rows);
         return QMM_EUNSUPPORTED;
     }
+    const bool f16 = dtype == QMM_F16, mx = x_scales != nullptr;
+    const int f4 = mx_f4_takes(rows, E, N, K, mx, true) ? mx_f4_item_rows(rows, E, N, K, mx, true) : 0;
+    if (!f4 && (rc = check_limits("mx_gather", rows, E, N, K))) return rc;
     if (rows == 0) return QMM_OK;
     if ((rc = check_aligned("mx_gather", {x, w, y}))) return rc;
     if (!scales || !rhs) {
@@ -270,10 +272,7 @@ int qmm_mx_gather(const void* x, const uint8_t* x_scales, const uint32_t* w, con
                               qmm_mx_gather_workspace_size(rows, E, N, K, dtype, x_scales != nullptr, sorted))))
         return rc;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    const bool f16 = dtype == QMM_F16;
-    const int f4 = mx_f4_takes(rows, E, N, K, true) ? mx_f4_item_rows(rows, E, N, K, true) : 0;
-    const bool tc = !f4 && mx_tc_takes(x_scales, scales, rows, E, N, K);
-    const int item_rows = f4 ? f4 : tc ? mx_tc_item_rows() : mx_warp_item_rows(rows, E);
+    const int item_rows = f4 ? f4 : mx_tc_item_rows();
     const GatherTables t = gather_tables(workspace, rows, E, sorted, item_rows);
     MxMatmul a{};
     a.x = x;
@@ -316,9 +315,7 @@ int qmm_mx_gather(const void* x, const uint8_t* x_scales, const uint32_t* w, con
     if (rc) return rc;
     fire("mx_gather");
     if (f4) return launch_mx_f4(a, t.items, n_items, rhs, f4, static_cast<char*>(workspace) + t.bytes);
-    if (tc) return launch_mx_tc(a, t.items, n_items, rhs, static_cast<char*>(workspace) + t.bytes);
-    if ((rc = launch_mx_zero_rows(rhs, rows, (int)E, y, N, st))) return rc;
-    return launch_mx_warp(a, t.items, n_items, t.items_max, t.item_rows);
+    return launch_mx_tc(a, t.items, n_items, rhs, static_cast<char*>(workspace) + t.bytes);
 }
 
 }  // extern "C"

@@ -472,7 +472,9 @@ __global__ void __launch_bounds__(C::THREADS, 1)
                 for (int q = 1; q < NL; ++q) v[q] = ld_v4(src[q] + 16 * grp);
             } else {
 #pragma unroll
-                for (int q = 0; q < NL; ++q) v[q] = mt_scale_bytes(src[q], 16 * grp, n_sf, p.c.vec);
+                for (int q = 0; q < NL; ++q)
+                    v[q] = mt_scale_bytes(src[q], 16 * grp, n_sf, p.c.vec, q ? p.c.sfb : p.c.sfw,
+                                          q ? p.c.sfb_end : p.c.sfw_end);
             }
             if (++grp > g1) {
                 grp = g0;
@@ -888,13 +890,19 @@ int launch_f4_bt(const MxMatmul& a, const CUtensorMap& mw, const CUtensorMap& mb
 bool mx_f4_direct(long long rows, long long E, bool grouped) { return grouped && rows <= 32 && 4 * rows <= E; }
 
 // Rows of a tile, 0 where the kernel is not for this size.
-int mx_f4_item_rows(long long rows, long long E, long long N, long long K, bool grouped) {
+int mx_f4_item_rows(long long rows, long long E, long long N, long long K, bool mx, bool grouped) {
     const long long mean = (rows + E - 1) / E;
-    // The kernel of mx_tc.cu does the same work in half the matrix instructions,
-    // on tiles that leave blocks idle when there are few: 64 rows of 17408x5120
-    // take 27 us here and 38 there, 96 rows of 1024x5120 F4A and F4B, 128 rows of
-    // 17408x5120 F4C and 51.
-    if (grouped ? mean > 32 : mean > 64 && (mean > 256 || (mean + 31) / 32 * ((N + 127) / 128) > kMxMaxBlocks)) return 0;
+    // The kernel of mx_tc.cu spreads the weights' codes, but multiplies by one to
+    // three planes where this one has the rate of four of them: it is ahead
+    // from few rows on for mxfp8 and later for 16-bit activations, later still
+    // where its larger tiles are few.  Here / there, us: mxfp8 16 rows of
+    // 17408x5120 14.7 / 18.9, 64 rows 27.1 / 20.0, 64 of 1024x5120 12.8 / 10.7;
+    // bf16 64 rows of 17408x5120 27.1 / 27.2, 96 rows 36.6 / 28.8, 96 of
+    // 6144x5120 16.4 / 21.5, 128 of it 25.2 / 24.0; 32 experts of 1024x2048 with
+    // 24 rows each 24.3 / 28.8 (mxfp8 24.5 / 23.3), with 32 rows 31.2 / 29.9.
+    if (mx ? mean > 16
+           : grouped ? mean > 24 : mean > 64 && (mean + 31) / 32 * ((N + 127) / 128) > kMxMaxBlocks)
+        return 0;
     if (mx_f4_direct(rows, E, grouped)) return 2;
     // One launch for a product that is about as short as a launch; with planes
     // made by a kernel before it the weight stream itself is faster (one row of
@@ -905,8 +913,8 @@ int mx_f4_item_rows(long long rows, long long E, long long N, long long K, bool 
     return (grouped ? 2 * mean : mean) <= 16 ? 16 : 32;
 }
 
-bool mx_f4_takes(long long rows, long long E, long long N, long long K, bool grouped) {
-    const int bt = mx_f4_item_rows(rows, E, N, K, grouped);
+bool mx_f4_takes(long long rows, long long E, long long N, long long K, bool mx, bool grouped) {
+    const int bt = mx_f4_item_rows(rows, E, N, K, mx, grouped);
     return bt && E * N <= (1LL << 31) - 256 && rows * qmm::F4_PLANES <= (1LL << 31) - 256 &&
            f4_items_max(rows, E, bt, true) * ((N + 127) / 128) * ((K + 255) / 256) < (1LL << 31);
 }
@@ -933,6 +941,8 @@ int launch_mx_f4(const MxMatmul& a, const int4* items, const int32_t* n_items, c
     p.c.K = (int)a.K;
     p.c.KB = (int)((a.K + qmm::F4_BK - 1) / qmm::F4_BK);
     p.c.n_tiles = (int)((a.N + 127) / 128);
+    p.c.sfw_end = a.ws + a.E * a.N * (a.K / 32);
+    p.c.sfb_end = own ? nullptr : scales + qmm::F4_PLANES * a.rows * (a.K / 32);
     p.c.vec = mx_scale_vec(a.K, a.ws, p.c.sfb);
     p.x = a.x;
     p.xs = a.xs;

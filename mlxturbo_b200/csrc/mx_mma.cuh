@@ -1,6 +1,6 @@
 // mx_mma.cuh -- what the two block-scaled tensor-core kernels (mx_f4.cu,
-// mx_tc.cu) share: bounded waits, scale copies, the division of the work over
-// persistent blocks and the joining of divided tiles.
+// mx_tc.cu) share: bounded waits, scale bytes, signals between the blocks of a
+// cluster, parameters.
 #pragma once
 
 #include "mx.cuh"
@@ -109,89 +109,36 @@ QMM_DEVINL void mt_copy_scales(uint32_t taddr, uint32_t saddr) {
 struct MxTcParams {
     const uint8_t* sfw;       // weight scale bytes [E * N, K/32]
     const uint8_t* sfb;       // plane scale bytes, rows of K/32
+    const uint8_t *sfw_end, *sfb_end;
     uint16_t* y;
     const int4* items;        // grouped: (expert, first row, rows); dense: null
     const int32_t* n_items;
     const uint32_t* dst;      // y row of each row, or null
-    float* partial;           // split: parts of tiles
-    uint32_t* counters;       // split: one per tile and 32 weight rows, zero
     int rows, N, K, KB;       // KB: k-blocks
-    int n_tiles, split;
-    int vec;                  // bytes that one load of scale bytes may take: 16, 4 or 1
-};
-
-// The stretches of k-blocks of one tile that worker `me` of `count` (a pair of
-// blocks) has, in order.  Whole tiles: every count-th.  Split: of g workers the
-// first `more` have base + 1 k-blocks and the others base, consecutive.  32-bit arithmetic: the
-// host keeps tiles * KB below 2^31.
-struct MxWalk {
-    uint32_t u, end, kb, step;
-    uint32_t base, more;
-    QMM_DEVINL MxWalk(const MxTcParams& p, uint32_t tiles, uint32_t me, uint32_t count) : kb((uint32_t)p.KB) {
-        if (p.split) {
-            const uint32_t all = tiles * kb, g = min(all, count);  // a worker with no k-block shares nothing
-            step = base = more = u = end = 0;
-            if (g) {
-                base = all / g;
-                more = all - base * g;
-            }
-            if (me < g) {
-                u = start_of(me);
-                end = start_of(me + 1);
-            }
-        } else {
-            base = more = 0;
-            step = count;
-            u = me;
-            end = tiles;
-        }
-    }
-    QMM_DEVINL uint32_t start_of(uint32_t block) const { return block * base + min(block, more); }
-    QMM_DEVINL uint32_t block_of(uint32_t unit) const {
-        const uint32_t big = more * (base + 1);
-        return unit < big ? unit / (base + 1) : more + (unit - big) / base;
-    }
-    QMM_DEVINL bool next(uint32_t& tile, int& k0, int& k1) {
-        if (u >= end) return false;
-        if (step) {
-            tile = u;
-            k0 = 0;
-            k1 = (int)kb;
-            u += step;
-        } else {
-            tile = u / kb;
-            k0 = (int)(u - tile * kb);
-            k1 = (int)min(kb, (uint32_t)k0 + (end - u));
-            u += (uint32_t)(k1 - k0);
-        }
-        return true;
-    }
+    int n_tiles;              // weight tiles
+    int vec;                  // alignment of rows of scale bytes: 16, 4 or 1
 };
 
 struct MxTile {
     int expert, row0, rows, n0;
 };
-QMM_DEVINL MxTile mt_tile(const MxTcParams& p, uint32_t tile, int bt, int weight_rows) {
-    MxTile t;
-    const int item = (int)(tile / (uint32_t)p.n_tiles);
-    t.n0 = ((int)tile - item * p.n_tiles) * weight_rows;
-    if (p.items) {
-        const int4 it = ld_dep(p.items + item);
-        t.expert = it.x;
-        t.row0 = it.y;
-        t.rows = it.z;
-    } else {
-        t.expert = 0;
-        t.row0 = item * bt;
-        t.rows = min(bt, p.rows - t.row0);
-    }
-    return t;
-}
 
 QMM_DEVINL void mt_prefetch(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
 
-// 16 scale bytes of a row from `at`, bytes at or past `n` zero.
-QMM_DEVINL uint4 mt_scale_bytes(const uint8_t* row, int at, int n, int vec) {
+// The word at w (4-byte aligned); bytes outside of [lo, hi) are not read.
+QMM_DEVINL uint32_t mt_word_within(const uint8_t* w, const uint8_t* lo, const uint8_t* hi) {
+    if (w >= lo && w + 4 <= hi) return ld_dep(reinterpret_cast<const uint32_t*>(w));
+    uint32_t v = 0;
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+        if (w + c >= lo && w + c < hi) v |= (uint32_t)ld_dep(w + c) << (8 * c);
+    return v;
+}
+
+// 16 bytes of a row of n scale bytes from `at`, those at or past n zero.  vec:
+// every row starts on a multiple of so many bytes.  lo, hi: of the whole tensor.
+// (Byte loads for vec = 1 held 16 rows of 6144x5152 at 36 us; 20 so.)
+QMM_DEVINL uint4 mt_scale_bytes(const uint8_t* row, int at, int n, int vec, const uint8_t* lo, const uint8_t* hi) {
     if (vec == 16) return ld_v4(row + at);
     uint32_t w[4] = {};
     if (vec == 4) {
@@ -199,48 +146,19 @@ QMM_DEVINL uint4 mt_scale_bytes(const uint8_t* row, int at, int n, int vec) {
         for (int c = 0; c < 4; ++c)
             if (at + 4 * c < n) w[c] = ld_dep(reinterpret_cast<const uint32_t*>(row + at) + c);
     } else {
+        const uint32_t off = (uint32_t)(uintptr_t)(row + at) & 3u;
+        const uint8_t* from = row + at - off;
+        const int left = min(n - at, 16);
+        uint32_t u[5];
 #pragma unroll
-        for (int c = 0; c < 16; ++c)
-            if (at + c < n) w[c >> 2] |= (uint32_t)ld_dep(row + at + c) << (8 * (c & 3));
+        for (int c = 0; c < 5; ++c) u[c] = 4 * c < left + (int)off ? mt_word_within(from + 4 * c, lo, hi) : 0;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            const int k = left - 4 * c;
+            w[c] = __funnelshift_r(u[c], u[c + 1], 8 * off) & (k >= 4 ? 0xFFFFFFFFu : k > 0 ? (1u << (8 * k)) - 1u : 0u);
+        }
     }
     return make_uint4(w[0], w[1], w[2], w[3]);
-}
-
-// A worker that computed a part of a tile stored it in its slot; true for the
-// warp that has to join the parts (of its 32 weight rows, with a counter of
-// their own): the last of the workers first .. final that share the tile.
-QMM_DEVINL bool mt_last_of(const MxWalk& w, uint32_t tile, uint32_t* counter, int& first, int& final_) {
-    first = (int)w.block_of(tile * w.kb);
-    final_ = (int)w.block_of(tile * w.kb + w.kb - 1);
-    __threadfence();
-    __syncwarp();
-    uint32_t before = 0;
-    if ((threadIdx.x & 31) == 0) before = atomicAdd(counter, 1u);
-    if (__shfl_sync(0xffffffffu, before, 0) != (uint32_t)(final_ - first)) return false;
-    __threadfence();
-    return true;
-}
-
-// The parts of eight columns (128 rows each, from `base` of the first worker's
-// slots), added in the order of k.  Slot 0 of a worker is a stretch that begins
-// inside a tile (its first), slot 1 one that begins with the tile and ends
-// inside it (its last).
-QMM_DEVINL void mt_join8(const float* base, long long slot, int first, int final_, int nj, float (&f)[8]) {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) f[j] = 0.0f;
-    for (int c = first; c <= final_; c += 4) {
-        float v[4][8];  // loads of four workers in flight
-#pragma unroll
-        for (int d = 0; d < 4; ++d) {
-            const float* from = base + (2 * (c + d) + (c + d == first)) * slot;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) v[d][j] = c + d <= final_ && j < nj ? __ldcg(from + j * MT_ROWS) : 0.0f;
-        }
-#pragma unroll
-        for (int d = 0; d < 4; ++d)
-#pragma unroll
-            for (int j = 0; j < 8; ++j) f[j] += v[d][j];
-    }
 }
 
 }  // namespace qmm

@@ -31,13 +31,12 @@
 //   warps 2..9  two sets of four, a k-block each in turn: spread the weights'
 //               codes, 8 to 16 bytes as the instruction reads them
 //   warps 10..13 scale bytes into the instruction's layout
-//   warps 14..17 epilogue: TMEM -> y, or a partial sum
+//   warps 14..17 epilogue: TMEM -> y
 // TMA could spread the codes itself, but at 8 packed bytes a clock and SM: 1024
 // clocks for 128 x 128, which the MMAs of one plane need 384 for.
 //
-// Pairs are persistent.  With enough tiles each takes whole ones; with few, the
-// k-blocks are divided evenly over the pairs and the last pair of a tile to
-// finish joins the parts in the order of k, so results do not depend on timing.
+// Pairs are persistent.  They take whole tiles, or, where there are fewer tiles than
+// pairs, parts of one along K, which a second kernel adds.
 
 #include "mx_mma.cuh"
 
@@ -75,7 +74,41 @@ struct MtParams {
     MxTcParams c;
     const int32_t* ids;   // grouped: expert of each y row
     int E;                // experts
+    int split, part;      // parts of a tile along K, k-blocks of a part
+    float* partial;       // split > 1: sums of the parts [split][rows][N]
 };
+
+// Every pairs-th tile, or part of one: k-blocks k0 .. k1 - 1, k0 a multiple of four.
+struct MtWalk {
+    uint32_t u, end, step;
+    QMM_DEVINL MtWalk(uint32_t tiles, const MtParams& p)
+        : u(blockIdx.x >> 1), end(tiles * (uint32_t)p.split), step(gridDim.x >> 1) {}
+    QMM_DEVINL bool next(const MtParams& p, uint32_t& tile, int& k0, int& k1) {
+        if (u >= end) return false;
+        tile = u / (uint32_t)p.split;
+        k0 = (int)(u - tile * (uint32_t)p.split) * p.part;
+        k1 = min(p.c.KB, k0 + p.part);
+        u += step;
+        return true;
+    }
+};
+
+QMM_DEVINL MxTile mt_tile(const MxTcParams& p, uint32_t tile) {
+    MxTile t;
+    const int item = (int)(tile / (uint32_t)p.n_tiles);
+    t.n0 = ((int)tile - item * p.n_tiles) * MT_W;
+    if (p.items) {
+        const int4 it = ld_dep(p.items + item);
+        t.expert = it.x;
+        t.row0 = it.y;
+        t.rows = it.z;
+    } else {
+        t.expert = 0;
+        t.row0 = item * MT_BT;
+        t.rows = min(MT_BT, p.rows - t.row0);
+    }
+    return t;
+}
 
 template <bool F16_, int P_, int STAGES_>
 struct MxTc {
@@ -169,7 +202,7 @@ __global__ void __launch_bounds__(C::THREADS, 1)
     if (warp != 0 || p.c.items) pdl_wait();
     const uint32_t tiles =
         (uint32_t)p.c.n_tiles * (uint32_t)(p.c.items ? ld_dep(p.c.n_items) : (p.c.rows + MT_BT - 1) / MT_BT);
-    MxWalk walk(p.c, tiles, blockIdx.x >> 1, gridDim.x >> 1);
+    MtWalk walk(tiles, p);
     uint32_t tile;
     int k0, k1;
     // columns of a tile's MMAs, and the first row of this block's half of them
@@ -184,20 +217,20 @@ __global__ void __launch_bounds__(C::THREADS, 1)
         };
         int i = 0, pack = 0, early = 0;  // k-blocks and pairs of them so far
         if (!p.c.items) {
-            MxWalk ahead = walk;
-            while (early < C::PACKS && ahead.next(tile, k0, k1)) {
-                const MxTile t = mt_tile(p.c, tile, MT_BT, MT_W);
-                for (int j = k0 >> 1; j <= (k1 - 1) >> 1 && early < C::PACKS; ++j, ++early)
+            MtWalk ahead = walk;
+            while (early < C::PACKS && ahead.next(p, tile, k0, k1)) {
+                const MxTile t = mt_tile(p.c, tile);
+                for (int j = k0 >> 1; 2 * j < k1 && early < C::PACKS; ++j, ++early)
                     if (elect_one()) load_w(t, j, early);
                 __syncwarp();
             }
             pdl_wait();
         }
-        while (walk.next(tile, k0, k1) && !*abort) {
-            const MxTile t = mt_tile(p.c, tile, MT_BT, MT_W);
+        while (walk.next(p, tile, k0, k1) && !*abort) {
+            const MxTile t = mt_tile(p.c, tile);
             const int half = cols(t) / 2, mine = t.row0 + (int)rank * half;
             for (int kb = k0; kb < k1; ++kb, ++i) {
-                if (kb == k0 || (kb & 1) == 0) {
+                if ((kb & 1) == 0) {
                     const int w = pack % C::PACKS;
                     if (pack >= early) {  // an early one may have been read and given back already
                         if (!mt_wait(empty_w(w), ((uint32_t)(pack / C::PACKS) & 1u) ^ 1u, abort, 64)) break;
@@ -222,14 +255,14 @@ __global__ void __launch_bounds__(C::THREADS, 1)
         // ---------------- scale copies and MMAs (first block) ----------------
         const uint64_t adesc0 = umma_desc_sw128(sbase + C::A_OFF), bdesc0 = umma_desc_sw128(sbase + C::B_OFF);
         int i = 0, seg = 0, g = -1;
-        while (rank == 0 && walk.next(tile, k0, k1) && !*abort) {
-            const int nb = cols(mt_tile(p.c, tile, MT_BT, MT_W)), b = seg & 1;
+        while (rank == 0 && walk.next(p, tile, k0, k1) && !*abort) {
+            const int nb = cols(mt_tile(p.c, tile)), b = seg & 1;
             const uint32_t acc = tmem + b * MT_BT;
             if (!mt_wait(acc_empty(b), ((uint32_t)(seg >> 1) & 1u) ^ 1u, abort, 2)) break;
             ++seg;
             for (int kb = k0; kb < k1; ++kb, ++i) {
                 const int s = i % STAGES;
-                if (kb == k0 || (kb & 3) == 0) {
+                if ((kb & 3) == 0) {
                     ++g;
                     if (!mt_wait(scaled(g % C::SG), (uint32_t)(g / C::SG) & 1u, abort, 256)) break;
                 }
@@ -262,11 +295,11 @@ __global__ void __launch_bounds__(C::THREADS, 1)
         // even k-blocks, set 1 the odd.
         const int set = (warp - 2) >> 2, r = ((warp - 2) & 3) * 32 + lane;
         const uint32_t ready0 = mt_remote(ready(0), 0);
-        int i0 = 0, pack = 0;  // k-blocks before this stretch, pairs so far
-        while (walk.next(tile, k0, k1) && !*abort) {
-            for (int j = k0 >> 1; j <= (k1 - 1) >> 1; ++j, ++pack) {
+        int i0 = 0, pack = 0;  // k-blocks before this part, pairs so far
+        while (walk.next(p, tile, k0, k1) && !*abort) {
+            for (int j = k0 >> 1; 2 * j < k1; ++j, ++pack) {
                 const int kb = 2 * j + set, w = pack % C::PACKS;
-                const bool in = kb >= k0 && kb < k1;
+                const bool in = kb < k1;
                 uint32_t c[4][4];
                 if (!mt_wait(full_w(w), (uint32_t)(pack / C::PACKS) & 1u, abort, 8)) break;
                 if (in) {
@@ -309,16 +342,16 @@ __global__ void __launch_bounds__(C::THREADS, 1)
         // AHEAD groups ahead, across tiles.
         constexpr int NL = 1 + 2 * C::P;
         constexpr int AHEAD = C::P == 3 ? 2 : 3;
-        const int r = (warp - 10) * 32 + lane, n_sf = p.c.KB * 4;
+        const int r = (warp - 10) * 32 + lane, n_sf = p.c.K / 32;
         const uint32_t sdst = sbase + C::S_OFF + (r & 31) * 16 + (r >> 5) * 4;
         const uint32_t scaled0 = mt_remote(scaled(0), 0);
         const uint8_t* src[NL];
         int grp = 0, last = -1;
         bool more = true;
-        auto enter = [&]() {  // the next stretch
-            more = walk.next(tile, k0, k1);
+        auto enter = [&]() {  // the next part
+            more = walk.next(p, tile, k0, k1);
             if (!more) return;
-            const MxTile t = mt_tile(p.c, tile, MT_BT, MT_W);
+            const MxTile t = mt_tile(p.c, tile);
             src[0] = p.c.sfw + ((long long)t.expert * p.c.N + min(t.n0 + (int)rank * MT_ROWS + r, p.c.N - 1)) * n_sf;
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
@@ -337,7 +370,9 @@ __global__ void __launch_bounds__(C::THREADS, 1)
                 for (int q = 1; q < NL; ++q) v[q] = ld_v4(src[q] + 16 * grp);
             } else {
 #pragma unroll
-                for (int q = 0; q < NL; ++q) v[q] = mt_scale_bytes(src[q], 16 * grp, n_sf, p.c.vec);
+                for (int q = 0; q < NL; ++q)
+                    v[q] = mt_scale_bytes(src[q], 16 * grp, n_sf, p.c.vec, q ? p.c.sfb : p.c.sfw,
+                                          q ? p.c.sfb_end : p.c.sfw_end);
             }
             if (++grp > last) enter();
             return true;
@@ -380,26 +415,18 @@ __global__ void __launch_bounds__(C::THREADS, 1)
             for (int q = blockIdx.x * 4 + warp - 14; q < p.c.rows; q += gridDim.x * 4)
                 if ((uint32_t)ld_dep(p.ids + q) >= (uint32_t)p.E)
                     for (int n = lane; n < p.c.N; n += 32) p.c.y[(long long)q * p.c.N + n] = 0;
-        constexpr long long SLOT = (long long)MT_BT * MT_ROWS;
-        float* parts = p.c.partial + (long long)rank * gridDim.x * SLOT + row;  // [2 blocks][2 * pairs] slots
         const uint32_t acc_empty0 = mt_remote(acc_empty(0), 0);
         int seg = 0;
-        while (walk.next(tile, k0, k1) && !*abort) {
-            const MxTile t = mt_tile(p.c, tile, MT_BT, MT_W);
+        while (walk.next(p, tile, k0, k1) && !*abort) {
+            const MxTile t = mt_tile(p.c, tile);
             const int b = seg & 1;
             if (!mt_wait(acc_full(b), (uint32_t)(seg >> 1) & 1u, abort, 32)) break;
             ++seg;
             tc_fence_after();
-            const bool whole = k0 == 0 && k1 == p.c.KB;
             const int n = t.n0 + (int)rank * MT_ROWS + row;
-            float* part = parts + (2 * (blockIdx.x >> 1) + (k0 == 0)) * SLOT;
-            auto store_y = [&](int j, float f) {
-                const long long out = p.c.dst ? (long long)ld_dep(p.c.dst + t.row0 + j) : t.row0 + j;
-                if (n < p.c.N) p.c.y[out * p.c.N + n] = H::from_f32(f);
-            };
             // Two lanes exchange halves, so that each stores two neighbouring
             // outputs at once: the even lane for even rows, the odd for odd.
-            const bool pairs = whole && (p.c.N & 1) == 0;
+            const bool pairs = (p.c.N & 1) == 0;
             const int n2 = n & ~1;
 #pragma unroll 1
             for (int c0 = 0; c0 < t.rows; c0 += 32) {
@@ -408,7 +435,12 @@ __global__ void __launch_bounds__(C::THREADS, 1)
                 int out_l = t.row0 + c0 + lane;  // y row of column c0 + lane
                 if (p.c.dst && c0 + lane < t.rows) out_l = (int)ld_dep(p.c.dst + out_l);
                 tmem_wait_ld();
-                if (pairs) {
+                if (p.split > 1) {  // 128 bytes of a row to a warp
+                    float* part = p.partial + ((long long)(k0 / p.part) * p.c.rows + t.row0 + c0) * p.c.N + n;
+#pragma unroll
+                    for (int j = 0; j < 32; ++j)
+                        if (c0 + j < t.rows && n < p.c.N) part[(long long)j * p.c.N] = __uint_as_float(u[j]);
+                } else if (pairs) {
 #pragma unroll
                     for (int j = 0; j < 32; j += 2) {
                         const uint32_t mine = lane & 1 ? u[j + 1] : u[j], give = lane & 1 ? u[j] : u[j + 1];
@@ -422,27 +454,17 @@ __global__ void __launch_bounds__(C::THREADS, 1)
                 } else {
 #pragma unroll
                     for (int j = 0; j < 32; ++j) {
-                        if (c0 + j >= t.rows) continue;
-                        if (!whole) part[(c0 + j) * MT_ROWS] = __uint_as_float(u[j]);
-                        else store_y(c0 + j, __uint_as_float(u[j]));
+                        const long long out = __shfl_sync(0xffffffffu, out_l, j);
+                        if (c0 + j < t.rows && n < p.c.N) p.c.y[out * p.c.N + n] = H::from_f32(__uint_as_float(u[j]));
                     }
                 }
             }
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mt_pair_arrive(acc_empty0 + 8 * b);
-            int first, final_;
-            if (whole || !mt_last_of(walk, tile, p.c.counters + tile * 8 + rank * 4 + quarter, first, final_)) continue;
-            for (int c0 = 0; c0 < t.rows; c0 += 8) {
-                float f[8];
-                const int nj = min(8, t.rows - c0);
-                mt_join8(parts + c0 * MT_ROWS, SLOT, first, final_, nj, f);
-#pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    if (j < nj) store_y(c0 + j, f[j]);
-            }
         }
     }
+    if (p.split > 1) pdl_launch_dependents();
     if (*abort) __nanosleep(1000000);  // after a wait gave up: let copies in flight land
     tc_fence_before();
     __syncwarp();
@@ -452,6 +474,50 @@ __global__ void __launch_bounds__(C::THREADS, 1)
     if (warp == 1) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(C::COLS) : "memory");
+    }
+}
+
+// y = the sum of a divided product's parts, in their order; four values to a thread.
+template <bool F16>
+__global__ void __launch_bounds__(256) mx_join_kernel(const float* partial, uint16_t* y, long long n, int split) {
+    using H = Half<F16>;
+    constexpr int RUN = 4;  // loads together
+    pdl_wait();
+    for (long long i = ((long long)blockIdx.x * blockDim.x + threadIdx.x) * 4; i < n;
+         i += (long long)gridDim.x * blockDim.x * 4) {
+        float f[4] = {};
+        for (int s0 = 0; s0 < split; s0 += RUN) {
+            float v[RUN][4];
+#pragma unroll
+            for (int s = 0; s < RUN; ++s)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) v[s][j] = 0.0f;
+#pragma unroll
+            for (int s = 0; s < RUN; ++s) {
+                if (s0 + s >= split) continue;
+                const float* from = partial + (s0 + s) * n + i;
+                if ((n & 3) == 0) {
+                    const uint4 w = ld_v4(from);
+                    v[s][0] = __uint_as_float(w.x), v[s][1] = __uint_as_float(w.y);
+                    v[s][2] = __uint_as_float(w.z), v[s][3] = __uint_as_float(w.w);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        if (i + j < n) v[s][j] = ld_dep(from + j);
+                }
+            }
+#pragma unroll
+            for (int s = 0; s < RUN; ++s)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) f[j] += v[s][j];
+        }
+        if ((n & 3) == 0) {
+            *reinterpret_cast<uint2*>(y + i) = make_uint2(H::pack2(f[0], f[1]), H::pack2(f[2], f[3]));
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (i + j < n) y[i + j] = H::from_f32(f[j]);
+        }
     }
 }
 
@@ -540,17 +606,12 @@ QMM_DEVINL uint32_t mt_max_finite(const uint4& raw) {
 }
 
 // Activations to P e4m3 planes [P][R][K] with scales [P][R][K/32], rows taken
-// through src; two lanes hold a block.  P = 1 copies mxfp8 rows.  Also clears
-// the counters of the product that follows.
+// through src; two lanes hold a block.  P = 1 copies mxfp8 rows.
 template <int T, int P>
 __global__ void __launch_bounds__(128) mx_planes_kernel(const void* x, const uint8_t* xs, uint8_t* planes,
-                                                        uint8_t* scales, const uint32_t* src, int x_rows, int R, int K,
-                                                        uint32_t* counters, int n_counters) {
+                                                        uint8_t* scales, const uint32_t* src, int x_rows, int R,
+                                                        int K) {
     pdl_launch_dependents();
-    const int tid = blockIdx.y * gridDim.x + blockIdx.x;
-    for (long long i = (long long)tid * blockDim.x + threadIdx.x; i < n_counters;
-         i += (long long)gridDim.x * gridDim.y * blockDim.x)
-        counters[i] = 0;
     // sixteen values (half a block) of RUN rows to a thread, their loads together
     constexpr int RUN = 4;
     const int g = K / 16, c = blockIdx.x * blockDim.x + threadIdx.x;
@@ -624,11 +685,9 @@ namespace qmm_host {
 
 namespace {
 
-constexpr int kPairs = kMxMaxBlocks / 2;
-
 // Workspace of a product behind the row tables.
 struct TcLayout {
-    size_t planes, scales, counters, partial, bytes;
+    size_t planes, scales, partial, bytes;
 };
 
 int planes_of(bool mx, bool f16) { return mx ? 1 : f16 ? 3 : 2; }
@@ -639,17 +698,27 @@ long long tc_tiles_max(long long rows, long long E, long long N, bool grouped) {
     return items * ((N + qmm::MT_W - 1) / qmm::MT_W);
 }
 
-// Whether the k-blocks of the tiles are divided over the pairs: with fewer
-// tiles than two for each pair, whole ones would leave many pairs idle in the
-// last round.
-bool tc_split(long long tiles) { return tiles < 2 * kPairs; }
+// Parts of a tile along K: as many as leave no pair idle, each of at least 8
+// k-blocks, in dense products.  Their sums meet in fp32 in the workspace, added
+// by mx_join_kernel.  (bf16, 512 rows of 1024x5120: 24 us, 27 a tile's whole K
+// alone.  Stretches of equal length over tile ends, with the parts added by the
+// pair that came last: 54 us, 128 rows of 17408x5120 52 against 31.)
+struct TcSplit {
+    int split, part;
+};
+TcSplit tc_split(long long rows, long long N, long long K, bool grouped) {
+    const long long tiles = tc_tiles_max(rows, 1, N, false), KB = (K + 127) / 128;
+    long long s = grouped ? 1 : kMxMaxBlocks / 2 / tiles;
+    s = s > KB / 8 ? KB / 8 : s;
+    if (s < 2) return {1, (int)KB};
+    const long long part = ((KB + s - 1) / s + 3) / 4 * 4;  // whole groups of scale bytes
+    return {(int)((KB + part - 1) / part), (int)part};
+}
 
 // planes: of every row of the product; mxfp8 rows that are taken in order are
 // read where they are
-TcLayout tc_layout(long long rows, long long E, long long N, long long K, bool mx, bool f16, bool grouped) {
+TcLayout tc_layout(long long rows, long long N, long long K, bool mx, bool f16, bool grouped) {
     TcLayout l{};
-    const long long tiles = tc_tiles_max(rows, E, N, grouped);
-    const bool split = tc_split(tiles);
     const int P = planes_of(mx, f16);
     size_t at = 0;
     auto take = [&](size_t n) {
@@ -659,8 +728,8 @@ TcLayout tc_layout(long long rows, long long E, long long N, long long K, bool m
     };
     l.planes = take(mx && !grouped ? 0 : (size_t)P * rows * K);
     l.scales = take(mx && !grouped ? 0 : (size_t)P * rows * (K / 32));
-    l.counters = take(split ? (size_t)tiles * 32 : 0);
-    l.partial = take(split ? (size_t)4 * kPairs * qmm::MT_BT * 128 * 4 : 0);
+    const TcSplit d = tc_split(rows, N, K, grouped);
+    l.partial = take(d.split > 1 ? (size_t)d.split * rows * N * 4 : 0);
     l.bytes = at;
     return l;
 }
@@ -691,49 +760,47 @@ int launch_tc(const MxMatmul& a, const CUtensorMap& mw, const CUtensorMap& mb, c
 
 int mx_tc_item_rows() { return qmm::MT_BT; }
 
-// Rows of packed weights are whole 16-byte runs and k-blocks whole.
-bool mx_tc_takes(const uint8_t* xs, const uint8_t* ws, long long rows, long long E, long long N, long long K) {
-    return K % 128 == 0 && ((uintptr_t)ws & 3u) == 0 && ((uintptr_t)xs & 3u) == 0 && E * N <= (1LL << 31) - 512 &&
-           3 * rows <= (1LL << 31) - 512 &&
-           tc_tiles_max(rows, E, N, true) * (K / 128) < (1LL << 31);
+bool mx_tc_takes(long long rows, long long E, long long N, long long K) {
+    return E * N <= (1LL << 31) - 512 && 3 * rows <= (1LL << 31) - 512 &&
+           tc_tiles_max(rows, E, N, true) * ((K + 127) / 128) < (1LL << 31);
 }
 
-size_t mx_tc_workspace(long long rows, long long E, long long N, long long K, bool mx, bool f16, bool grouped) {
-    return tc_layout(rows, E, N, K, mx, f16, grouped).bytes;
+size_t mx_tc_workspace(long long rows, long long N, long long K, bool mx, bool f16, bool grouped) {
+    return tc_layout(rows, N, K, mx, f16, grouped).bytes;
 }
 
 int launch_mx_tc(const MxMatmul& a, const int4* items, const int32_t* n_items, const int32_t* ids, void* ws) {
     const bool mx = a.xs != nullptr, grouped = items != nullptr, in_place = mx && !a.src;
     const int P = planes_of(mx, a.f16);
-    const TcLayout l = tc_layout(a.rows, a.E, a.N, a.K, mx, a.f16, grouped);
+    const TcLayout l = tc_layout(a.rows, a.N, a.K, mx, a.f16, grouped);
     char* const base = static_cast<char*>(ws);
     const long long tiles = tc_tiles_max(a.rows, a.E, a.N, grouped);
     uint8_t* planes = reinterpret_cast<uint8_t*>(base + l.planes);
     uint8_t* scales = reinterpret_cast<uint8_t*>(base + l.scales);
     qmm::MtParams p{};
-    p.c.split = tc_split(tiles);
     p.c.sfw = a.ws;
     p.c.sfb = in_place ? a.xs : scales;
     p.c.y = static_cast<uint16_t*>(a.y);
     p.c.items = items;
     p.c.n_items = n_items;
     p.c.dst = a.dst;
-    p.c.partial = reinterpret_cast<float*>(base + l.partial);
-    p.c.counters = reinterpret_cast<uint32_t*>(base + l.counters);
     p.c.rows = (int)a.rows;
     p.c.N = (int)a.N;
     p.c.K = (int)a.K;
-    p.c.KB = (int)(a.K / 128);
+    p.c.KB = (int)((a.K + 127) / 128);
     p.c.n_tiles = (int)((a.N + qmm::MT_W - 1) / qmm::MT_W);
+    p.c.sfw_end = a.ws + a.E * a.N * (a.K / 32);
+    p.c.sfb_end = p.c.sfb + P * (in_place ? a.x_rows : a.rows) * (a.K / 32);
     p.c.vec = mx_scale_vec(a.K, p.c.sfw, p.c.sfb);
     p.ids = ids;
     p.E = (int)a.E;
+    const TcSplit d = tc_split(a.rows, a.N, a.K, grouped);
+    p.split = d.split;
+    p.part = d.part;
+    p.partial = reinterpret_cast<float*>(base + l.partial);
     const int most = mx_sm_count() / 2;
-    long long pairs = tiles;
-    if (p.c.split) pairs = (tiles * p.c.KB + 7) / 8;  // at least eight k-blocks each: a join reads every part
-    if (pairs > most) pairs = most;
+    const long long pairs = tiles * d.split < most ? tiles * d.split : most;
 
-    const size_t n_counters = p.c.split ? (size_t)tiles * 8 : 0;
     int rc = QMM_OK;
     if (!in_place) {
         const int g = (int)(a.K / 16);
@@ -741,14 +808,12 @@ int launch_mx_tc(const MxMatmul& a, const int4* items, const int32_t* n_items, c
         const dim3 grid((unsigned)((g + 127) / 128), (unsigned)(runs < 32768 ? runs : 32768));
 #define QMM_PLANES(T, PP)                                                                                         \
     qmm::mx_planes_kernel<T, PP><<<grid, 128, 0, a.st>>>(a.x, a.xs, planes, scales, a.src, (int)a.x_rows,          \
-                                                         (int)a.rows, (int)a.K, p.c.counters, (int)n_counters)
+                                                         (int)a.rows, (int)a.K)
         if (mx) QMM_PLANES(qmm::MX_BF16, 1);
         else if (a.f16) QMM_PLANES(qmm::MX_F16, 3);
         else QMM_PLANES(qmm::MX_BF16, 2);
 #undef QMM_PLANES
         rc = cuda_status(cudaGetLastError(), "mx_planes launch");
-    } else if (n_counters) {
-        rc = cuda_status(cudaMemsetAsync(p.c.counters, 0, n_counters * 4, a.st), "mx_tc: clearing the counters");
     }
     if (rc) return rc;
     CUtensorMap mw, mb;
@@ -759,10 +824,24 @@ int launch_mx_tc(const MxMatmul& a, const int4* items, const int32_t* n_items, c
                        (uint64_t)(P * a.rows), (uint64_t)a.K, 128, qmm::MT_HALF, CU_TENSOR_MAP_SWIZZLE_128B);
     if (rc) return rc;
     using namespace qmm;
-    if (mx) return a.f16 ? launch_tc<MxTc<true, 1, 6>>(a, mw, mb, p, (int)pairs, !in_place)
-                         : launch_tc<MxTc<false, 1, 6>>(a, mw, mb, p, (int)pairs, !in_place);
-    return a.f16 ? launch_tc<MxTc<true, 3, 3>>(a, mw, mb, p, (int)pairs, true)
-                 : launch_tc<MxTc<false, 2, 4>>(a, mw, mb, p, (int)pairs, true);
+    if (mx) rc = a.f16 ? launch_tc<MxTc<true, 1, 6>>(a, mw, mb, p, (int)pairs, !in_place)
+                       : launch_tc<MxTc<false, 1, 6>>(a, mw, mb, p, (int)pairs, !in_place);
+    else rc = a.f16 ? launch_tc<MxTc<true, 3, 3>>(a, mw, mb, p, (int)pairs, true)
+                    : launch_tc<MxTc<false, 2, 4>>(a, mw, mb, p, (int)pairs, true);
+    if (rc || d.split == 1) return rc;
+    const long long n = a.rows * a.N, blocks = (n + 1023) / 1024;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)(blocks < 2 * kMxMaxBlocks ? blocks : 2 * kMxMaxBlocks));
+    cfg.blockDim = dim3(256);
+    cfg.stream = a.st;
+    cudaLaunchAttribute at[1]{};
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = pdl_enabled() ? 1 : 0;
+    return cuda_status(cudaLaunchKernelEx(&cfg, a.f16 ? mx_join_kernel<true> : mx_join_kernel<false>,
+                                          (const float*)p.partial, p.c.y, n, d.split),
+                       "mx_join launch");
 }
 
 int mx_tc_device_error(int reset) { return mx_error_flag(reset); }
