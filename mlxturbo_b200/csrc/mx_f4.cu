@@ -461,20 +461,19 @@ __global__ void __launch_bounds__(C::THREADS, 1)
             for (int q = 1; q < NL; ++q) {
                 const int c = min((q - 1) * 128 + r, C::NB - 1);
                 const long long row = min((long long)t.row0 * F4_PLANES + c, (long long)p.c.rows * F4_PLANES - 1);
-                src[q] = p.c.sfb + row * n_sf;
+                src[q] = p.c.sfb + row * p.c.sfb_row;
             }
         };
         auto load = [&](uint4 (&v)[NL]) {
             if (!tiles.more()) return;
-            if (p.c.vec == 16) {
+            if (p.c.vec_w == 16) {
                 v[0] = ldg_v4(src[0] + 16 * grp);
 #pragma unroll
                 for (int q = 1; q < NL; ++q) v[q] = ld_v4(src[q] + 16 * grp);
             } else {
+                v[0] = mt_scale_bytes(src[0], 16 * grp, n_sf, p.c.vec_w, p.c.sfw, p.c.sfw_end);
 #pragma unroll
-                for (int q = 0; q < NL; ++q)
-                    v[q] = mt_scale_bytes(src[q], 16 * grp, n_sf, p.c.vec, q ? p.c.sfb : p.c.sfw,
-                                          q ? p.c.sfb_end : p.c.sfw_end);
+                for (int q = 1; q < NL; ++q) v[q] = ld_v4(src[q] + 16 * grp);
             }
             if (++grp > g1) {
                 grp = g0;
@@ -761,14 +760,14 @@ __global__ void __launch_bounds__(C::THREADS, 1)
     }
 }
 
-// The planes, where another kernel makes them: [R][8][K/2] with scales [R][8][K/32],
-// rows taken through src and lhs; four lanes hold a block.
+// The planes, where another kernel makes them: [R][8][K/2] with scales [R][8][K/32
+// rounded up to 16], rows taken through src and lhs; four lanes hold a block.
 template <int X>
 __global__ void __launch_bounds__(64) mx_f4_planes_kernel(const void* x, const uint8_t* xs, uint32_t* planes,
                                                            uint8_t* scales, const uint32_t* src, const int32_t* lhs,
                                                            int x_rows, int R, int K) {
     pdl_launch_dependents();
-    const int n8 = K / 8;
+    const int n8 = K / 8, pitch = (K / 32 + 15) & ~15;
     const long long total = (long long)R * n8, step = (long long)gridDim.x * blockDim.x;
     for (long long base = ((long long)blockIdx.x * blockDim.x + threadIdx.x) & ~31LL; base < total; base += step) {
         const long long i = base + (threadIdx.x & 31);
@@ -794,11 +793,18 @@ __global__ void __launch_bounds__(64) mx_f4_planes_kernel(const void* x, const u
         uint32_t plane[8];
         f4_digits(g, plane);
         if (!in) continue;
+        uint32_t* to = planes + (long long)r * F4_PLANES * n8 + c;
+        uint8_t* sf = scales + (long long)r * F4_PLANES * pitch + (c >> 2);
 #pragma unroll
         for (int q = 0; q < F4_PLANES; ++q) {
-            const long long o = ((long long)r * F4_PLANES + q) * n8 + c;
-            planes[o] = plane[q];
-            if ((c & 3) == 0) scales[o >> 2] = (uint8_t)f4_plane_scale(g.byte, q);
+            to[q * n8] = plane[q];
+            if ((c & 3) == 0) sf[q * pitch] = (uint8_t)f4_plane_scale(g.byte, q);
+        }
+        if (c + 4 == n8 && n8 < 4 * pitch) {  // the last block's first lane: the rest of the rows
+#pragma unroll 1
+            for (int q = 0; q < F4_PLANES; ++q)
+#pragma unroll 1
+                for (int k = 1; k <= pitch - n8 / 4; ++k) sf[q * pitch + k] = 0;
         }
     }
 }
@@ -922,7 +928,7 @@ bool mx_f4_takes(long long rows, long long E, long long N, long long K, bool mx,
 size_t mx_f4_workspace(long long rows, long long K, int bt) {
     return bt == 2 ? 0
                    : mx_al256((size_t)qmm::F4_PLANES * rows * (K / 2)) +
-                         mx_al256((size_t)qmm::F4_PLANES * rows * (K / 32));
+                         mx_al256((size_t)qmm::F4_PLANES * rows * mx_plane_row(K));
 }
 
 int launch_mx_f4(const MxMatmul& a, const int4* items, const int32_t* n_items, const int32_t* ids, int bt, void* ws) {
@@ -942,8 +948,8 @@ int launch_mx_f4(const MxMatmul& a, const int4* items, const int32_t* n_items, c
     p.c.KB = (int)((a.K + qmm::F4_BK - 1) / qmm::F4_BK);
     p.c.n_tiles = (int)((a.N + 127) / 128);
     p.c.sfw_end = a.ws + a.E * a.N * (a.K / 32);
-    p.c.sfb_end = own ? nullptr : scales + qmm::F4_PLANES * a.rows * (a.K / 32);
-    p.c.vec = mx_scale_vec(a.K, a.ws, p.c.sfb);
+    p.c.sfb_row = (int)mx_plane_row(a.K);
+    p.c.vec_w = mx_scale_vec(a.K, a.ws);
     p.x = a.x;
     p.xs = a.xs;
     p.src = a.src;

@@ -357,22 +357,22 @@ __global__ void __launch_bounds__(C::THREADS, 1)
             for (int h = 0; h < 2; ++h) {
                 const int row = t.row0 + min(h * 128 + r, t.rows - 1);
 #pragma unroll
-                for (int q = 0; q < C::P; ++q) src[1 + 2 * q + h] = p.c.sfb + ((long long)q * p.c.rows + row) * n_sf;
+                for (int q = 0; q < C::P; ++q) src[1 + 2 * q + h] = p.c.sfb + ((long long)q * p.c.rows + row) * p.c.sfb_row;
             }
             grp = k0 >> 2;
             last = (k1 - 1) >> 2;
         };
         auto load = [&](uint4 (&v)[NL]) {  // false past the end
             if (!more) return false;
-            if (p.c.vec == 16) {
+            if (p.c.vec_w == 16 && p.c.vec_b == 16) {
                 v[0] = ldg_v4(src[0] + 16 * grp);
 #pragma unroll
                 for (int q = 1; q < NL; ++q) v[q] = ld_v4(src[q] + 16 * grp);
             } else {
+                v[0] = mt_scale_bytes(src[0], 16 * grp, n_sf, p.c.vec_w, p.c.sfw, p.c.sfw_end);
 #pragma unroll
-                for (int q = 0; q < NL; ++q)
-                    v[q] = mt_scale_bytes(src[q], 16 * grp, n_sf, p.c.vec, q ? p.c.sfb : p.c.sfw,
-                                          q ? p.c.sfb_end : p.c.sfw_end);
+                for (int q = 1; q < NL; ++q)
+                    v[q] = mt_scale_bytes(src[q], 16 * grp, n_sf, p.c.vec_b, p.c.sfb, p.c.sfb_end);
             }
             if (++grp > last) enter();
             return true;
@@ -605,8 +605,8 @@ QMM_DEVINL uint32_t mt_max_finite(const uint4& raw) {
     return max_abs_f32<F16>(m);
 }
 
-// Activations to P e4m3 planes [P][R][K] with scales [P][R][K/32], rows taken
-// through src; two lanes hold a block.  P = 1 copies mxfp8 rows.
+// Activations to P e4m3 planes [P][R][K] with scales [P][R][K/32 rounded
+// up to 16], rows taken through src; two lanes hold a block.  P = 1 copies mxfp8 rows.
 template <int T, int P>
 __global__ void __launch_bounds__(128) mx_planes_kernel(const void* x, const uint8_t* xs, uint8_t* planes,
                                                         uint8_t* scales, const uint32_t* src, int x_rows, int R,
@@ -617,6 +617,17 @@ __global__ void __launch_bounds__(128) mx_planes_kernel(const void* x, const uin
     const int g = K / 16, c = blockIdx.x * blockDim.x + threadIdx.x;
     const bool in = c < g;  // whole blocks of 32 are in or out
     const long long plane = (long long)R * g;
+    const int n_sf = K / 32, pitch = (n_sf + 15) & ~15;
+    // scale byte of plane q of a row's block, by the first lane of two; the last block's clears the rest of the row
+    auto put_scale = [&](int q, long long row, uint32_t byte) {
+        if (c & 1) return;
+        uint8_t* to = scales + ((long long)q * R + row) * pitch;
+        to[c >> 1] = (uint8_t)byte;
+        if (c + 2 == g) {
+#pragma unroll 1
+            for (int j = n_sf; j < pitch; ++j) to[j] = 0;
+        }
+    };
     for (int r0 = blockIdx.y * RUN; r0 < R; r0 += gridDim.y * RUN) {
         long long from[RUN];
 #pragma unroll
@@ -646,7 +657,7 @@ __global__ void __launch_bounds__(128) mx_planes_kernel(const void* x, const uin
             if constexpr (P == 1) {
                 if (!live) continue;
                 out[0] = raw[k][0];
-                if ((c & 1) == 0) scales[i >> 1] = (uint8_t)e[k];
+                put_scale(0, r0 + k, e[k]);
             } else {
                 if constexpr (T == MX_BF16) {
                     uint4 two[2];
@@ -655,10 +666,8 @@ __global__ void __launch_bounds__(128) mx_planes_kernel(const void* x, const uin
                         if (!live) continue;
                         out[0] = two[0];
                         out[plane] = two[1];
-                        if ((c & 1) == 0) {
-                            scales[i >> 1] = (uint8_t)byte;
-                            scales[(plane + i) >> 1] = (uint8_t)(byte - 4);
-                        }
+                        put_scale(0, r0 + k, byte);
+                        put_scale(1, r0 + k, byte - 4);
                         continue;
                     }
                 }
@@ -672,7 +681,7 @@ __global__ void __launch_bounds__(128) mx_planes_kernel(const void* x, const uin
 #pragma unroll
                 for (int q = 0; q < P; ++q) {
                     out[q * plane] = make_uint4(lo[q].x, lo[q].y, hi[q].x, hi[q].y);
-                    if ((c & 1) == 0) scales[(q * plane + i) >> 1] = (uint8_t)bytes[q];
+                    put_scale(q, r0 + k, bytes[q]);
                 }
             }
         }
@@ -727,7 +736,7 @@ TcLayout tc_layout(long long rows, long long N, long long K, bool mx, bool f16, 
         return o;
     };
     l.planes = take(mx && !grouped ? 0 : (size_t)P * rows * K);
-    l.scales = take(mx && !grouped ? 0 : (size_t)P * rows * (K / 32));
+    l.scales = take(mx && !grouped ? 0 : (size_t)P * rows * mx_plane_row(K));
     const TcSplit d = tc_split(rows, N, K, grouped);
     l.partial = take(d.split > 1 ? (size_t)d.split * rows * N * 4 : 0);
     l.bytes = at;
@@ -790,8 +799,10 @@ int launch_mx_tc(const MxMatmul& a, const int4* items, const int32_t* n_items, c
     p.c.KB = (int)((a.K + 127) / 128);
     p.c.n_tiles = (int)((a.N + qmm::MT_W - 1) / qmm::MT_W);
     p.c.sfw_end = a.ws + a.E * a.N * (a.K / 32);
-    p.c.sfb_end = p.c.sfb + P * (in_place ? a.x_rows : a.rows) * (a.K / 32);
-    p.c.vec = mx_scale_vec(a.K, p.c.sfw, p.c.sfb);
+    p.c.sfb_row = (int)(in_place ? a.K / 32 : mx_plane_row(a.K));
+    p.c.sfb_end = p.c.sfb + P * (in_place ? a.x_rows : a.rows) * p.c.sfb_row;
+    p.c.vec_w = mx_scale_vec(a.K, a.ws);
+    p.c.vec_b = in_place ? mx_scale_vec(a.K, a.xs) : 16;
     p.ids = ids;
     p.E = (int)a.E;
     const TcSplit d = tc_split(a.rows, a.N, a.K, grouped);

@@ -206,6 +206,29 @@ def test_mx_matmul(ops, M, N, K, dtype):
     check_product(y, xv, wv, dtype == "f16")
 
 
+@pytest.mark.parametrize("kind", ["bf16", "f16", "mx"])
+@pytest.mark.parametrize("M,N,K", [(70, 300, 96), (193, 257, 4128), (400, 640, 2880), (90, 200, 8224), (17, 515, 2080),
+                                   (65, 2500, 1056), (1000, 100, 32)])
+def test_widths_of_many_rows(ops, M, N, K, kind):
+    """Widths that end inside a k-block, parts of K that meet, rows of scale bytes on odd addresses."""
+    rng = np.random.default_rng(M + N + K)
+    w, s, wv = _mx.random_weights(rng, (N + 1, K))
+    s[0] = s[3] = 255  # outside of the slice, and a row of its own
+    w, s = dev(w)[1:], dev(s)[1:]
+    if kind == "mx":
+        xq, xs, xv = _mx.random_weights(rng, (M + 1, K), 8, 1.0)
+        xs[0] = 255
+        y = ops.mx_matmul(dev(xq)[1:], dev(xs)[1:], w, s)
+        xv = xv[1:]
+    else:
+        x = activations(rng, M, K, kind)
+        y = ops.quantized_matmul(x, w, s, None, group_size=32, bits=4, mode="mxfp4")
+        xv = host(x)
+    assert y[:, 2].isnan().all()
+    keep = [n for n in range(N) if n != 2]
+    check_product(y[:, keep], xv, wv[1:][keep], kind == "f16")
+
+
 @pytest.mark.parametrize("dtype", ["bf16", "f16"])
 @pytest.mark.parametrize("M", [1, 7, 40, 300])
 def test_product_range(ops, M, dtype):
@@ -343,7 +366,7 @@ IDS = {
 @pytest.mark.parametrize("sort", [False, True])
 @pytest.mark.parametrize("rows,E,N,K,dtype", [
     (1, 1, 8, 32, "bf16"), (10, 16, 128, 256, "bf16"), (10, 4, 72, 96, "f16"), (40, 8, 256, 512, "f16"),
-    (64, 64, 200, 128, "bf16"), (300, 3, 130, 640, "bf16"), (700, 8, 256, 256, "f16"),
+    (64, 64, 200, 128, "bf16"), (300, 3, 130, 640, "bf16"), (700, 8, 256, 256, "f16"), (300, 3, 130, 672, "f16"),
 ])
 def test_gather_qmm(ops, rows, E, N, K, dtype, sort, kind):
     rng = np.random.default_rng(rows + E + N + K)
@@ -365,7 +388,7 @@ def test_gather_qmm(ops, rows, E, N, K, dtype, sort, kind):
 
 
 @pytest.mark.parametrize("sort", [False, True])
-@pytest.mark.parametrize("rows,E,N,K", [(10, 16, 128, 256), (90, 8, 72, 96), (500, 4, 256, 384)])
+@pytest.mark.parametrize("rows,E,N,K", [(10, 16, 128, 256), (90, 8, 72, 96), (500, 4, 256, 384), (500, 4, 136, 1056)])
 def test_mx_matmul_grouped(ops, rows, E, N, K, sort):
     rng = np.random.default_rng(rows)
     w, s, wv = _mx.random_weights(rng, (E, N, K))
