@@ -364,8 +364,13 @@ QMM_API int qmm_mx_rms_norm(const void* x, const void* residual, const void* wei
  * [N, K/32] and fp32 accumulation (mx.quantized_matmul with mode="mxfp4").
  * x is [M, K] of dtype when x_scales is NULL, else mxfp8: words [M, K/4] and
  * x_scales [M, K/32].
+ * Activations of dtype are held to 2^-21 (or better) of the largest value of
+ * their block of 32 along K; mxfp8 ones exactly.  A row with an infinity or a
+ * NaN gives NaN; where a few rows share a launch, magnitudes of 2^127 and above
+ * count as infinite.  Equal calls give equal bits.
  * workspace: qmm_mx_matmul_workspace_size bytes of device scratch, 256-byte
- * aligned (NULL when that is 0), with no requirement on its content.
+ * aligned (NULL when that is 0), with no requirement on its content; not shared
+ * by calls that run at the same time.  M < 2^31 / 3.
  */
 QMM_API size_t qmm_mx_matmul_workspace_size(int64_t M, int64_t N, int64_t K, int dtype, int x_is_mx);
 QMM_API int qmm_mx_matmul(const void* x, const uint8_t* x_scales, const uint32_t* w, const uint8_t* scales, void* y,
@@ -378,7 +383,7 @@ QMM_API int qmm_mx_matmul(const void* x, const uint8_t* x_scales, const uint32_t
  * scales [E, N, K/32], x of x_rows rows, lhs int32 [rows] or NULL (row r).
  * sorted != 0 promises that rhs is non-decreasing; otherwise rows are sorted
  * by expert on the device first.  Rows whose expert is outside [0, E) become
- * zero.  rows, x_rows <= 2^30, E <= 16384.
+ * zero.  rows < 2^31 / 3, x_rows <= 2^30, E <= 16384.
  */
 QMM_API size_t qmm_mx_gather_workspace_size(int64_t rows, int64_t E, int64_t N, int64_t K, int dtype, int x_is_mx,
                                             int sorted);

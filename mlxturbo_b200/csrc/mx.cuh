@@ -129,10 +129,9 @@ QMM_DEVINL uint32_t max_abs_f32(uint32_t two) {
     else return m << 16;
 }
 
-// Four lanes of a warp hold a block, eight values each: quantise and store the
-// words and (the first of the four) the scale byte.  `o8` counts groups of
+// Four lanes of a warp hold a block, eight values each: to mxfp8, words and (by
+// the first of the four) scale byte.  `o8` counts groups of
 // eight values; lanes with `in` false only take part in the shuffles.
-template <int BITS>
 QMM_DEVINL void mx_store_block(const float (&v)[8], uint32_t* words, uint8_t* scales, long long o8, bool in) {
     uint32_t m = 0;
 #pragma unroll
@@ -140,18 +139,14 @@ QMM_DEVINL void mx_store_block(const float (&v)[8], uint32_t* words, uint8_t* sc
     m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
     m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
     float inv;
-    const uint32_t byte = mx_scale_byte<BITS == 4 ? 2 : 8>(m, inv);
+    const uint32_t byte = mx_scale_byte<8>(m, inv);
     if (!in) return;
     float s[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) s[j] = byte == 255u ? 0.0f : v[j] * inv;
-    if constexpr (BITS == 4) {
-        words[o8] = cvt8_e2m1(s);
-    } else {
-        const uint32_t lo = cvt2_e4m3(s[0], s[1]) | (cvt2_e4m3(s[2], s[3]) << 16);
-        const uint32_t hi = cvt2_e4m3(s[4], s[5]) | (cvt2_e4m3(s[6], s[7]) << 16);
-        reinterpret_cast<uint2*>(words)[o8] = make_uint2(lo, hi);
-    }
+    const uint32_t lo = cvt2_e4m3(s[0], s[1]) | (cvt2_e4m3(s[2], s[3]) << 16);
+    const uint32_t hi = cvt2_e4m3(s[4], s[5]) | (cvt2_e4m3(s[6], s[7]) << 16);
+    reinterpret_cast<uint2*>(words)[o8] = make_uint2(lo, hi);
     if ((o8 & 3) == 0) scales[o8 >> 2] = (uint8_t)byte;
 }
 

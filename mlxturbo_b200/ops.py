@@ -182,11 +182,12 @@ def quantized_matmul(x: torch.Tensor, w: torch.Tensor, scales: torch.Tensor, bia
     same C ABI entry and raise the same exception types.
 
     mode="mxfp4" (group_size=32, bits=4, biases=None): w holds e2m1 codes and
-    scales uint8 [N, K/32].  bf16 activations enter without rounding, fp16 ones
-    too, as long as a value is no more than 2^14 below the largest of its 32
-    (below that to 2^-21 of that largest value); sums are in fp32.  A row with
-    an infinity or a NaN gives NaN where the product does not depend on it
-    alone.
+    scales uint8 [N, K/32].  Activations enter the products without rounding
+    as long as a value is not far below the largest of its block of 32 (along
+    K): each is held to 2^-21 of that largest value at least (bf16 exactly down
+    to 2^-14 of it; fp16 down to 2^-11 of it in calls of a few rows, to 2^-14 in
+    others).  Sums are in fp32.  A row with an infinity or a NaN gives NaN;
+    in calls of a few rows magnitudes of 2^127 and above count as infinite.
     """
     if mode != "affine" and mode in _MX_BITS:
         _check_mx_weight(mode, group_size, bits, biases, transpose)
@@ -510,7 +511,9 @@ def mx_matmul(xq: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor, scales:
 
     xq int32 [..., K/4] and x_scales uint8 [..., K/32] as ``quantize`` (mode
     "mxfp8") or ``rms_norm_quantize`` make them, w int32 [N, K/8] and scales
-    uint8 [N, K/32] of mode "mxfp4"; the result [..., N] has `dtype`.
+    uint8 [N, K/32] of mode "mxfp4"; the result [..., N] has `dtype`.  Codes
+    enter exactly; a block whose scale byte is 255 (in calls of a few rows: above
+    245, values of 2^127 and more) makes its row NaN.
 
     With rhs_indices [rows] the weights are a bank [E, N, K/8] and row r of the
     result [rows, N] is row lhs_indices[r] (r without lhs_indices) of the
