@@ -19,6 +19,7 @@
 // calls these directly and leaves every check to them.
 
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/library.h>
 #include <torch/types.h>
@@ -91,6 +92,13 @@ at::Tensor& decode_workspace(const at::Device& device, size_t bytes) {
         buf = at::zeros({(int64_t)size}, at::TensorOptions().dtype(at::kByte).device(device));
     }
     return buf;
+}
+
+// A new tensor on the device of `like`, allocated without another pass through
+// the dispatcher (about 0.3 us each: a norm and a dequantisation, four tensors,
+// take 14.0 us of host time, with at::empty 14.9).
+at::Tensor empty_like_device(at::IntArrayRef shape, at::ScalarType dtype, const at::Tensor& like) {
+    return at::detail::empty_cuda(shape, dtype, like.device(), std::nullopt);
 }
 
 at::Tensor contiguous16(const at::Tensor& t) {
@@ -203,7 +211,7 @@ int64_t mx_check_words(const char* what, const char* name, const at::Tensor& w, 
 
 at::Tensor mx_scratch(const at::Tensor& like, size_t bytes) {
     if (!bytes) return at::Tensor();
-    return at::empty({(int64_t)bytes + 256}, at::TensorOptions().dtype(at::kByte).device(like.device()));
+    return empty_like_device({(int64_t)bytes + 256}, at::kByte, like);
 }
 void* mx_scratch_ptr(const at::Tensor& t) {
     return t.defined() ? reinterpret_cast<void*>((reinterpret_cast<uintptr_t>(t.data_ptr()) + 255) & ~(uintptr_t)255)
@@ -222,9 +230,9 @@ std::tuple<at::Tensor, at::Tensor> mx_quantize(const at::Tensor& v_in, int64_t b
     const int64_t K = v.size(-1), rows = v.numel() / K;
     std::vector<int64_t> shape(v.sizes().begin(), v.sizes().end());
     shape.back() = K * bits / 32;
-    at::Tensor w = at::empty(shape, v.options().dtype(at::kInt));
+    at::Tensor w = empty_like_device(shape, at::kInt, v);
     shape.back() = K / 32;
-    at::Tensor s = at::empty(shape, v.options().dtype(at::kByte));
+    at::Tensor s = empty_like_device(shape, at::kByte, v);
     check(qmm_mx_quantize(v.data_ptr(), static_cast<uint32_t*>(w.data_ptr()), static_cast<uint8_t*>(s.data_ptr()),
                           rows, K, (int)bits, dt, at::cuda::getCurrentCUDAStream(v.device().index()).stream()),
           "quantize");
@@ -240,7 +248,7 @@ at::Tensor mx_dequantize(const at::Tensor& w_in, const at::Tensor& s_in, int64_t
     const at::Tensor w = contiguous16(w_in), s = s_in.contiguous();
     std::vector<int64_t> shape(w.sizes().begin(), w.sizes().end());
     shape.back() = K;
-    at::Tensor out = at::empty(shape, w.options().dtype(dtype));
+    at::Tensor out = empty_like_device(shape, dtype, w);
     if (out.numel() == 0) return out;
     check(qmm_mx_dequantize(static_cast<const uint32_t*>(w.data_ptr()), static_cast<const uint8_t*>(s.data_ptr()),
                             out.data_ptr(), out.numel() / K, K, (int)bits, dt,
@@ -269,13 +277,13 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> mx_rms_norm(const at::Tensor& x_i
     at::Tensor r, h;
     if (res) {
         r = contiguous16(*res_in);
-        h = at::empty(x.sizes(), x.options());
+        h = empty_like_device(x.sizes(), x.scalar_type(), x);
     }
     std::vector<int64_t> shape(x.sizes().begin(), x.sizes().end());
     shape.back() = K / 4;
-    at::Tensor xq = at::empty(shape, x.options().dtype(at::kInt));
+    at::Tensor xq = empty_like_device(shape, at::kInt, x);
     shape.back() = K / 32;
-    at::Tensor xs = at::empty(shape, x.options().dtype(at::kByte));
+    at::Tensor xs = empty_like_device(shape, at::kByte, x);
     check(qmm_mx_rms_norm(x.data_ptr(), res ? r.data_ptr() : nullptr, weight.data_ptr(), res ? h.data_ptr() : nullptr,
                           static_cast<uint32_t*>(xq.data_ptr()), static_cast<uint8_t*>(xs.data_ptr()), rows, K,
                           (float)eps, dt, at::cuda::getCurrentCUDAStream(x.device().index()).stream()),
@@ -311,7 +319,7 @@ at::Tensor run_mx_matmul(const at::Tensor& x_in, const std::optional<at::Tensor>
             fail(Err::kValue, "out must be a contiguous, 16-byte aligned tensor of the result shape %s and dtype",
                  dims(at::IntArrayRef(shape)).c_str());
     } else {
-        y = at::empty(shape, x.options().dtype(dtype));
+        y = empty_like_device(shape, dtype, x);
     }
     if (M == 0) return y;
     const size_t need = qmm_mx_matmul_workspace_size(M, N, K, dt, mx);
@@ -358,7 +366,7 @@ at::Tensor mx_gather(const at::Tensor& x_in, const std::optional<at::Tensor>& xs
     const at::Tensor x = contiguous16(x_in), w = contiguous16(w_in), s = s_in.contiguous(), rhs = rhs_in.contiguous();
     const at::Tensor xs = mx ? xs_in->contiguous() : at::Tensor(), l = lhs ? lhs_in->contiguous() : at::Tensor();
     const int64_t rows = rhs.size(0);
-    at::Tensor y = one ? at::empty({rows, 1, N}, x.options().dtype(dtype)) : at::empty({rows, N}, x.options().dtype(dtype));
+    at::Tensor y = one ? empty_like_device({rows, 1, N}, dtype, x) : empty_like_device({rows, N}, dtype, x);
     if (rows == 0) return y;
     const size_t need = qmm_mx_gather_workspace_size(rows, E, N, K, dt, mx, sorted);
     const at::Tensor ws = mx_scratch(x, need);
