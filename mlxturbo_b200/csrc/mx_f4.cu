@@ -36,6 +36,7 @@
 // persistent over tiles.
 
 #include "mx_mma.cuh"
+#include "mx_ring.cuh"
 
 namespace qmm {
 
@@ -339,12 +340,7 @@ __global__ void __launch_bounds__(C::THREADS, 1)
     if (warp != 0 || p.c.items) pdl_wait();
     const F4Walk walk(p, rank);
     const int k0 = walk.k0, k1 = walk.k1;
-    // The ring in use.  With a whole number of tiles in it, a slot holds the
-    // same k-block of one tile after another: own planes made for an item's
-    // first `fresh` tiles serve all of its tiles.
-    const int nk = k1 - k0;
-    const int L = C::OWN && nk <= STAGES ? STAGES - STAGES % nk : STAGES;
-    const int fresh = C::OWN && nk <= STAGES ? L / nk : 0x7fffffff;
+    const int nk = k1 - k0, L = f4_ring_slots(C::OWN, nk, STAGES), fresh = f4_ring_fresh(C::OWN, nk, STAGES);
 
     if (warp == 0) {
         // ---------------- TMA ----------------
@@ -705,19 +701,20 @@ __global__ void __launch_bounds__(C::THREADS, 1)
                 for (int c = 0; c < 4; ++c)
                     four |= __shfl_sync(0xffffffffu, g.byte, (lane & 16) + 4 * c) << (8 * c);
             }
-            // A wait tells two phases of a slot apart, not three: a warp that
-            // had nothing to do for more than a ring first lets the MMA warp
-            // come within one (it then holds that i - 2 L was consumed, and it
-            // cannot pass i without this warp).
-            bool ok = true;
+            // a warp that had nothing to do for more than a ring first lets the
+            // MMA warp come within one (which it can without this warp)
+            bool gone = false;
             if (i - seen > L) {
                 int tries = 0;
-                while (*reached < i - L && ok) {
+                while (!f4_ring_may_wait(*reached, i, L) && !*abort) {
                     __nanosleep(100);
-                    ok = !*abort && ++tries < (1 << 20);
+                    if (++tries < (1 << 20)) continue;
+                    *abort = 1;
+                    atomicCAS(&g_mx_error, 0, 2048);
                 }
+                gone = __any_sync(0xffffffffu, *abort);
             }
-            if (!ok || !mt_wait(empty(s), ((uint32_t)turn & 1u) ^ 1u, abort, 512)) break;
+            if (gone || !mt_wait(empty(s), ((uint32_t)turn & 1u) ^ 1u, abort, 512)) break;
             seen = i;
             if (st[0].live) {
                 const uint32_t b =
