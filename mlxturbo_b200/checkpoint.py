@@ -134,8 +134,17 @@ class QuantConfig:
             return self.group_size, self.bits
         return int(o.get("group_size", self.group_size)), int(o.get("bits", self.bits))
 
-    def mode_for_layer(self, prefix: str) -> str:
-        return self.overrides.get(prefix, {}).get("mode", self.mode)
+    def mode_for_layer(self, prefix: str, biases: bool = True) -> str:
+        """The layer's mode; `biases`: whether the layer has such a tensor.
+
+        An override stands for the whole of a layer's settings in MLX, whose mode
+        defaults to affine whatever the model's.  A layer without biases cannot be
+        affine and takes the model's.
+        """
+        o = self.overrides.get(prefix)
+        if o is None or not (biases or "mode" in o):
+            return self.mode
+        return o.get("mode", "affine")
 
 
 def quantized_prefixes(tensors: dict[str, torch.Tensor]) -> list[str]:
@@ -209,7 +218,7 @@ def load_model_dir(model_dir: str, device=None) -> tuple[dict[str, torch.nn.Modu
         for prefix in quantized_prefixes(t):
             gs, bits = qc.for_layer(prefix)
             load = load_switch_linear if t[f"{prefix}.weight"].dim() == 3 else load_quantized_linear
-            layers[prefix] = load(t, prefix, gs, bits, device=device, mode=qc.mode_for_layer(prefix))
+            layers[prefix] = load(t, prefix, gs, bits, device=device, mode=qc.mode_for_layer(prefix, f"{prefix}.biases" in t))
     return layers, qc
 
 
