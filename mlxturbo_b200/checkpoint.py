@@ -42,6 +42,8 @@ _DTYPES = {
 _TORCH_TO_ST = {torch.bfloat16: "BF16", torch.float16: "F16", torch.float32: "F32", torch.int32: "I32",
                 torch.int64: "I64", torch.uint8: "U8", torch.int8: "I8", torch.bool: "BOOL"}
 
+_HALF = {"bfloat16": torch.bfloat16, "float16": torch.float16}
+
 
 def read_header(path: str) -> tuple[dict, int]:
     """(header dict, byte offset of the data section)."""
@@ -113,9 +115,12 @@ def write_safetensors(path: str, tensors: dict[str, torch.Tensor], metadata: dic
 
 
 class QuantConfig:
-    """config.json's "quantization": default group_size/bits plus per-prefix overrides."""
+    """config.json's "quantization": default group_size/bits plus per-prefix overrides.
 
-    def __init__(self, quantization: dict | None):
+    ``dtype``: the model's own ("torch_dtype" or "dtype") where it is a 16-bit one, else None."""
+
+    def __init__(self, quantization: dict | None, dtype: torch.dtype | None = None):
+        self.dtype = dtype
         q = dict(quantization or {})
         self.group_size = int(q.pop("group_size", 64))
         self.bits = int(q.pop("bits", 4))
@@ -126,7 +131,8 @@ class QuantConfig:
     def from_model_dir(cls, model_dir: str) -> "QuantConfig":
         with open(os.path.join(model_dir, "config.json")) as f:
             cfg = json.load(f)
-        return cls(cfg.get("quantization") or cfg.get("quantization_config"))
+        dtype = _HALF.get(str(cfg.get("torch_dtype") or cfg.get("dtype")))
+        return cls(cfg.get("quantization") or cfg.get("quantization_config"), dtype)
 
     def for_layer(self, prefix: str) -> tuple[int, int]:
         o = self.overrides.get(prefix)
@@ -165,17 +171,26 @@ def _check(prefix: str, w: torch.Tensor, s: torch.Tensor, b: torch.Tensor | None
     return K
 
 
+def _layer_dtype(s: torch.Tensor, bias: torch.Tensor | None, mode: str, dtype: torch.dtype | None) -> torch.dtype:
+    if mode == "affine":
+        return s.dtype
+    if dtype is None and bias is not None and bias.dtype in _HALF.values():
+        return bias.dtype
+    return dtype or torch.bfloat16
+
+
 def load_quantized_linear(tensors: dict[str, torch.Tensor], prefix: str, group_size: int = 64, bits: int = 4,
-                          device=None, mode: str = "affine", dtype=torch.bfloat16) -> QuantizedLinear:
+                          device=None, mode: str = "affine", dtype: torch.dtype | None = None) -> QuantizedLinear:
     """A QuantizedLinear from `<prefix>.weight/.scales/.biases` (+ `.bias` if present).
 
-    `dtype` is the activations' of an mxfp4 layer; an affine one's is its scales'."""
+    `dtype` is the activations' of an mxfp4 layer (default: the bias's if 16-bit, else
+    bfloat16); an affine one's is its scales'."""
     w, s, b = tensors[f"{prefix}.weight"], tensors[f"{prefix}.scales"], tensors.get(f"{prefix}.biases")
     K = _check(prefix, w, s, b, group_size, bits, mode)
     dev = device if device is not None else w.device
     bias = tensors.get(f"{prefix}.bias")
     layer = QuantizedLinear(K, w.shape[0], bias is not None, group_size, bits, mode,
-                            dtype=s.dtype if mode == "affine" else dtype, device=dev)
+                            dtype=_layer_dtype(s, bias, mode, dtype), device=dev)
     layer.weight.copy_(w.view(torch.int32))
     layer.scales.copy_(s)
     if b is not None:
@@ -186,14 +201,14 @@ def load_quantized_linear(tensors: dict[str, torch.Tensor], prefix: str, group_s
 
 
 def load_switch_linear(tensors: dict[str, torch.Tensor], prefix: str, group_size: int = 64, bits: int = 4,
-                       device=None, mode: str = "affine", dtype=torch.bfloat16) -> QuantizedSwitchLinear:
+                       device=None, mode: str = "affine", dtype: torch.dtype | None = None) -> QuantizedSwitchLinear:
     """A QuantizedSwitchLinear (expert bank, leading E axis) from its tensors."""
     w, s, b = tensors[f"{prefix}.weight"], tensors[f"{prefix}.scales"], tensors.get(f"{prefix}.biases")
     K = _check(prefix, w, s, b, group_size, bits, mode)
     dev = device if device is not None else w.device
     bias = tensors.get(f"{prefix}.bias")
     layer = QuantizedSwitchLinear(K, w.shape[1], w.shape[0], bias is not None, group_size, bits, mode,
-                                  dtype=s.dtype if mode == "affine" else dtype, device=dev)
+                                  dtype=_layer_dtype(s, bias, mode, dtype), device=dev)
     layer.weight.copy_(w.view(torch.int32))
     layer.scales.copy_(s)
     if b is not None:
@@ -203,11 +218,14 @@ def load_switch_linear(tensors: dict[str, torch.Tensor], prefix: str, group_size
     return layer
 
 
-def load_model_dir(model_dir: str, device=None) -> tuple[dict[str, torch.nn.Module], QuantConfig]:
+def load_model_dir(model_dir: str, device=None,
+                   dtype: torch.dtype | None = None) -> tuple[dict[str, torch.nn.Module], QuantConfig]:
     """Every quantized layer of an MLX model directory (*.safetensors + config.json).
 
     Returns {prefix: QuantizedLinear or QuantizedSwitchLinear} (a 3-D weight is
-    an expert bank) and the quantization config.
+    an expert bank) and the quantization config.  `dtype` is the activations' of
+    its mxfp4 layers (default: the model's, else the bias's if 16-bit, else
+    bfloat16).
     """
     qc = QuantConfig.from_model_dir(model_dir)
     layers: dict[str, torch.nn.Module] = {}
@@ -218,7 +236,8 @@ def load_model_dir(model_dir: str, device=None) -> tuple[dict[str, torch.nn.Modu
         for prefix in quantized_prefixes(t):
             gs, bits = qc.for_layer(prefix)
             load = load_switch_linear if t[f"{prefix}.weight"].dim() == 3 else load_quantized_linear
-            layers[prefix] = load(t, prefix, gs, bits, device=device, mode=qc.mode_for_layer(prefix, f"{prefix}.biases" in t))
+            layers[prefix] = load(t, prefix, gs, bits, device=device,
+                                  mode=qc.mode_for_layer(prefix, f"{prefix}.biases" in t), dtype=dtype or qc.dtype)
     return layers, qc
 
 

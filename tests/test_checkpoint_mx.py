@@ -55,3 +55,25 @@ def test_mode_that_the_tensors_contradict(tmp_path):
         ck.load_model_dir(model_dir(tmp_path, {"group_size": 32, "bits": 4}, mx_layer("a")))
     with pytest.raises(ValueError):
         ck.load_model_dir(model_dir(tmp_path, {**MX, "b": dict(MX)}, affine_layer("b", bits=4, group=32)))
+
+
+@pytest.mark.parametrize("config", [{"torch_dtype": "float16"}, {"dtype": "float16"}, {}])
+def test_layers_of_an_fp16_model(tmp_path, config):
+    """mxfp4 tensors do not say the activations' type: the model does, or the bias, which keeps its bits."""
+    bias = (torch.randn(64, generator=torch.Generator().manual_seed(1)) / 3).half()
+    t = {**mx_layer("a"), "a.bias": bias, **mx_layer("b"), **affine_layer("c", dtype=torch.float16)}
+    layers, _ = ck.load_model_dir(model_dir(tmp_path, {**MX, "c": {"group_size": 64, "bits": 8}}, t, **config))
+    assert layers["a"].bias.dtype == torch.float16 and torch.equal(layers["a"].bias.data, bias)
+    assert layers["a"].dtype == torch.float16 and layers["c"].scales.dtype == torch.float16
+    assert layers["b"].dtype == (torch.float16 if config else torch.bfloat16)
+    layers, _ = ck.load_model_dir(model_dir(tmp_path, {**MX, "c": {"group_size": 64, "bits": 8}}, t, **config),
+                                  dtype=torch.bfloat16)
+    assert layers["a"].dtype == layers["a"].bias.dtype == layers["b"].dtype == torch.bfloat16
+
+
+def test_dtype_of_one_layer():
+    t = {**mx_layer("a"), "a.bias": torch.zeros(64, dtype=torch.float16)}
+    assert ck.load_quantized_linear(t, "a", 32, 4, mode="mxfp4").dtype == torch.float16
+    assert ck.load_quantized_linear(t, "a", 32, 4, mode="mxfp4", dtype=torch.bfloat16).dtype == torch.bfloat16
+    t["a.bias"] = t["a.bias"].float()
+    assert ck.load_quantized_linear(t, "a", 32, 4, mode="mxfp4").dtype == torch.bfloat16
