@@ -22,14 +22,22 @@ def _quantized_buffers(module: nn.Module, lead: tuple, input_dims: int, dtype, d
         raise NotImplementedError(f"mode={module.mode!r} with group_size={group_size} bits={bits}: layers have affine "
                                   "weights, or mxfp4 ones with group_size=32 and bits=4")
     affine = module.mode == "affine"
-    module.dtype = dtype
     module.register_buffer("weight", torch.zeros((*lead, input_dims * bits // 32), dtype=torch.int32, device=device))
     module.register_buffer("scales", torch.zeros((*lead, input_dims // group_size),
                                                  dtype=dtype if affine else torch.uint8, device=device))
     module.register_buffer("biases", torch.zeros_like(module.scales) if affine else None)
+    # empty: the type of an mxfp4 layer's activations, which follows the module's (half(), to())
+    module.register_buffer("_like", None if affine else torch.empty(0, dtype=dtype, device=device), persistent=False)
 
 
-class QuantizedLinear(nn.Module):
+class _Quantized(nn.Module):
+    @property
+    def dtype(self) -> torch.dtype:
+        """The type of activations and outputs."""
+        return self.scales.dtype if self.mode == "affine" else self._like.dtype
+
+
+class QuantizedLinear(_Quantized):
     """y = x @ dequant(weight)^T (+ bias); weight uint32-as-int32 [N, K*bits/32]."""
 
     def __init__(self, input_dims: int, output_dims: int, bias: bool = False, group_size: int = 64, bits: int = 4,
@@ -81,7 +89,7 @@ class RMSNormQuantized(nn.Module):
         return ops.rms_norm_quantize(x, self.weight, self.eps, residual=residual)
 
 
-class QuantizedSwitchLinear(nn.Module):
+class QuantizedSwitchLinear(_Quantized):
     """Expert bank: weight [E, N, K*bits/32]; forward(x, indices, sorted_indices)."""
 
     def __init__(self, input_dims: int, output_dims: int, num_experts: int, bias: bool = False,
