@@ -398,23 +398,34 @@ TORCH_LIBRARY(mlxturbo_b200, m) {
           "-> Tensor");
     m.def("quantized_matmul_out(Tensor x, Tensor w, Tensor scales, Tensor biases, int group_size, int bits, "
           "*, Tensor(a!) out) -> Tensor(a!)");
-    m.def("mx_quantize(Tensor v, int bits) -> (Tensor, Tensor)", &mx_quantize);
-    m.def("mx_dequantize(Tensor w, Tensor scales, int bits, ScalarType dtype) -> Tensor", &mx_dequantize);
-    m.def("mx_rms_norm(Tensor x, Tensor? residual, Tensor weight, float eps) -> (Tensor, Tensor, Tensor)",
-          &mx_rms_norm);
-    m.def("mx_matmul(Tensor x, Tensor? x_scales, Tensor w, Tensor scales, ScalarType dtype) -> Tensor", &mx_matmul);
-    m.def("mx_matmul_out(Tensor x, Tensor? x_scales, Tensor w, Tensor scales, *, Tensor(a!) out) -> Tensor(a!)",
-          &mx_matmul_out);
+    m.def("mx_quantize(Tensor v, int bits) -> (Tensor, Tensor)");
+    m.def("mx_dequantize(Tensor w, Tensor scales, int bits, ScalarType dtype) -> Tensor");
+    m.def("mx_rms_norm(Tensor x, Tensor? residual, Tensor weight, float eps) -> (Tensor, Tensor, Tensor)");
+    m.def("mx_matmul(Tensor x, Tensor? x_scales, Tensor w, Tensor scales, ScalarType dtype) -> Tensor");
+    m.def("mx_matmul_out(Tensor x, Tensor? x_scales, Tensor w, Tensor scales, *, Tensor(a!) out) -> Tensor(a!)");
     m.def("mx_gather(Tensor x, Tensor? x_scales, Tensor w, Tensor scales, Tensor? lhs, Tensor rhs, ScalarType dtype, "
-          "bool sorted) -> Tensor", &mx_gather);
+          "bool sorted) -> Tensor");
+}
+
+// Per device, not for every dispatch key: autograd and the dispatch modes above
+// see the calls.  All-CPU arguments reach the same functions, which refuse them.
+void mx_impl(torch::Library& m) {
+    m.impl("mx_quantize", &mx_quantize);
+    m.impl("mx_dequantize", &mx_dequantize);
+    m.impl("mx_rms_norm", &mx_rms_norm);
+    m.impl("mx_matmul", &mx_matmul);
+    m.impl("mx_matmul_out", &mx_matmul_out);
+    m.impl("mx_gather", &mx_gather);
 }
 
 TORCH_LIBRARY_IMPL(mlxturbo_b200, CUDA, m) {
     m.impl("quantized_matmul", &quantized_matmul);
     m.impl("quantized_matmul_out", &quantized_matmul_out);
+    mx_impl(m);
 }
 
 TORCH_LIBRARY_IMPL(mlxturbo_b200, CPU, m) {
     m.impl("quantized_matmul", &quantized_matmul_cpu);
     m.impl("quantized_matmul_out", &quantized_matmul_out_cpu);
+    mx_impl(m);
 }
