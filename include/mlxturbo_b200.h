@@ -383,7 +383,8 @@ QMM_API int qmm_mx_matmul(const void* x, const uint8_t* x_scales, const uint32_t
  * scales [E, N, K/32], x of x_rows rows, lhs int32 [rows] or NULL (row r).
  * sorted != 0 promises that rhs is non-decreasing; otherwise rows are sorted
  * by expert on the device first.  Rows whose expert is outside [0, E) become
- * zero.  rows < 2^31 / 3, x_rows <= 2^30, E <= 16384.
+ * zero.  rows < 2^31 / 3, x_rows <= 2^30, E <= 16384; unsorted rows / 256 * (E + 1)
+ * < 2^31.
  */
 QMM_API size_t qmm_mx_gather_workspace_size(int64_t rows, int64_t E, int64_t N, int64_t K, int dtype, int x_is_mx,
                                             int sorted);

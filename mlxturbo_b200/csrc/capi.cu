@@ -82,7 +82,7 @@ int launch_ep_pack(const int32_t* ids, int n, int e_local, int world, int top_k,
 int launch_moe_route(const uint32_t* ids, int M, int E, int top_k, int ir, uint32_t* order, uint32_t* idx_s,
                      uint32_t* row_src, uint32_t* inv, int32_t* row_start, int32_t* item_prefix, int4* item_info,
                      cudaStream_t st, const int32_t* lhs = nullptr);
-int launch_sort_rows(const uint32_t* ids, int M, int E, int top_k, uint32_t* order, uint32_t* idx_s,
+int launch_sort_rows(const uint32_t* ids, long long rows, int E, int top_k, uint32_t* order, uint32_t* idx_s,
                      uint32_t* row_src, uint32_t* inv, void* ws, size_t ws_bytes, cudaStream_t st);
 int launch_moe_combine(const uint16_t* out_sorted, long long src_rows, const uint32_t* inv, const float* w,
                        uint16_t* y, int rows, int top_k, int N, bool f16, cudaStream_t st, bool pdl);
@@ -692,7 +692,7 @@ int qmm_sort_rows(const uint32_t* ids, int64_t M, int64_t E, int top_k, uint32_t
         return QMM_EINVAL;
     }
     fire("sort_rows");
-    return launch_sort_rows(ids, (int)M, (int)E, top_k, order, idx_s, row_src, inv, workspace, workspace_bytes,
+    return launch_sort_rows(ids, M, (int)E, top_k, order, idx_s, row_src, inv, workspace, workspace_bytes,
                             as_stream(stream));
 }
 

@@ -588,10 +588,22 @@ int launch_moe_route(const uint32_t* ids, int M, int E, int top_k, int ir, uint3
     return cuda_status(cudaGetLastError(), "moe_route launch");
 }
 
-int launch_sort_rows(const uint32_t* ids, int M, int E, int top_k, uint32_t* order, uint32_t* idx_s,
+// The histogram of (expert, block of rows) is indexed and scanned in ints, a
+// thread block beyond its end.
+bool sort_rows_takes(long long M, long long E) {
+    const long long B = (M + qmm::kSortBlock - 1) / qmm::kSortBlock;
+    return M <= (1LL << 30) && E < (1LL << 30) && (E + 1) * B <= (1LL << 31) - 2048;
+}
+
+int launch_sort_rows(const uint32_t* ids, long long rows, int E, int top_k, uint32_t* order, uint32_t* idx_s,
                      uint32_t* row_src, uint32_t* inv, void* ws, size_t ws_bytes, cudaStream_t st) {
-    if (M == 0) return QMM_OK;
-    const int B = (M + qmm::kSortBlock - 1) / qmm::kSortBlock;
+    if (rows == 0) return QMM_OK;
+    if (!sort_rows_takes(rows, E)) {
+        set_error("sort_rows: M=%lld E=%d: more than 2^31 counts of experts in blocks of %d rows", rows, E,
+                  qmm::kSortBlock);
+        return QMM_EUNSUPPORTED;
+    }
+    const int M = (int)rows, B = (M + qmm::kSortBlock - 1) / qmm::kSortBlock;
     if (ws_bytes < sort_workspace(M, E)) {
         set_error("sort_rows: workspace %zu < %zu bytes", ws_bytes, sort_workspace(M, E));
         return QMM_EINVAL;

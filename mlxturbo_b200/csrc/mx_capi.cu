@@ -8,10 +8,11 @@
 namespace qmm_host {
 size_t sort_workspace(long long M, long long E);
 size_t route_smem(long long M, long long E);
+bool sort_rows_takes(long long M, long long E);
 int launch_moe_route(const uint32_t* ids, int M, int E, int top_k, int ir, uint32_t* order, uint32_t* idx_s,
                      uint32_t* row_src, uint32_t* inv, int32_t* row_start, int32_t* item_prefix, int4* item_info,
                      cudaStream_t st, const int32_t* lhs = nullptr);
-int launch_sort_rows(const uint32_t* ids, int M, int E, int top_k, uint32_t* order, uint32_t* idx_s,
+int launch_sort_rows(const uint32_t* ids, long long rows, int E, int top_k, uint32_t* order, uint32_t* idx_s,
                      uint32_t* row_src, uint32_t* inv, void* ws, size_t ws_bytes, cudaStream_t st);
 int launch_compose(const int32_t* lhs, const uint32_t* order, uint32_t* out, long long n, cudaStream_t st);
 }  // namespace qmm_host
@@ -255,8 +256,9 @@ int qmm_mx_gather(const void* x, const uint8_t* x_scales, const uint32_t* w, con
                   (long long)E);
         return QMM_EINVAL;
     }
-    if (E > 16384 || x_rows > kMaxDim) {
-        set_error("mx_gather: E=%lld x_rows=%lld beyond limits", (long long)E, (long long)x_rows);
+    if (E > 16384 || x_rows > kMaxDim || (!sorted && !route_smem(rows, E) && !sort_rows_takes(rows, E))) {
+        set_error("mx_gather: rows=%lld E=%lld x_rows=%lld beyond limits", (long long)rows, (long long)E,
+                  (long long)x_rows);
         return QMM_EUNSUPPORTED;
     }
     const bool f16 = dtype == QMM_F16, mx = x_scales != nullptr;
@@ -302,8 +304,8 @@ int qmm_mx_gather(const void* x, const uint8_t* x_scales, const uint32_t* w, con
                                   t.idx_s, t.row_src, t.inv, t.row_start, t.item_prefix, t.items, st, lhs);
             n_items = t.item_prefix + E;
         } else {
-            rc = launch_sort_rows(reinterpret_cast<const uint32_t*>(rhs), (int)rows, (int)E, 1, t.order, t.idx_s,
-                                  t.row_src, t.inv, t.sort_ws, t.sort_bytes, st);
+            rc = launch_sort_rows(reinterpret_cast<const uint32_t*>(rhs), rows, (int)E, 1, t.order, t.idx_s, t.row_src,
+                                  t.inv, t.sort_ws, t.sort_bytes, st);
             if (!rc)
                 rc = launch_mx_items(reinterpret_cast<const int32_t*>(t.idx_s), rows, (int)E, t.item_rows, t.row_start,
                                      t.items, t.items_max, t.n_items, st);
