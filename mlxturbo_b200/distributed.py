@@ -87,9 +87,16 @@ def _qmm(x, w, s, b, group_size, bits):
     return ops.quantized_matmul(x, w, s, b, transpose=True, group_size=group_size, bits=bits)
 
 
+def _check_affine(biases) -> None:
+    if biases is None:
+        raise NotImplementedError("the sharded linears take affine weights; weights without biases (mode \"mxfp4\") "
+                                  "are replicated, or split by expert (ExpertParallelSwitchGLU)")
+
+
 class _ShardedBase(nn.Module):
     def __init__(self, weight, scales, biases, bias, group_size, bits, group, matmul):
         super().__init__()
+        _check_affine(biases)
         self.group = group
         self.group_size, self.bits, self.mode = group_size, bits, "affine"
         self.register_buffer("weight", weight.contiguous())
@@ -107,6 +114,7 @@ class QuantizedAllToShardedLinear(_ShardedBase):
 
     @classmethod
     def from_full(cls, weight, scales, biases, bias=None, *, group_size=64, bits=4, group=None, matmul=None):
+        _check_affine(biases)
         rank, world = _group_rank_world(group)
         a, b = shard_range(weight.shape[0], rank, world)
         return cls(weight[a:b], scales[a:b], biases[a:b], None if bias is None else bias[a:b], group_size, bits,
@@ -122,6 +130,7 @@ class QuantizedShardedToAllLinear(_ShardedBase):
 
     @classmethod
     def from_full(cls, weight, scales, biases, bias=None, *, group_size=64, bits=4, group=None, matmul=None):
+        _check_affine(biases)
         rank, world = _group_rank_world(group)
         K = weight.shape[1] * 32 // bits
         a, b = shard_range(K, rank, world)
@@ -147,6 +156,7 @@ class ColumnShardedLMHead(_ShardedBase):
 
     @classmethod
     def from_full(cls, weight, scales, biases, bias=None, *, group_size=64, bits=8, group=None, matmul=None):
+        _check_affine(biases)
         rank, world = _group_rank_world(group)
         a, b = shard_range(weight.shape[0], rank, world)
         return cls(weight[a:b], scales[a:b], biases[a:b], None if bias is None else bias[a:b], group_size, bits,
