@@ -35,6 +35,8 @@
 // the others' sums from its shared memory in the order of k.  Clusters are
 // persistent over tiles.
 
+#include <cmath>
+
 #include "mx_mma.cuh"
 #include "mx_ring.cuh"
 
@@ -963,8 +965,8 @@ int launch_mx_f4(const MxMatmul& a, const int4* items, const int32_t* n_items, c
     double n = (double)f4_items_max(a.rows, a.E, bt, false);
     if (p.direct) n = (double)a.rows;
     else if (grouped) {
-        double miss = 1.0;  // share of experts without a row: (1 - 1/E)^rows
-        for (long long r = 0; r < a.rows && miss > 1e-3; ++r) miss *= 1.0 - 1.0 / (double)a.E;
+        // share of experts without a row: (1 - 1/E)^rows
+        const double miss = a.E > 1 ? std::exp((double)a.rows * std::log1p(-1.0 / (double)a.E)) : 0.0;
         n += (1.0 - miss) * (double)a.E;
         if (n > (double)a.rows) n = (double)a.rows;
     }
