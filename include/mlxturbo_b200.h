@@ -366,8 +366,9 @@ QMM_API int qmm_mx_rms_norm(const void* x, const void* residual, const void* wei
  * x_scales [M, K/32].
  * Activations of dtype are held to 2^-21 (or better) of the largest value of
  * their block of 32 along K; mxfp8 ones exactly.  A row with an infinity or a
- * NaN gives NaN; where a few rows share a launch, magnitudes of 2^127 and above
- * count as infinite.  Equal calls give equal bits.
+ * NaN gives NaN.  In small products (few rows or few outputs) a block below
+ * 2^-103 is held to 2^-126, an mxfp8 value of 2^128 or more counts as infinite,
+ * and results of 2^127 and above may become infinite.  Equal calls give equal bits.
  * workspace: qmm_mx_matmul_workspace_size bytes of device scratch, 256-byte
  * aligned (NULL when that is 0), with no requirement on its content; not shared
  * by calls that run at the same time.  M < 2^31 / 3.

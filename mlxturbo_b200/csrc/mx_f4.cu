@@ -14,8 +14,10 @@
 // activation is held to 2^-22 of the largest of its block of 32 (bf16 exactly
 // down to 2^-14 of it, fp16 to 2^-11, an e4m3 block exactly).  Products and
 // sums are fp32 in TMEM, where a plane is a column; the epilogue adds the
-// eight, small ones first.  Values of 2^127 and above count as infinite, and a
-// block with an infinity or a NaN makes its row NaN.
+// eight, small ones first.  A block below 2^-103 is held to 2^-126, the smallest
+// scale's limit; one with an infinity or a NaN, or with an mxfp8 value of 2^128
+// or more, makes its row NaN.  The first plane's sum may be twice the whole, so
+// results of 2^127 and above may become infinite.
 //
 // 5 rows of 17408x5120 (47 MB) take 13.6 us, 1 of 248320x5120 (675 MB) 115 us,
 // 5.9 TB/s: the difference is ramp and tail, and the kernel that makes the planes.
@@ -68,10 +70,14 @@ QMM_DEVINL void f4_mma(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t
 
 // Eight activations of four lanes' block of 32 as fp32, and the scale byte of
 // the block's first plane (255: not a number) with the factor to 2^22 units.
+// twice: the block reaches 2^127 and 2^128 is no scale.  Its digits are those of
+// half the values, the first plane's codes those of d instead of d / 2, the other
+// planes' scales one up.
 struct F4Group {
     float v[8];
     uint32_t byte;
     float mul;
+    bool twice;
 };
 
 template <int X>
@@ -102,14 +108,21 @@ QMM_DEVINL F4Group f4_group(uint4 raw, uint32_t mx_byte) {
     // values are v * 2^(own - 127); an e4m3 code is below 2^9
     const uint32_t own = X == F4_MX8 ? mx_byte : 127u;
     const uint32_t top = X == F4_MX8 ? own + 9 : (m >> 23) + 1;
-    const bool bad = m >= 0x7F800000u || top > 254u || (X == F4_MX8 && own == 255u);
     // 24: the eighth plane's scale stays above 2^-127 (smaller blocks keep 2^-125)
-    const uint32_t byte = max(top, 24u);
-    g.byte = bad ? 255u : byte;
-    g.mul = bad ? 0.0f : __uint_as_float((127u + 22u + own - byte) << 23);
-    if (bad) {
+    g.byte = max(top, 24u);
+    g.mul = __uint_as_float((127u + 22u + own - g.byte) << 23);
+    g.twice = false;
+    if (m >= 0x7F800000u || top > 254u) {
+        // up to 2^128 after all, by the largest value there is (the smallest code is 2^-9)?
+        const uint32_t most = own + max(m >> 23, 118u) - 126u;
+        const bool good = m < 0x7F800000u && most <= 255u && own != 255u;
+        g.twice = good && most == 255u;
+        g.byte = good ? most - g.twice : 255u;
+        g.mul = good ? __uint_as_float((127u + 22u + own - most) << 23) : 0.0f;
+        if (!good) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) g.v[j] = 0.0f;
+            for (int j = 0; j < 8; ++j) g.v[j] = 0.0f;
+        }
     }
     return g;
 }
@@ -155,6 +168,10 @@ QMM_DEVINL void f4_digits(const F4Group& g, uint32_t (&plane)[8]) {
         const uint32_t u = b[7 - q];
         const uint32_t n = (~u >> 2) & 0x11111111u;
         plane[q] = ((u & 0x33333333u) ^ (3u * n)) + 9u * n;
+    }
+    if (g.twice) {  // codes 0 .. 4 of 0 .. 2 to those of 0 .. 4
+        const uint32_t c = plane[0], M = 0x11111111u;
+        plane[0] = c + (c & ~(c >> 1) & M) + 2u * (((c >> 1) | (c >> 2)) & M);
     }
 }
 
@@ -702,6 +719,11 @@ __global__ void __launch_bounds__(C::THREADS, 1)
 #pragma unroll
                 for (int c = 0; c < 4; ++c)
                     four |= __shfl_sync(0xffffffffu, g.byte, (lane & 16) + 4 * c) << (8 * c);
+                if (const uint32_t twice = __ballot_sync(0xffffffffu, g.twice)) {
+#pragma unroll
+                    for (int c = 0; c < 4; ++c)
+                        four += (lane & 15) ? ((twice >> ((lane & 16) + 4 * c)) & 1u) << (8 * c) : 0u;
+                }
             }
             // a warp that had nothing to do for more than a ring first lets the
             // MMA warp come within one (which it can without this warp)
@@ -800,7 +822,7 @@ __global__ void __launch_bounds__(64) mx_f4_planes_kernel(const void* x, const u
 #pragma unroll
         for (int q = 0; q < F4_PLANES; ++q) {
             to[q * n8] = plane[q];
-            if ((c & 3) == 0) sf[q * pitch] = (uint8_t)f4_plane_scale(g.byte, q);
+            if ((c & 3) == 0) sf[q * pitch] = (uint8_t)(f4_plane_scale(g.byte, q) + (q ? g.twice : 0));
         }
         if (c + 4 == n8 && n8 < 4 * pitch) {  // the last block's first lane: the rest of the rows
 #pragma unroll 1

@@ -185,9 +185,10 @@ def quantized_matmul(x: torch.Tensor, w: torch.Tensor, scales: torch.Tensor, bia
     scales uint8 [N, K/32].  Activations enter the products without rounding
     as long as a value is not far below the largest of its block of 32 (along
     K): each is held to 2^-21 of that largest value at least (bf16 exactly down
-    to 2^-14 of it; fp16 down to 2^-11 of it in calls of a few rows, to 2^-14 in
-    others).  Sums are in fp32.  A row with an infinity or a NaN gives NaN;
-    in calls of a few rows magnitudes of 2^127 and above count as infinite.
+    to 2^-14 of it; fp16 down to 2^-11 of it in small products, those of few rows
+    or few outputs, to 2^-14 in others; a block all below 2^-103, in small
+    products, to 2^-126).  Sums are in fp32; in small products results of 2^127
+    and above may become infinite.  A row with an infinity or a NaN gives NaN.
     """
     if mode != "affine" and mode in _MX_BITS:
         _check_mx_weight(mode, group_size, bits, biases, transpose)
@@ -512,8 +513,9 @@ def mx_matmul(xq: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor, scales:
     xq int32 [..., K/4] and x_scales uint8 [..., K/32] as ``quantize`` (mode
     "mxfp8") or ``rms_norm_quantize`` make them, w int32 [N, K/8] and scales
     uint8 [N, K/32] of mode "mxfp4"; the result [..., N] has `dtype`.  Codes
-    enter exactly; a block whose scale byte is 255 (in calls of a few rows: above
-    245, values of 2^127 and more) makes its row NaN.
+    enter exactly (in small products, those of few rows, to 2^-126 below a scale
+    byte of 15); a block whose scale byte is 255 makes its row NaN, in small
+    products also one with a value of 2^128 or more.
 
     With rhs_indices [rows] the weights are a bank [E, N, K/8] and row r of the
     result [rows, N] is row lhs_indices[r] (r without lhs_indices) of the
