@@ -19,8 +19,9 @@
 // or more, makes its row NaN.  The first plane's sum may be twice the whole, so
 // results of 2^127 and above may become infinite.
 //
-// 5 rows of 17408x5120 (47 MB) take 13.6 us, 1 of 248320x5120 (675 MB) 115 us,
-// 5.9 TB/s: the difference is ramp and tail, and the kernel that makes the planes.
+// 5 rows of 17408x5120 (47 MB) take 13.9 us, 1 of 248320x5120 (675 MB) 115 us,
+// 5.9 TB/s: start and end of the launch, and the kernel that makes the planes,
+// cost every call the same.
 //
 // Eight-bit planes (mx_tc.cu) were tried here first: they need the codes spread
 // to bytes in shared memory, and TMA spreads 8 packed bytes a clock and SM,
