@@ -465,6 +465,95 @@ QMM_API int qmm_stream_read(const void* p, size_t bytes, int blocks, void* sink,
  */
 QMM_API int qmm_copy_kernel(void* dst, const void* src, size_t bytes, void* stream);
 
+/*
+ * Rows of logits.  What follows reads rows of V logits (bf16, fp16 or fp32;
+ * any start that is a multiple of an element, rows `row_stride` elements apart,
+ * at most 2^30 logits a row and 2^26 rows).  The order of a row's tokens is
+ * (logit descending, id ascending), -0 equals +0, and but for the distillation
+ * a NaN counts as -infinity.
+ */
+
+/*
+ * A token a row from a given uniform number u in [0, 1) (sampled counterpart of
+ * qmm_quantized_matmul_argmax; no reference counterpart here, its SpecEngine
+ * samples through mlx-lm).  With w_i = exp((l_i - max) / temperature): kept are
+ * the first top_k tokens of the order (0, or V and more: all); of these, as
+ * long as the mass before a token is below top_p times theirs (the first
+ * always; 1: all); and those with w_i >= min_p (0: all).  ids[r] is the first
+ * id, in the order of ids, at which the kept weights add up to more than u
+ * times their sum.  Temperature 0: the lowest id of the largest logit.  A
+ * logit of -infinity is never drawn; a row of nothing else gives -1.  The ids
+ * are those of 64-bit arithmetic, the same in every call.
+ * Each setting is one number, or (pointer not null) one a row; a row's
+ * temperature <= 0 or NaN is 0, top_k <= 0 all, top_p >= 1 or NaN all and <= 0
+ * the first token, min_p <= 0 or NaN all and >= 1 the largest.
+ */
+QMM_API int qmm_sample(const void* logits, int64_t row_stride, int64_t rows, int64_t V, int dtype, const float* u,
+                       const float* temperature_rows, double temperature, const int32_t* top_k_rows, int64_t top_k,
+                       const float* top_p_rows, double top_p, const float* min_p_rows, double min_p, int64_t* ids,
+                       void* stream);
+
+/*
+ * The k <= 1024 first tokens of a row's order: values [rows, k] (the logits'
+ * dtype), ids [rows, k], and unless null logsumexp [rows], the logarithm of the
+ * sum of exp(l / temperature).
+ */
+QMM_API int qmm_topk(const void* logits, int64_t row_stride, int64_t rows, int64_t V, int dtype, int64_t k,
+                     double temperature, void* values, int64_t* ids, float* logsumexp, void* stream);
+
+/*
+ * Which drafted tokens stand, and the token after them.  logits [B, n + 1, V]
+ * (row i of sequence b at b seq_stride + i row_stride elements) are the
+ * model's at the drafted positions and the one after, draft_logits [B, n, V]
+ * the draft's, draft_ids [B, n] its tokens; an id outside [0, V) ends that
+ * sequence's draft, and rows behind it are not read.  With p and q the softmax
+ * of a position's logits and draft logits over their temperatures (0: all on
+ * the lowest id of the maximum), token i stands while u[b, i] q(id) < p(id).
+ * At the first that does not, a token is drawn as qmm_sample draws, from
+ * u[b, n] and max(p - q, 0); where the draft ends, from p.  tokens [B, n + 1]
+ * are the standing tokens, the drawn one (-1 if every logit there is
+ * -infinity), then -1; accepted [B] counts the standing ones.
+ * `workspace` (16-byte aligned) needs no clearing and is not shared by
+ * concurrent calls.
+ */
+QMM_API size_t qmm_speculative_sample_workspace_size(int64_t B, int64_t n);
+QMM_API int qmm_speculative_sample(const void* logits, int64_t seq_stride, int64_t row_stride,
+                                   const void* draft_logits, int64_t draft_seq_stride, int64_t draft_row_stride,
+                                   int64_t B, int64_t n, int64_t V, int dtype, const int64_t* draft_ids,
+                                   const float* u, const float* temperature_rows, double temperature,
+                                   const float* draft_temperature_rows, double draft_temperature, int64_t* tokens,
+                                   int64_t* accepted, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * Divergence from a teacher's top logits.  teacher_values [rows, k] (k <= 512)
+ * and teacher_ids [rows, k] (int32 or int64 by id_bytes; an id outside [0, V)
+ * is an empty place, an id listed twice adds up).  p are the softmax of the
+ * listed values over `temperature`, or with teacher_logsumexp [rows] (of the
+ * teacher's row over the same temperature) exp(value / temperature -
+ * logsumexp), the rest of 1 being the class of all tokens not listed.
+ * loss [rows] = KL(p || softmax(logits / temperature)).  A row with nothing
+ * listed, or whose logsumexp is -infinity, has loss 0 and gradient 0.
+ * Gradients are with respect to the logits, in their dtype, times row_weight /
+ * grad_loss [rows] (null: 1); a weight of 0 gives zeros.
+ *
+ * qmm_distill_loss writes the loss and, unless null, stats (16 bytes a row,
+ * 16-byte aligned), which qmm_distill_backward takes.  qmm_distill_loss_grad
+ * is both in one launch; grad may be the logits themselves.
+ */
+QMM_API int qmm_distill_loss(const void* logits, int64_t row_stride, int64_t rows, int64_t V, int dtype,
+                             const void* teacher_values, int teacher_dtype, const void* teacher_ids, int id_bytes,
+                             const float* teacher_logsumexp, int64_t k, double temperature, float* loss, void* stats,
+                             void* stream);
+QMM_API int qmm_distill_loss_grad(const void* logits, int64_t row_stride, int64_t rows, int64_t V, int dtype,
+                                  const void* teacher_values, int teacher_dtype, const void* teacher_ids,
+                                  int id_bytes, const float* teacher_logsumexp, int64_t k, double temperature,
+                                  const float* row_weight, float* loss, void* grad, int64_t grad_stride,
+                                  void* stream);
+QMM_API int qmm_distill_backward(const void* logits, int64_t row_stride, int64_t rows, int64_t V, int dtype,
+                                 const void* teacher_values, int teacher_dtype, const void* teacher_ids, int id_bytes,
+                                 const float* teacher_logsumexp, int64_t k, double temperature, const void* stats,
+                                 const float* grad_loss, void* grad, int64_t grad_stride, void* stream);
+
 /* The K-split warp count the decode kernel uses for (N, K) (never depends on M). */
 QMM_API int qmm_qmv_k_warps(int64_t N, int64_t K, int group_size);
 

@@ -23,6 +23,7 @@ _i64 = ctypes.c_int64
 _i = ctypes.c_int
 _sz = ctypes.c_size_t
 _f = ctypes.c_float
+_d = ctypes.c_double
 
 # name -> (restype, argtypes); must match include/mlxturbo_b200.h
 SIGNATURES = {
@@ -64,6 +65,14 @@ SIGNATURES = {
     "qmm_mx_matmul": (_i, [_p, _p, _p, _p, _p, _i64, _i64, _i64, _i, _p, _sz, _p]),
     "qmm_mx_gather_workspace_size": (_sz, [_i64, _i64, _i64, _i64, _i, _i, _i]),
     "qmm_mx_gather": (_i, [_p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i, _i, _p, _sz, _p]),
+    "qmm_sample": (_i, [_p, _i64, _i64, _i64, _i, _p, _p, _d, _p, _i64, _p, _d, _p, _d, _p, _p]),
+    "qmm_topk": (_i, [_p, _i64, _i64, _i64, _i, _i64, _d, _p, _p, _p, _p]),
+    "qmm_speculative_sample_workspace_size": (_sz, [_i64, _i64]),
+    "qmm_speculative_sample": (_i, [_p, _i64, _i64, _p, _i64, _i64, _i64, _i64, _i64, _i, _p, _p, _p, _d, _p, _d, _p,
+                                    _p, _p, _sz, _p]),
+    "qmm_distill_loss": (_i, [_p, _i64, _i64, _i64, _i, _p, _i, _p, _i, _p, _i64, _d, _p, _p, _p]),
+    "qmm_distill_loss_grad": (_i, [_p, _i64, _i64, _i64, _i, _p, _i, _p, _i, _p, _i64, _d, _p, _p, _p, _i64, _p]),
+    "qmm_distill_backward": (_i, [_p, _i64, _i64, _i64, _i, _p, _i, _p, _i, _p, _i64, _d, _p, _p, _p, _i64, _p]),
     "qmm_gather_tables": (_i, [_p, _i64, _i64, _p, _sz, _p]),
     "qmm_moe_route": (_i, [_p, _i64, _i64, _i, _p, _p, _p, _p, _p, _sz, _p]),
     "qmm_ep_pack": (_i, [_p, _i64, _i64, _i64, _i, _p, _i64, _p, _i64, _p, _p]),

@@ -22,7 +22,8 @@ NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 SOURCES = ["capi.cu", "qmv.cu", "qmv_sk.cu", "moe.cu", "prefill.cu", "layout.cu", "tmap.cu", "noalloc.cu", "floor.cu", "qmv_i8.cu", "argmax.cu", "moe_decode.cu", "hostcopy.cu",
-           "mx_quant.cu", "mx_items.cu", "mx_f4.cu", "mx_tc.cu", "mx_capi.cu"]
+           "mx_quant.cu", "mx_items.cu", "mx_f4.cu", "mx_tc.cu", "mx_capi.cu",
+           "sample.cu", "topk.cu", "speculative.cu", "distill.cu", "logits_capi.cu"]
 
 
 def _flags(debug: bool) -> list[str]:

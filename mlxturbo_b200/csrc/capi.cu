@@ -40,6 +40,7 @@ static const char* const kFireNames[] = {
     "qmv",       "qmv_gather", "qmm_prefill", "segment_tables", "sort_rows", "moe_combine",
     "dequantize", "qmv_chunked", "qmv_i8",     "moe_glu_decode",
     "mx_quantize", "mx_dequantize", "mx_rms_norm", "mx_matmul", "mx_gather",
+    "sample",     "topk",       "speculative", "distill_loss",   "distill_grad",
 };
 constexpr int kNumFire = sizeof(kFireNames) / sizeof(kFireNames[0]);
 static std::atomic<long long> g_fire[kNumFire];

@@ -1,0 +1,327 @@
+// distill.cu -- Kullback-Leibler divergence of a row of logits from a
+// teacher's top logits, and its gradient (ops.distill_loss).
+//
+// The teacher's list of a row is k (logit, id) pairs; ids outside [0, V) are
+// empty places.  p are the listed probabilities: exp(t_j / tau) over their
+// sum, or, with the teacher's log-sum-exp given, over the whole sum, the rest
+// 1 - sum p being one more class that holds every token not listed.  With
+// q = softmax(l / tau), Z its sum and O the part of it that is not listed:
+//
+//   loss  = sum_j p_j (log p_j - log q_j)  [ + rest (log rest - log (O / Z)) ]
+//   dloss/dl_i = (q_i - p_i) / tau                     listed tokens
+//              = e_i (1 / Z  [ - rest / O ]) / tau     the others, e_i / Z = q_i
+//
+// O is summed on its own (a bit to an element marks the listed ones), not as a
+// difference: it may be a billionth of Z.  Its weights are taken against the
+// largest logit that is not listed, so neither O nor rest / O leaves the range
+// of 32 bits.
+//
+// Bound by memory: the loss reads the logits once, the gradient reads and
+// writes them once.  Loss and gradient in one call are one launch, a cluster to
+// a row, whose second reading is from L2.
+
+#include "logits.cuh"
+
+namespace qmm {
+
+struct DistillShared {
+    double logp[kMaxList];
+    float x[kMaxList];   // the student's logits of the list
+    int id[kMaxList];    // or -1
+    int slot[kMaxList];  // place in the table of distinct ids
+    int table[2 * kMaxList], owner[2 * kMaxList];
+    double slots[kMaxRowWarps];
+    float tops[kMaxRowWarps];
+    double red[kRowWarps];
+    double top_ref;
+    int twice;
+};
+
+// Sum or maximum over the CTA, the same in every thread and every run.
+template <bool MAX>
+QMM_DEVINL double cta_reduce(double* red, double x) {
+#pragma unroll
+    for (int o = 16; o >= 1; o >>= 1) {
+        const double y = __shfl_xor_sync(~0u, x, o);
+        x = MAX ? (y > x ? y : x) : x + y;
+    }
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = x;
+    __syncthreads();
+    x = red[0];
+    for (int i = 1; i < kRowWarps; ++i) x = MAX ? (red[i] > x ? red[i] : x) : x + red[i];
+    return x;
+}
+
+// The list into shared memory: ids, log p, the student's logits; duplicates
+// share a slot whose owner is the first of them.  Returns sum p.
+template <int DT>
+QMM_DEVINL double load_list(const DistillArgs& a, DistillShared& sh, const Row<DT>& row, long long r) {
+    int size = 2;
+    while (size < 2 * a.k) size <<= 1;
+    for (int i = threadIdx.x; i < size; i += kRowThreads) {
+        sh.table[i] = -1;
+        sh.owner[i] = kMaxList;
+    }
+    if (threadIdx.x == 0) sh.twice = 0;
+    __syncthreads();
+    double best = -CUDART_INF;
+    for (int j = threadIdx.x; j < a.k; j += kRowThreads) {
+        const long long at = r * a.k + j;
+        const long long id = a.ti_bytes == 8 ? static_cast<const long long*>(a.ti)[at]
+                                             : (long long)static_cast<const int*>(a.ti)[at];
+        const float t = a.tv_dtype == 2 ? elem_f32<2>(a.tv, at) : a.tv_dtype == 1 ? elem_f32<1>(a.tv, at)
+                                                                                 : elem_f32<0>(a.tv, at);
+        const bool in = id >= 0 && id < a.V;
+        sh.id[j] = in ? (int)id : -1;
+        sh.x[j] = in ? row.at((int)id) : 0.0f;
+        const double l = in ? (double)t * a.inv_t : -CUDART_INF;
+        sh.logp[j] = l;
+        best = fmax(best, l);  // a NaN shows in the sum
+        if (in) {
+            int h = (int)((uint32_t)id * 2654435761u >> 16) & (size - 1);
+            for (;;) {
+                const int was = atomicCAS(&sh.table[h], -1, (int)id);
+                if (was == -1 || was == (int)id) {
+                    if (was != -1) sh.twice = 1;
+                    break;
+                }
+                h = (h + 1) & (size - 1);
+            }
+            sh.slot[j] = h;
+            atomicMin(&sh.owner[h], j);
+        }
+    }
+    double norm;
+    if (a.tlse) {
+        norm = (double)a.tlse[r];
+    } else {
+        const double m = cta_reduce<true>(sh.red, best);
+        if (m == -CUDART_INF) {
+            norm = 0.0;  // nothing listed
+        } else {
+            double sum = 0.0;
+            for (int j = threadIdx.x; j < a.k; j += kRowThreads) sum += exp(sh.logp[j] - m);
+            sum = cta_reduce<false>(sh.red, sum);
+            norm = m + log(sum);
+        }
+    }
+    double mass = 0.0;
+    for (int j = threadIdx.x; j < a.k; j += kRowThreads) {
+        sh.logp[j] -= norm;
+        mass += exp(sh.logp[j]);
+    }
+    return cta_reduce<false>(sh.red, mass);
+}
+
+// Every listed element of this vector set to -infinity; bit j of m is element j.
+template <int DT>
+QMM_DEVINL void take_out(uint4& u, uint32_t m) {
+    uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if (DT == 2) {
+            if (m >> i & 1) w[i] = 0xFF800000u;
+        } else {
+            if (m >> (2 * i) & 1) w[i] = (w[i] & 0xFFFF0000u) | (neg_inf_word<DT>() & 0xFFFFu);
+            if (m >> (2 * i + 1) & 1) w[i] = (w[i] & 0xFFFFu) | (neg_inf_word<DT>() & 0xFFFF0000u);
+        }
+    }
+    u = make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+template <int DT>
+QMM_DEVINL uint4 encode(const float (&x)[Elem<DT>::kVec]) {
+    if constexpr (DT == 2) {
+        return make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3]));
+    } else {
+        using H = Half<DT == 1>;
+        return make_uint4(H::pack2(x[0], x[1]), H::pack2(x[2], x[3]), H::pack2(x[4], x[5]), H::pack2(x[6], x[7]));
+    }
+}
+
+// TAIL: the teacher's log-sum-exp is given.  MODE kBackward needs no cluster.
+template <int DT, bool TAIL, int MODE>
+__global__ void __launch_bounds__(kRowThreads) distill_kernel(const DistillArgs a, int C) {
+    __shared__ DistillShared sh;
+    extern __shared__ uint32_t marks[];  // TAIL: a byte to a vector of this CTA
+    constexpr int N = Elem<DT>::kVec;
+    cg::cluster_group cl = cg::this_cluster();
+    if (MODE != kBackward) cl.barrier_arrive();
+    const int rank = (int)(blockIdx.x % C), warps = C * kRowWarps;
+    const int g = rank * kRowWarps + (threadIdx.x >> 5);
+    const long long r = blockIdx.x / C;
+    const Row<DT> row(a.logits, a.stride, r, a.V);
+    const Slice s = warp_slice(row.nv, g, warps);
+    const int per = (row.nv + warps - 1) / warps, cta_begin = per * kRowWarps * rank;
+    const int cta_end = cta_begin + per * kRowWarps;
+    const Scale c(a.inv_t);
+    // a teacher's row that is masked throughout carries no loss
+    const bool none = TAIL && a.tlse[r] == -CUDART_INF_F;
+    const float weight = none ? 0.0f : a.weight ? a.weight[r] : 1.0f;
+
+    float ref, mx;         // the others' reference; the row's maximum
+    double others, sum;    // factor of the others' gradient; sum against mx
+    double mass = 0.0;     // sum p
+    if (MODE == kBackward) {
+        const float4 st = a.stats[r];
+        ref = st.x;
+        others = st.y;
+        mx = st.z;
+        sum = st.w;
+        if (weight != 0.0f) mass = load_list<DT>(a, sh, row, r);
+        __syncthreads();
+    } else {
+        if (TAIL)
+            for (int i = threadIdx.x; i < (per * kRowWarps + 3) / 4; i += kRowThreads) marks[i] = 0;
+        mass = load_list<DT>(a, sh, row, r);
+        if (TAIL) {
+            __syncthreads();
+            for (int j = threadIdx.x; j < a.k; j += kRowThreads) {
+                const int at = sh.id[j] + row.shift, v = at / N - cta_begin;
+                if (sh.id[j] >= 0 && v >= 0 && v < per * kRowWarps)
+                    atomicOr(&marks[v / 4], 1u << (8 * (v & 3) + at % N));
+            }
+        }
+        __syncthreads();
+        LaneSum acc;
+        const uint8_t* mark = reinterpret_cast<const uint8_t*>(marks);
+        const float top = stream_slice<DT, true, true>(row, s, c, acc, [&](int v, uint4& u) {
+            if (TAIL) {
+                const uint32_t m = mark[v - cta_begin];
+                if (m) take_out<DT>(u, m);
+            }
+        });
+        cl.barrier_wait();
+        all_gather(cl, sh.tops, g, warp_max(top));
+        cl.sync();
+        ref = slots_max(sh.tops, warps);
+        all_gather(cl, sh.slots, g, warp_mass(acc, c, ref));
+        cl.sync();
+        const double s_ref = ref == -CUDART_INF_F ? 0.0 : slots_sum(sh.slots, warps);
+        // the list's part of the sum
+        double rest = 0.0, log_other = 0.0;
+        mx = ref;
+        sum = s_ref;
+        if (TAIL) {
+            double best = -CUDART_INF;
+            for (int j = threadIdx.x; j < a.k; j += kRowThreads)
+                if (sh.id[j] >= 0) best = fmax(best, (double)sh.x[j]);
+            best = cta_reduce<true>(sh.red, best);
+            mx = fmaxf(ref, (float)best);
+            double part = 0.0;
+            for (int j = threadIdx.x; j < a.k; j += kRowThreads)
+                if (sh.id[j] >= 0 && sh.owner[sh.slot[j]] == j) part += exp(((double)sh.x[j] - (double)mx) * a.inv_t);
+            part = cta_reduce<false>(sh.red, part);
+            const double lift = ref == -CUDART_INF_F ? 0.0 : exp(((double)ref - (double)mx) * a.inv_t);
+            sum = s_ref * lift + part;
+            rest = mass < 1.0 ? 1.0 - mass : mass >= 1.0 ? 0.0 : mass;
+            log_other = ref == -CUDART_INF_F ? -CUDART_INF
+                                             : ((double)ref - (double)mx) * a.inv_t + log(s_ref) - log(sum);
+            others = lift / sum - (s_ref > 0.0 ? rest / s_ref : 0.0);
+            if (ref == -CUDART_INF_F) others = 0.0;  // no token that is not listed has any probability
+        } else {
+            others = mass == 0.0 ? 0.0 : 1.0 / sum;
+        }
+        if (rank == 0) {
+            const double log_z = (double)mx * a.inv_t + log(sum);
+            double part = 0.0;
+            for (int j = threadIdx.x; j < a.k; j += kRowThreads) {
+                const double lp = sh.logp[j], p = exp(lp);
+                if (sh.id[j] >= 0 && p != 0.0) part += p * (lp - ((double)sh.x[j] * a.inv_t - log_z));
+            }
+            part = cta_reduce<false>(sh.red, part);
+            if (TAIL && rest != 0.0) part += rest * (log(rest) - log_other);
+            if (threadIdx.x == 0) {
+                a.loss[r] = none ? 0.0f : (float)part;
+                if (MODE == kLoss && a.stats) a.stats[r] = make_float4(ref, (float)others, mx, (float)sum);
+            }
+        }
+        if (MODE == kLoss) return;
+    }
+
+    // gradient
+    char* const out = static_cast<char*>(a.grad) + r * a.grad_stride * Elem<DT>::kBytes;
+    const bool aligned = ((reinterpret_cast<uintptr_t>(out) - row.shift * Elem<DT>::kBytes) & 15u) == 0;
+    auto store = [&](int v, const float (&y)[N]) {
+        const int f = row.first(v);
+        if (aligned && row.whole(v)) {
+            *reinterpret_cast<uint4*>(out + (long long)f * Elem<DT>::kBytes) = encode<DT>(y);
+        } else {
+#pragma unroll
+            for (int j = 0; j < N; ++j)
+                if (f + j >= 0 && f + j < row.V) store_elem<DT>(out, f + j, y[j]);
+        }
+    };
+    const double scale = (double)weight * a.inv_t;
+    const float factor = weight == 0.0f ? 0.0f : (float)(scale * others);
+    if (factor == 0.0f) {  // a row that carries no loss, or one whose other tokens get none: whatever their logits
+        const float zero[N] = {};
+        for (int v = s.begin + s.lane; v < s.end; v += 32) store(v, zero);
+        if (weight == 0.0f) return;
+    } else {
+        for_vectors<DT>(row, s, [&](int v, const uint4& u) {
+            float x[N];
+            decode<DT>(u, x);
+#pragma unroll
+            for (int j = 0; j < N; ++j) x[j] = factor * ex2(c.exponent(below<true>(x[j], ref)));
+            store(v, x);
+        });
+    }
+    __syncthreads();  // the listed tokens' values after the others' formula has been written in their place
+    for (int j = threadIdx.x; j < a.k; j += kRowThreads) {
+        const int id = sh.id[j];
+        if (id < 0 || sh.owner[sh.slot[j]] != j) continue;
+        const int v = (id + row.shift) / N;
+        if (v < cta_begin || v >= cta_end) continue;
+        double p = exp(sh.logp[j]);
+        if (sh.twice) {
+            for (int i = j + 1; i < a.k; ++i)
+                if (sh.id[i] == id) p += exp(sh.logp[i]);
+        }
+        const double q = mass == 0.0 && !TAIL ? 0.0 : exp(((double)sh.x[j] - (double)mx) * a.inv_t) / sum;
+        store_elem<DT>(out, id, (float)(scale * (q - p)));
+    }
+}
+
+}  // namespace qmm
+
+namespace qmm_host {
+
+template <int DT, bool TAIL, int MODE>
+static int distill_launch(const qmm::DistillArgs& a, long long rows, cudaStream_t st) {
+    const int C = row_cluster(rows, a.V, qmm::Elem<DT>::kBytes);
+    if (MODE == qmm::kBackward)  // CTAs on their own
+        return launch_rows(qmm::distill_kernel<DT, TAIL, MODE>, rows * C, 1, 0, st, "distill launch", a, C);
+    size_t smem = 0;
+    if (TAIL) {
+        const long long vecs = (a.V + 2LL * qmm::Elem<DT>::kVec - 2) / qmm::Elem<DT>::kVec;  // any start of a row
+        const int warps = C * qmm::kRowWarps;
+        smem = (size_t)(((vecs + warps - 1) / warps) * qmm::kRowWarps + 3) / 4 * 4;
+        if (smem + sizeof(qmm::DistillShared) > 48 * 1024) {
+            set_error("distill: V=%d is too long for teacher_logsumexp", a.V);
+            return QMM_EUNSUPPORTED;
+        }
+    }
+    return launch_rows(qmm::distill_kernel<DT, TAIL, MODE>, rows, C, smem, st, "distill launch", a, C);
+}
+
+template <int DT, bool TAIL>
+static int distill_mode(const qmm::DistillArgs& a, long long rows, int mode, cudaStream_t st) {
+    if (mode == qmm::kLoss) return distill_launch<DT, TAIL, qmm::kLoss>(a, rows, st);
+    if (mode == qmm::kLossGrad) return distill_launch<DT, TAIL, qmm::kLossGrad>(a, rows, st);
+    return distill_launch<DT, TAIL, qmm::kBackward>(a, rows, st);
+}
+
+template <int DT>
+static int distill_dt(const qmm::DistillArgs& a, long long rows, int mode, cudaStream_t st) {
+    return a.tlse ? distill_mode<DT, true>(a, rows, mode, st) : distill_mode<DT, false>(a, rows, mode, st);
+}
+
+int launch_distill(const qmm::DistillArgs& a, long long rows, int dtype, int mode, cudaStream_t st) {
+    if (dtype == QMM_BF16) return distill_dt<0>(a, rows, mode, st);
+    if (dtype == QMM_F16) return distill_dt<1>(a, rows, mode, st);
+    return distill_dt<2>(a, rows, mode, st);
+}
+
+}  // namespace qmm_host

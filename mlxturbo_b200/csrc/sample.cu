@@ -1,0 +1,327 @@
+// sample.cu -- a token a row from a given uniform number: temperature, top-k,
+// top-p, min-p (ops.sample).
+//
+// With w_i = exp((l_i - max) / T) and the tokens in the order of (logit
+// descending, id ascending), kept are the first top_k; of these, as long as
+// the mass before a token is below top_p times theirs; and those with
+// w_i >= min_p.  The answer is the first id, in the order of ids, at which the
+// kept weights add up to more than u times their sum.  Every kept set is a
+// prefix of the order, so it is {key >= border} for one 64-bit key.
+//
+// The ids are those of 64-bit arithmetic.  Where sums over the whole row are
+// needed (top-p without top-k, no filter at all) a 32-bit pass gives them with
+// a bound on their error; only a row whose decision lies within that bound of
+// a border takes a second pass in 64 bits.
+
+#include "logits_select.cuh"
+
+namespace qmm {
+
+// What CTA 0 makes of the candidates: the answer; a sum in 64 bits is needed;
+// the border, but more kept tokens than it draws from itself; not enough of them.
+enum { kDone, kNeedSum, kBorder, kGeneral };
+constexpr int kDrawHere = 2 * kRowThreads;
+
+// Running sums over the sorted candidates' weights, in place, by the whole CTA.
+QMM_DEVINL void scan_weights(SelectShared& sh, int n) {
+    const int per = (n + kRowThreads - 1) / kRowThreads, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int b = threadIdx.x * per, e = b + per < n ? b + per : n;
+    double run = 0.0;
+    for (int i = b; i < e; ++i) run += sh.w[i];
+    double incl = run;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const double y = __shfl_up_sync(~0u, incl, o);
+        if (lane >= o) incl += y;
+    }
+    if (lane == 31) sh.scan[warp] = incl;
+    __syncthreads();
+    double base = incl - run;
+    for (int i = 0; i < warp; ++i) base += sh.scan[i];
+    for (int i = b; i < e; ++i) {
+        base += sh.w[i];
+        sh.w[i] = base;
+    }
+    __syncthreads();
+}
+
+// How many of the first n running sums stand before `limit`: the tokens whose
+// mass before them (the sum of the one above) is below it.  The first always is.
+QMM_DEVINL int count_before(const double* sums, int n, double limit) {
+    int lo = 1, hi = n;  // the first i >= 1 with sums[i - 1] >= limit
+    while (lo < hi) {
+        const int mid = (lo + hi) / 2;
+        if (sums[mid - 1] >= limit) hi = mid;
+        else lo = mid + 1;
+    }
+    return lo;
+}
+
+template <int DT>
+__global__ void __launch_bounds__(kRowThreads) sample_kernel(const SampleArgs a) {
+    __shared__ SelectShared sh;
+    cg::cluster_group cl = cg::this_cluster();
+    cl.barrier_arrive();  // waited for before the first access to another CTA
+    if (threadIdx.x == 0) sh.n_cand = 0;
+    const int C = (int)cl.num_blocks(), rank = (int)cl.block_rank(), warps = C * kRowWarps;
+    const int g = rank * kRowWarps + (threadIdx.x >> 5);
+    const long long r = blockIdx.x / C;
+    const Row<DT> row(a.logits, a.stride, r, a.V);
+    const Slice s = warp_slice(row.nv, g, warps);
+
+    double T = a.t_rows ? (double)a.t_rows[r] : a.t;
+    const bool greedy = !(T > 0.0);
+    int k = a.k_rows ? a.k_rows[r] : a.k;
+    double p = a.p_rows ? (double)a.p_rows[r] : a.p;
+    double mp = a.m_rows ? (double)a.m_rows[r] : a.m;
+    if (greedy) {
+        T = 1.0;
+        k = 1;
+    }
+    const bool k_on = k >= 1 && k < a.V, p_on = p < 1.0 && !(k_on && k == 1);
+    const bool m_on = mp > 0.0 && !(k_on && k == 1);
+    if (mp > 1.0) mp = 1.0;
+    const double inv_t = 1.0 / T, u = (double)a.u[r];
+    const bool sum = !k_on && (p_on || !m_on);
+    const Scale c(inv_t);
+
+    // one pass over memory
+    LaneSum acc;
+    const float top = sum ? stream_slice<DT, true>(row, s, c, acc) : stream_slice<DT, false>(row, s, c, acc);
+    const float wtop = warp_max(top);
+    cl.barrier_wait();
+    all_gather(cl, sh.tops, g, wtop);
+    const bool select = k_on || p_on;  // a bound from the threads' maxima
+    if (select) *cl.map_shared_rank(&sh.maxima[rank * kRowThreads + threadIdx.x], 0) = top;
+    cl.sync();
+    const float mx = slots_max(sh.tops, warps);
+    if (mx == -CUDART_INF_F) {  // nothing to draw from
+        if (rank == 0 && threadIdx.x == 0) a.ids[r] = -1;
+        return;
+    }
+    bool fast = sum && mx < CUDART_INF_F && T >= kFastMinT && T <= kFastMaxT &&
+                (row.nv + warps - 1) / warps <= 32 * kFastVectors;
+
+    // the warps' masses against the row's maximum, to every CTA
+    if (sum) {
+        const double mass = warp_mass(acc, c, mx);
+        all_gather(cl, sh.slots[0], g, fast ? mass : CUDART_NAN);
+    }
+    // smallest key that min-p keeps; masked tokens have none
+    uint32_t kmin = kKeyNegInf + 1;
+    if (m_on) {
+        const float guess = (float)((double)mx + T * log(mp));
+        uint32_t b = guess == guess && key32(guess) > kmin ? key32(guess) : kmin;
+        const uint32_t top_key = key32(mx);
+        if (b > top_key) b = top_key;
+        while (b > kmin && weight64(key32_value(b - 1), mx, inv_t) >= mp) --b;
+        while (b < top_key && weight64(key32_value(b), mx, inv_t) < mp) ++b;
+        kmin = b;
+    }
+    // Top-k without top-p: tokens below min-p play no part.
+    uint32_t bound = kmin;
+    const int want = k_on ? k : kRowThreads;
+    const bool listed = select ? want <= C * kRowThreads / 2 || want <= kRowThreads : m_on;
+    if (select && listed) {
+        if (rank == 0) {
+            const uint32_t b = kth_prefix(sh, C * kRowThreads, want) << 16;
+            if (threadIdx.x < C) *cl.map_shared_rank(&sh.bound, threadIdx.x) = b;
+        }
+        cl.sync();
+        bound = sh.bound > kKeyNegInf ? sh.bound : kKeyNegInf + 1;
+        if (!(k_on && p_on) && bound < kmin) bound = kmin;
+    } else {
+        cl.sync();
+    }
+    double total = sum ? slots_sum(sh.slots[0], warps) : 0.0;
+    if (!(total >= 0.5)) fast = false;  // NaN, or a pass that missed the maximum: 64 bits
+    unsigned long long border = (unsigned long long)kmin << 32;
+    bool bordered = false;
+
+    if (listed) {
+        const uint32_t mine = push_candidates<DT>(cl, sh, row, s, top, bound);
+        all_gather(cl, sh.found, g, mine);
+        cl.sync();
+        uint32_t n = 0;
+        for (int i = s.lane; i < warps; i += 32) n += sh.found[i];
+        n = warp_sum(n);
+        if (n <= kCand) {
+            // one CTA's work; the others wait only where it may end otherwise
+            const bool sure = k_on && k <= kRowThreads;
+            if (rank != 0 && sure) return;
+            bool sorted = false;
+            double eps = k_on ? 0.0 : fast ? kFastEps : 1.0;
+            for (;;) {
+                if (rank == 0) {
+                    if (!sorted) {
+                        sort_candidates(sh.cand, (int)n);
+                        for (int i = threadIdx.x; i < (int)n; i += kRowThreads)
+                            sh.w[i] = weight64(key32_value((uint32_t)(sh.cand[i] >> 32)), mx, inv_t);
+                        __syncthreads();
+                        scan_weights(sh, (int)n);
+                        sorted = true;
+                    }
+                    int verdict = kDone;
+                    int kept = (int)n;
+                    if (k_on && k < kept) kept = k;
+                    if (p_on) {
+                        const double all = k_on ? sh.w[kept - 1] : total;
+                        const int lo = count_before(sh.w, kept, p * all * (1.0 - eps));
+                        const int hi = count_before(sh.w, kept, p * all * (1.0 + eps));
+                        const bool open = !k_on && bound > kmin && !(sh.w[kept - 1] >= p * all * (1.0 + eps));
+                        if (eps == 1.0) verdict = kNeedSum;
+                        else if (open) verdict = eps > 0.0 && sh.w[kept - 1] >= p * all * (1.0 - eps) ? kNeedSum : kGeneral;
+                        else if (lo != hi) verdict = kNeedSum;
+                        kept = hi;
+                    }
+                    // of them, those that min-p keeps
+                    int lo = 0, hi = kept;
+                    while (lo < hi) {
+                        const int mid = (lo + hi) / 2;
+                        if ((uint32_t)(sh.cand[mid] >> 32) >= kmin) lo = mid + 1;
+                        else hi = mid;
+                    }
+                    kept = lo;
+                    if (verdict == kDone && kept > kDrawHere) verdict = kBorder;
+                    if (verdict == kDone) {
+                        // the first id at which the sum over kept tokens with ids up to it passes u W
+                        const double target = u * sh.w[kept - 1];
+                        if (threadIdx.x == 0) sh.best = ~0ull;
+                        __syncthreads();
+                        unsigned long long best = ~0ull;
+                        for (int j = threadIdx.x; j < kept; j += kRowThreads) {
+                            const int id = key_id(sh.cand[j]);
+                            double run = 0.0, prev = 0.0;
+                            const double own = sh.w[j] - (j ? sh.w[j - 1] : 0.0);
+                            for (int i = 0; i < kept; ++i) {
+                                const double cum = sh.w[i];
+                                if (key_id(sh.cand[i]) <= id) run += cum - prev;
+                                prev = cum;
+                            }
+                            if (own > 0.0) {
+                                // past the target: the smallest id; if none is, the largest id of all
+                                const unsigned long long code =
+                                    run > target ? (unsigned long long)id : (1ull << 40) + (0xFFFFFFFFu - (uint32_t)id);
+                                best = code < best ? code : best;
+                            }
+                        }
+                        atomicMin(&sh.best, best);
+                        __syncthreads();
+                        if (threadIdx.x == 0) {
+                            const unsigned long long b = sh.best;
+                            a.ids[r] = b < (1ull << 40) ? (int64_t)b : (int64_t)(0xFFFFFFFFu - (uint32_t)(b - (1ull << 40)));
+                        }
+                    }
+                    if (!sure && threadIdx.x < C) {
+                        *cl.map_shared_rank(&sh.verdict, threadIdx.x) = verdict;
+                        if (verdict == kBorder) *cl.map_shared_rank(&sh.best, threadIdx.x) = sh.cand[kept - 1];
+                    }
+                }
+                if (sure) return;
+                cl.sync();
+                const int verdict = sh.verdict;
+                if (verdict == kDone) return;
+                if (verdict == kBorder) border = sh.best;
+                if (verdict != kNeedSum) {
+                    bordered = verdict == kBorder;
+                    break;
+                }
+                // the row's sum in 64 bits, then again
+                double mass = 0.0;
+                for_vectors<DT>(row, s, [&](int v, const uint4& q) {
+                    float x[Elem<DT>::kVec];
+                    decode<DT>(q, x);
+#pragma unroll
+                    for (int j = 0; j < Elem<DT>::kVec; ++j) mass += x[j] == x[j] ? weight64(x[j], mx, inv_t) : 0.0;
+                });
+                all_gather(cl, sh.slots[1], g, warp_sum(mass));
+                cl.sync();
+                total = slots_sum(sh.slots[1], warps);
+                eps = 0.0;
+            }
+        }
+    }
+
+    if (!select && !m_on && fast) {  // no filter: the warps' fast masses are the distribution
+        const double target = u * total, slack = 2.0 * kFastEps * total;
+        const Place at = locate(sh.slots[0], warps, target);
+        if (g == at.g) {
+            const Found f = find_in_slice<DT>(row, s, at.base, target, [&](int, float x) {
+                return weight64(x, mx, inv_t);
+            });
+            const bool sure = f.id >= 0 && f.before + slack <= target && f.after - slack > target;
+            if (sure && s.lane == 0) a.ids[r] = f.id;
+            if (s.lane < C) *cl.map_shared_rank(&sh.verdict, s.lane) = sure ? kDone : kGeneral;
+        }
+        cl.sync();
+        if (sh.verdict == kDone) return;
+    }
+
+    // the general way: borders by search, masses and place in 64 bits
+    const unsigned long long lo = (unsigned long long)(kKeyNegInf + 1) << 32;
+    const unsigned long long hi = ((unsigned long long)key32(mx) + 1) << 32;
+    if (select && !bordered) {
+        unsigned long long first = lo;
+        if (k_on) first = border_key<DT, false>(cl, sh, row, s, g, warps, mx, inv_t, lo, hi, (double)k);
+        if (p_on) {
+            double mass = 0.0;
+            for_vectors<DT>(row, s, [&](int v, const uint4& q) {
+                float x[Elem<DT>::kVec];
+                decode<DT>(q, x);
+#pragma unroll
+                for (int j = 0; j < Elem<DT>::kVec; ++j) {
+                    const int id = row.first(v) + j;
+                    if (id >= 0 && id < row.V && row_key(x[j], id) >= first) mass += weight64(x[j], mx, inv_t);
+                }
+            });
+            cl.sync();
+            all_gather(cl, sh.slots[1], g, warp_sum(mass));
+            cl.sync();
+            first = border_key<DT, true>(cl, sh, row, s, g, warps, mx, inv_t, first, hi,
+                                         fmax(p * slots_sum(sh.slots[1], warps), 1e-300));
+        }
+        if (first > border) border = first;
+    }
+    auto weight = [&](int id, float x) { return row_key(x, id) >= border ? weight64(x, mx, inv_t) : 0.0; };
+    double mass = 0.0;
+    for_vectors<DT>(row, s, [&](int v, const uint4& q) {
+        float x[Elem<DT>::kVec];
+        decode<DT>(q, x);
+#pragma unroll
+        for (int j = 0; j < Elem<DT>::kVec; ++j) {
+            const int id = row.first(v) + j;
+            if (id >= 0 && id < row.V) mass += weight(id, x[j]);
+        }
+    });
+    cl.sync();
+    all_gather(cl, sh.slots[0], g, warp_sum(mass));
+    cl.sync();
+    const double target = u * slots_sum(sh.slots[0], warps);
+    const Place at = locate(sh.slots[0], warps, target);
+    if (g == at.g) {
+        const Found f = find_in_slice<DT>(row, s, at.base, target, weight);
+        if (s.lane == 0) a.ids[r] = f.id;
+    }
+}
+
+}  // namespace qmm
+
+namespace qmm_host {
+
+int row_cluster(long long rows, long long V, int elem_bytes) {
+    const long long vecs = (V * elem_bytes + 15) / 16;
+    int C = 1;
+    // up to 16 vectors to a lane; a call of few rows goes down to 2 vectors as long as SMs are idle
+    while (C < 8 && vecs > 16LL * C * qmm::kRowThreads) C *= 2;
+    while (C < 16 && rows * C * 2 <= 148 && vecs > 2LL * C * qmm::kRowThreads) C *= 2;
+    return C;
+}
+
+int launch_sample(const qmm::SampleArgs& a, long long rows, int dtype, cudaStream_t st) {
+    const int C = row_cluster(rows, a.V, dtype == QMM_F32 ? 4 : 2);
+    if (dtype == QMM_BF16) return launch_rows(qmm::sample_kernel<0>, rows, C, 0, st, "sample launch", a);
+    if (dtype == QMM_F16) return launch_rows(qmm::sample_kernel<1>, rows, C, 0, st, "sample launch", a);
+    return launch_rows(qmm::sample_kernel<2>, rows, C, 0, st, "sample launch", a);
+}
+
+}  // namespace qmm_host

@@ -1,0 +1,115 @@
+// topk.cu -- the k largest logits of a row with their ids, and the row's
+// log-sum-exp (ops.topk): what a distillation takes from its teacher and a
+// sharded lm_head exchanges instead of its logits.
+//
+// One pass over memory.  The k-th largest of the threads' maxima bounds the
+// k-th largest logit from below, and with 2048 threads to a row little more
+// than k logits reach it: the lanes that hold one read their share again
+// (from L2), CTA 0 sorts what they find.  Rows where too many reach the bound
+// (many equal logits, k near the number of threads) search the border key and
+// collect above it.
+
+#include "logits_select.cuh"
+
+namespace qmm {
+
+template <int DT, bool LSE>
+__global__ void __launch_bounds__(kRowThreads) topk_kernel(const TopkArgs a) {
+    __shared__ SelectShared sh;
+    cg::cluster_group cl = cg::this_cluster();
+    cl.barrier_arrive();  // waited for before the first access to another CTA
+    if (threadIdx.x == 0) sh.n_cand = 0;
+    const int C = (int)cl.num_blocks(), rank = (int)cl.block_rank(), warps = C * kRowWarps;
+    const int g = rank * kRowWarps + (threadIdx.x >> 5);
+    const long long r = blockIdx.x / C;
+    const Row<DT> row(a.logits, a.stride, r, a.V);
+    const Slice s = warp_slice(row.nv, g, warps);
+    const Scale c(a.inv_t);
+
+    LaneSum acc;
+    const float top = stream_slice<DT, LSE>(row, s, c, acc);
+    cl.barrier_wait();
+    if (LSE) all_gather(cl, sh.tops, g, warp_max(top));
+    *cl.map_shared_rank(&sh.maxima[rank * kRowThreads + threadIdx.x], 0) = top;
+    cl.sync();
+    float mx = 0.0f;
+    if (LSE) {
+        mx = slots_max(sh.tops, warps);
+        all_gather(cl, sh.slots[0], g, warp_mass(acc, c, mx));
+    }
+    const bool listed = a.k <= C * kRowThreads;
+    uint32_t bound = 0;
+    if (listed) {
+        if (rank == 0) {
+            const uint32_t b = kth_prefix(sh, C * kRowThreads, a.k) << 16;
+            if (threadIdx.x < C) *cl.map_shared_rank(&sh.bound, threadIdx.x) = b;
+        }
+        cl.sync();
+        bound = sh.bound;
+    } else {
+        cl.sync();
+    }
+    if (LSE && rank == 0 && threadIdx.x < 32) {
+        const double total = slots_sum(sh.slots[0], warps);
+        // no finite maximum: the sum is that of the largest alone
+        const double l = mx == -CUDART_INF_F || mx == CUDART_INF_F ? (double)mx : (double)mx * a.inv_t + log(total);
+        if (threadIdx.x == 0) a.lse[r] = (float)l;
+    }
+    uint32_t n = kCand + 1;
+    if (listed) {
+        const uint32_t mine = push_candidates<DT>(cl, sh, row, s, top, bound);
+        all_gather(cl, sh.found, g, mine);
+        cl.sync();
+        n = 0;
+        for (int i = s.lane; i < warps; i += 32) n += sh.found[i];
+        n = warp_sum(n);
+    }
+    if (n > kCand) {  // the border, then the k tokens from it on
+        const unsigned long long border =
+            border_key<DT, false>(cl, sh, row, s, g, warps, 0.0f, 1.0, 0ull, ~0ull, (double)a.k);
+        if (threadIdx.x == 0) sh.n_cand = 0;
+        cl.sync();
+        uint32_t* count = cl.map_shared_rank(&sh.n_cand, 0);
+        unsigned long long* list = cl.map_shared_rank(sh.cand, 0);
+        for_vectors<DT>(row, s, [&](int v, const uint4& q) {
+            float x[Elem<DT>::kVec];
+            decode<DT>(q, x);
+#pragma unroll
+            for (int j = 0; j < Elem<DT>::kVec; ++j) {
+                const int id = row.first(v) + j;
+                if (id < 0 || id >= row.V || row_key(x[j], id) < border) continue;
+                const uint32_t at = atomicAdd(count, 1u);
+                if (at < kCand) list[at] = row_key(x[j], id);
+            }
+        });
+        cl.sync();
+        n = (uint32_t)a.k;
+    }
+    if (rank != 0) return;
+    sort_candidates(sh.cand, (int)n);
+    for (int i = threadIdx.x; i < a.k; i += kRowThreads) {
+        const int id = key_id(sh.cand[i]);
+        const float x = row.at(id);  // the bits of memory: -0 stays -0
+        store_elem<DT>(a.values, r * a.k + i, x == x ? x : -CUDART_INF_F);
+        a.ids[r * a.k + i] = id;
+    }
+}
+
+}  // namespace qmm
+
+namespace qmm_host {
+
+template <int DT>
+static int topk_dt(const qmm::TopkArgs& a, long long rows, cudaStream_t st) {
+    const int C = row_cluster(rows, a.V, qmm::Elem<DT>::kBytes);
+    if (a.lse) return launch_rows(qmm::topk_kernel<DT, true>, rows, C, 0, st, "topk launch", a);
+    return launch_rows(qmm::topk_kernel<DT, false>, rows, C, 0, st, "topk launch", a);
+}
+
+int launch_topk(const qmm::TopkArgs& a, long long rows, int dtype, cudaStream_t st) {
+    if (dtype == QMM_BF16) return topk_dt<0>(a, rows, st);
+    if (dtype == QMM_F16) return topk_dt<1>(a, rows, st);
+    return topk_dt<2>(a, rows, st);
+}
+
+}  // namespace qmm_host

@@ -380,6 +380,255 @@ at::Tensor mx_gather(const at::Tensor& x_in, const std::optional<at::Tensor>& xs
     return y;
 }
 
+// ---- rows of logits -------------------------------------------------------------
+
+// [.., V] as rows of one stride: as it is where the rows lie evenly, else a copy.
+at::Tensor logits_rows(const char* what, const at::Tensor& l) {
+    if (l.dim() < 1 || l.size(-1) == 0)
+        fail(Err::kValue, "%s: logits of shape %s have no vocabulary axis", what, dims(l.sizes()).c_str());
+    const int64_t V = l.size(-1);
+    if (l.dim() == 2 && (l.stride(1) == 1 || V == 1)) return l;
+    if (l.dim() == 1 && (l.stride(0) == 1 || V == 1)) return l.unsqueeze(0);
+    return l.contiguous().view({l.numel() / V, V});
+}
+
+// One number a row, of dtype, or nothing.
+at::Tensor per_row(const char* what, const char* name, const std::optional<at::Tensor>& t, at::ScalarType dtype,
+                   at::IntArrayRef lead) {
+    if (!t.has_value()) return at::Tensor();
+    if (t->dim() > (int64_t)lead.size())
+        fail(Err::kValue, "%s: %s of shape %s for rows of shape %s", what, name, dims(t->sizes()).c_str(),
+             dims(lead).c_str());
+    for (int64_t i = 0; i < t->dim(); ++i) {
+        const int64_t n = t->size(t->dim() - 1 - i), m = lead[lead.size() - 1 - i];
+        if (n != 1 && n != m)
+            fail(Err::kValue, "%s: %s of shape %s for rows of shape %s", what, name, dims(t->sizes()).c_str(),
+                 dims(lead).c_str());
+    }
+    return t->to(dtype).expand(lead).contiguous();
+}
+
+template <typename T>
+const T* ptr_or_null(const at::Tensor& t) {
+    return t.defined() ? static_cast<const T*>(t.data_ptr()) : nullptr;
+}
+
+const at::Tensor* opt(const std::optional<at::Tensor>& t) { return t.has_value() ? &*t : nullptr; }
+
+void* logits_stream(const at::Tensor& t) { return at::cuda::getCurrentCUDAStream(t.device().index()).stream(); }
+
+at::Tensor sample(const at::Tensor& logits, const at::Tensor& u_in, const std::optional<at::Tensor>& t_in, double t,
+                  const std::optional<at::Tensor>& k_in, int64_t k, const std::optional<at::Tensor>& p_in, double p,
+                  const std::optional<at::Tensor>& m_in, double m) {
+    mx_same_device("sample", {&logits, &u_in, opt(t_in), opt(k_in), opt(p_in), opt(m_in)});
+    const int dt = mx_dtype_code(logits.scalar_type());
+    c10::cuda::CUDAGuard guard(logits.device());
+    const at::Tensor l = logits_rows("sample", logits);
+    const at::IntArrayRef lead = logits.sizes().slice(0, logits.dim() - 1);
+    if (u_in.sizes() != lead || u_in.scalar_type() != at::kFloat)
+        fail(Err::kValue, "sample: u must be float32 of shape %s, one number a row", dims(lead).c_str());
+    if (k_in.has_value() && k_in->is_floating_point()) fail(Err::kValue, "sample: top_k must hold integers");
+    const at::Tensor u = u_in.contiguous();
+    const at::Tensor tr = per_row("sample", "temperature", t_in, at::kFloat, lead);
+    const at::Tensor kr = per_row("sample", "top_k",
+                                  k_in.has_value() && k_in->scalar_type() == at::kLong
+                                      ? std::optional<at::Tensor>(k_in->clamp(0, 0x7FFFFFFF)) : k_in,
+                                  at::kInt, lead);
+    const at::Tensor pr = per_row("sample", "top_p", p_in, at::kFloat, lead);
+    const at::Tensor mr = per_row("sample", "min_p", m_in, at::kFloat, lead);
+    at::Tensor ids = empty_like_device(lead, at::kLong, l);
+    check(qmm_sample(l.data_ptr(), l.stride(0), l.size(0), l.size(1), dt, static_cast<const float*>(u.data_ptr()),
+                     ptr_or_null<float>(tr), t, ptr_or_null<int32_t>(kr), k, ptr_or_null<float>(pr), p,
+                     ptr_or_null<float>(mr), m, static_cast<int64_t*>(ids.data_ptr()), logits_stream(l)),
+          "sample");
+    return ids;
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor> topk(const at::Tensor& logits, int64_t k, bool lse, double t) {
+    mx_same_device("topk", {&logits});
+    const int dt = mx_dtype_code(logits.scalar_type());
+    c10::cuda::CUDAGuard guard(logits.device());
+    const at::Tensor l = logits_rows("topk", logits);
+    std::vector<int64_t> shape(logits.sizes().begin(), logits.sizes().end());
+    shape.back() = k < 0 ? 0 : k;
+    at::Tensor values = empty_like_device(shape, l.scalar_type(), l), ids = empty_like_device(shape, at::kLong, l);
+    shape.pop_back();
+    at::Tensor sums = lse ? empty_like_device(shape, at::kFloat, l) : at::Tensor();
+    check(qmm_topk(l.data_ptr(), l.stride(0), l.size(0), l.size(1), dt, k, t, values.data_ptr(),
+                   static_cast<int64_t*>(ids.data_ptr()), lse ? static_cast<float*>(sums.data_ptr()) : nullptr,
+                   logits_stream(l)),
+          "topk");
+    return {values, ids, sums};
+}
+
+std::tuple<at::Tensor, at::Tensor> speculative_sample(const at::Tensor& logits, const at::Tensor& draft,
+                                                      const at::Tensor& ids_in, const at::Tensor& u_in,
+                                                      const std::optional<at::Tensor>& t_in, double t,
+                                                      const std::optional<at::Tensor>& dt_in, double draft_t) {
+    const char* what = "speculative_sample";
+    mx_same_device(what, {&logits, &draft, &ids_in, &u_in, opt(t_in), opt(dt_in)});
+    const int dt = mx_dtype_code(logits.scalar_type());
+    if (logits.dim() < 2 || logits.size(-1) == 0 || logits.size(-2) == 0)
+        fail(Err::kValue, "%s: logits of shape %s are not [.., n + 1, V]", what, dims(logits.sizes()).c_str());
+    const int64_t V = logits.size(-1), n = logits.size(-2) - 1;
+    std::vector<int64_t> lead(logits.sizes().begin(), logits.sizes().end() - 2), shape = lead;
+    int64_t B = 1;
+    for (int64_t d : lead) B *= d;
+    shape.push_back(n);
+    if (ids_in.sizes() != at::IntArrayRef(shape) || ids_in.is_floating_point())
+        fail(Err::kValue, "%s: draft_ids must be integers of shape %s", what, dims(shape).c_str());
+    shape.push_back(V);
+    if (draft.sizes() != at::IntArrayRef(shape) || draft.scalar_type() != logits.scalar_type())
+        fail(Err::kValue, "%s: draft_logits must have shape %s and the logits' dtype", what, dims(shape).c_str());
+    shape.pop_back();
+    shape.back() = n + 1;
+    if (u_in.sizes() != at::IntArrayRef(shape) || u_in.scalar_type() != at::kFloat)
+        fail(Err::kValue, "%s: u must be float32 of shape %s", what, dims(shape).c_str());
+    c10::cuda::CUDAGuard guard(logits.device());
+    auto rows3 = [&](const at::Tensor& x, int64_t rows) {  // [B, rows, V] with any strides of the first two
+        if (x.dim() == 3 && (x.stride(2) == 1 || V == 1)) return x;
+        return x.contiguous().view({B, rows, V});
+    };
+    const at::Tensor l = rows3(logits, n + 1), q = rows3(draft, n);
+    const at::Tensor ids = ids_in.to(at::kLong).contiguous(), u = u_in.contiguous();
+    const at::Tensor tr = per_row(what, "temperature", t_in, at::kFloat, lead);
+    const at::Tensor dtr = per_row(what, "draft_temperature", dt_in, at::kFloat, lead);
+    at::Tensor tokens = empty_like_device(shape, at::kLong, l), accepted = empty_like_device(lead, at::kLong, l);
+    if (B == 0) return {tokens, accepted};
+    const size_t need = qmm_speculative_sample_workspace_size(B, n);
+    const at::Tensor ws = mx_scratch(l, need);
+    check(qmm_speculative_sample(l.data_ptr(), l.stride(0), l.stride(1), n ? q.data_ptr() : nullptr,
+                                 n ? q.stride(0) : 0, n ? q.stride(1) : 0, B, n, V, dt,
+                                 n ? static_cast<const int64_t*>(ids.data_ptr()) : nullptr,
+                                 static_cast<const float*>(u.data_ptr()), ptr_or_null<float>(tr), t,
+                                 ptr_or_null<float>(dtr), draft_t, static_cast<int64_t*>(tokens.data_ptr()),
+                                 static_cast<int64_t*>(accepted.data_ptr()), mx_scratch_ptr(ws), need,
+                                 logits_stream(l)),
+          what);
+    return {tokens, accepted};
+}
+
+// The teacher's side of a distillation, checked against the logits' rows.
+struct Teacher {
+    at::Tensor values, ids, lse;
+    int dtype, id_bytes;
+    int64_t k;
+};
+
+Teacher teacher_of(const char* what, const at::Tensor& logits, const at::Tensor& tv, const at::Tensor& ti,
+                   const std::optional<at::Tensor>& lse) {
+    const at::IntArrayRef lead = logits.sizes().slice(0, logits.dim() - 1);
+    Teacher t;
+    t.dtype = mx_dtype_code(tv.scalar_type());
+    if (tv.dim() != logits.dim() || tv.sizes().slice(0, tv.dim() - 1) != lead || ti.sizes() != tv.sizes())
+        fail(Err::kValue, "%s: teacher_values %s and teacher_ids %s do not list entries for logits %s", what,
+             dims(tv.sizes()).c_str(), dims(ti.sizes()).c_str(), dims(logits.sizes()).c_str());
+    if (ti.scalar_type() != at::kLong && ti.scalar_type() != at::kInt)
+        fail(Err::kValue, "%s: teacher_ids must be int32 or int64", what);
+    if (lse.has_value() && (lse->sizes() != lead || lse->scalar_type() != at::kFloat))
+        fail(Err::kValue, "%s: teacher_logsumexp must be float32 of shape %s", what, dims(lead).c_str());
+    t.k = tv.size(-1);
+    t.id_bytes = ti.scalar_type() == at::kLong ? 8 : 4;
+    t.values = tv.contiguous();
+    t.ids = ti.contiguous();
+    if (lse.has_value()) t.lse = lse->contiguous();
+    return t;
+}
+
+// stats: what the backward pass takes (empty where it is not asked for).
+std::tuple<at::Tensor, at::Tensor> distill_loss(const at::Tensor& logits, const at::Tensor& tv, const at::Tensor& ti,
+                                                const std::optional<at::Tensor>& lse, double t, bool stats) {
+    const char* what = "distill_loss";
+    mx_same_device(what, {&logits, &tv, &ti, opt(lse)});
+    const int dt = mx_dtype_code(logits.scalar_type());
+    c10::cuda::CUDAGuard guard(logits.device());
+    const at::Tensor l = logits_rows(what, logits);
+    const Teacher te = teacher_of(what, logits, tv, ti, lse);
+    at::Tensor loss = empty_like_device(logits.sizes().slice(0, logits.dim() - 1), at::kFloat, l);
+    at::Tensor st = empty_like_device({stats ? l.size(0) : 0, 4}, at::kFloat, l);
+    check(qmm_distill_loss(l.data_ptr(), l.stride(0), l.size(0), l.size(1), dt, te.values.data_ptr(), te.dtype,
+                           te.ids.data_ptr(), te.id_bytes, ptr_or_null<float>(te.lse), te.k, t,
+                           static_cast<float*>(loss.data_ptr()), stats ? st.data_ptr() : nullptr, logits_stream(l)),
+          what);
+    return {loss, st};
+}
+
+at::Tensor distill_backward(const at::Tensor& logits, const at::Tensor& tv, const at::Tensor& ti,
+                            const std::optional<at::Tensor>& lse, double t, const at::Tensor& stats,
+                            const at::Tensor& grad_loss) {
+    const char* what = "distill_backward";
+    mx_same_device(what, {&logits, &tv, &ti, opt(lse), &stats, &grad_loss});
+    const int dt = mx_dtype_code(logits.scalar_type());
+    c10::cuda::CUDAGuard guard(logits.device());
+    const at::Tensor l = logits_rows(what, logits);
+    const Teacher te = teacher_of(what, logits, tv, ti, lse);
+    if (stats.scalar_type() != at::kFloat || stats.numel() != 4 * l.size(0) || !stats.is_contiguous())
+        fail(Err::kValue, "%s: stats are not those of the loss", what);
+    if (grad_loss.numel() != l.size(0)) fail(Err::kValue, "%s: grad_loss must hold one number a row", what);
+    const at::Tensor g = grad_loss.to(at::kFloat).contiguous();
+    at::Tensor grad = empty_like_device(logits.sizes(), l.scalar_type(), l);
+    check(qmm_distill_backward(l.data_ptr(), l.stride(0), l.size(0), l.size(1), dt, te.values.data_ptr(), te.dtype,
+                               te.ids.data_ptr(), te.id_bytes, ptr_or_null<float>(te.lse), te.k, t, stats.data_ptr(),
+                               static_cast<const float*>(g.data_ptr()), grad.data_ptr(), l.size(1),
+                               logits_stream(l)),
+          what);
+    return grad;
+}
+
+// grad: a new tensor, or (out) one given, which may be the logits themselves.
+at::Tensor run_distill_loss_grad(const at::Tensor& logits, const at::Tensor& tv, const at::Tensor& ti,
+                                 const std::optional<at::Tensor>& weight, const std::optional<at::Tensor>& lse,
+                                 double t, at::Tensor& grad, bool given) {
+    const char* what = "distill_loss_and_grad";
+    mx_same_device(what, {&logits, &tv, &ti, opt(weight), opt(lse), given ? &grad : nullptr});
+    const int dt = mx_dtype_code(logits.scalar_type());
+    c10::cuda::CUDAGuard guard(logits.device());
+    const at::Tensor l = logits_rows(what, logits);
+    const at::IntArrayRef lead = logits.sizes().slice(0, logits.dim() - 1);
+    const Teacher te = teacher_of(what, logits, tv, ti, lse);
+    if (weight.has_value() && (weight->sizes() != lead || weight->scalar_type() != at::kFloat))
+        fail(Err::kValue, "%s: row_weight must be float32 of shape %s", what, dims(lead).c_str());
+    const at::Tensor w = weight.has_value() ? weight->contiguous() : at::Tensor();
+    if (given) {
+        if (grad.sizes() != logits.sizes() || grad.scalar_type() != logits.scalar_type() || !grad.is_contiguous())
+            fail(Err::kValue, "%s: out must be contiguous, of the logits' shape %s and dtype", what,
+                 dims(logits.sizes()).c_str());
+        // over the logits, or clear of everything that is read
+        const bool same = grad.data_ptr() == l.data_ptr() && l.stride(0) == l.size(1);
+        auto touches = [&](const at::Tensor& x, int64_t bytes) {
+            const char *a = static_cast<const char*>(grad.data_ptr()), *b = static_cast<const char*>(x.data_ptr());
+            return a < b + bytes && b < a + grad.numel() * grad.element_size();
+        };
+        auto clash = [&](const at::Tensor& x) { return x.defined() && touches(x, x.numel() * x.element_size()); };
+        const int64_t span = l.size(0) ? ((l.size(0) - 1) * l.stride(0) + l.size(1)) * l.element_size() : 0;
+        if ((!same && touches(l, span)) || clash(te.values) || clash(te.ids) || clash(te.lse) || clash(w))
+            fail(Err::kValue, "%s: out overlaps an argument without being the logits", what);
+    } else {
+        grad = empty_like_device(logits.sizes(), l.scalar_type(), l);
+    }
+    at::Tensor loss = empty_like_device(lead, at::kFloat, l);
+    check(qmm_distill_loss_grad(l.data_ptr(), l.stride(0), l.size(0), l.size(1), dt, te.values.data_ptr(), te.dtype,
+                                te.ids.data_ptr(), te.id_bytes, ptr_or_null<float>(te.lse), te.k, t,
+                                ptr_or_null<float>(w), static_cast<float*>(loss.data_ptr()), grad.data_ptr(),
+                                l.size(1), logits_stream(l)),
+          what);
+    return loss;
+}
+
+std::tuple<at::Tensor, at::Tensor> distill_loss_grad(const at::Tensor& logits, const at::Tensor& tv,
+                                                     const at::Tensor& ti, const std::optional<at::Tensor>& weight,
+                                                     const std::optional<at::Tensor>& lse, double t) {
+    at::Tensor grad;
+    at::Tensor loss = run_distill_loss_grad(logits, tv, ti, weight, lse, t, grad, false);
+    return {loss, grad};
+}
+
+at::Tensor distill_loss_grad_out(const at::Tensor& logits, const at::Tensor& tv, const at::Tensor& ti,
+                                 const std::optional<at::Tensor>& weight, const std::optional<at::Tensor>& lse,
+                                 double t, at::Tensor& grad) {
+    return run_distill_loss_grad(logits, tv, ti, weight, lse, t, grad, true);
+}
+
 // All-CPU arguments: the same error as a CPU tensor among CUDA ones.
 at::Tensor quantized_matmul_cpu(const at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&, int64_t,
                                 int64_t) {
@@ -405,6 +654,20 @@ TORCH_LIBRARY(mlxturbo_b200, m) {
     m.def("mx_matmul_out(Tensor x, Tensor? x_scales, Tensor w, Tensor scales, *, Tensor(a!) out) -> Tensor(a!)");
     m.def("mx_gather(Tensor x, Tensor? x_scales, Tensor w, Tensor scales, Tensor? lhs, Tensor rhs, ScalarType dtype, "
           "bool sorted) -> Tensor");
+    m.def("sample(Tensor logits, Tensor u, Tensor? temperature_rows, float temperature, Tensor? top_k_rows, int top_k, "
+          "Tensor? top_p_rows, float top_p, Tensor? min_p_rows, float min_p) -> Tensor");
+    m.def("topk(Tensor logits, int k, bool logsumexp, float temperature) -> (Tensor, Tensor, Tensor)");
+    m.def("speculative_sample(Tensor logits, Tensor draft_logits, Tensor draft_ids, Tensor u, "
+          "Tensor? temperature_rows, float temperature, Tensor? draft_temperature_rows, float draft_temperature) "
+          "-> (Tensor, Tensor)");
+    m.def("distill_loss(Tensor logits, Tensor teacher_values, Tensor teacher_ids, Tensor? teacher_logsumexp, "
+          "float temperature, bool stats) -> (Tensor, Tensor)");
+    m.def("distill_backward(Tensor logits, Tensor teacher_values, Tensor teacher_ids, Tensor? teacher_logsumexp, "
+          "float temperature, Tensor stats, Tensor grad_loss) -> Tensor");
+    m.def("distill_loss_grad(Tensor logits, Tensor teacher_values, Tensor teacher_ids, Tensor? row_weight, "
+          "Tensor? teacher_logsumexp, float temperature) -> (Tensor, Tensor)");
+    m.def("distill_loss_grad_out(Tensor logits, Tensor teacher_values, Tensor teacher_ids, Tensor? row_weight, "
+          "Tensor? teacher_logsumexp, float temperature, *, Tensor(a!) grad) -> Tensor");
 }
 
 // Per device, not for every dispatch key: autograd and the dispatch modes above
@@ -418,14 +681,26 @@ void mx_impl(torch::Library& m) {
     m.impl("mx_gather", &mx_gather);
 }
 
+void logits_impl(torch::Library& m) {
+    m.impl("sample", &sample);
+    m.impl("topk", &topk);
+    m.impl("speculative_sample", &speculative_sample);
+    m.impl("distill_loss", &distill_loss);
+    m.impl("distill_backward", &distill_backward);
+    m.impl("distill_loss_grad", &distill_loss_grad);
+    m.impl("distill_loss_grad_out", &distill_loss_grad_out);
+}
+
 TORCH_LIBRARY_IMPL(mlxturbo_b200, CUDA, m) {
     m.impl("quantized_matmul", &quantized_matmul);
     m.impl("quantized_matmul_out", &quantized_matmul_out);
     mx_impl(m);
+    logits_impl(m);
 }
 
 TORCH_LIBRARY_IMPL(mlxturbo_b200, CPU, m) {
     m.impl("quantized_matmul", &quantized_matmul_cpu);
     m.impl("quantized_matmul_out", &quantized_matmul_out_cpu);
     mx_impl(m);
+    logits_impl(m);
 }

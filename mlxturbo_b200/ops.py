@@ -537,6 +537,164 @@ def mx_matmul(xq: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor, scales:
                                flat[0], flat[1], dtype, bool(sorted_indices))
 
 
+# --------------------------------------------------------------------------
+# rows of logits
+# --------------------------------------------------------------------------
+
+class _LogitsOps:
+    """The overloads of the operators on rows of logits, looked up once."""
+
+    def __init__(self):
+        ops = _lib.torch_ops()
+        if ops is None:
+            raise ImportError(f"{_lib.TORCH_OPS_PATH} is not built; run `python -m mlxturbo_b200.build`")
+        self.sample = ops.sample.default
+        self.topk = ops.topk.default
+        self.speculative = ops.speculative_sample.default
+        self.distill = ops.distill_loss.default
+        self.distill_backward = ops.distill_backward.default
+        self.distill_grad = ops.distill_loss_grad.default
+        self.distill_grad_out = ops.distill_loss_grad_out.default
+
+
+_LOGITS: _LogitsOps | None = None
+
+
+def _logits_ops() -> _LogitsOps:
+    global _LOGITS
+    if _LOGITS is None:
+        _LOGITS = _LogitsOps()
+    return _LOGITS
+
+
+def _rows_or_one(x, other):
+    """(tensor or None, number) of a setting that is one number or a tensor of one a row."""
+    return (x, other) if isinstance(x, torch.Tensor) else (None, x)
+
+
+def sample(logits: torch.Tensor, u: torch.Tensor, *, temperature=1.0, top_k=0, top_p=1.0,
+           min_p=0.0) -> torch.Tensor:
+    """A token id (int64) for each row of logits [..., V], drawn with the uniform numbers u [...] in [0, 1).
+
+    With w = exp((logits - max) / temperature) and a row's tokens in the order
+    of (logit descending, id ascending): kept are the first ``top_k`` (0: all);
+    of these, as long as the mass before a token is below ``top_p`` times
+    theirs; and those with w >= ``min_p``.  The token is the first id, in the
+    order of ids, at which the kept weights add up to more than u times their
+    sum.  temperature=0 is the lowest id of the largest logit, as
+    ``argmax_from_keys`` gives it.  A logit of -inf is never drawn (a NaN counts
+    as one); a row of nothing else gives -1.
+
+    logits are bf16, fp16 or fp32, u float32.  Each setting is a number, or a
+    tensor of one a row (broadcast over the leading axes), where a temperature
+    below 0 is 0, a top_k below 1 and a top_p above 1 keep all.  The ids are
+    those of 64-bit arithmetic: equal arguments give equal ids, alone or in a
+    batch.
+    """
+    return _logits_ops().sample(logits, u, *_rows_or_one(temperature, 0.0), *_rows_or_one(top_k, 0),
+                                *_rows_or_one(top_p, 1.0), *_rows_or_one(min_p, 0.0))
+
+
+TOPK_MAX = 1024
+
+
+def topk(logits: torch.Tensor, k: int, *, logsumexp: bool = False, temperature: float = 1.0):
+    """(values, ids) of the k <= 1024 largest logits of each row [..., V], in the order of (value
+    descending, id ascending): values [..., k] in the logits' dtype, ids int64.  A NaN counts as -inf.
+
+    With ``logsumexp`` also the float32 [...] logarithm of the sum of
+    exp(logits / temperature): a teacher's side of ``distill_loss``.
+    """
+    values, ids, lse = _logits_ops().topk(logits, k, logsumexp, temperature)
+    return (values, ids, lse) if logsumexp else (values, ids)
+
+
+def speculative_sample(logits: torch.Tensor, draft_logits: torch.Tensor, draft_ids: torch.Tensor, u: torch.Tensor, *,
+                       temperature=1.0, draft_temperature=None) -> tuple[torch.Tensor, torch.Tensor]:
+    """Which drafted tokens stand, and the token after them: (tokens [..., n + 1], accepted [...]), int64.
+
+    logits [..., n + 1, V] are the model's at the n drafted positions and the
+    one after, draft_logits [..., n, V] what draft_ids [..., n] were drawn
+    from; an id outside [0, V) (-1) ends a shorter draft.  With
+    p = softmax(logits / temperature) and q = softmax(draft_logits /
+    draft_temperature) (default: temperature), token i stands while
+    u[..., i] * q(id) < p(id).  At the first that does not, a token is drawn,
+    as ``sample`` draws, with u[..., n] from max(p - q, 0); where the draft
+    ends, from p.  tokens are the standing ones, the drawn one, then -1.
+    Filters go into the logits of either side as -inf.  Temperatures are
+    numbers, or tensors of one a sequence; 0 puts everything on the lowest id
+    of the maximum.
+    """
+    if draft_temperature is None:
+        draft_temperature = temperature
+    return _logits_ops().speculative(logits, draft_logits, draft_ids, u, *_rows_or_one(temperature, 0.0),
+                                     *_rows_or_one(draft_temperature, 0.0))
+
+
+class _DistillLoss(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, teacher_values, teacher_ids, teacher_logsumexp, temperature):
+        loss, stats = _logits_ops().distill(logits, teacher_values, teacher_ids, teacher_logsumexp, temperature, True)
+        ctx.save_for_backward(logits, teacher_values, teacher_ids, teacher_logsumexp, stats)
+        ctx.temperature = temperature
+        return loss
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad_loss):
+        logits, teacher_values, teacher_ids, teacher_logsumexp, stats = ctx.saved_tensors
+        grad = _logits_ops().distill_backward(logits, teacher_values, teacher_ids, teacher_logsumexp,
+                                              ctx.temperature, stats, grad_loss)
+        return grad, None, None, None, None
+
+
+def _no_teacher_grad(*tensors) -> None:
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise NotImplementedError("the distillation loss has no gradient for the teacher's side; detach it")
+
+
+def distill_loss(logits: torch.Tensor, teacher_values: torch.Tensor, teacher_ids: torch.Tensor, *,
+                 temperature: float = 1.0, teacher_logsumexp: torch.Tensor | None = None) -> torch.Tensor:
+    """KL divergence (float32 [...]) of each row's softmax(logits / temperature) from a teacher's top logits.
+
+    logits are [..., V]; teacher_values and teacher_ids [..., k], k <= 512, as
+    ``topk`` gives them.  An id outside [0, V) is an empty place; an id listed
+    twice adds up.  The teacher's probabilities are those of the listed values,
+    renormalised; with ``teacher_logsumexp`` [...] (``topk`` with logsumexp=True
+    and the same temperature) they are taken as they are, and the rest of the
+    teacher's mass is compared with the model's on all tokens not listed.  A row
+    with nothing listed, or whose teacher_logsumexp is -inf, has loss 0.
+
+    Differentiable in the logits.  The gradient of a row whose incoming
+    gradient is 0 is 0, whatever its logits; the loss is not multiplied by
+    temperature squared.
+    """
+    _no_teacher_grad(teacher_values, teacher_logsumexp)
+    if torch.is_grad_enabled() and logits.requires_grad:
+        return _DistillLoss.apply(logits, teacher_values, teacher_ids, teacher_logsumexp, temperature)
+    return _logits_ops().distill(logits, teacher_values, teacher_ids, teacher_logsumexp, temperature, False)[0]
+
+
+def distill_loss_and_grad(logits: torch.Tensor, teacher_values: torch.Tensor, teacher_ids: torch.Tensor,
+                          row_weight: torch.Tensor | None = None, *, temperature: float = 1.0,
+                          teacher_logsumexp: torch.Tensor | None = None,
+                          out: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """``distill_loss`` and the gradient of sum(row_weight * loss) in the logits, in one launch.
+
+    Returns (loss [...], grad [..., V] in the logits' dtype); row_weight is
+    float32 [...] (None: 1).  For training in chunks of rows, where the logits
+    are read once and never kept; ``out`` may be the logits themselves.
+    Outside autograd: logits that require a gradient are refused.
+    """
+    _no_teacher_grad(teacher_values, teacher_logsumexp, row_weight)
+    if torch.is_grad_enabled() and logits.requires_grad:
+        raise NotImplementedError("distill_loss_and_grad is outside autograd: detach the logits, or use distill_loss")
+    args = (logits, teacher_values, teacher_ids, row_weight, teacher_logsumexp, temperature)
+    if out is None:
+        return _logits_ops().distill_grad(*args)
+    return _logits_ops().distill_grad_out(*args, grad=out), out
+
+
 def copy_(dst: torch.Tensor, src: torch.Tensor) -> torch.Tensor:
     """dst <- src with one kernel on the current stream of the CUDA side
     (qmm_copy_kernel), where one side is pinned host memory and the other a
