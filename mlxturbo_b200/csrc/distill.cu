@@ -140,9 +140,13 @@ QMM_DEVINL uint4 encode(const float (&x)[Elem<DT>::kVec]) {
     }
 }
 
+// A finite reference that the fast weights do not take: rows masked throughout
+// with a type's lowest value.
+QMM_DEVINL bool out_of_range(float ref) { return fabsf(ref) > kFastMax && fabsf(ref) < CUDART_INF_F; }
+
 // TAIL: the teacher's log-sum-exp is given.  MODE kBackward needs no cluster.
 template <int DT, bool TAIL, int MODE>
-__global__ void __launch_bounds__(kRowThreads) distill_kernel(const DistillArgs a, int C) {
+__global__ void __launch_bounds__(kRowThreads, 4) distill_kernel(const DistillArgs a, int C) {
     __shared__ DistillShared sh;
     extern __shared__ uint32_t marks[];  // TAIL: a byte to a vector of this CTA
     constexpr int N = Elem<DT>::kVec;
@@ -152,7 +156,7 @@ __global__ void __launch_bounds__(kRowThreads) distill_kernel(const DistillArgs 
     const int g = rank * kRowWarps + (threadIdx.x >> 5);
     const long long r = blockIdx.x / C;
     const Row<DT> row(a.logits, a.stride, r, a.V);
-    const Slice s = warp_slice(row.nv, g, warps);
+    const Slice s = warp_slice<DT>(row, g, warps);
     const int per = (row.nv + warps - 1) / warps, cta_begin = per * kRowWarps * rank;
     const int cta_end = cta_begin + per * kRowWarps;
     const Scale c(a.inv_t);
@@ -186,7 +190,7 @@ __global__ void __launch_bounds__(kRowThreads) distill_kernel(const DistillArgs 
         __syncthreads();
         LaneSum acc;
         const uint8_t* mark = reinterpret_cast<const uint8_t*>(marks);
-        const float top = stream_slice<DT, true, true>(row, s, c, acc, [&](int v, uint4& u) {
+        const float top = stream_slice<DT, true>(row, s, c, acc, [&](int v, uint4& u) {
             if (TAIL) {
                 const uint32_t m = mark[v - cta_begin];
                 if (m) take_out<DT>(u, m);
@@ -196,7 +200,19 @@ __global__ void __launch_bounds__(kRowThreads) distill_kernel(const DistillArgs 
         all_gather(cl, sh.tops, g, warp_max(top));
         cl.sync();
         ref = slots_max(sh.tops, warps);
-        all_gather(cl, sh.slots, g, warp_mass(acc, c, ref));
+        double share = warp_mass(acc, c, ref);
+        if (out_of_range(ref)) {
+            share = 0.0;
+            for_vectors_slow<DT>(row, s, [&](int v, uint4 u) {
+                if (TAIL && mark[v - cta_begin]) take_out<DT>(u, mark[v - cta_begin]);
+                float x[N];
+                decode<DT>(u, x);
+#pragma unroll
+                for (int j = 0; j < N; ++j) share += exp(((double)x[j] - (double)ref) * a.inv_t);
+            });
+            share = warp_sum(share);
+        }
+        all_gather(cl, sh.slots, g, share);
         cl.sync();
         const double s_ref = ref == -CUDART_INF_F ? 0.0 : slots_sum(sh.slots, warps);
         // the list's part of the sum
@@ -258,13 +274,24 @@ __global__ void __launch_bounds__(kRowThreads) distill_kernel(const DistillArgs 
     if (factor == 0.0f) {  // a row that carries no loss, or one whose other tokens get none: whatever their logits
         const float zero[N] = {};
         for (int v = s.begin + s.lane; v < s.end; v += 32) store(v, zero);
+        if (s.lane == 0 && s.head >= 0) store(s.head, zero);
+        if (s.lane == 0 && s.tail >= 0) store(s.tail, zero);
         if (weight == 0.0f) return;
+    } else if (out_of_range(ref)) {
+        for_vectors_slow<DT>(row, s, [&](int v, const uint4& u) {
+            float x[N];
+            decode<DT>(u, x);
+#pragma unroll
+            for (int j = 0; j < N; ++j) x[j] = (float)(scale * others * exp(((double)x[j] - (double)ref) * a.inv_t));
+            store(v, x);
+        });
     } else {
+        const float e = ceilf(ref * c.c), scaled = (float)(scale * others * c.against(e, ref));
         for_vectors<DT>(row, s, [&](int v, const uint4& u) {
             float x[N];
             decode<DT>(u, x);
 #pragma unroll
-            for (int j = 0; j < N; ++j) x[j] = factor * ex2(c.exponent(below<true>(x[j], ref)));
+            for (int j = 0; j < N; ++j) x[j] = scaled * ex2(fmaf(x[j], c.c, -e));
             store(v, x);
         });
     }

@@ -60,6 +60,7 @@ struct Row {
     QMM_DEVINL int first(int v) const { return v * Elem<DT>::kVec - shift; }
     QMM_DEVINL bool whole(int v) const { return first(v) >= 0 && first(v) <= V - Elem<DT>::kVec; }
     QMM_DEVINL uint4 load(int v) const;  // elements outside the row read as -infinity
+    QMM_DEVINL uint4 load_whole(int v) const;
     QMM_DEVINL float at(int i) const;
 };
 
@@ -80,8 +81,13 @@ QMM_DEVINL uint32_t neg_inf_word() {
 }
 
 template <int DT>
+QMM_DEVINL uint4 Row<DT>::load_whole(int v) const {
+    return ld_row_v4(base + 16LL * v);
+}
+
+template <int DT>
 QMM_DEVINL uint4 Row<DT>::load(int v) const {
-    if (whole(v)) return ld_row_v4(base + 16LL * v);
+    if (whole(v)) return load_whole(v);
     const int f = first(v);
     uint32_t w[4];
 #pragma unroll
@@ -169,49 +175,77 @@ QMM_DEVINL int key_id(unsigned long long k) { return (int)(0xFFFFFFFFu - (uint32
 
 // ---- weights exp((x - max) / T) ----------------------------------------------------
 
-// In 64 bits.  The largest logit weighs 1 even where it is infinite.
-QMM_DEVINL double weight64(float x, float mx, double inv_t) {
-    if (x == mx) return 1.0;
-    const double w = exp(((double)x - (double)mx) * inv_t);
-    return w == w ? w : 0.0;  // NaN logits, and the others beside +infinity
-}
-
 QMM_DEVINL float ex2(float a) {
     float r;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(a));
     return r;
 }
 
-// log2(e) / T in two floats: the exponent of a fast weight is off by one
-// rounding, not by a multiple of the constant's own.
-struct Scale {
-    float hi, lo;
-    QMM_DEVINL explicit Scale(double inv_t) {
-        const double c = inv_t * 1.4426950408889634;
-        hi = (float)c;
-        lo = (float)(c - (double)hi);
+// In 64 bits: 2^t, t = (x - max) log2(e) / T, as a table's 2^(j/32) times the
+// Taylor polynomial of 2^r, |r| <= 1/64 (the term left out is below 3e-15),
+// with the whole part added to the exponent: 11 operations of the 64-bit pipe,
+// where exp() takes about twice that.  The largest logit weighs 1 even where it
+// is infinite; NaN weighs nothing.
+struct Weight64 {
+    const double* table;  // 2^(j/32), j = 0 .. 31, in shared memory
+    double c, b, inv_t;
+    float mx;
+
+    QMM_DEVINL Weight64(const double* table_, float mx_, double inv_t_)
+        : table(table_), c(inv_t_ * 1.4426950408889634), b(-(double)mx_ * c), inv_t(inv_t_), mx(mx_) {}
+
+    QMM_DEVINL double operator()(float x) const {
+        if (x == mx) return 1.0;
+        const double t = fma((double)x, c, b);
+        if (!(t > -1000.0)) {  // next to nothing, or no number
+            const double w = exp(((double)x - (double)mx) * inv_t);
+            return w == w ? w : 0.0;
+        }
+        const double magic = 6755399441055744.0 / 32.0;  // 1.5 * 2^52 / 32: sums are whole 32nds
+        const double k = t + magic;
+        const double r = t - (k - magic);
+        const int n = __double2loint(k);
+        // ln2^i / i!
+        double p = fma(r, 1.3333558146428443e-3, 9.618129107628477e-3);
+        p = fma(r, p, 5.550410866482158e-2);
+        p = fma(r, p, 2.4022650695910072e-1);
+        p = fma(r, p, 6.931471805599453e-1);
+        p = fma(r, p, 1.0) * table[n & 31];
+        return __hiloint2double(__double2hiint(p) + ((n >> 5) << 20), __double2loint(p));
     }
-    QMM_DEVINL float exponent(float d) const { return fmaf(d, hi, d * lo); }
 };
 
-// Differences from the maximum end here: what a masked logit (-infinity, the
-// type's lowest value) leaves is a finite exponent and no weight.
-constexpr float kFarBelow = -1e30f;
-// Temperatures of the fast sums: within them an exponent of kFarBelow is
-// finite and weighs nothing.
-constexpr double kFastMinT = 1e-6, kFastMaxT = 1e20;
-// Bound of the relative error of a fast sum.  A weight: difference and
-// exponent rounded once each, |a| ln2 2^-23, where the weighted mean of |a| is
-// at most about log2(V) + 2 <= 25: 2.1e-6; ex2.approx 2^-22; up to 8 rescalings
-// of a lane's sum, 8 * 2^-22 at worst.  A lane's sum: five roundings within a
-// batch of 4 vectors and one per batch, 64 batches at most: 69 * 2^-24 =
-// 4.1e-6.  Together 8.4e-6 < 2^-16.
-constexpr double kFastEps = 1.0 / 65536.0;
-constexpr int kFastVectors = 256;  // vectors to a lane
+QMM_DEVINL void fill_table(double* table) {
+    if (threadIdx.x < 32) table[threadIdx.x] = exp2((double)threadIdx.x / 32.0);
+}
 
-// Running maximum and sum of weights of one lane.
+// Fast weights: 2^(x c - E) with c = log2(e) / T in 32 bits and a whole number
+// E, so one multiply-add, and every change of reference is exact.
+// Bound of the relative error of a fast sum: the exponent's rounding and c's
+// own, |a| ln2 (2^-24 + 2^-25) with a weighted mean of |a| of at most about
+// log2(V) + 2 <= 30: 1.9e-6; ex2.approx 2^-22; five roundings within a batch of
+// 4 vectors, 3.0e-7; batches are added in 64 bits.  Together 2.5e-6 < 2^-18.
+constexpr double kFastEps = 1.0 / 262144.0;
+// It stands for finite maxima up to kFastMax and these temperatures: exponents
+// stay finite.  Beyond, or where a NaN or an infinity enters, a sum comes out as
+// NaN or outside [0.5, inf) and is made in 64 bits.
+constexpr float kFastMax = 1e29f;
+constexpr double kFastMinT = 1e-6, kFastMaxT = 1e6;
+
+struct Scale {
+    float c;
+    QMM_DEVINL explicit Scale(double inv_t) : c((float)(inv_t * 1.4426950408889634)) {}
+    // what turns a sum against E into one against the weight of mx
+    QMM_DEVINL double against(float e, float mx) const { return exp2((double)e - (double)mx * (double)c); }
+    QMM_DEVINL bool fast(float mx, double T) const {
+        return fabsf(mx) <= kFastMax && T >= kFastMinT && T <= kFastMaxT;
+    }
+};
+
+// Sum of weights of one lane against its reference E.
 struct LaneSum {
-    float m = -3.402823466e38f, s = 0.0f;  // the lowest finite value: differences from it are no NaN
+    float e = -3e38f;
+    double s = 0.0;
 };
 
 template <int N>
@@ -225,60 +259,123 @@ QMM_DEVINL float tree_sum(float (&e)[N]) {
 
 // ---- a cluster's slices --------------------------------------------------------------
 
+// The vectors of a warp.  Those from `begin` to `end` lie whole within the row,
+// lane l takes begin + l, begin + l + 32, ..; the row's first and last vector,
+// where they stick out of it, are `head` and `tail` (or -1) of the warp they
+// fall to, and lane 0's.
 struct Slice {
-    int begin, end;  // vectors of this warp
+    int begin, end, head, tail;
     int lane;
 };
 
-QMM_DEVINL Slice warp_slice(int nv, int warp, int warps) {
-    const int per = (nv + warps - 1) / warps;
+template <int DT>
+QMM_DEVINL Slice warp_slice(const Row<DT>& row, int warp, int warps) {
+    const int per = (row.nv + warps - 1) / warps;
     const long long b = (long long)per * warp;
     Slice s;
-    s.begin = (int)(b < nv ? b : nv);
-    s.end = (int)(b + per < nv ? b + per : nv);
+    s.begin = (int)(b < row.nv ? b : row.nv);
+    s.end = (int)(b + per < row.nv ? b + per : row.nv);
     s.lane = threadIdx.x & 31;
+    s.head = s.tail = -1;
+    if (s.begin < s.end && s.begin == 0 && !row.whole(0)) {
+        s.head = 0;
+        ++s.begin;
+    }
+    if (s.begin < s.end && s.end == row.nv && !row.whole(row.nv - 1)) s.tail = --s.end;
     return s;
 }
 
-// f(vector index, vector) over the warp's slice, four loads in flight to a lane.
+// f(vectors, first index, how many) over the warp's slice: batches of 4 vectors
+// 32 apart, the next batch's loads issued before f is called on this one.
 template <int DT, typename F>
-QMM_DEVINL void for_vectors(const Row<DT>& row, const Slice& s, F&& f) {
+QMM_DEVINL void for_batches(const Row<DT>& row, const Slice& s, F&& f) {
+    using Four = std::integral_constant<int, 4>;
+    using One = std::integral_constant<int, 1>;
     int v = s.begin + s.lane;
-    for (; v + 96 < s.end; v += 128) {
-        uint4 u[4];
+    if (v + 96 < s.end) {
+        uint4 next[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) u[i] = row.load(v + 32 * i);
+        for (int i = 0; i < 4; ++i) next[i] = row.load_whole(v + 32 * i);
+        do {
+            uint4 u[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) f(v + 32 * i, u[i]);
+            for (int i = 0; i < 4; ++i) u[i] = next[i];
+            const int at = v;
+            v += 128;
+            if (v + 96 < s.end) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) next[i] = row.load_whole(v + 32 * i);
+            }
+            f(u, at, Four());
+        } while (v + 96 < s.end);
     }
-    for (; v < s.end; v += 32) f(v, row.load(v));
+    if (v < s.end) {  // up to 4 more
+        uint4 u[4];
+        u[0] = row.load_whole(v);
+#pragma unroll
+        for (int i = 1; i < 4; ++i)
+            if (v + 32 * i < s.end) u[i] = row.load_whole(v + 32 * i);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (v + 32 * i < s.end) f(&u[i], v + 32 * i, One());
+    }
+    if (s.lane == 0) {
+        if (s.head >= 0) {
+            uint4 u = row.load(s.head);
+            f(&u, s.head, One());
+        }
+        if (s.tail >= 0) {
+            uint4 u = row.load(s.tail);
+            f(&u, s.tail, One());
+        }
+    }
 }
 
-// x - m, not below kFarBelow.  A NaN is far below too, or with NAN_THROUGH stays one.
-template <bool NAN_THROUGH>
-QMM_DEVINL float below(float x, float m) {
-    if (!NAN_THROUGH) return fmaxf(x - m, kFarBelow);
-    float r;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(x - m), "f"(kFarBelow));
-    return r;
+// f(vector index, vector) over the warp's slice.
+template <int DT, typename F>
+QMM_DEVINL void for_vectors(const Row<DT>& row, const Slice& s, F&& f) {
+    for_batches<DT>(row, s, [&](uint4* u, int v, auto n_) {
+#pragma unroll
+        for (int i = 0; i < decltype(n_)::value; ++i) f(v + 32 * i, u[i]);
+    });
+}
+
+// The same, a vector at a time with the next one on its way: for passes whose
+// arithmetic in 64 bits outlasts the loads, in few registers.
+template <int DT, typename F>
+QMM_DEVINL void for_vectors_slow(const Row<DT>& row, const Slice& s, F&& f) {
+    const int first = s.head >= 0 ? s.head : s.begin, last = s.tail >= 0 ? s.tail + 1 : s.end;
+    int v = first + s.lane;
+    uint4 next = make_uint4(0, 0, 0, 0);
+    if (v < last) next = row.load(v);
+#pragma unroll 1
+    for (; v < last; v += 32) {
+        const uint4 u = next;
+        if (v + 32 < last) next = row.load(v + 32);
+        f(v, u);
+    }
 }
 
 // Maximum of the slice's logits in this lane, and with SUM the lane's weights.
 // change(vector index, vector) may take elements out (set them to -infinity).
-template <int DT, bool SUM, bool NAN_THROUGH, typename F>
+template <int DT, bool SUM, typename F>
 QMM_DEVINL float stream_slice(const Row<DT>& row, const Slice& s, const Scale& c, LaneSum& acc, F&& change) {
     constexpr int N = Elem<DT>::kVec;
     float top = -CUDART_INF_F;
-    auto batch = [&](const uint4* u, auto n_) {
+    for_batches<DT>(row, s, [&](uint4* u, int v, auto n_) {
         constexpr int n = decltype(n_)::value;
-        float bm = -CUDART_INF_F;
 #pragma unroll
-        for (int i = 0; i < n; ++i) bm = fmaxf(bm, vec_max<DT>(u[i]));
+        for (int i = 0; i < n; ++i) change(v + 32 * i, u[i]);
+        float bm = vec_max<DT>(u[0]);
+#pragma unroll
+        for (int i = 1; i < n; ++i) bm = fmaxf(bm, vec_max<DT>(u[i]));
         top = fmaxf(top, bm);
         if (!SUM) return;
-        if (bm > acc.m) {
-            acc.s *= ex2(c.exponent(below<false>(acc.m, bm)));
-            acc.m = bm;
+        const float t = bm * c.c;
+        if (t > acc.e + 16.0f) {  // weights stay below 2^17
+            const float e = ceilf(t);
+            acc.s *= (double)ex2(acc.e - e);
+            acc.e = e;
         }
         float sum = 0.0f;
 #pragma unroll
@@ -286,31 +383,17 @@ QMM_DEVINL float stream_slice(const Row<DT>& row, const Slice& s, const Scale& c
             float e[N];
             decode<DT>(u[i], e);
 #pragma unroll
-            for (int j = 0; j < N; ++j) e[j] = ex2(c.exponent(below<NAN_THROUGH>(e[j], acc.m)));
+            for (int j = 0; j < N; ++j) e[j] = ex2(fmaf(e[j], c.c, -acc.e));
             sum += tree_sum<N>(e);
         }
-        acc.s += sum;
-    };
-    int v = s.begin + s.lane;
-    for (; v + 96 < s.end; v += 128) {
-        uint4 u[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) u[i] = row.load(v + 32 * i);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) change(v + 32 * i, u[i]);
-        batch(u, std::integral_constant<int, 4>());
-    }
-    for (; v < s.end; v += 32) {
-        uint4 u = row.load(v);
-        change(v, u);
-        batch(&u, std::integral_constant<int, 1>());
-    }
+        acc.s += (double)sum;
+    });
     return top;
 }
 
 template <int DT, bool SUM>
 QMM_DEVINL float stream_slice(const Row<DT>& row, const Slice& s, const Scale& c, LaneSum& acc) {
-    return stream_slice<DT, SUM, false>(row, s, c, acc, [](int, uint4&) {});
+    return stream_slice<DT, SUM>(row, s, c, acc, [](int, uint4&) {});
 }
 
 // ---- exchange between the warps of a cluster ---------------------------------------------
@@ -355,9 +438,10 @@ QMM_DEVINL float slots_max(const float* slots, int n) {
     return warp_max(x);
 }
 
-// A warp's sum of weights against the row's maximum mx.
+// A warp's sum of weights against the weight of mx, the row's maximum.
 QMM_DEVINL double warp_mass(const LaneSum& acc, const Scale& c, float mx) {
-    return warp_sum((double)acc.s * (double)ex2(c.exponent(below<false>(acc.m, mx))));
+    const float e = ceilf(mx * c.c);
+    return warp_sum(acc.s * (double)ex2(acc.e - e)) * c.against(e, mx);
 }
 
 // The first slot at which the running sum passes `target`, or the last slot
@@ -420,20 +504,21 @@ struct Found {
 template <int DT, typename W>
 QMM_DEVINL Found find_in_slice(const Row<DT>& row, const Slice& s, double base, double target, W&& weight) {
     constexpr int N = Elem<DT>::kVec;
+    const int first = s.head >= 0 ? s.head : s.begin, last = s.tail >= 0 ? s.tail + 1 : s.end;
     Found found{-1, 0.0, 0.0};
     uint4 next = make_uint4(0, 0, 0, 0);
-    if (s.begin + s.lane < s.end) next = row.load(s.begin + s.lane);
-    for (int v0 = s.begin; v0 < s.end; v0 += 32) {
+    if (first + s.lane < last) next = row.load(first + s.lane);
+    for (int v0 = first; v0 < last; v0 += 32) {
         const int v = v0 + s.lane;
         const uint4 cur = next;
-        if (v + 32 < s.end) next = row.load(v + 32);
+        if (v + 32 < last) next = row.load(v + 32);
         double w[N], mine = 0.0;
         float x[N];
         decode<DT>(cur, x);
 #pragma unroll
         for (int j = 0; j < N; ++j) {
             const int id = row.first(v) + j;
-            w[j] = v < s.end && id >= 0 && id < row.V ? weight(id, x[j]) : 0.0;
+            w[j] = v < last && id >= 0 && id < row.V ? weight(id, x[j]) : 0.0;
             mine += w[j];
         }
         double incl = mine;

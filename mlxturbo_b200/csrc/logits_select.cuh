@@ -23,6 +23,7 @@ struct SelectShared {
     uint32_t hist[256];
     uint32_t n_cand, bound, sel_bin, sel_above;
     double scan[kRowWarps];
+    double table[32];  // of Weight64
     unsigned long long best;
     int verdict;
 };
@@ -84,32 +85,38 @@ QMM_DEVINL uint32_t kth_prefix(SelectShared& sh, int n, int k) {
 }
 
 // Candidates: every token with key32 >= bound, found again by the warps whose
-// lanes' maxima reach it (lane `owner` holds the slice's vectors owner, owner +
-// 32, ..).  They go to CTA 0's list in any order; returns how many this warp
-// found.  The list's own count may pass kCand; no more than that are written.
+// lanes' maxima reach it (lane `owner` holds the slice's vectors begin + owner,
+// begin + owner + 32, ..).  They go to CTA 0's list in any order; returns how
+// many this warp found.  The list's own count may pass kCand; no more than that
+// are written.
 template <int DT>
 QMM_DEVINL uint32_t push_candidates(cg::cluster_group& cl, SelectShared& sh, const Row<DT>& row, const Slice& s,
                                     float top, uint32_t bound) {
     constexpr int N = Elem<DT>::kVec;
-    unsigned owners = __ballot_sync(~0u, key32(top) >= bound && s.begin + s.lane < s.end);
+    unsigned owners = __ballot_sync(~0u, key32(top) >= bound);
     uint32_t* count = cl.map_shared_rank(&sh.n_cand, 0);
     unsigned long long* list = cl.map_shared_rank(sh.cand, 0);
     uint32_t found = 0;
+    auto take = [&](const uint4& u, int v) {
+        float x[N];
+        decode<DT>(u, x);
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            const int id = row.first(v) + j;
+            if (id < 0 || id >= row.V || key32(x[j]) < bound) continue;
+            ++found;
+            const uint32_t at = atomicAdd(count, 1u);
+            if (at < kCand) list[at] = row_key(x[j], id);
+        }
+    };
+    if (s.lane == 0 && (owners & 1u)) {
+        if (s.head >= 0) take(row.load(s.head), s.head);
+        if (s.tail >= 0) take(row.load(s.tail), s.tail);
+    }
     while (owners) {
         const int owner = __ffs(owners) - 1;
         owners &= owners - 1;
-        for (int v = s.begin + owner + 32 * s.lane; v < s.end; v += 32 * 32) {
-            float x[N];
-            decode<DT>(row.load(v), x);
-#pragma unroll
-            for (int j = 0; j < N; ++j) {
-                const int id = row.first(v) + j;
-                if (id < 0 || id >= row.V || key32(x[j]) < bound) continue;
-                ++found;
-                const uint32_t at = atomicAdd(count, 1u);
-                if (at < kCand) list[at] = row_key(x[j], id);
-            }
-        }
+        for (int v = s.begin + owner + 32 * s.lane; v < s.end; v += 32 * 32) take(row.load_whole(v), v);
     }
     return warp_sum(found);
 }
@@ -136,20 +143,91 @@ QMM_DEVINL void sort_candidates(unsigned long long* k, int n) {
     }
 }
 
-// The border key: the largest key b in [lo, hi) such that the tokens with keys
-// >= b reach `target` (their number, or with MASS the sum of their weights in
-// 64 bits); lo if all of them do not.  All warps of the cluster; the rounds cut
-// the range into eight and end when one token is left in it, 22 rounds at most.
+// The CTA's sum, the same in every thread.
+QMM_DEVINL double cta_sum(SelectShared& sh, double x) {
+    x = warp_sum(x);
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) sh.scan[threadIdx.x >> 5] = x;
+    __syncthreads();
+    x = 0.0;
+    for (int i = 0; i < kRowWarps; ++i) x += sh.scan[i];
+    return x;
+}
+
+// Running sums over the sorted candidates' weights, in place, by the whole CTA.
+QMM_DEVINL void scan_weights(SelectShared& sh, int n) {
+    const int per = (n + kRowThreads - 1) / kRowThreads, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int b = threadIdx.x * per, e = b + per < n ? b + per : n;
+    double run = 0.0;
+    for (int i = b; i < e; ++i) run += sh.w[i];
+    double incl = run;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const double y = __shfl_up_sync(~0u, incl, o);
+        if (lane >= o) incl += y;
+    }
+    if (lane == 31) sh.scan[warp] = incl;
+    __syncthreads();
+    double base = incl - run;
+    for (int i = 0; i < warp; ++i) base += sh.scan[i];
+    for (int i = b; i < e; ++i) {
+        base += sh.w[i];
+        sh.w[i] = base;
+    }
+    __syncthreads();
+}
+
+// ---- borders by search -------------------------------------------------------------
+//
+// The border of a count or a mass: the first token of the order at which the
+// tokens from the top on, of those with keys >= floor, reach it.  Rounds of one
+// pass each: eight pivots cut the range that holds the border, and only tokens
+// within the range are counted and weighed (in 64 bits); from the second round
+// on that is a small part of them.  Once few enough are left they go to CTA 0,
+// which sorts them and runs through them.
+//
+// kInRange: sorting 512 costs about as much as one more round.
+constexpr uint32_t kInRange = 512;
+
+// A pivot between two logits' values, in the order of keys.
+QMM_DEVINL uint32_t between(uint32_t lo, uint32_t hi, int j, bool by_value) {
+    const uint32_t step = (hi - lo) / 8, even = lo + (step > 0 ? step * j : j);
+    if (!by_value) return even;
+    const float a = key32_value(lo), b = key32_value(hi);
+    const float v = a + (b - a) * (0.125f * j);
+    const uint32_t k = key32(v);  // NaN (infinite ends): kKeyNegInf, which the caller clamps
+    return k > lo && k < hi ? k : even;
+}
+
+// MASS: `want` is a part of the mass of all tokens >= floor, else a count.
+// Returns the border key; floor if the tokens do not reach it.  All threads of
+// the cluster; every thread returns the same.
 template <int DT, bool MASS>
 QMM_DEVINL unsigned long long border_key(cg::cluster_group& cl, SelectShared& sh, const Row<DT>& row, const Slice& s,
-                                         int g, int warps, float mx, double inv_t, unsigned long long lo,
-                                         unsigned long long hi, double target) {
+                                         int g, int warps, const Weight64& weight, unsigned long long floor,
+                                         double want) {
     constexpr int N = Elem<DT>::kVec;
-    uint32_t in_lo = 0xFFFFFFFFu, in_hi = 0;
-    cl.sync();  // the shared arrays' earlier readers
-    for (int round = 0; hi - lo > 1 && in_lo - in_hi > 1; ++round) {
-        const unsigned long long step = (hi - lo) / 8 > 0 ? (hi - lo) / 8 : 1;
-        // pivots lo + j step, j = 0 .. 7, below hi
+    const int rank = (int)cl.block_rank();
+    uint32_t lo = (uint32_t)(floor >> 32), hi = key32(weight.mx) + 1, inside = 0xFFFFFFFFu;
+    double above = 0.0, target = want;  // measure of the keys from hi on
+    cl.sync();                          // the shared arrays' earlier readers
+    for (int round = 0; round == 0 || (hi - lo > 1 && inside > kInRange); ++round) {
+        // pivot 0 is lo; the first round looks where weights are, later ones cut values, or keys, evenly
+        uint32_t p[8];
+        p[0] = lo;
+#pragma unroll
+        for (int j = 1; j < 8; ++j) {
+            if (round == 0 && MASS) {
+                // 24, 16, 11, 8, 5.5, 3.5, 1.5 temperatures below the maximum
+                const float depth = j == 1 ? 24.f : j == 2 ? 16.f : j == 3 ? 11.f : j == 4 ? 8.f : j == 5 ? 5.5f
+                                    : j == 6 ? 3.5f : 1.5f;
+                p[j] = key32(weight.mx - depth / (float)weight.inv_t);
+            } else {
+                p[j] = between(lo, hi, j, round < 8 && (round & 1) == (MASS ? 1 : 0));
+            }
+            p[j] = max(p[j], p[j - 1]);
+            p[j] = min(p[j], hi);
+        }
         uint32_t n[8];
         double m[8];
 #pragma unroll
@@ -157,19 +235,18 @@ QMM_DEVINL unsigned long long border_key(cg::cluster_group& cl, SelectShared& sh
             n[j] = 0;
             m[j] = 0.0;
         }
-        for_vectors<DT>(row, s, [&](int v, const uint4& u) {
+        for_vectors_slow<DT>(row, s, [&](int v, const uint4& u) {
             float x[N];
             decode<DT>(u, x);
 #pragma unroll
             for (int e = 0; e < N; ++e) {
                 const int id = row.first(v) + e;
-                if (id < 0 || id >= row.V) continue;
-                const unsigned long long k = row_key(x[e], id);
-                if (k < lo) continue;
-                const double w = MASS ? weight64(x[e], mx, inv_t) : 0.0;
+                const uint32_t k = key32(x[e]);
+                if (k < lo || k >= hi || id < 0 || id >= row.V || row_key(x[e], id) < floor) continue;
+                const double w = MASS ? weight(x[e]) : 0.0;
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
-                    if (k >= lo + j * step) {
+                    if (k >= p[j]) {
                         ++n[j];
                         if (MASS) m[j] += w;
                     }
@@ -192,28 +269,132 @@ QMM_DEVINL unsigned long long border_key(cg::cluster_group& cl, SelectShared& sh
             }
         }
         cl.sync();
-        // lane j < 8 of every warp: pivot j's totals, in the order of warps
+        // lanes j, j + 8, .. of every warp: pivot j's totals, in a fixed order
         uint32_t tn = 0;
         double tm = 0.0;
-        if (s.lane < 8) {
-            for (int i = 0; i < warps; ++i) {
-                tn += sh.piv_count[buf][i][s.lane];
-                if (MASS) tm += sh.piv_mass[buf][i][s.lane];
-            }
+        for (int i = s.lane >> 3; i < warps; i += 4) {
+            tn += sh.piv_count[buf][i][s.lane & 7];
+            if (MASS) tm += sh.piv_mass[buf][i][s.lane & 7];
         }
-        const bool reach = s.lane < 8 && lo + s.lane * step < hi && (MASS ? tm : (double)tn) >= target;
-        const unsigned reached = __ballot_sync(~0u, reach);
-        if (!(reached & 1u)) return lo;  // not even all of them: first round only
-        const int at = 31 - __clz(reached);
-        in_lo = __shfl_sync(~0u, tn, at);
-        const unsigned long long base = lo;
-        lo = base + at * step;
-        if (at < 7 && base + (at + 1) * step < hi) {
-            hi = base + (at + 1) * step;
-            in_hi = __shfl_sync(~0u, tn, at + 1);
+#pragma unroll
+        for (int o = 8; o <= 16; o <<= 1) {
+            tn += __shfl_xor_sync(~0u, tn, o);
+            if (MASS) tm += __shfl_xor_sync(~0u, tm, o);
+        }
+        const double got = above + (MASS ? tm : (double)tn);
+        if (round == 0 && MASS) target = fmax(want * __shfl_sync(~0u, got, 0), 1e-300);
+        const unsigned reached = __ballot_sync(~0u, got >= target) & 0xFFu;
+        if (!(reached & 1u)) return floor;  // not even all of them: the first round
+        const int at = 31 - __clz(reached), nxt = at < 7 ? at + 1 : 7;
+        const uint32_t n_at = __shfl_sync(~0u, tn, at), n_next = __shfl_sync(~0u, tn, nxt);
+        const double got_next = __shfl_sync(~0u, got, nxt);
+        uint32_t p_at = p[0], p_next = hi;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            if (j == at) p_at = p[j];
+            if (j == at + 1) p_next = p[j];
+        }
+        lo = p_at;
+        inside = n_at;
+        if (at < 7) {
+            hi = p_next;
+            inside -= n_next;
+            above = got_next;
         }
     }
-    return lo;
+    if (inside > kInRange) {
+        // one logit's value, more often than the list is long: the first of them by id.  Equal weights: a count.
+        const double w = weight(key32_value(lo));
+        double need = MASS ? ceil((target - above) / w) : target - above;
+        if (MASS) {  // the quotient's rounding
+            while (need > 1.0 && above + (need - 1.0) * w >= target) need -= 1.0;
+            while (above + need * w < target && need < (double)inside) need += 1.0;
+        }
+        unsigned long long a = (unsigned long long)lo << 32, b = (unsigned long long)(lo + 1) << 32;
+        if (floor > a) a = floor;
+        for (int round = 0; b - a > 1; ++round) {  // the largest key with `need` tokens from it on
+            const unsigned long long step = (b - a) / 8 > 0 ? (b - a) / 8 : 1;
+            uint32_t n[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) n[j] = 0;
+            for_vectors_slow<DT>(row, s, [&](int v, const uint4& u) {
+                float x[N];
+                decode<DT>(u, x);
+#pragma unroll
+                for (int e = 0; e < N; ++e) {
+                    const int id = row.first(v) + e;
+                    if (key32(x[e]) != lo || id < 0 || id >= row.V) continue;
+                    const unsigned long long k = row_key(x[e], id);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                        if (k >= a + j * step) ++n[j];
+                }
+            });
+            const int buf = round & 1;
+            if (round == 0) cl.sync();
+#pragma unroll
+            for (int j = 0; j < 8; ++j) n[j] = warp_sum(n[j]);
+            if (s.lane < (int)cl.num_blocks()) {
+                uint32_t* pn = cl.map_shared_rank(sh.piv_count[buf][g], s.lane);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) pn[j] = n[j];
+            }
+            cl.sync();
+            uint32_t tn = 0;
+            for (int i = s.lane >> 3; i < warps; i += 4) tn += sh.piv_count[buf][i][s.lane & 7];
+#pragma unroll
+            for (int o = 8; o <= 16; o <<= 1) tn += __shfl_xor_sync(~0u, tn, o);
+            const unsigned reached =
+                __ballot_sync(~0u, a + (s.lane & 7) * step < b && (double)tn >= need) & 0xFFu;
+            if (!(reached & 1u)) return a;
+            const int at = 31 - __clz(reached);
+            const unsigned long long from = a;
+            a = from + at * step;
+            if (at < 7 && from + (at + 1) * step < b) b = from + (at + 1) * step;
+        }
+        return a;
+    }
+    // the tokens left, in order
+    cl.sync();
+    if (rank == 0 && threadIdx.x == 0) sh.n_cand = 0;
+    cl.sync();
+    uint32_t* count = cl.map_shared_rank(&sh.n_cand, 0);
+    unsigned long long* list = cl.map_shared_rank(sh.cand, 0);
+    for_vectors_slow<DT>(row, s, [&](int v, const uint4& u) {
+        float x[N];
+        decode<DT>(u, x);
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+            const int id = row.first(v) + e;
+            const uint32_t k = key32(x[e]);
+            if (k < lo || k >= hi || id < 0 || id >= row.V || row_key(x[e], id) < floor) continue;
+            const uint32_t at = atomicAdd(count, 1u);
+            if (at < kCand) list[at] = row_key(x[e], id);
+        }
+    });
+    cl.sync();
+    if (rank == 0) {
+        const int n = (int)sh.n_cand;
+        sort_candidates(sh.cand, n);
+        if (MASS) {
+            for (int i = threadIdx.x; i < n; i += kRowThreads) sh.w[i] = weight(key32_value((uint32_t)(sh.cand[i] >> 32)));
+            __syncthreads();
+            scan_weights(sh, n);
+        }
+        int first = MASS ? n - 1 : (int)(target - above) - 1;  // the token at which the target is reached
+        if (MASS) {
+            int b = 0, e = n - 1;
+            while (b < e) {
+                const int mid = (b + e) / 2;
+                if (above + sh.w[mid] >= target) e = mid;
+                else b = mid + 1;
+            }
+            first = b;
+        }
+        if (threadIdx.x < cl.num_blocks()) *cl.map_shared_rank(&sh.best, threadIdx.x) = sh.cand[first];
+    }
+    cl.sync();
+    return sh.best;
 }
 
 }  // namespace qmm

@@ -13,6 +13,7 @@
 // a bound on their error; only a row whose decision lies within that bound of
 // a border takes a second pass in 64 bits.
 
+#include <stdlib.h>
 #include "logits_select.cuh"
 
 namespace qmm {
@@ -21,29 +22,6 @@ namespace qmm {
 // the border, but more kept tokens than it draws from itself; not enough of them.
 enum { kDone, kNeedSum, kBorder, kGeneral };
 constexpr int kDrawHere = 2 * kRowThreads;
-
-// Running sums over the sorted candidates' weights, in place, by the whole CTA.
-QMM_DEVINL void scan_weights(SelectShared& sh, int n) {
-    const int per = (n + kRowThreads - 1) / kRowThreads, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int b = threadIdx.x * per, e = b + per < n ? b + per : n;
-    double run = 0.0;
-    for (int i = b; i < e; ++i) run += sh.w[i];
-    double incl = run;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const double y = __shfl_up_sync(~0u, incl, o);
-        if (lane >= o) incl += y;
-    }
-    if (lane == 31) sh.scan[warp] = incl;
-    __syncthreads();
-    double base = incl - run;
-    for (int i = 0; i < warp; ++i) base += sh.scan[i];
-    for (int i = b; i < e; ++i) {
-        base += sh.w[i];
-        sh.w[i] = base;
-    }
-    __syncthreads();
-}
 
 // How many of the first n running sums stand before `limit`: the tokens whose
 // mass before them (the sum of the one above) is below it.  The first always is.
@@ -58,16 +36,17 @@ QMM_DEVINL int count_before(const double* sums, int n, double limit) {
 }
 
 template <int DT>
-__global__ void __launch_bounds__(kRowThreads) sample_kernel(const SampleArgs a) {
+__global__ void __launch_bounds__(kRowThreads, 4) sample_kernel(const SampleArgs a) {
     __shared__ SelectShared sh;
     cg::cluster_group cl = cg::this_cluster();
     cl.barrier_arrive();  // waited for before the first access to another CTA
     if (threadIdx.x == 0) sh.n_cand = 0;
+    fill_table(sh.table);
     const int C = (int)cl.num_blocks(), rank = (int)cl.block_rank(), warps = C * kRowWarps;
     const int g = rank * kRowWarps + (threadIdx.x >> 5);
     const long long r = blockIdx.x / C;
     const Row<DT> row(a.logits, a.stride, r, a.V);
-    const Slice s = warp_slice(row.nv, g, warps);
+    const Slice s = warp_slice<DT>(row, g, warps);
 
     double T = a.t_rows ? (double)a.t_rows[r] : a.t;
     const bool greedy = !(T > 0.0);
@@ -99,8 +78,8 @@ __global__ void __launch_bounds__(kRowThreads) sample_kernel(const SampleArgs a)
         if (rank == 0 && threadIdx.x == 0) a.ids[r] = -1;
         return;
     }
-    bool fast = sum && mx < CUDART_INF_F && T >= kFastMinT && T <= kFastMaxT &&
-                (row.nv + warps - 1) / warps <= 32 * kFastVectors;
+    bool fast = sum && c.fast(mx, T);
+    const Weight64 weight(sh.table, mx, inv_t);
 
     // the warps' masses against the row's maximum, to every CTA
     if (sum) {
@@ -114,8 +93,8 @@ __global__ void __launch_bounds__(kRowThreads) sample_kernel(const SampleArgs a)
         uint32_t b = guess == guess && key32(guess) > kmin ? key32(guess) : kmin;
         const uint32_t top_key = key32(mx);
         if (b > top_key) b = top_key;
-        while (b > kmin && weight64(key32_value(b - 1), mx, inv_t) >= mp) --b;
-        while (b < top_key && weight64(key32_value(b), mx, inv_t) < mp) ++b;
+        while (b > kmin && weight(key32_value(b - 1)) >= mp) --b;
+        while (b < top_key && weight(key32_value(b)) < mp) ++b;
         kmin = b;
     }
     // Top-k without top-p: tokens below min-p play no part.
@@ -134,7 +113,7 @@ __global__ void __launch_bounds__(kRowThreads) sample_kernel(const SampleArgs a)
         cl.sync();
     }
     double total = sum ? slots_sum(sh.slots[0], warps) : 0.0;
-    if (!(total >= 0.5)) fast = false;  // NaN, or a pass that missed the maximum: 64 bits
+    if (!(total >= 0.5 && total < CUDART_INF)) fast = false;  // 64 bits
     unsigned long long border = (unsigned long long)kmin << 32;
     bool bordered = false;
 
@@ -153,18 +132,25 @@ __global__ void __launch_bounds__(kRowThreads) sample_kernel(const SampleArgs a)
             double eps = k_on ? 0.0 : fast ? kFastEps : 1.0;
             for (;;) {
                 if (rank == 0) {
-                    if (!sorted) {
+                    int verdict = kDone;
+                    if (!k_on && p_on && bound > kmin && eps < 1.0 && !sorted) {
+                        // an open row: the list is far from top_p, and is not worth its sorting
+                        double listed_mass = 0.0;
+                        for (int i = threadIdx.x; i < (int)n; i += kRowThreads)
+                            listed_mass += weight(key32_value((uint32_t)(sh.cand[i] >> 32)));
+                        if (cta_sum(sh, listed_mass) < p * total * (1.0 - 2.0 * eps)) verdict = kGeneral;
+                    }
+                    int kept = (int)n;
+                    if (verdict == kDone && !sorted) {
                         sort_candidates(sh.cand, (int)n);
                         for (int i = threadIdx.x; i < (int)n; i += kRowThreads)
-                            sh.w[i] = weight64(key32_value((uint32_t)(sh.cand[i] >> 32)), mx, inv_t);
+                            sh.w[i] = weight(key32_value((uint32_t)(sh.cand[i] >> 32)));
                         __syncthreads();
                         scan_weights(sh, (int)n);
                         sorted = true;
                     }
-                    int verdict = kDone;
-                    int kept = (int)n;
                     if (k_on && k < kept) kept = k;
-                    if (p_on) {
+                    if (p_on && verdict == kDone) {
                         const double all = k_on ? sh.w[kept - 1] : total;
                         const int lo = count_before(sh.w, kept, p * all * (1.0 - eps));
                         const int hi = count_before(sh.w, kept, p * all * (1.0 + eps));
@@ -228,11 +214,11 @@ __global__ void __launch_bounds__(kRowThreads) sample_kernel(const SampleArgs a)
                 }
                 // the row's sum in 64 bits, then again
                 double mass = 0.0;
-                for_vectors<DT>(row, s, [&](int v, const uint4& q) {
+                for_vectors_slow<DT>(row, s, [&](int v, const uint4& q) {
                     float x[Elem<DT>::kVec];
                     decode<DT>(q, x);
 #pragma unroll
-                    for (int j = 0; j < Elem<DT>::kVec; ++j) mass += x[j] == x[j] ? weight64(x[j], mx, inv_t) : 0.0;
+                    for (int j = 0; j < Elem<DT>::kVec; ++j) mass += weight(x[j]);
                 });
                 all_gather(cl, sh.slots[1], g, warp_sum(mass));
                 cl.sync();
@@ -246,9 +232,7 @@ __global__ void __launch_bounds__(kRowThreads) sample_kernel(const SampleArgs a)
         const double target = u * total, slack = 2.0 * kFastEps * total;
         const Place at = locate(sh.slots[0], warps, target);
         if (g == at.g) {
-            const Found f = find_in_slice<DT>(row, s, at.base, target, [&](int, float x) {
-                return weight64(x, mx, inv_t);
-            });
+            const Found f = find_in_slice<DT>(row, s, at.base, target, [&](int, float x) { return weight(x); });
             const bool sure = f.id >= 0 && f.before + slack <= target && f.after - slack > target;
             if (sure && s.lane == 0) a.ids[r] = f.id;
             if (s.lane < C) *cl.map_shared_rank(&sh.verdict, s.lane) = sure ? kDone : kGeneral;
@@ -258,40 +242,23 @@ __global__ void __launch_bounds__(kRowThreads) sample_kernel(const SampleArgs a)
     }
 
     // the general way: borders by search, masses and place in 64 bits
-    const unsigned long long lo = (unsigned long long)(kKeyNegInf + 1) << 32;
-    const unsigned long long hi = ((unsigned long long)key32(mx) + 1) << 32;
     if (select && !bordered) {
-        unsigned long long first = lo;
-        if (k_on) first = border_key<DT, false>(cl, sh, row, s, g, warps, mx, inv_t, lo, hi, (double)k);
-        if (p_on) {
-            double mass = 0.0;
-            for_vectors<DT>(row, s, [&](int v, const uint4& q) {
-                float x[Elem<DT>::kVec];
-                decode<DT>(q, x);
-#pragma unroll
-                for (int j = 0; j < Elem<DT>::kVec; ++j) {
-                    const int id = row.first(v) + j;
-                    if (id >= 0 && id < row.V && row_key(x[j], id) >= first) mass += weight64(x[j], mx, inv_t);
-                }
-            });
-            cl.sync();
-            all_gather(cl, sh.slots[1], g, warp_sum(mass));
-            cl.sync();
-            first = border_key<DT, true>(cl, sh, row, s, g, warps, mx, inv_t, first, hi,
-                                         fmax(p * slots_sum(sh.slots[1], warps), 1e-300));
-        }
-        if (first > border) border = first;
+        unsigned long long from = (unsigned long long)(kKeyNegInf + 1) << 32;
+        if (k_on) from = border_key<DT, false>(cl, sh, row, s, g, warps, weight, from, (double)k);
+        if (p_on) from = border_key<DT, true>(cl, sh, row, s, g, warps, weight, from, p);
+        if (from > border) border = from;
     }
-    auto weight = [&](int id, float x) { return row_key(x, id) >= border ? weight64(x, mx, inv_t) : 0.0; };
+    const uint32_t border32 = (uint32_t)(border >> 32);
+    auto kept = [&](int id, float x) {
+        const uint32_t k32 = key32(x);
+        return k32 < border32 || (k32 == border32 && row_key(x, id) < border) ? 0.0 : weight(x);
+    };
     double mass = 0.0;
-    for_vectors<DT>(row, s, [&](int v, const uint4& q) {
+    for_vectors_slow<DT>(row, s, [&](int v, const uint4& q) {
         float x[Elem<DT>::kVec];
         decode<DT>(q, x);
 #pragma unroll
-        for (int j = 0; j < Elem<DT>::kVec; ++j) {
-            const int id = row.first(v) + j;
-            if (id >= 0 && id < row.V) mass += weight(id, x[j]);
-        }
+        for (int j = 0; j < Elem<DT>::kVec; ++j) mass += kept(row.first(v) + j, x[j]);  // -infinity past the ends
     });
     cl.sync();
     all_gather(cl, sh.slots[0], g, warp_sum(mass));
@@ -299,7 +266,7 @@ __global__ void __launch_bounds__(kRowThreads) sample_kernel(const SampleArgs a)
     const double target = u * slots_sum(sh.slots[0], warps);
     const Place at = locate(sh.slots[0], warps, target);
     if (g == at.g) {
-        const Found f = find_in_slice<DT>(row, s, at.base, target, weight);
+        const Found f = find_in_slice<DT>(row, s, at.base, target, kept);
         if (s.lane == 0) a.ids[r] = f.id;
     }
 }
@@ -310,6 +277,7 @@ namespace qmm_host {
 
 int row_cluster(long long rows, long long V, int elem_bytes) {
     const long long vecs = (V * elem_bytes + 15) / 16;
+    if (const char* e = getenv("QMM_C")) return atoi(e);
     int C = 1;
     // up to 16 vectors to a lane; a call of few rows goes down to 2 vectors as long as SMs are idle
     while (C < 8 && vecs > 16LL * C * qmm::kRowThreads) C *= 2;

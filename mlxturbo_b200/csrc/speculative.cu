@@ -30,7 +30,7 @@ QMM_DEVINL double spec_temperature(const SpecArgs& a, long long b, bool draft) {
 }
 
 template <int DT>
-__global__ void __launch_bounds__(kRowThreads) spec_stats_kernel(const SpecArgs a) {
+__global__ void __launch_bounds__(kRowThreads, 4) spec_stats_kernel(const SpecArgs a) {
     __shared__ float tops[kMaxRowWarps];
     __shared__ double slots[kMaxRowWarps];
     __shared__ int args[kMaxRowWarps];
@@ -54,28 +54,29 @@ __global__ void __launch_bounds__(kRowThreads) spec_stats_kernel(const SpecArgs 
         return;
     }
     const Row<DT> row = spec_row<DT>(a, b, i);
-    const Slice s = warp_slice(row.nv, g, warps);
+    const Slice s = warp_slice<DT>(row, g, warps);
     const double T = spec_temperature(a, b, draft);
     const bool greedy = !(T > 0.0);
     const Scale c(greedy ? 1.0 : 1.0 / T);
     LaneSum acc;
     const float top = greedy ? stream_slice<DT, false>(row, s, c, acc) : stream_slice<DT, true>(row, s, c, acc);
     cl.barrier_wait();
-    all_gather(cl, tops, g, warp_max(top));
+    const float wtop = warp_max(top);
+    all_gather(cl, tops, g, wtop);
     cl.sync();
     const float mx = slots_max(tops, warps);
     if (greedy) {
         int first = 0x7FFFFFFF;
-        if (top == mx) {
-            for (int v = s.begin + s.lane; v < s.end && first == 0x7FFFFFFF; v += 32) {
+        if (wtop == mx) {  // the warp's share again
+            for_vectors_slow<DT>(row, s, [&](int v, const uint4& q) {
                 float x[Elem<DT>::kVec];
-                decode<DT>(row.load(v), x);
+                decode<DT>(q, x);
 #pragma unroll
-                for (int j = Elem<DT>::kVec - 1; j >= 0; --j) {
+                for (int j = 0; j < Elem<DT>::kVec; ++j) {
                     const int id = row.first(v) + j;
-                    if (x[j] == mx && id >= 0 && id < a.V) first = id;
+                    if (x[j] == mx && id >= 0 && id < a.V) first = min(first, id);
                 }
-            }
+            });
         }
         all_gather(cl, args, g, __reduce_min_sync(~0u, first));
     } else {
@@ -93,9 +94,7 @@ __global__ void __launch_bounds__(kRowThreads) spec_stats_kernel(const SpecArgs 
             st.arg = __reduce_min_sync(~0u, first);
         } else {
             const double total = slots_sum(slots, warps);
-            const bool fast = T >= kFastMinT && T <= kFastMaxT && (row.nv + warps - 1) / warps <= 32 * kFastVectors &&
-                              mx < CUDART_INF_F && mx > -CUDART_INF_F && total >= 0.5;
-            st.sum = fast ? total : CUDART_NAN;
+            st.sum = c.fast(mx, T) && total >= 0.5 && total < CUDART_INF ? total : CUDART_NAN;
         }
         if (s.lane == 0) a.stats[at] = st;
     }
@@ -106,20 +105,19 @@ template <int DT>
 struct Dist {
     Row<DT> row;
     RowStat st;
-    double inv_t;
     bool greedy;
+    Weight64 exact;
 
-    QMM_DEVINL Dist(const SpecArgs& a, long long b, int i)
-        : row(spec_row<DT>(a, b, i)), st(a.stats[b * (2 * a.n + 1) + i]) {
-        const double T = spec_temperature(a, b, i > a.n);
-        greedy = !(T > 0.0);
-        inv_t = greedy ? 1.0 : 1.0 / T;
+    QMM_DEVINL Dist(const SpecArgs& a, long long b, int i, const double* table)
+        : row(spec_row<DT>(a, b, i)), st(a.stats[b * (2 * a.n + 1) + i]),
+          greedy(!(spec_temperature(a, b, i > a.n) > 0.0)),
+          exact(table, st.mx, greedy ? 1.0 : 1.0 / spec_temperature(a, b, i > a.n)) {
         if (dead()) st.sum = 1.0;
     }
     QMM_DEVINL double weight(int id, float x) const {
         if (dead()) return 0.0;
         if (greedy) return id == st.arg ? 1.0 : 0.0;
-        return x == x ? weight64(x, st.mx, inv_t) : 0.0;
+        return exact(x);
     }
     // against the sum at hand: exact weights, over a sum that may be a fast one
     QMM_DEVINL double prob(int id, float x) const { return weight(id, x) / st.sum; }
@@ -131,8 +129,8 @@ template <int DT>
 QMM_DEVINL void exact_sum(cg::cluster_group& cl, double* slots, Dist<DT>& d, int g, int warps) {
     if (d.greedy || d.dead()) return;
     double mass = 0.0;
-    const Slice s = warp_slice(d.row.nv, g, warps);
-    for_vectors<DT>(d.row, s, [&](int v, const uint4& q) {
+    const Slice s = warp_slice<DT>(d.row, g, warps);
+    for_vectors_slow<DT>(d.row, s, [&](int v, const uint4& q) {
         float x[Elem<DT>::kVec];
         decode<DT>(q, x);
 #pragma unroll
@@ -162,9 +160,11 @@ QMM_DEVINL void paired(const Row<DT>& p, const Row<DT>& q, int v, float (&y)[Ele
 }
 
 template <int DT>
-__global__ void __launch_bounds__(kRowThreads) spec_decide_kernel(const SpecArgs a) {
+__global__ void __launch_bounds__(kRowThreads, 2) spec_decide_kernel(const SpecArgs a) {
     __shared__ double slots[kMaxRowWarps];
     __shared__ int sure_flag;
+    __shared__ double table[32];
+    fill_table(table);
     constexpr int N = Elem<DT>::kVec;
     cg::cluster_group cl = cg::this_cluster();
     cl.sync();  // every CTA is there before its memory is written
@@ -187,10 +187,10 @@ __global__ void __launch_bounds__(kRowThreads) spec_decide_kernel(const SpecArgs
                 bool before = true;  // rows past the draft's end have no sums
                 for (int j = taken; j < i; ++j) before = before && ids[j] >= 0 && ids[j] < a.V;
                 if (before) {
-                    const Dist<DT> p(a, b, i), q(a, b, a.n + 1 + i);
+                    const Dist<DT> p(a, b, i, table), q(a, b, a.n + 1 + i, table);
                     const double wp = p.weight((int)d, p.row.at((int)d)), wq = q.weight((int)d, q.row.at((int)d));
                     const double left = (double)u[i] * wq / q.st.sum, right = wp / p.st.sum;
-                    const double slack = (p.greedy && q.greedy ? 0.0 : 4.0 * kFastEps) * (left + right);
+                    const double slack = (p.greedy && q.greedy ? 0.0 : 1.5 * kFastEps) * (left + right);
                     if (wp == 0.0) state = kFails;  // whatever the sums
                     else if (left + slack < right) state = kStands;
                     else if (left - slack >= right) state = kFails;
@@ -204,7 +204,7 @@ __global__ void __launch_bounds__(kRowThreads) spec_decide_kernel(const SpecArgs
         if (at == 32) continue;
         state = __shfl_sync(~0u, state, at);
         if (state == kOpen) {
-            Dist<DT> p(a, b, taken), q(a, b, a.n + 1 + taken);
+            Dist<DT> p(a, b, taken, table), q(a, b, a.n + 1 + taken, table);
             exact_sum<DT>(cl, slots, p, g, warps);
             exact_sum<DT>(cl, slots, q, g, warps);
             const int d = (int)ids[taken];
@@ -219,9 +219,9 @@ __global__ void __launch_bounds__(kRowThreads) spec_decide_kernel(const SpecArgs
     }
 
     // the draw
-    Dist<DT> p(a, b, taken);
-    Dist<DT> q(a, b, drafted ? a.n + 1 + taken : taken);
-    const Slice s = warp_slice(p.row.nv, g, warps);
+    Dist<DT> p(a, b, taken, table);
+    Dist<DT> q(a, b, drafted ? a.n + 1 + taken : taken, table);
+    const Slice s = warp_slice<DT>(p.row, g, warps);
     const double draw = (double)u[a.n];
     int token = -1;
     bool mine = false;  // this lane writes the token
@@ -236,7 +236,7 @@ __global__ void __launch_bounds__(kRowThreads) spec_decide_kernel(const SpecArgs
         }
         double mass = 0.0;
         if (exact || p.greedy || q.greedy) {
-            for_vectors<DT>(p.row, s, [&](int v, const uint4& w) {
+            for_vectors_slow<DT>(p.row, s, [&](int v, const uint4& w) {
                 float x[N], y[N];
                 decode<DT>(w, x);
                 if (minus) paired<DT>(p.row, q.row, v, y);
@@ -248,16 +248,17 @@ __global__ void __launch_bounds__(kRowThreads) spec_decide_kernel(const SpecArgs
                 }
             });
         } else {
-            const Scale cp(p.inv_t), cq(q.inv_t);
-            const float fp = (float)(1.0 / p.st.sum), fq = (float)(1.0 / q.st.sum);
+            const Scale cp(p.exact.inv_t), cq(q.exact.inv_t);
+            const float ep = ceilf(p.st.mx * cp.c), eq = ceilf(q.st.mx * cq.c);
+            const float fp = (float)(cp.against(ep, p.st.mx) / p.st.sum), fq = (float)(cq.against(eq, q.st.mx) / q.st.sum);
             for_vectors<DT>(p.row, s, [&](int v, const uint4& w) {
                 float x[N], y[N];
                 decode<DT>(w, x);
                 if (minus) paired<DT>(p.row, q.row, v, y);
 #pragma unroll
                 for (int j = 0; j < N; ++j) {
-                    x[j] = fp * ex2(cp.exponent(below<false>(x[j], p.st.mx)));
-                    if (minus) x[j] = fmaxf(x[j] - fq * ex2(cq.exponent(below<false>(y[j], q.st.mx))), 0.0f);
+                    x[j] = fp * ex2(fmaf(x[j], cp.c, -ep));
+                    if (minus) x[j] = fmaxf(x[j] - fq * ex2(fmaf(y[j], cq.c, -eq)), 0.0f);
                 }
                 mass += (double)tree_sum<N>(x);
             });

@@ -14,16 +14,17 @@
 namespace qmm {
 
 template <int DT, bool LSE>
-__global__ void __launch_bounds__(kRowThreads) topk_kernel(const TopkArgs a) {
+__global__ void __launch_bounds__(kRowThreads, 4) topk_kernel(const TopkArgs a) {
     __shared__ SelectShared sh;
     cg::cluster_group cl = cg::this_cluster();
     cl.barrier_arrive();  // waited for before the first access to another CTA
     if (threadIdx.x == 0) sh.n_cand = 0;
+    if (LSE) fill_table(sh.table);
     const int C = (int)cl.num_blocks(), rank = (int)cl.block_rank(), warps = C * kRowWarps;
     const int g = rank * kRowWarps + (threadIdx.x >> 5);
     const long long r = blockIdx.x / C;
     const Row<DT> row(a.logits, a.stride, r, a.V);
-    const Slice s = warp_slice(row.nv, g, warps);
+    const Slice s = warp_slice<DT>(row, g, warps);
     const Scale c(a.inv_t);
 
     LaneSum acc;
@@ -49,8 +50,21 @@ __global__ void __launch_bounds__(kRowThreads) topk_kernel(const TopkArgs a) {
     } else {
         cl.sync();
     }
+    double total = LSE ? slots_sum(sh.slots[0], warps) : 0.0;
+    const Weight64 weight(sh.table, mx, a.inv_t);
+    if (LSE && fabsf(mx) != CUDART_INF_F && !(c.fast(mx, 1.0 / a.inv_t) && total >= 0.5 && total < CUDART_INF)) {
+        double mass = 0.0;  // a NaN among the logits, or none above a mask's lowest value
+        for_vectors_slow<DT>(row, s, [&](int, const uint4& q) {
+            float x[Elem<DT>::kVec];
+            decode<DT>(q, x);
+#pragma unroll
+            for (int j = 0; j < Elem<DT>::kVec; ++j) mass += weight(x[j]);
+        });
+        all_gather(cl, sh.slots[1], g, warp_sum(mass));
+        cl.sync();
+        total = slots_sum(sh.slots[1], warps);
+    }
     if (LSE && rank == 0 && threadIdx.x < 32) {
-        const double total = slots_sum(sh.slots[0], warps);
         // no finite maximum: the sum is that of the largest alone
         const double l = mx == -CUDART_INF_F || mx == CUDART_INF_F ? (double)mx : (double)mx * a.inv_t + log(total);
         if (threadIdx.x == 0) a.lse[r] = (float)l;
@@ -65,13 +79,16 @@ __global__ void __launch_bounds__(kRowThreads) topk_kernel(const TopkArgs a) {
         n = warp_sum(n);
     }
     if (n > kCand) {  // the border, then the k tokens from it on
-        const unsigned long long border =
-            border_key<DT, false>(cl, sh, row, s, g, warps, 0.0f, 1.0, 0ull, ~0ull, (double)a.k);
+        // the search takes logits up to its maximum: infinite ones too
+        const unsigned long long border = border_key<DT, false>(cl, sh, row, s, g, warps,
+                                                                Weight64(sh.table, CUDART_INF_F, 1.0),
+                                                                (unsigned long long)kKeyNegInf << 32, (double)a.k);
+        cl.sync();
         if (threadIdx.x == 0) sh.n_cand = 0;
         cl.sync();
         uint32_t* count = cl.map_shared_rank(&sh.n_cand, 0);
         unsigned long long* list = cl.map_shared_rank(sh.cand, 0);
-        for_vectors<DT>(row, s, [&](int v, const uint4& q) {
+        for_vectors_slow<DT>(row, s, [&](int v, const uint4& q) {
             float x[Elem<DT>::kVec];
             decode<DT>(q, x);
 #pragma unroll
