@@ -24,94 +24,104 @@
 
 namespace qmm {
 
+// A CTA: eight warps read logits, a ninth works through the list meanwhile.
+constexpr int kDistillThreads = kRowThreads + 32;
+
 struct DistillShared {
     double logp[kMaxList];
     float x[kMaxList];   // the student's logits of the list
     int id[kMaxList];    // or -1
     int slot[kMaxList];  // place in the table of distinct ids
     int table[2 * kMaxList], owner[2 * kMaxList];
-    double slots[kMaxRowWarps];
-    float tops[kMaxRowWarps];
-    double red[kRowWarps];
-    double top_ref;
-    int twice;
+    WarpStat stats[kMaxRowWarps];
+    double mass;   // sum p
+    double cross;  // sum p (log p - l / tau)
+    double part;   // sum over distinct listed tokens of exp((l - best) / tau)
+    float best;    // largest listed logit
+    int twice;     // an id is listed more than once
 };
 
-// Sum or maximum over the CTA, the same in every thread and every run.
-template <bool MAX>
-QMM_DEVINL double cta_reduce(double* red, double x) {
-#pragma unroll
-    for (int o = 16; o >= 1; o >>= 1) {
-        const double y = __shfl_xor_sync(~0u, x, o);
-        x = MAX ? (y > x ? y : x) : x + y;
-    }
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = x;
-    __syncthreads();
-    x = red[0];
-    for (int i = 1; i < kRowWarps; ++i) x = MAX ? (red[i] > x ? red[i] : x) : x + red[i];
-    return x;
-}
-
-// The list into shared memory: ids, log p, the student's logits; duplicates
-// share a slot whose owner is the first of them.  Returns sum p.
-template <int DT>
-QMM_DEVINL double load_list(const DistillArgs& a, DistillShared& sh, const Row<DT>& row, long long r) {
-    int size = 2;
-    while (size < 2 * a.k) size <<= 1;
-    for (int i = threadIdx.x; i < size; i += kRowThreads) {
-        sh.table[i] = -1;
-        sh.owner[i] = kMaxList;
-    }
-    if (threadIdx.x == 0) sh.twice = 0;
-    __syncthreads();
-    double best = -CUDART_INF;
-    for (int j = threadIdx.x; j < a.k; j += kRowThreads) {
+// The ids of the list, by one warp.
+QMM_DEVINL void list_ids(const DistillArgs& a, DistillShared& sh, long long r) {
+    for (int j = threadIdx.x & 31; j < a.k; j += 32) {
         const long long at = r * a.k + j;
         const long long id = a.ti_bytes == 8 ? static_cast<const long long*>(a.ti)[at]
                                              : (long long)static_cast<const int*>(a.ti)[at];
+        sh.id[j] = id >= 0 && id < a.V ? (int)id : -1;
+    }
+    __syncwarp();
+}
+
+// The rest of it, by one warp: log p and the student's logits; entries of one
+// id share a slot whose owner is the first of them; the sums.
+template <int DT>
+QMM_DEVINL void list_sums(const DistillArgs& a, DistillShared& sh, const Row<DT>& row, long long r) {
+    const int lane = threadIdx.x & 31;
+    int size = 2;
+    while (size < 2 * a.k) size <<= 1;
+    for (int i = lane; i < size; i += 32) {
+        sh.table[i] = -1;
+        sh.owner[i] = kMaxList;
+    }
+    __syncwarp();
+    double top = -CUDART_INF;
+    float best = -CUDART_INF_F;
+    bool twice = false;
+    for (int j = lane; j < a.k; j += 32) {
+        const long long at = r * a.k + j;
+        const int id = sh.id[j];
         const float t = a.tv_dtype == 2 ? elem_f32<2>(a.tv, at) : a.tv_dtype == 1 ? elem_f32<1>(a.tv, at)
                                                                                  : elem_f32<0>(a.tv, at);
-        const bool in = id >= 0 && id < a.V;
-        sh.id[j] = in ? (int)id : -1;
-        sh.x[j] = in ? row.at((int)id) : 0.0f;
-        const double l = in ? (double)t * a.inv_t : -CUDART_INF;
+        const float x = id >= 0 ? row.at(id) : 0.0f;
+        sh.x[j] = x;
+        const double l = id >= 0 ? (double)t * a.inv_t : -CUDART_INF;
         sh.logp[j] = l;
-        best = fmax(best, l);  // a NaN shows in the sum
-        if (in) {
+        top = fmax(top, l);  // a NaN shows in the sums
+        if (id >= 0) {
+            best = fmaxf(best, x);
             int h = (int)((uint32_t)id * 2654435761u >> 16) & (size - 1);
             for (;;) {
-                const int was = atomicCAS(&sh.table[h], -1, (int)id);
-                if (was == -1 || was == (int)id) {
-                    if (was != -1) sh.twice = 1;
-                    break;
-                }
+                const int was = atomicCAS(&sh.table[h], -1, id);
+                twice |= was == id;
+                if (was == -1 || was == id) break;
                 h = (h + 1) & (size - 1);
             }
             sh.slot[j] = h;
             atomicMin(&sh.owner[h], j);
         }
     }
-    double norm;
+    __syncwarp();
+#pragma unroll
+    for (int o = 16; o >= 1; o >>= 1) top = fmax(top, __shfl_xor_sync(~0u, top, o));
+    best = warp_max(best);
+    double norm = 0.0;
     if (a.tlse) {
         norm = (double)a.tlse[r];
-    } else {
-        const double m = cta_reduce<true>(sh.red, best);
-        if (m == -CUDART_INF) {
-            norm = 0.0;  // nothing listed
-        } else {
-            double sum = 0.0;
-            for (int j = threadIdx.x; j < a.k; j += kRowThreads) sum += exp(sh.logp[j] - m);
-            sum = cta_reduce<false>(sh.red, sum);
-            norm = m + log(sum);
-        }
+    } else if (top != -CUDART_INF) {  // else nothing is listed
+        double sum = 0.0;
+        for (int j = lane; j < a.k; j += 32) sum += exp(sh.logp[j] - top);
+        norm = top + log(warp_sum(sum));
     }
-    double mass = 0.0;
-    for (int j = threadIdx.x; j < a.k; j += kRowThreads) {
-        sh.logp[j] -= norm;
-        mass += exp(sh.logp[j]);
+    double mass = 0.0, cross = 0.0, part = 0.0;
+    for (int j = lane; j < a.k; j += 32) {
+        const double lp = sh.logp[j] - norm, p = exp(lp);
+        sh.logp[j] = lp;
+        mass += p;
+        if (sh.id[j] < 0) continue;
+        if (p != 0.0) cross += p * (lp - (double)sh.x[j] * a.inv_t);
+        if (sh.owner[sh.slot[j]] == j) part += exp(((double)sh.x[j] - (double)best) * a.inv_t);
     }
-    return cta_reduce<false>(sh.red, mass);
+    mass = warp_sum(mass);
+    cross = warp_sum(cross);
+    part = warp_sum(part);
+    twice = __any_sync(~0u, twice);
+    if (lane == 0) {
+        sh.mass = mass;
+        sh.cross = cross;
+        sh.part = part;
+        sh.best = best;
+        sh.twice = twice;
+    }
 }
 
 // Every listed element of this vector set to -infinity; bit j of m is element j.
@@ -146,91 +156,103 @@ QMM_DEVINL bool out_of_range(float ref) { return fabsf(ref) > kFastMax && fabsf(
 
 // TAIL: the teacher's log-sum-exp is given.  MODE kBackward needs no cluster.
 template <int DT, bool TAIL, int MODE>
-__global__ void __launch_bounds__(kRowThreads, 4) distill_kernel(const DistillArgs a, int C) {
+__global__ void __launch_bounds__(kDistillThreads, MODE == kLossGrad ? 3 : 4)
+    distill_kernel(const DistillArgs a, int C) {
     __shared__ DistillShared sh;
     extern __shared__ uint32_t marks[];  // TAIL: a byte to a vector of this CTA
     constexpr int N = Elem<DT>::kVec;
     cg::cluster_group cl = cg::this_cluster();
     if (MODE != kBackward) cl.barrier_arrive();
-    const int rank = (int)(blockIdx.x % C), warps = C * kRowWarps;
-    const int g = rank * kRowWarps + (threadIdx.x >> 5);
+    const int rank = (int)(blockIdx.x % C), warps = C * kRowWarps, warp = threadIdx.x >> 5;
+    const bool reader = warp < kRowWarps;
+    const int g = rank * kRowWarps + warp;
     const long long r = blockIdx.x / C;
     const Row<DT> row(a.logits, a.stride, r, a.V);
-    const Slice s = warp_slice<DT>(row, g, warps);
     const int per = (row.nv + warps - 1) / warps, cta_begin = per * kRowWarps * rank;
     const int cta_end = cta_begin + per * kRowWarps;
+    const Slice s = warp_slice<DT>(row, g, warps);
     const Scale c(a.inv_t);
     // a teacher's row that is masked throughout carries no loss
     const bool none = TAIL && a.tlse[r] == -CUDART_INF_F;
     const float weight = none ? 0.0f : a.weight ? a.weight[r] : 1.0f;
 
-    float ref, mx;         // the others' reference; the row's maximum
-    double others, sum;    // factor of the others' gradient; sum against mx
-    double mass = 0.0;     // sum p
+    float ref, mx;       // the others' reference; the row's maximum
+    double others, sum;  // factor of the others' gradient; sum against mx
     if (MODE == kBackward) {
         const float4 st = a.stats[r];
         ref = st.x;
         others = st.y;
         mx = st.z;
         sum = st.w;
-        if (weight != 0.0f) mass = load_list<DT>(a, sh, row, r);
-        __syncthreads();
+        if (!reader && weight != 0.0f) {
+            list_ids(a, sh, r);
+            list_sums<DT>(a, sh, row, r);
+        }
     } else {
-        if (TAIL)
-            for (int i = threadIdx.x; i < (per * kRowWarps + 3) / 4; i += kRowThreads) marks[i] = 0;
-        mass = load_list<DT>(a, sh, row, r);
+        if (!reader) list_ids(a, sh, r);
         if (TAIL) {
+            for (int i = threadIdx.x; i < (per * kRowWarps + 3) / 4; i += kDistillThreads) marks[i] = 0;
             __syncthreads();
-            for (int j = threadIdx.x; j < a.k; j += kRowThreads) {
-                const int at = sh.id[j] + row.shift, v = at / N - cta_begin;
-                if (sh.id[j] >= 0 && v >= 0 && v < per * kRowWarps)
-                    atomicOr(&marks[v / 4], 1u << (8 * (v & 3) + at % N));
+            if (!reader) {
+                for (int j = s.lane; j < a.k; j += 32) {
+                    const int at = sh.id[j] + row.shift, v = at / N - cta_begin;
+                    if (sh.id[j] >= 0 && v >= 0 && v < per * kRowWarps)
+                        atomicOr(&marks[v / 4], 1u << (8 * (v & 3) + at % N));
+                }
             }
+            __syncthreads();
         }
-        __syncthreads();
-        LaneSum acc;
         const uint8_t* mark = reinterpret_cast<const uint8_t*>(marks);
-        const float top = stream_slice<DT, true>(row, s, c, acc, [&](int v, uint4& u) {
-            if (TAIL) {
-                const uint32_t m = mark[v - cta_begin];
-                if (m) take_out<DT>(u, m);
-            }
-        });
-        cl.barrier_wait();
-        all_gather(cl, sh.tops, g, warp_max(top));
-        cl.sync();
-        ref = slots_max(sh.tops, warps);
-        double share = warp_mass(acc, c, ref);
-        if (out_of_range(ref)) {
-            share = 0.0;
-            for_vectors_slow<DT>(row, s, [&](int v, uint4 u) {
-                if (TAIL && mark[v - cta_begin]) take_out<DT>(u, mark[v - cta_begin]);
-                float x[N];
-                decode<DT>(u, x);
-#pragma unroll
-                for (int j = 0; j < N; ++j) share += exp(((double)x[j] - (double)ref) * a.inv_t);
+        WarpStat stat{};
+        if (reader) {
+            LaneSum acc;
+            const float top = stream_slice<DT, true>(row, s, c, acc, [&](int v, uint4& u) {
+                if (TAIL) {
+                    const uint32_t m = mark[v - cta_begin];
+                    if (m) take_out<DT>(u, m);
+                }
             });
-            share = warp_sum(share);
+            stat = warp_stat(top, acc);
+        } else {
+            list_sums<DT>(a, sh, row, r);
         }
-        all_gather(cl, sh.slots, g, share);
+        cl.barrier_wait();
+        if (reader) all_gather(cl, sh.stats, g, stat);
         cl.sync();
-        const double s_ref = ref == -CUDART_INF_F ? 0.0 : slots_sum(sh.slots, warps);
+        double s_ref;
+        row_stat(sh.stats, warps, c, ref, s_ref, nullptr);
+        if (ref == -CUDART_INF_F) s_ref = 0.0;
+        if (out_of_range(ref)) {
+            double share = 0.0;
+            if (reader) {
+                for_vectors_slow<DT>(row, s, [&](int v, uint4 u) {
+                    if (TAIL && mark[v - cta_begin]) take_out<DT>(u, mark[v - cta_begin]);
+                    float x[N];
+                    decode<DT>(u, x);
+#pragma unroll
+                    for (int j = 0; j < N; ++j) share += exp(((double)x[j] - (double)ref) * a.inv_t);
+                });
+            }
+            share = warp_sum(share);
+            cl.sync();
+            if (reader) all_gather(cl, sh.stats, g, WarpStat{share, 0.0f, 0.0f});
+            cl.sync();
+            s_ref = 0.0;
+            for (int i = s.lane; i < warps; i += 32) s_ref += sh.stats[i].s;
+            s_ref = warp_sum(s_ref);
+        }
+        if (MODE == kLoss && (rank != 0 || reader)) return;
         // the list's part of the sum
+        const double mass = sh.mass;
         double rest = 0.0, log_other = 0.0;
         mx = ref;
         sum = s_ref;
         if (TAIL) {
-            double best = -CUDART_INF;
-            for (int j = threadIdx.x; j < a.k; j += kRowThreads)
-                if (sh.id[j] >= 0) best = fmax(best, (double)sh.x[j]);
-            best = cta_reduce<true>(sh.red, best);
-            mx = fmaxf(ref, (float)best);
-            double part = 0.0;
-            for (int j = threadIdx.x; j < a.k; j += kRowThreads)
-                if (sh.id[j] >= 0 && sh.owner[sh.slot[j]] == j) part += exp(((double)sh.x[j] - (double)mx) * a.inv_t);
-            part = cta_reduce<false>(sh.red, part);
+            mx = fmaxf(ref, sh.best);
             const double lift = ref == -CUDART_INF_F ? 0.0 : exp(((double)ref - (double)mx) * a.inv_t);
-            sum = s_ref * lift + part;
+            const double listed =
+                sh.best == -CUDART_INF_F ? 0.0 : sh.part * exp(((double)sh.best - (double)mx) * a.inv_t);
+            sum = s_ref * lift + listed;
             rest = mass < 1.0 ? 1.0 - mass : mass >= 1.0 ? 0.0 : mass;
             log_other = ref == -CUDART_INF_F ? -CUDART_INF
                                              : ((double)ref - (double)mx) * a.inv_t + log(s_ref) - log(sum);
@@ -239,19 +261,12 @@ __global__ void __launch_bounds__(kRowThreads, 4) distill_kernel(const DistillAr
         } else {
             others = mass == 0.0 ? 0.0 : 1.0 / sum;
         }
-        if (rank == 0) {
-            const double log_z = (double)mx * a.inv_t + log(sum);
-            double part = 0.0;
-            for (int j = threadIdx.x; j < a.k; j += kRowThreads) {
-                const double lp = sh.logp[j], p = exp(lp);
-                if (sh.id[j] >= 0 && p != 0.0) part += p * (lp - ((double)sh.x[j] * a.inv_t - log_z));
-            }
-            part = cta_reduce<false>(sh.red, part);
-            if (TAIL && rest != 0.0) part += rest * (log(rest) - log_other);
-            if (threadIdx.x == 0) {
-                a.loss[r] = none ? 0.0f : (float)part;
-                if (MODE == kLoss && a.stats) a.stats[r] = make_float4(ref, (float)others, mx, (float)sum);
-            }
+        if (rank == 0 && threadIdx.x == kRowThreads) {
+            double loss = sh.cross;
+            if (mass != 0.0) loss += mass * ((double)mx * a.inv_t + log(sum));
+            if (TAIL && rest != 0.0) loss += rest * (log(rest) - log_other);
+            a.loss[r] = none ? 0.0f : (float)loss;
+            if (MODE == kLoss && a.stats) a.stats[r] = make_float4(ref, (float)others, mx, (float)sum);
         }
         if (MODE == kLoss) return;
     }
@@ -271,32 +286,36 @@ __global__ void __launch_bounds__(kRowThreads, 4) distill_kernel(const DistillAr
     };
     const double scale = (double)weight * a.inv_t;
     const float factor = weight == 0.0f ? 0.0f : (float)(scale * others);
-    if (factor == 0.0f) {  // a row that carries no loss, or one whose other tokens get none: whatever their logits
-        const float zero[N] = {};
-        for (int v = s.begin + s.lane; v < s.end; v += 32) store(v, zero);
-        if (s.lane == 0 && s.head >= 0) store(s.head, zero);
-        if (s.lane == 0 && s.tail >= 0) store(s.tail, zero);
-        if (weight == 0.0f) return;
-    } else if (out_of_range(ref)) {
-        for_vectors_slow<DT>(row, s, [&](int v, const uint4& u) {
-            float x[N];
-            decode<DT>(u, x);
+    if (reader) {
+        if (factor == 0.0f) {  // a row that carries no loss, or one whose other tokens get none: whatever their logits
+            const float zero[N] = {};
+            for (int v = s.begin + s.lane; v < s.end; v += 32) store(v, zero);
+            if (s.lane == 0 && s.head >= 0) store(s.head, zero);
+            if (s.lane == 0 && s.tail >= 0) store(s.tail, zero);
+        } else if (out_of_range(ref)) {
+            for_vectors_slow<DT>(row, s, [&](int v, const uint4& u) {
+                float x[N];
+                decode<DT>(u, x);
 #pragma unroll
-            for (int j = 0; j < N; ++j) x[j] = (float)(scale * others * exp(((double)x[j] - (double)ref) * a.inv_t));
-            store(v, x);
-        });
-    } else {
-        const float e = ceilf(ref * c.c), scaled = (float)(scale * others * c.against(e, ref));
-        for_vectors<DT>(row, s, [&](int v, const uint4& u) {
-            float x[N];
-            decode<DT>(u, x);
+                for (int j = 0; j < N; ++j)
+                    x[j] = (float)(scale * others * exp(((double)x[j] - (double)ref) * a.inv_t));
+                store(v, x);
+            });
+        } else {
+            const float e = ceilf(ref * c.c), scaled = (float)(scale * others * c.against(e, ref));
+            for_vectors<DT>(row, s, [&](int v, const uint4& u) {
+                float x[N];
+                decode<DT>(u, x);
 #pragma unroll
-            for (int j = 0; j < N; ++j) x[j] = scaled * ex2(fmaf(x[j], c.c, -e));
-            store(v, x);
-        });
+                for (int j = 0; j < N; ++j) x[j] = scaled * ex2(fmaf(x[j], c.c, -e));
+                store(v, x);
+            });
+        }
     }
+    if (weight == 0.0f) return;
     __syncthreads();  // the listed tokens' values after the others' formula has been written in their place
-    for (int j = threadIdx.x; j < a.k; j += kRowThreads) {
+    const bool empty = !TAIL && sh.mass == 0.0;
+    for (int j = threadIdx.x; j < a.k; j += kDistillThreads) {
         const int id = sh.id[j];
         if (id < 0 || sh.owner[sh.slot[j]] != j) continue;
         const int v = (id + row.shift) / N;
@@ -306,7 +325,7 @@ __global__ void __launch_bounds__(kRowThreads, 4) distill_kernel(const DistillAr
             for (int i = j + 1; i < a.k; ++i)
                 if (sh.id[i] == id) p += exp(sh.logp[i]);
         }
-        const double q = mass == 0.0 && !TAIL ? 0.0 : exp(((double)sh.x[j] - (double)mx) * a.inv_t) / sum;
+        const double q = empty ? 0.0 : exp(((double)sh.x[j] - (double)mx) * a.inv_t) / sum;
         store_elem<DT>(out, id, (float)(scale * (q - p)));
     }
 }
@@ -317,9 +336,10 @@ namespace qmm_host {
 
 template <int DT, bool TAIL, int MODE>
 static int distill_launch(const qmm::DistillArgs& a, long long rows, cudaStream_t st) {
-    const int C = row_cluster(rows, a.V, qmm::Elem<DT>::kBytes);
+    const int C = row_cluster(rows, a.V, qmm::Elem<DT>::kBytes, 3 * 148);
     if (MODE == qmm::kBackward)  // CTAs on their own
-        return launch_rows(qmm::distill_kernel<DT, TAIL, MODE>, rows * C, 1, 0, st, "distill launch", a, C);
+        return launch_rows(qmm::distill_kernel<DT, TAIL, MODE>, qmm::kDistillThreads, rows * C, 1, 0, st, "distill launch",
+                           a, C);
     size_t smem = 0;
     if (TAIL) {
         const long long vecs = (a.V + 2LL * qmm::Elem<DT>::kVec - 2) / qmm::Elem<DT>::kVec;  // any start of a row
@@ -330,7 +350,7 @@ static int distill_launch(const qmm::DistillArgs& a, long long rows, cudaStream_
             return QMM_EUNSUPPORTED;
         }
     }
-    return launch_rows(qmm::distill_kernel<DT, TAIL, MODE>, rows, C, smem, st, "distill launch", a, C);
+    return launch_rows(qmm::distill_kernel<DT, TAIL, MODE>, qmm::kDistillThreads, rows, C, smem, st, "distill launch", a, C);
 }
 
 template <int DT, bool TAIL>

@@ -183,24 +183,21 @@ QMM_DEVINL float ex2(float a) {
 
 // In 64 bits: 2^t, t = (x - max) log2(e) / T, as a table's 2^(j/32) times the
 // Taylor polynomial of 2^r, |r| <= 1/64 (the term left out is below 3e-15),
-// with the whole part added to the exponent: 11 operations of the 64-bit pipe,
-// where exp() takes about twice that.  The largest logit weighs 1 even where it
-// is infinite; NaN weighs nothing.
+// with the whole part added to the exponent: 12 operations of the 64-bit pipe
+// and no branch, so the elements of a vector overlap (with exp() and its
+// branches a vector of 8 took 3.4 us of a warp's time).  The largest logit
+// weighs 1 even where it is infinite; NaN weighs nothing.
 struct Weight64 {
     const double* table;  // 2^(j/32), j = 0 .. 31, in shared memory
     double c, b, inv_t;
-    float mx;
+    float mx, least, far;  // below `least` nothing is left; below `far` the result is made in two steps
 
     QMM_DEVINL Weight64(const double* table_, float mx_, double inv_t_)
-        : table(table_), c(inv_t_ * 1.4426950408889634), b(-(double)mx_ * c), inv_t(inv_t_), mx(mx_) {}
+        : table(table_), c(inv_t_ * 1.4426950408889634), b(-(double)mx_ * c), inv_t(inv_t_), mx(mx_),
+          least((float)((double)mx_ - 1080.0 / c)), far((float)((double)mx_ - 900.0 / c)) {}
 
     QMM_DEVINL double operator()(float x) const {
-        if (x == mx) return 1.0;
         const double t = fma((double)x, c, b);
-        if (!(t > -1000.0)) {  // next to nothing, or no number
-            const double w = exp(((double)x - (double)mx) * inv_t);
-            return w == w ? w : 0.0;
-        }
         const double magic = 6755399441055744.0 / 32.0;  // 1.5 * 2^52 / 32: sums are whole 32nds
         const double k = t + magic;
         const double r = t - (k - magic);
@@ -211,7 +208,12 @@ struct Weight64 {
         p = fma(r, p, 2.4022650695910072e-1);
         p = fma(r, p, 6.931471805599453e-1);
         p = fma(r, p, 1.0) * table[n & 31];
-        return __hiloint2double(__double2hiint(p) + ((n >> 5) << 20), __double2loint(p));
+        const bool small = x < far;
+        const int up = (n >> 5) + (small ? 300 : 0);
+        double w = __hiloint2double(__double2hiint(p) + (up << 20), __double2loint(p));
+        w *= small ? 4.909093465297727e-91 : 1.0;  // 2^-300
+        w = x > least ? w : 0.0;
+        return x == mx ? 1.0 : w;
     }
 };
 
@@ -419,6 +421,41 @@ QMM_DEVINL void all_gather(cg::cluster_group& cl, T* slots, int g, const T& valu
     if (lane < (int)cl.num_blocks()) *cl.map_shared_rank(slots + g, lane) = value;
 }
 
+// What a warp knows of a row after its pass: the maximum, and the sum of
+// weights against 2^e.
+struct alignas(16) WarpStat {
+    double s;
+    float top, e;
+};
+
+QMM_DEVINL WarpStat warp_stat(float top, const LaneSum& acc) {
+    WarpStat w;
+    w.top = warp_max(top);
+    w.e = warp_max(acc.e);
+    w.s = warp_sum(acc.s * (double)ex2(acc.e - w.e));
+    return w;
+}
+
+// From the gathered warps: the row's maximum, its sum against the weight of the
+// maximum (NaN where 32 bits do not do), and each warp's part of it into
+// `slots` (by warp 0; null: not wanted).  Alike in every warp.
+template <typename S>
+QMM_DEVINL void row_stat(const WarpStat* stats, int warps, const S& c, float& mx, double& total, double* slots) {
+    const int lane = threadIdx.x & 31;
+    mx = -CUDART_INF_F;
+    for (int i = lane; i < warps; i += 32) mx = fmaxf(mx, stats[i].top);
+    mx = warp_max(mx);
+    const float e = ceilf(mx * c.c);
+    const double back = c.against(e, mx);
+    total = 0.0;
+    for (int i = lane; i < warps; i += 32) {
+        const double x = stats[i].s * (double)ex2(stats[i].e - e) * back;
+        if (slots && threadIdx.x < 32) slots[i] = x;
+        total += x;
+    }
+    total = warp_sum(total);
+}
+
 // Sum of n slots in their order, the same in every thread.
 QMM_DEVINL double slots_sum(const double* slots, int n) {
     const int lane = threadIdx.x & 31;
@@ -431,18 +468,6 @@ struct Place {
     int g;        // slot
     double base;  // sum of the slots before it
 };
-
-QMM_DEVINL float slots_max(const float* slots, int n) {
-    float x = -CUDART_INF_F;
-    for (int i = threadIdx.x & 31; i < n; i += 32) x = fmaxf(x, slots[i]);
-    return warp_max(x);
-}
-
-// A warp's sum of weights against the weight of mx, the row's maximum.
-QMM_DEVINL double warp_mass(const LaneSum& acc, const Scale& c, float mx) {
-    const float e = ceilf(mx * c.c);
-    return warp_sum(acc.s * (double)ex2(acc.e - e)) * c.against(e, mx);
-}
 
 // The first slot at which the running sum passes `target`, or the last slot
 // that holds anything.  Called by whole warps; equal in every warp.
@@ -493,83 +518,112 @@ QMM_DEVINL Place locate(const double* slots, int n, double target) {
     return p;
 }
 
-// Within one warp's slice: the first id at which base + the running sum of
-// weights passes `target`, with the sums just before and after it; the last id
-// of any weight if none does.  weight(id, logit) is in 64 bits.
+// Within slice `s` of another warp: the first id at which base + the running sum
+// of weights passes `target`, with the sums just before and after it; the last
+// id of any weight if none does.  By a whole CTA (one warp takes 10 us for the
+// 500 vectors of a slice): its warps sum an eighth each, one walks through the
+// eighth that holds the place.  weights(v, vector, w) fills a vector's weights
+// in 64 bits, 0 for elements outside the row.
 struct Found {
     int id;
     double before, after;
 };
 
+struct FindShared {
+    double sums[kRowWarps];
+    Found found;
+};
+
 template <int DT, typename W>
-QMM_DEVINL Found find_in_slice(const Row<DT>& row, const Slice& s, double base, double target, W&& weight) {
+QMM_DEVINL Found find_in_slice(const Row<DT>& row, const Slice& s, double base, double target, FindShared& sh,
+                               W&& weights) {
     constexpr int N = Elem<DT>::kVec;
-    const int first = s.head >= 0 ? s.head : s.begin, last = s.tail >= 0 ? s.tail + 1 : s.end;
-    Found found{-1, 0.0, 0.0};
-    uint4 next = make_uint4(0, 0, 0, 0);
-    if (first + s.lane < last) next = row.load(first + s.lane);
-    for (int v0 = first; v0 < last; v0 += 32) {
-        const int v = v0 + s.lane;
-        const uint4 cur = next;
-        if (v + 32 < last) next = row.load(v + 32);
-        double w[N], mine = 0.0;
-        float x[N];
-        decode<DT>(cur, x);
+    const int from = s.head >= 0 ? s.head : s.begin, to = s.tail >= 0 ? s.tail + 1 : s.end;
+    const int warp = threadIdx.x >> 5, per = (to - from + kRowWarps - 1) / kRowWarps;
+    const int first = min(from + per * warp, to), last = min(first + per, to);
+    double mass = 0.0;
+    for (int v = first + s.lane; v < last; v += 32) {
+        double w[N];
+        weights(v, row.load(v), w);
 #pragma unroll
-        for (int j = 0; j < N; ++j) {
-            const int id = row.first(v) + j;
-            w[j] = v < last && id >= 0 && id < row.V ? weight(id, x[j]) : 0.0;
-            mine += w[j];
-        }
-        double incl = mine;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const double y = __shfl_up_sync(~0u, incl, o);
-            if (s.lane >= o) incl += y;
-        }
-        const unsigned hits = __ballot_sync(~0u, mine > 0.0 && base + incl > target);
-        const unsigned any = __ballot_sync(~0u, mine > 0.0);
-        if (any) {
-            // the first lane that passes, else the last with a weight (kept for the end)
-            const int src = hits ? __ffs(hits) - 1 : 31 - __clz(any);
-            double run = base + incl - mine;
-            Found f{-1, 0.0, 0.0};
-            bool done = false;
-#pragma unroll
-            for (int j = 0; j < N; ++j) {
-                if (w[j] > 0.0 && !done) {
-                    f.id = row.first(v) + j;
-                    f.before = run;
-                    f.after = run + w[j];
-                    run += w[j];
-                    done = run > target;
-                }
-            }
-            found.id = __shfl_sync(~0u, f.id, src);
-            found.before = __shfl_sync(~0u, f.before, src);
-            found.after = __shfl_sync(~0u, f.after, src);
-            if (hits) return found;
-        }
-        base += __shfl_sync(~0u, incl, 31);
+        for (int j = 0; j < N; ++j) mass += w[j];
     }
-    return found;
+    mass = warp_sum(mass);
+    __syncthreads();
+    if (s.lane == 0) sh.sums[warp] = mass;
+    __syncthreads();
+    int hit = -1;
+    double start = 0.0, run = base;
+    for (int i = 0; i < kRowWarps; ++i) {
+        const double x = sh.sums[i];
+        if (x > 0.0) {
+            hit = i;
+            start = run;
+            if (run + x > target) break;
+        }
+        run += x;
+    }
+    if (warp == max(hit, 0)) {
+        run = start;
+        for (int v0 = first; v0 < last; v0 += 32) {
+            const int v = v0 + s.lane;
+            double w[N], mine = 0.0;
+#pragma unroll
+            for (int j = 0; j < N; ++j) w[j] = 0.0;
+            if (v < last) weights(v, row.load(v), w);
+#pragma unroll
+            for (int j = 0; j < N; ++j) mine += w[j];
+            double incl = mine;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const double y = __shfl_up_sync(~0u, incl, o);
+                if (s.lane >= o) incl += y;
+            }
+            const unsigned hits = __ballot_sync(~0u, mine > 0.0 && run + incl > target);
+            const unsigned any = __ballot_sync(~0u, mine > 0.0);
+            if (any) {
+                // the first lane that passes, else the last with a weight (kept for the end)
+                const int src = hits ? __ffs(hits) - 1 : 31 - __clz(any);
+                double sum = run + incl - mine;
+                Found f{-1, 0.0, 0.0};
+                bool done = false;
+#pragma unroll
+                for (int j = 0; j < N; ++j) {
+                    if (w[j] > 0.0 && !done) {
+                        f.id = row.first(v) + j;
+                        f.before = sum;
+                        f.after = sum + w[j];
+                        sum += w[j];
+                        done = sum > target;
+                    }
+                }
+                if (s.lane == src) sh.found = f;
+                __syncwarp();
+            }
+            if (hits) break;
+            run += __shfl_sync(~0u, incl, 31);
+        }
+    }
+    __syncthreads();
+    if (hit < 0) return Found{-1, 0.0, 0.0};
+    return sh.found;
 }
 
 }  // namespace qmm
 
 namespace qmm_host {
 
-// CTAs to a row: enough that a lane holds few vectors, and that a call of few
-// rows reaches every SM.
-int row_cluster(long long rows, long long V, int elem_bytes);
+// CTAs to a row: so many that a lane holds at most 64 vectors, and more, down to
+// 2 vectors to a lane, until the call has `ctas` of them.
+int row_cluster(long long rows, long long V, int elem_bytes, int ctas);
 
-// Launch `kernel` over rows * C CTAs of kRowThreads in clusters of C.
+// Launch `kernel` over rows * C CTAs in clusters of C.
 template <typename... P, typename... A>
-int launch_rows(void (*kernel)(P...), long long rows, int C, size_t smem, cudaStream_t st, const char* what,
+int launch_rows(void (*kernel)(P...), int threads, long long rows, int C, size_t smem, cudaStream_t st, const char* what,
                 A... args) {
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)(rows * C));
-    cfg.blockDim = dim3(qmm::kRowThreads);
+    cfg.blockDim = dim3((unsigned)threads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
     cudaLaunchAttribute at{};

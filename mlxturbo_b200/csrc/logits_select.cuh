@@ -9,7 +9,7 @@ namespace qmm {
 // A cluster's candidates are in its CTA 0.
 struct SelectShared {
     union {
-        float maxima[kRowThreads * kMaxCluster];  // one of each thread of the cluster (CTA 0's copy is used)
+        float maxima[kRowThreads * kMaxCluster];  // of groups of lanes of the cluster
         double w[kCand];                          // the sorted candidates' weights
         uint32_t piv_count[2][kMaxRowWarps][8];
     };
@@ -18,11 +18,12 @@ struct SelectShared {
         double piv_mass[2][kMaxRowWarps][8];
     };
     double slots[2][kMaxRowWarps];
-    float tops[kMaxRowWarps];
+    WarpStat stats[kMaxRowWarps];
     uint32_t found[kMaxRowWarps];
     uint32_t hist[256];
-    uint32_t n_cand, bound, sel_bin, sel_above;
+    uint32_t n_cand, sel_bin, sel_above;
     double scan[kRowWarps];
+    FindShared find;
     double table[32];  // of Weight64
     unsigned long long best;
     int verdict;
@@ -84,6 +85,45 @@ QMM_DEVINL uint32_t kth_prefix(SelectShared& sh, int n, int k) {
     return prefix;
 }
 
+// How many lanes share one published maximum: the k-th largest of the maxima
+// bounds the k-th largest logit from below, and with at least twice as many
+// maxima as k about 1.4 k logits reach it.  Few maxima are searched by every
+// warp on its own.
+QMM_DEVINL int lanes_to_group(int warps, int k) {
+    int lanes = 32;
+    while (lanes > 1 && warps * (32 / lanes) < 2 * k) lanes >>= 1;
+    return lanes;
+}
+
+// The maxima of a warp's groups to every CTA of the cluster.
+QMM_DEVINL void publish_maxima(cg::cluster_group& cl, SelectShared& sh, int g, int lanes, float top) {
+    const int lane = threadIdx.x & 31;
+    for (int o = 1; o < lanes; o <<= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
+    if (lane % lanes == 0) {
+        float* to = sh.maxima + g * (32 / lanes) + lane / lanes;
+        for (int i = 0; i < (int)cl.num_blocks(); ++i) *cl.map_shared_rank(to, i) = top;
+    }
+}
+
+// key32 of a bound that at least k of the n maxima reach (0: fewer than k are
+// there).  All threads of a CTA.
+constexpr int kWarpSearch = 256;
+QMM_DEVINL uint32_t kth_bound(SelectShared& sh, int n, int k) {
+    if (n > kWarpSearch) return kth_prefix(sh, n, k) << 16;
+    const int lane = threadIdx.x & 31;
+    uint32_t key[kWarpSearch / 32];
+#pragma unroll
+    for (int i = 0; i < kWarpSearch / 32; ++i) key[i] = i * 32 + lane < n ? key32(sh.maxima[i * 32 + lane]) >> 16 : 0;
+    uint32_t b = 0;  // bit by bit: the largest prefix that k keys reach
+    for (uint32_t bit = 0x8000u; bit; bit >>= 1) {
+        int reach = 0;
+#pragma unroll
+        for (int i = 0; i < kWarpSearch / 32; ++i) reach += __popc(__ballot_sync(~0u, key[i] >= (b | bit)));
+        if (reach >= k) b |= bit;
+    }
+    return b << 16;
+}
+
 // Candidates: every token with key32 >= bound, found again by the warps whose
 // lanes' maxima reach it (lane `owner` holds the slice's vectors begin + owner,
 // begin + owner + 32, ..).  They go to CTA 0's list in any order; returns how
@@ -121,9 +161,18 @@ QMM_DEVINL uint32_t push_candidates(cg::cluster_group& cl, SelectShared& sh, con
     return warp_sum(found);
 }
 
-// Descending bitonic sort of the first n candidates in place (padded with 0,
-// which no token's key is).  One CTA.
+// Descending sort of the first n candidates (distinct keys) in place, above 256
+// bitonic, padded with 0, which no token's key is.  One CTA, in step before it.
 QMM_DEVINL void sort_candidates(unsigned long long* k, int n) {
+    if (n <= kRowThreads) {  // a thread to a key: its place is the number of larger ones
+        const unsigned long long mine = (int)threadIdx.x < n ? k[threadIdx.x] : 0;
+        int place = 0;
+        for (int i = 0; i < n; ++i) place += k[i] > mine;
+        __syncthreads();
+        if ((int)threadIdx.x < n) k[place] = mine;
+        __syncthreads();
+        return;
+    }
     int size = 2;
     while (size < n) size <<= 1;
     for (int i = n + threadIdx.x; i < size; i += kRowThreads) k[i] = 0;
@@ -237,18 +286,30 @@ QMM_DEVINL unsigned long long border_key(cg::cluster_group& cl, SelectShared& sh
         }
         for_vectors_slow<DT>(row, s, [&](int v, const uint4& u) {
             float x[N];
+            uint32_t k[N];
+            bool any = false;
             decode<DT>(u, x);
 #pragma unroll
             for (int e = 0; e < N; ++e) {
                 const int id = row.first(v) + e;
-                const uint32_t k = key32(x[e]);
-                if (k < lo || k >= hi || id < 0 || id >= row.V || row_key(x[e], id) < floor) continue;
-                const double w = MASS ? weight(x[e]) : 0.0;
+                k[e] = key32(x[e]);
+                const bool in = k[e] >= lo && k[e] < hi && id >= 0 && id < row.V && row_key(x[e], id) >= floor;
+                if (!in) k[e] = 0;  // below every pivot
+                any |= in;
+            }
+            if (!any) return;
+            double w[N];
+            if (MASS) {
+#pragma unroll
+                for (int e = 0; e < N; ++e) w[e] = weight(x[e]);
+            }
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
-                    if (k >= p[j]) {
+                    if (k[e] >= p[j]) {
                         ++n[j];
-                        if (MASS) m[j] += w;
+                        if (MASS) m[j] += w[e];
                     }
                 }
             }

@@ -67,25 +67,25 @@ __global__ void __launch_bounds__(kRowThreads, 4) sample_kernel(const SampleArgs
     // one pass over memory
     LaneSum acc;
     const float top = sum ? stream_slice<DT, true>(row, s, c, acc) : stream_slice<DT, false>(row, s, c, acc);
-    const float wtop = warp_max(top);
+    const WarpStat stat = warp_stat(top, acc);
+    const bool select = k_on || p_on;  // a bound from maxima
+    const int want = k_on ? k : kRowThreads;
+    const int lanes = lanes_to_group(warps, want);
+    const bool listed = select ? 2 * want <= C * kRowThreads || want <= kRowThreads : m_on;
     cl.barrier_wait();
-    all_gather(cl, sh.tops, g, wtop);
-    const bool select = k_on || p_on;  // a bound from the threads' maxima
-    if (select) *cl.map_shared_rank(&sh.maxima[rank * kRowThreads + threadIdx.x], 0) = top;
+    all_gather(cl, sh.stats, g, stat);
+    if (select && listed) publish_maxima(cl, sh, g, lanes, top);
     cl.sync();
-    const float mx = slots_max(sh.tops, warps);
+    float mx;
+    double total;
+    row_stat(sh.stats, warps, c, mx, total, sh.slots[0]);
     if (mx == -CUDART_INF_F) {  // nothing to draw from
         if (rank == 0 && threadIdx.x == 0) a.ids[r] = -1;
         return;
     }
-    bool fast = sum && c.fast(mx, T);
+    const bool fast = sum && c.fast(mx, T) && total >= 0.5 && total < CUDART_INF;  // else 64 bits
     const Weight64 weight(sh.table, mx, inv_t);
 
-    // the warps' masses against the row's maximum, to every CTA
-    if (sum) {
-        const double mass = warp_mass(acc, c, mx);
-        all_gather(cl, sh.slots[0], g, fast ? mass : CUDART_NAN);
-    }
     // smallest key that min-p keeps; masked tokens have none
     uint32_t kmin = kKeyNegInf + 1;
     if (m_on) {
@@ -99,21 +99,11 @@ __global__ void __launch_bounds__(kRowThreads, 4) sample_kernel(const SampleArgs
     }
     // Top-k without top-p: tokens below min-p play no part.
     uint32_t bound = kmin;
-    const int want = k_on ? k : kRowThreads;
-    const bool listed = select ? want <= C * kRowThreads / 2 || want <= kRowThreads : m_on;
     if (select && listed) {
-        if (rank == 0) {
-            const uint32_t b = kth_prefix(sh, C * kRowThreads, want) << 16;
-            if (threadIdx.x < C) *cl.map_shared_rank(&sh.bound, threadIdx.x) = b;
-        }
-        cl.sync();
-        bound = sh.bound > kKeyNegInf ? sh.bound : kKeyNegInf + 1;
-        if (!(k_on && p_on) && bound < kmin) bound = kmin;
-    } else {
-        cl.sync();
+        const uint32_t b = kth_bound(sh, warps * (32 / lanes), want);
+        bound = max(b, kKeyNegInf + 1);
+        if (!(k_on && p_on)) bound = max(bound, kmin);
     }
-    double total = sum ? slots_sum(sh.slots[0], warps) : 0.0;
-    if (!(total >= 0.5 && total < CUDART_INF)) fast = false;  // 64 bits
     unsigned long long border = (unsigned long long)kmin << 32;
     bool bordered = false;
 
@@ -229,13 +219,20 @@ __global__ void __launch_bounds__(kRowThreads, 4) sample_kernel(const SampleArgs
     }
 
     if (!select && !m_on && fast) {  // no filter: the warps' fast masses are the distribution
+        __syncthreads();
         const double target = u * total, slack = 2.0 * kFastEps * total;
         const Place at = locate(sh.slots[0], warps, target);
-        if (g == at.g) {
-            const Found f = find_in_slice<DT>(row, s, at.base, target, [&](int, float x) { return weight(x); });
+        if (rank == at.g / kRowWarps) {
+            const Found f = find_in_slice<DT>(row, warp_slice<DT>(row, at.g, warps), at.base, target, sh.find,
+                                              [&](int, const uint4& q, double (&w)[Elem<DT>::kVec]) {
+                float x[Elem<DT>::kVec];
+                decode<DT>(q, x);
+#pragma unroll
+                for (int j = 0; j < Elem<DT>::kVec; ++j) w[j] = weight(x[j]);
+            });
             const bool sure = f.id >= 0 && f.before + slack <= target && f.after - slack > target;
-            if (sure && s.lane == 0) a.ids[r] = f.id;
-            if (s.lane < C) *cl.map_shared_rank(&sh.verdict, s.lane) = sure ? kDone : kGeneral;
+            if (sure && threadIdx.x == 0) a.ids[r] = f.id;
+            if (threadIdx.x < C) *cl.map_shared_rank(&sh.verdict, threadIdx.x) = sure ? kDone : kGeneral;
         }
         cl.sync();
         if (sh.verdict == kDone) return;
@@ -249,25 +246,30 @@ __global__ void __launch_bounds__(kRowThreads, 4) sample_kernel(const SampleArgs
         if (from > border) border = from;
     }
     const uint32_t border32 = (uint32_t)(border >> 32);
-    auto kept = [&](int id, float x) {
-        const uint32_t k32 = key32(x);
-        return k32 < border32 || (k32 == border32 && row_key(x, id) < border) ? 0.0 : weight(x);
-    };
-    double mass = 0.0;
-    for_vectors_slow<DT>(row, s, [&](int v, const uint4& q) {
+    auto kept = [&](int v, const uint4& q, double (&w)[Elem<DT>::kVec]) {
         float x[Elem<DT>::kVec];
         decode<DT>(q, x);
 #pragma unroll
-        for (int j = 0; j < Elem<DT>::kVec; ++j) mass += kept(row.first(v) + j, x[j]);  // -infinity past the ends
+        for (int j = 0; j < Elem<DT>::kVec; ++j) {  // -infinity past the ends
+            const uint32_t k32 = key32(x[j]);
+            w[j] = k32 < border32 || (k32 == border32 && row_key(x[j], row.first(v) + j) < border) ? 0.0 : weight(x[j]);
+        }
+    };
+    double mass = 0.0;
+    for_vectors_slow<DT>(row, s, [&](int v, const uint4& q) {
+        double w[Elem<DT>::kVec];
+        kept(v, q, w);
+#pragma unroll
+        for (int j = 0; j < Elem<DT>::kVec; ++j) mass += w[j];
     });
     cl.sync();
     all_gather(cl, sh.slots[0], g, warp_sum(mass));
     cl.sync();
     const double target = u * slots_sum(sh.slots[0], warps);
     const Place at = locate(sh.slots[0], warps, target);
-    if (g == at.g) {
-        const Found f = find_in_slice<DT>(row, s, at.base, target, kept);
-        if (s.lane == 0) a.ids[r] = f.id;
+    if (rank == at.g / kRowWarps) {
+        const Found f = find_in_slice<DT>(row, warp_slice<DT>(row, at.g, warps), at.base, target, sh.find, kept);
+        if (threadIdx.x == 0) a.ids[r] = f.id;
     }
 }
 
@@ -275,21 +277,21 @@ __global__ void __launch_bounds__(kRowThreads, 4) sample_kernel(const SampleArgs
 
 namespace qmm_host {
 
-int row_cluster(long long rows, long long V, int elem_bytes) {
-    const long long vecs = (V * elem_bytes + 15) / 16;
+int row_cluster(long long rows, long long V, int elem_bytes, int ctas) {
     if (const char* e = getenv("QMM_C")) return atoi(e);
+    const long long vecs = (V * elem_bytes + 15) / 16, lanes = qmm::kRowThreads;
     int C = 1;
-    // up to 16 vectors to a lane; a call of few rows goes down to 2 vectors as long as SMs are idle
-    while (C < 8 && vecs > 16LL * C * qmm::kRowThreads) C *= 2;
-    while (C < 16 && rows * C * 2 <= 148 && vecs > 2LL * C * qmm::kRowThreads) C *= 2;
+    while (C < 8 && vecs > 2 * C * lanes && (vecs > 64 * C * lanes || rows * C < ctas)) C *= 2;
+    // clusters of 16 find room on fewer SMs: for calls that fit at once
+    if (C == 8 && rows * 16 <= 148 && vecs > 16 * lanes) C = 16;
     return C;
 }
 
 int launch_sample(const qmm::SampleArgs& a, long long rows, int dtype, cudaStream_t st) {
-    const int C = row_cluster(rows, a.V, dtype == QMM_F32 ? 4 : 2);
-    if (dtype == QMM_BF16) return launch_rows(qmm::sample_kernel<0>, rows, C, 0, st, "sample launch", a);
-    if (dtype == QMM_F16) return launch_rows(qmm::sample_kernel<1>, rows, C, 0, st, "sample launch", a);
-    return launch_rows(qmm::sample_kernel<2>, rows, C, 0, st, "sample launch", a);
+    const int C = row_cluster(rows, a.V, dtype == QMM_F32 ? 4 : 2, 4 * 148);
+    if (dtype == QMM_BF16) return launch_rows(qmm::sample_kernel<0>, qmm::kRowThreads, rows, C, 0, st, "sample launch", a);
+    if (dtype == QMM_F16) return launch_rows(qmm::sample_kernel<1>, qmm::kRowThreads, rows, C, 0, st, "sample launch", a);
+    return launch_rows(qmm::sample_kernel<2>, qmm::kRowThreads, rows, C, 0, st, "sample launch", a);
 }
 
 }  // namespace qmm_host

@@ -31,8 +31,7 @@ QMM_DEVINL double spec_temperature(const SpecArgs& a, long long b, bool draft) {
 
 template <int DT>
 __global__ void __launch_bounds__(kRowThreads, 4) spec_stats_kernel(const SpecArgs a) {
-    __shared__ float tops[kMaxRowWarps];
-    __shared__ double slots[kMaxRowWarps];
+    __shared__ WarpStat stats[kMaxRowWarps];
     __shared__ int args[kMaxRowWarps];
     cg::cluster_group cl = cg::this_cluster();
     cl.barrier_arrive();
@@ -60,14 +59,16 @@ __global__ void __launch_bounds__(kRowThreads, 4) spec_stats_kernel(const SpecAr
     const Scale c(greedy ? 1.0 : 1.0 / T);
     LaneSum acc;
     const float top = greedy ? stream_slice<DT, false>(row, s, c, acc) : stream_slice<DT, true>(row, s, c, acc);
+    const WarpStat stat = warp_stat(top, acc);
     cl.barrier_wait();
-    const float wtop = warp_max(top);
-    all_gather(cl, tops, g, wtop);
+    all_gather(cl, stats, g, stat);
     cl.sync();
-    const float mx = slots_max(tops, warps);
+    float mx;
+    double total;
+    row_stat(stats, warps, c, mx, total, nullptr);
     if (greedy) {
         int first = 0x7FFFFFFF;
-        if (wtop == mx) {  // the warp's share again
+        if (stat.top == mx) {  // the warp's share again
             for_vectors_slow<DT>(row, s, [&](int v, const uint4& q) {
                 float x[Elem<DT>::kVec];
                 decode<DT>(q, x);
@@ -79,10 +80,8 @@ __global__ void __launch_bounds__(kRowThreads, 4) spec_stats_kernel(const SpecAr
             });
         }
         all_gather(cl, args, g, __reduce_min_sync(~0u, first));
-    } else {
-        all_gather(cl, slots, g, warp_mass(acc, c, mx));
+        cl.sync();
     }
-    cl.sync();
     if (rank == 0 && threadIdx.x < 32) {
         RowStat st;
         st.mx = mx;
@@ -93,7 +92,6 @@ __global__ void __launch_bounds__(kRowThreads, 4) spec_stats_kernel(const SpecAr
             for (int w = s.lane; w < warps; w += 32) first = min(first, args[w]);
             st.arg = __reduce_min_sync(~0u, first);
         } else {
-            const double total = slots_sum(slots, warps);
             st.sum = c.fast(mx, T) && total >= 0.5 && total < CUDART_INF ? total : CUDART_NAN;
         }
         if (s.lane == 0) a.stats[at] = st;
@@ -121,29 +119,19 @@ struct Dist {
     }
     // against the sum at hand: exact weights, over a sum that may be a fast one
     QMM_DEVINL double prob(int id, float x) const { return weight(id, x) / st.sum; }
+    // a vector's, whose element 0 is token `first`
+    QMM_DEVINL void probs(int first, const float (&x)[Elem<DT>::kVec], double (&w)[Elem<DT>::kVec]) const {
+        const double part = dead() ? 0.0 : 1.0 / st.sum;
+        if (greedy) {
+#pragma unroll
+            for (int j = 0; j < Elem<DT>::kVec; ++j) w[j] = first + j == st.arg ? part : 0.0;
+        } else {
+#pragma unroll
+            for (int j = 0; j < Elem<DT>::kVec; ++j) w[j] = exact(x[j]) * part;
+        }
+    }
     QMM_DEVINL bool dead() const { return st.mx == -CUDART_INF_F; }  // masked throughout
 };
-
-// The row's sum in 64 bits, by the whole cluster.
-template <int DT>
-QMM_DEVINL void exact_sum(cg::cluster_group& cl, double* slots, Dist<DT>& d, int g, int warps) {
-    if (d.greedy || d.dead()) return;
-    double mass = 0.0;
-    const Slice s = warp_slice<DT>(d.row, g, warps);
-    for_vectors_slow<DT>(d.row, s, [&](int v, const uint4& q) {
-        float x[Elem<DT>::kVec];
-        decode<DT>(q, x);
-#pragma unroll
-        for (int j = 0; j < Elem<DT>::kVec; ++j) {
-            const int id = d.row.first(v) + j;
-            if (id >= 0 && id < d.row.V) mass += d.weight(id, x[j]);
-        }
-    });
-    cl.sync();
-    all_gather(cl, slots, g, warp_sum(mass));
-    cl.sync();
-    d.st.sum = slots_sum(slots, warps);
-}
 
 // Ids of a vector of p's row in q's row (whose start may lie otherwise).
 template <int DT>
@@ -159,10 +147,50 @@ QMM_DEVINL void paired(const Row<DT>& p, const Row<DT>& q, int v, float (&y)[Ele
     }
 }
 
+// The sums of both rows (BOTH false: of p's) in 64 bits, by the whole cluster.
+struct TwoSums {
+    double p, q;
+};
+
+template <int DT, bool BOTH>
+QMM_DEVINL void exact_sums(cg::cluster_group& cl, TwoSums* slots, Dist<DT>& p, Dist<DT>& q, int g, int warps) {
+    constexpr int N = Elem<DT>::kVec;
+    TwoSums mass{0.0, 0.0};
+    const Slice s = warp_slice<DT>(p.row, g, warps);
+    for_vectors_slow<DT>(p.row, s, [&](int v, const uint4& u) {
+        float x[N], y[N];
+        decode<DT>(u, x);
+        if (BOTH) paired<DT>(p.row, q.row, v, y);
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            const int id = p.row.first(v) + j;
+            const bool in = id >= 0 && id < p.row.V;
+            mass.p += in ? p.exact(x[j]) : 0.0;
+            if (BOTH) mass.q += in ? q.exact(y[j]) : 0.0;
+        }
+    });
+    mass.p = warp_sum(mass.p);
+    mass.q = warp_sum(mass.q);
+    cl.sync();
+    all_gather(cl, slots, g, mass);
+    cl.sync();
+    double sp = 0.0, sq = 0.0;
+    for (int i = s.lane; i < warps; i += 32) {
+        sp += slots[i].p;
+        sq += slots[i].q;
+    }
+    sp = warp_sum(sp);
+    sq = warp_sum(sq);
+    if (!p.greedy && !p.dead()) p.st.sum = sp;
+    if (BOTH && !q.greedy && !q.dead()) q.st.sum = sq;
+}
+
 template <int DT>
 __global__ void __launch_bounds__(kRowThreads, 2) spec_decide_kernel(const SpecArgs a) {
-    __shared__ double slots[kMaxRowWarps];
+    __shared__ double slots[2][kMaxRowWarps];
+    __shared__ TwoSums sums[kMaxRowWarps];
     __shared__ int sure_flag;
+    __shared__ FindShared find;
     __shared__ double table[32];
     fill_table(table);
     constexpr int N = Elem<DT>::kVec;
@@ -205,8 +233,7 @@ __global__ void __launch_bounds__(kRowThreads, 2) spec_decide_kernel(const SpecA
         state = __shfl_sync(~0u, state, at);
         if (state == kOpen) {
             Dist<DT> p(a, b, taken, table), q(a, b, a.n + 1 + taken, table);
-            exact_sum<DT>(cl, slots, p, g, warps);
-            exact_sum<DT>(cl, slots, q, g, warps);
+            exact_sums<DT, true>(cl, sums, p, q, g, warps);
             const int d = (int)ids[taken];
             state = (double)u[taken] * q.prob(d, q.row.at(d)) < p.prob(d, p.row.at(d)) ? kStands : kFails;
         }
@@ -224,72 +251,91 @@ __global__ void __launch_bounds__(kRowThreads, 2) spec_decide_kernel(const SpecA
     const Slice s = warp_slice<DT>(p.row, g, warps);
     const double draw = (double)u[a.n];
     int token = -1;
-    bool mine = false;  // this lane writes the token
+    bool mine = false;  // this thread writes the token
     // 0: fast sums; 1: sums in 64 bits; 2: nothing left of p - q, from p
     for (int tries = 0; tries < 3 && !p.dead(); ++tries) {
         const bool exact = tries > 0;
         const bool minus = drafted && tries < 2 && !q.dead();
         if (tries == 0 && !(p.st.sum > 0.0 && q.st.sum > 0.0)) continue;  // a sum is missing
         if (tries == 1) {
-            exact_sum<DT>(cl, slots, p, g, warps);
-            if (minus) exact_sum<DT>(cl, slots, q, g, warps);
+            if (minus) exact_sums<DT, true>(cl, sums, p, q, g, warps);
+            else exact_sums<DT, false>(cl, sums, p, q, g, warps);
         }
+        auto weights = [&](int v, const uint4& w, double (&out)[N]) {
+            float x[N], y[N];
+            double minus_w[N];
+            const int first = p.row.first(v);
+            if (minus) paired<DT>(p.row, q.row, v, y);
+            decode<DT>(w, x);
+            p.probs(first, x, out);
+            if (minus) q.probs(first, y, minus_w);
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+                if (minus) out[j] = fmax(out[j] - minus_w[j], 0.0);
+                if (first + j < 0 || first + j >= a.V) out[j] = 0.0;
+            }
+        };
         double mass = 0.0;
         if (exact || p.greedy || q.greedy) {
             for_vectors_slow<DT>(p.row, s, [&](int v, const uint4& w) {
-                float x[N], y[N];
-                decode<DT>(w, x);
-                if (minus) paired<DT>(p.row, q.row, v, y);
+                double out[N];
+                weights(v, w, out);
 #pragma unroll
-                for (int j = 0; j < N; ++j) {
-                    const int id = p.row.first(v) + j;
-                    if (id < 0 || id >= a.V) continue;
-                    mass += minus ? fmax(p.prob(id, x[j]) - q.prob(id, y[j]), 0.0) : p.prob(id, x[j]);
-                }
+                for (int j = 0; j < N; ++j) mass += out[j];
             });
         } else {
             const Scale cp(p.exact.inv_t), cq(q.exact.inv_t);
             const float ep = ceilf(p.st.mx * cp.c), eq = ceilf(q.st.mx * cq.c);
             const float fp = (float)(cp.against(ep, p.st.mx) / p.st.sum), fq = (float)(cq.against(eq, q.st.mx) / q.st.sum);
-            for_vectors<DT>(p.row, s, [&](int v, const uint4& w) {
-                float x[N], y[N];
-                decode<DT>(w, x);
-                if (minus) paired<DT>(p.row, q.row, v, y);
+            for_batches<DT>(p.row, s, [&](uint4* w, int v, auto n_) {
+                constexpr int n = decltype(n_)::value;
+                uint4 other[n];
+                const bool even = p.row.shift == q.row.shift;
+                if (minus && even) {
 #pragma unroll
-                for (int j = 0; j < N; ++j) {
-                    x[j] = fp * ex2(fmaf(x[j], cp.c, -ep));
-                    if (minus) x[j] = fmaxf(x[j] - fq * ex2(fmaf(y[j], cq.c, -eq)), 0.0f);
+                    for (int i = 0; i < n; ++i) other[i] = q.row.load(v + 32 * i);
                 }
-                mass += (double)tree_sum<N>(x);
+#pragma unroll
+                for (int i = 0; i < n; ++i) {
+                    float x[N], y[N];
+                    decode<DT>(w[i], x);
+                    if (minus) {
+                        if (even) decode<DT>(other[i], y);
+                        else paired<DT>(p.row, q.row, v + 32 * i, y);
+                    }
+#pragma unroll
+                    for (int j = 0; j < N; ++j) {
+                        x[j] = fp * ex2(fmaf(x[j], cp.c, -ep));
+                        if (minus) x[j] = fmaxf(x[j] - fq * ex2(fmaf(y[j], cq.c, -eq)), 0.0f);
+                    }
+                    mass += (double)tree_sum<N>(x);
+                }
             });
         }
+        double* const places = slots[tries & 1];
+        all_gather(cl, places, g, warp_sum(mass));
         cl.sync();
-        all_gather(cl, slots, g, warp_sum(mass));
-        cl.sync();
-        const double total = slots_sum(slots, warps), target = draw * total;
+        const double total = slots_sum(places, warps), target = draw * total;
         if (exact && minus && !(total > 0.0)) continue;
         // each of p and q is off by kFastEps of itself, in sums and in the target
         const double slack = exact || (p.greedy && (!minus || q.greedy)) ? 0.0 : 8.0 * kFastEps;
-        const Place at = locate(slots, warps, target);
-        bool sure = true;
-        if (g == at.g) {
-            const Found f = find_in_slice<DT>(p.row, s, at.base, target, [&](int id, float x) {
-                const double w = p.prob(id, x);
-                return minus ? fmax(w - q.prob(id, q.row.at(id)), 0.0) : w;
-            });
+        const Place at = locate(places, warps, target);
+        if (at.g >= 0 && rank == at.g / kRowWarps) {
+            const Found f =
+                find_in_slice<DT>(p.row, warp_slice<DT>(p.row, at.g, warps), at.base, target, find, weights);
             token = f.id;
-            if (slack > 0.0) sure = f.id >= 0 && f.before + slack <= target && f.after - slack > target;
-            mine = lane == 0;
-            if (lane < C) *cl.map_shared_rank(&sure_flag, lane) = sure;
-        } else if (at.g < 0 && g == 0) {
-            if (lane < C) *cl.map_shared_rank(&sure_flag, lane) = exact;
-            mine = lane == 0;
+            const bool sure = slack == 0.0 || (f.id >= 0 && f.before + slack <= target && f.after - slack > target);
+            if (threadIdx.x < C) *cl.map_shared_rank(&sure_flag, threadIdx.x) = sure;
+            mine = threadIdx.x == 0;
+        } else if (at.g < 0 && rank == 0) {
+            if (threadIdx.x < C) *cl.map_shared_rank(&sure_flag, threadIdx.x) = exact;
+            mine = threadIdx.x == 0;
         }
         cl.sync();
         if (sure_flag) break;
         mine = false;
     }
-    if (p.dead()) mine = g == 0 && lane == 0;  // nothing to draw from: -1
+    if (p.dead()) mine = rank == 0 && threadIdx.x == 0;  // nothing to draw from: -1
     if (mine) {
         int64_t* out = a.tokens + b * (a.n + 1);
         for (int i = 0; i <= a.n; ++i) out[i] = i < taken ? ids[i] : i == taken ? (int64_t)token : -1;
@@ -307,10 +353,10 @@ template <int DT>
 static int speculative_dt(const qmm::SpecArgs& a, cudaStream_t st) {
     const long long rows = (long long)a.B * (2 * a.n + 1);
     const int bytes = qmm::Elem<DT>::kBytes;
-    const int rc = launch_rows(qmm::spec_stats_kernel<DT>, rows, row_cluster(rows, a.V, bytes), 0, st,
+    const int rc = launch_rows(qmm::spec_stats_kernel<DT>, qmm::kRowThreads, rows, row_cluster(rows, a.V, bytes, 4 * 148), 0, st,
                                "speculative sums launch", a);
     if (rc) return rc;
-    return launch_rows(qmm::spec_decide_kernel<DT>, a.B, row_cluster(a.B, a.V, bytes), 0, st, "speculative launch", a);
+    return launch_rows(qmm::spec_decide_kernel<DT>, qmm::kRowThreads, a.B, row_cluster(a.B, a.V, bytes, 4 * 148), 0, st, "speculative launch", a);
 }
 
 int launch_speculative(const qmm::SpecArgs& a, int dtype, cudaStream_t st) {

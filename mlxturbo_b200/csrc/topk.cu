@@ -29,28 +29,17 @@ __global__ void __launch_bounds__(kRowThreads, 4) topk_kernel(const TopkArgs a) 
 
     LaneSum acc;
     const float top = stream_slice<DT, LSE>(row, s, c, acc);
+    const bool listed = a.k <= C * kRowThreads;
+    const int lanes = lanes_to_group(warps, a.k);
+    const WarpStat stat = warp_stat(top, acc);
     cl.barrier_wait();
-    if (LSE) all_gather(cl, sh.tops, g, warp_max(top));
-    *cl.map_shared_rank(&sh.maxima[rank * kRowThreads + threadIdx.x], 0) = top;
+    if (LSE) all_gather(cl, sh.stats, g, stat);
+    if (listed) publish_maxima(cl, sh, g, lanes, top);
     cl.sync();
     float mx = 0.0f;
-    if (LSE) {
-        mx = slots_max(sh.tops, warps);
-        all_gather(cl, sh.slots[0], g, warp_mass(acc, c, mx));
-    }
-    const bool listed = a.k <= C * kRowThreads;
-    uint32_t bound = 0;
-    if (listed) {
-        if (rank == 0) {
-            const uint32_t b = kth_prefix(sh, C * kRowThreads, a.k) << 16;
-            if (threadIdx.x < C) *cl.map_shared_rank(&sh.bound, threadIdx.x) = b;
-        }
-        cl.sync();
-        bound = sh.bound;
-    } else {
-        cl.sync();
-    }
-    double total = LSE ? slots_sum(sh.slots[0], warps) : 0.0;
+    double total = 0.0;
+    if (LSE) row_stat(sh.stats, warps, c, mx, total, nullptr);
+    const uint32_t bound = listed ? kth_bound(sh, warps * (32 / lanes), a.k) : 0;
     const Weight64 weight(sh.table, mx, a.inv_t);
     if (LSE && fabsf(mx) != CUDART_INF_F && !(c.fast(mx, 1.0 / a.inv_t) && total >= 0.5 && total < CUDART_INF)) {
         double mass = 0.0;  // a NaN among the logits, or none above a mask's lowest value
@@ -118,9 +107,9 @@ namespace qmm_host {
 
 template <int DT>
 static int topk_dt(const qmm::TopkArgs& a, long long rows, cudaStream_t st) {
-    const int C = row_cluster(rows, a.V, qmm::Elem<DT>::kBytes);
-    if (a.lse) return launch_rows(qmm::topk_kernel<DT, true>, rows, C, 0, st, "topk launch", a);
-    return launch_rows(qmm::topk_kernel<DT, false>, rows, C, 0, st, "topk launch", a);
+    const int C = row_cluster(rows, a.V, qmm::Elem<DT>::kBytes, 4 * 148);
+    if (a.lse) return launch_rows(qmm::topk_kernel<DT, true>, qmm::kRowThreads, rows, C, 0, st, "topk launch", a);
+    return launch_rows(qmm::topk_kernel<DT, false>, qmm::kRowThreads, rows, C, 0, st, "topk launch", a);
 }
 
 int launch_topk(const qmm::TopkArgs& a, long long rows, int dtype, cudaStream_t st) {
