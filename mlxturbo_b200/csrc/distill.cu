@@ -206,13 +206,13 @@ __global__ void __launch_bounds__(kDistillThreads, MODE == kLossGrad ? 3 : 4)
         WarpStat stat{};
         if (reader) {
             LaneSum acc;
-            const float top = stream_slice<DT, true>(row, s, c, acc, [&](int v, uint4& u) {
+            const LaneTop top = stream_slice<DT, true, false>(row, s, c, acc, [&](int v, uint4& u) {
                 if (TAIL) {
                     const uint32_t m = mark[v - cta_begin];
                     if (m) take_out<DT>(u, m);
                 }
             });
-            stat = warp_stat(top, acc);
+            stat = warp_stat(top.first, acc);
         } else {
             list_sums<DT>(a, sh, row, r);
         }
@@ -225,7 +225,7 @@ __global__ void __launch_bounds__(kDistillThreads, MODE == kLossGrad ? 3 : 4)
         if (out_of_range(ref)) {
             double share = 0.0;
             if (reader) {
-                for_vectors_slow<DT>(row, s, [&](int v, uint4 u) {
+                for_vectors_rare<DT>(row, s, [&](int v, uint4 u) {
                     if (TAIL && mark[v - cta_begin]) take_out<DT>(u, mark[v - cta_begin]);
                     float x[N];
                     decode<DT>(u, x);
@@ -277,7 +277,7 @@ __global__ void __launch_bounds__(kDistillThreads, MODE == kLossGrad ? 3 : 4)
     auto store = [&](int v, const float (&y)[N]) {
         const int f = row.first(v);
         if (aligned && row.whole(v)) {
-            *reinterpret_cast<uint4*>(out + (long long)f * Elem<DT>::kBytes) = encode<DT>(y);
+            __stcs(reinterpret_cast<uint4*>(out + (long long)f * Elem<DT>::kBytes), encode<DT>(y));
         } else {
 #pragma unroll
             for (int j = 0; j < N; ++j)
@@ -293,7 +293,7 @@ __global__ void __launch_bounds__(kDistillThreads, MODE == kLossGrad ? 3 : 4)
             if (s.lane == 0 && s.head >= 0) store(s.head, zero);
             if (s.lane == 0 && s.tail >= 0) store(s.tail, zero);
         } else if (out_of_range(ref)) {
-            for_vectors_slow<DT>(row, s, [&](int v, const uint4& u) {
+            for_vectors_rare<DT>(row, s, [&](int v, const uint4& u) {
                 float x[N];
                 decode<DT>(u, x);
 #pragma unroll

@@ -342,36 +342,94 @@ QMM_DEVINL void for_vectors(const Row<DT>& row, const Slice& s, F&& f) {
     });
 }
 
-// The same, a vector at a time with the next one on its way: for passes whose
-// arithmetic in 64 bits outlasts the loads, in few registers.
+// The same in few instructions, for what hardly ever runs.
 template <int DT, typename F>
-QMM_DEVINL void for_vectors_slow(const Row<DT>& row, const Slice& s, F&& f) {
+QMM_DEVINL void for_vectors_rare(const Row<DT>& row, const Slice& s, F&& f) {
     const int first = s.head >= 0 ? s.head : s.begin, last = s.tail >= 0 ? s.tail + 1 : s.end;
-    int v = first + s.lane;
-    uint4 next = make_uint4(0, 0, 0, 0);
-    if (v < last) next = row.load(v);
 #pragma unroll 1
-    for (; v < last; v += 32) {
-        const uint4 u = next;
-        if (v + 32 < last) next = row.load(v + 32);
-        f(v, u);
-    }
+    for (int v = first + s.lane; v < last; v += 32) f(v, row.load(v));
 }
 
-// Maximum of the slice's logits in this lane, and with SUM the lane's weights.
-// change(vector index, vector) may take elements out (set them to -infinity).
-template <int DT, bool SUM, typename F>
-QMM_DEVINL float stream_slice(const Row<DT>& row, const Slice& s, const Scale& c, LaneSum& acc, F&& change) {
+// The same for passes whose arithmetic in 64 bits needs the registers: vectors
+// one at a time, the next seven on their way into shared memory (cp.async, each
+// thread's own slots, so nothing has to be synchronised).  With one load ahead
+// instead, a pass of 30 vectors to a lane took 30 us under a busy memory.
+constexpr int kRing = 8;
+using Ring = uint4 (*)[kRowThreads];  // [kRing][kRowThreads] in shared memory
+
+QMM_DEVINL void async_copy16(uint4* to, const void* from) {
+    const uint32_t at = (uint32_t)__cvta_generic_to_shared(to);
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(at), "l"(from) : "memory");
+}
+QMM_DEVINL void async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+QMM_DEVINL void async_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+template <int DT, typename F>
+QMM_DEVINL void for_vectors_slow(const Row<DT>& row, const Slice& s, Ring ring, F&& f) {
+    const int t = threadIdx.x;
+    int v = s.begin + s.lane;
+#pragma unroll
+    for (int i = 0; i < kRing - 1; ++i) {
+        if (v + 32 * i < s.end) async_copy16(&ring[i][t], row.base + 16LL * (v + 32 * i));
+        async_commit();
+    }
+    // the row's ends meanwhile
+    if (s.lane == 0 && s.head >= 0) f(s.head, row.load(s.head));
+    int slot = 0;
+#pragma unroll 1
+    for (; v < s.end; v += 32) {
+        async_wait<kRing - 2>();
+        const uint4 u = ring[slot][t];
+        // into the slot that the round before has used up
+        const int free = slot == 0 ? kRing - 1 : slot - 1, ahead = v + 32 * (kRing - 1);
+        if (ahead < s.end) async_copy16(&ring[free][t], row.base + 16LL * ahead);
+        async_commit();
+        slot = slot == kRing - 1 ? 0 : slot + 1;
+        f(v, u);
+    }
+    async_wait<0>();
+    if (s.lane == 0 && s.tail >= 0) f(s.tail, row.load(s.tail));
+}
+
+// The two vectors of a lane with the largest maxima, these, and the largest of
+// the lane's other vectors (or more, beside a NaN).
+struct LaneTop {
+    float first = kLow, second = kLow, others = kLow;
+    int at = -1, at2 = -1;
+    static constexpr float kLow = -__builtin_huge_valf();
+
+    QMM_DEVINL void add(float m, int v) {
+        const bool up = m > first, mid = m > second;
+        others = fmaxf(others, fminf(m, second));
+        second = up ? first : fmaxf(second, m);
+        at2 = up ? at : mid ? v : at2;
+        first = fmaxf(first, m);
+        at = up ? v : at;
+    }
+};
+
+// Maxima of the slice's logits in this lane (WHERE: and where they are), and
+// with SUM the lane's weights.  change(vector index, vector) may take elements
+// out (set them to -infinity).
+template <int DT, bool SUM, bool WHERE, typename F>
+QMM_DEVINL LaneTop stream_slice(const Row<DT>& row, const Slice& s, const Scale& c, LaneSum& acc, F&& change) {
     constexpr int N = Elem<DT>::kVec;
-    float top = -CUDART_INF_F;
+    LaneTop top;
     for_batches<DT>(row, s, [&](uint4* u, int v, auto n_) {
         constexpr int n = decltype(n_)::value;
 #pragma unroll
         for (int i = 0; i < n; ++i) change(v + 32 * i, u[i]);
-        float bm = vec_max<DT>(u[0]);
+        float bm = -CUDART_INF_F;
 #pragma unroll
-        for (int i = 1; i < n; ++i) bm = fmaxf(bm, vec_max<DT>(u[i]));
-        top = fmaxf(top, bm);
+        for (int i = 0; i < n; ++i) {
+            const float m = vec_max<DT>(u[i]);
+            if (WHERE) top.add(m, v + 32 * i);
+            bm = fmaxf(bm, m);
+        }
+        if (!WHERE) top.first = fmaxf(top.first, bm);
         if (!SUM) return;
         const float t = bm * c.c;
         if (t > acc.e + 16.0f) {  // weights stay below 2^17
@@ -393,9 +451,9 @@ QMM_DEVINL float stream_slice(const Row<DT>& row, const Slice& s, const Scale& c
     return top;
 }
 
-template <int DT, bool SUM>
-QMM_DEVINL float stream_slice(const Row<DT>& row, const Slice& s, const Scale& c, LaneSum& acc) {
-    return stream_slice<DT, SUM>(row, s, c, acc, [](int, uint4&) {});
+template <int DT, bool SUM, bool WHERE>
+QMM_DEVINL LaneTop stream_slice(const Row<DT>& row, const Slice& s, const Scale& c, LaneSum& acc) {
+    return stream_slice<DT, SUM, WHERE>(row, s, c, acc, [](int, uint4&) {});
 }
 
 // ---- exchange between the warps of a cluster ---------------------------------------------
@@ -542,11 +600,19 @@ QMM_DEVINL Found find_in_slice(const Row<DT>& row, const Slice& s, double base, 
     const int warp = threadIdx.x >> 5, per = (to - from + kRowWarps - 1) / kRowWarps;
     const int first = min(from + per * warp, to), last = min(first + per, to);
     double mass = 0.0;
-    for (int v = first + s.lane; v < last; v += 32) {
-        double w[N];
-        weights(v, row.load(v), w);
+    for (int v = first + s.lane; v < last; v += 128) {
+        uint4 u[4];
 #pragma unroll
-        for (int j = 0; j < N; ++j) mass += w[j];
+        for (int i = 0; i < 4; ++i)
+            if (v + 32 * i < last) u[i] = row.load(v + 32 * i);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (v + 32 * i >= last) break;
+            double w[N];
+            weights(v + 32 * i, u[i], w);
+#pragma unroll
+            for (int j = 0; j < N; ++j) mass += w[j];
+        }
     }
     mass = warp_sum(mass);
     __syncthreads();
@@ -565,12 +631,16 @@ QMM_DEVINL Found find_in_slice(const Row<DT>& row, const Slice& s, double base, 
     }
     if (warp == max(hit, 0)) {
         run = start;
+        uint4 next = make_uint4(0, 0, 0, 0);
+        if (first + s.lane < last) next = row.load(first + s.lane);
         for (int v0 = first; v0 < last; v0 += 32) {
             const int v = v0 + s.lane;
+            const uint4 u = next;
+            if (v + 32 < last) next = row.load(v + 32);
             double w[N], mine = 0.0;
 #pragma unroll
             for (int j = 0; j < N; ++j) w[j] = 0.0;
-            if (v < last) weights(v, row.load(v), w);
+            if (v < last) weights(v, u, w);
 #pragma unroll
             for (int j = 0; j < N; ++j) mine += w[j];
             double incl = mine;
@@ -634,6 +704,8 @@ int launch_rows(void (*kernel)(P...), int threads, long long rows, int C, size_t
     cfg.numAttrs = 1;
     cudaError_t e = cudaSuccess;
     if (C > 8) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e == cudaSuccess && smem > 48 * 1024)
+        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e == cudaSuccess) e = cudaLaunchKernelEx(&cfg, kernel, args...);
     return cuda_status(e, what);
 }

@@ -29,6 +29,8 @@ struct SelectShared {
     int verdict;
 };
 
+constexpr size_t kSelectSmem = sizeof(SelectShared) + kRing * kRowThreads * sizeof(uint4);
+
 // The largest 16-bit prefix b such that at least k of the n maxima have
 // key32 >> 16 >= b; 0 if there are fewer than k.  One CTA, all threads.
 QMM_DEVINL uint32_t kth_prefix(SelectShared& sh, int n, int k) {
@@ -124,41 +126,113 @@ QMM_DEVINL uint32_t kth_bound(SelectShared& sh, int n, int k) {
     return b << 16;
 }
 
-// Candidates: every token with key32 >= bound, found again by the warps whose
-// lanes' maxima reach it (lane `owner` holds the slice's vectors begin + owner,
-// begin + owner + 32, ..).  They go to CTA 0's list in any order; returns how
-// many this warp found.  The list's own count may pass kCand; no more than that
-// are written.
-template <int DT>
-QMM_DEVINL uint32_t push_candidates(cg::cluster_group& cl, SelectShared& sh, const Row<DT>& row, const Slice& s,
-                                    float top, uint32_t bound) {
+// The tokens of K vectors to a lane with key32 in [lo, hi) and key >= floor to
+// CTA 0's list, in any order.  By a whole warp; v < 0: none.  The list's count
+// may pass kCand; no more than that are written.  Returns the warp's number.
+template <int DT, int K>
+QMM_DEVINL uint32_t append(cg::cluster_group& cl, SelectShared& sh, const Row<DT>& row, const int (&v)[K],
+                           const uint4 (&u)[K], uint32_t lo, uint32_t hi, unsigned long long floor) {
     constexpr int N = Elem<DT>::kVec;
-    unsigned owners = __ballot_sync(~0u, key32(top) >= bound);
-    uint32_t* count = cl.map_shared_rank(&sh.n_cand, 0);
-    unsigned long long* list = cl.map_shared_rank(sh.cand, 0);
-    uint32_t found = 0;
-    auto take = [&](const uint4& u, int v) {
+    const int lane = threadIdx.x & 31;
+    uint32_t hit = 0;
+#pragma unroll
+    for (int i = 0; i < K; ++i) {
         float x[N];
-        decode<DT>(u, x);
+        decode<DT>(u[i], x);
 #pragma unroll
         for (int j = 0; j < N; ++j) {
-            const int id = row.first(v) + j;
-            if (id < 0 || id >= row.V || key32(x[j]) < bound) continue;
-            ++found;
-            const uint32_t at = atomicAdd(count, 1u);
-            if (at < kCand) list[at] = row_key(x[j], id);
+            const int id = row.first(v[i]) + j;
+            const uint32_t k = key32(x[j]);
+            if (v[i] >= 0 && k >= lo && k < hi && id >= 0 && id < row.V && row_key(x[j], id) >= floor)
+                hit |= 1u << (i * N + j);
         }
-    };
-    if (s.lane == 0 && (owners & 1u)) {
-        if (s.head >= 0) take(row.load(s.head), s.head);
-        if (s.tail >= 0) take(row.load(s.tail), s.tail);
     }
+    if (!__any_sync(~0u, hit != 0)) return 0;
+    const uint32_t mine = __popc(hit);
+    uint32_t incl = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t y = __shfl_up_sync(~0u, incl, o);
+        if (lane >= o) incl += y;
+    }
+    const uint32_t total = __shfl_sync(~0u, incl, 31);
+    uint32_t at = 0;
+    if (lane == 0) at = atomicAdd(cl.map_shared_rank(&sh.n_cand, 0), total);
+    at = __shfl_sync(~0u, at, 0) + incl - mine;
+    unsigned long long* list = cl.map_shared_rank(sh.cand, 0);
+#pragma unroll
+    for (int i = 0; i < K; ++i) {
+        float x[N];
+        decode<DT>(u[i], x);
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            if (!(hit >> (i * N + j) & 1)) continue;
+            if (at < kCand) list[at] = row_key(x[j], row.first(v[i]) + j);
+            ++at;
+        }
+    }
+    return total;
+}
+
+// The same over the whole slice.
+template <int DT>
+QMM_DEVINL uint32_t append_slice(cg::cluster_group& cl, SelectShared& sh, const Row<DT>& row, const Slice& s,
+                                 uint32_t lo, uint32_t hi, unsigned long long floor) {
+    const int first = s.head >= 0 ? s.head : s.begin, last = s.tail >= 0 ? s.tail + 1 : s.end;
+    uint32_t found = 0;
+    for (int v0 = first; v0 < last; v0 += 128) {
+        uint4 u[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int v = v0 + 32 * i + s.lane;
+            u[i] = v < last ? row.load(v) : make_uint4(0, 0, 0, 0);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int v = v0 + 32 * i + s.lane;
+            const int at[1] = {v < last ? v : -1};
+            const uint4 one[1] = {u[i]};
+            found += append<DT, 1>(cl, sh, row, at, one, lo, hi, floor);
+        }
+    }
+    return found;
+}
+
+// Candidates: every token with key32 >= bound.  A lane reads its two vectors
+// of the largest maxima again, as far as they reach the bound; one where a third
+// may reach it has all of its vectors (begin + owner, begin + owner + 32, .., and
+// lane 0 the row's ends) read by the warp.  What is read is read at once: under a
+// busy memory every wait here is 2 us.
+template <int DT>
+QMM_DEVINL uint32_t push_candidates(cg::cluster_group& cl, SelectShared& sh, const Row<DT>& row, const Slice& s,
+                                    const LaneTop& top, uint32_t bound) {
+    const bool more = key32(top.others) >= bound;
+    unsigned owners = __ballot_sync(~0u, more);
+    if (__popc(owners) > 6) return append_slice<DT>(cl, sh, row, s, bound, 0xFFFFFFFFu, 0);
+    const int v[2] = {!more && key32(top.first) >= bound ? top.at : -1,
+                      !more && key32(top.second) >= bound ? top.at2 : -1};
+    uint4 u[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) u[i] = v[i] >= 0 ? row.load(v[i]) : make_uint4(0, 0, 0, 0);
+    uint32_t found = append<DT, 2>(cl, sh, row, v, u, bound, 0xFFFFFFFFu, 0);
     while (owners) {
         const int owner = __ffs(owners) - 1;
         owners &= owners - 1;
-        for (int v = s.begin + owner + 32 * s.lane; v < s.end; v += 32 * 32) take(row.load_whole(v), v);
+        for (int v0 = s.begin + owner; v0 < s.end; v0 += 64 * 32) {
+            const int w[2] = {v0 + 32 * s.lane < s.end ? v0 + 32 * s.lane : -1,
+                              v0 + 32 * (s.lane + 32) < s.end ? v0 + 32 * (s.lane + 32) : -1};
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+                if (w[i] >= 0) u[i] = row.load_whole(w[i]);
+            found += append<DT, 2>(cl, sh, row, w, u, bound, 0xFFFFFFFFu, 0);
+        }
+        if (owner == 0) {
+            const int w[1] = {s.lane == 0 ? s.head : s.lane == 1 ? s.tail : -1};
+            const uint4 end[1] = {w[0] >= 0 ? row.load(w[0]) : make_uint4(0, 0, 0, 0)};
+            found += append<DT, 1>(cl, sh, row, w, end, bound, 0xFFFFFFFFu, 0);
+        }
     }
-    return warp_sum(found);
+    return found;
 }
 
 // Descending sort of the first n candidates (distinct keys) in place, above 256
@@ -253,8 +327,8 @@ QMM_DEVINL uint32_t between(uint32_t lo, uint32_t hi, int j, bool by_value) {
 // the cluster; every thread returns the same.
 template <int DT, bool MASS>
 QMM_DEVINL unsigned long long border_key(cg::cluster_group& cl, SelectShared& sh, const Row<DT>& row, const Slice& s,
-                                         int g, int warps, const Weight64& weight, unsigned long long floor,
-                                         double want) {
+                                         int g, int warps, Ring ring, const Weight64& weight,
+                                         unsigned long long floor, double want) {
     constexpr int N = Elem<DT>::kVec;
     const int rank = (int)cl.block_rank();
     uint32_t lo = (uint32_t)(floor >> 32), hi = key32(weight.mx) + 1, inside = 0xFFFFFFFFu;
@@ -284,7 +358,7 @@ QMM_DEVINL unsigned long long border_key(cg::cluster_group& cl, SelectShared& sh
             n[j] = 0;
             m[j] = 0.0;
         }
-        for_vectors_slow<DT>(row, s, [&](int v, const uint4& u) {
+        for_vectors_slow<DT>(row, s, ring, [&](int v, const uint4& u) {
             float x[N];
             uint32_t k[N];
             bool any = false;
@@ -378,7 +452,7 @@ QMM_DEVINL unsigned long long border_key(cg::cluster_group& cl, SelectShared& sh
             uint32_t n[8];
 #pragma unroll
             for (int j = 0; j < 8; ++j) n[j] = 0;
-            for_vectors_slow<DT>(row, s, [&](int v, const uint4& u) {
+            for_vectors_slow<DT>(row, s, ring, [&](int v, const uint4& u) {
                 float x[N];
                 decode<DT>(u, x);
 #pragma unroll
@@ -419,20 +493,7 @@ QMM_DEVINL unsigned long long border_key(cg::cluster_group& cl, SelectShared& sh
     cl.sync();
     if (rank == 0 && threadIdx.x == 0) sh.n_cand = 0;
     cl.sync();
-    uint32_t* count = cl.map_shared_rank(&sh.n_cand, 0);
-    unsigned long long* list = cl.map_shared_rank(sh.cand, 0);
-    for_vectors_slow<DT>(row, s, [&](int v, const uint4& u) {
-        float x[N];
-        decode<DT>(u, x);
-#pragma unroll
-        for (int e = 0; e < N; ++e) {
-            const int id = row.first(v) + e;
-            const uint32_t k = key32(x[e]);
-            if (k < lo || k >= hi || id < 0 || id >= row.V || row_key(x[e], id) < floor) continue;
-            const uint32_t at = atomicAdd(count, 1u);
-            if (at < kCand) list[at] = row_key(x[e], id);
-        }
-    });
+    append_slice<DT>(cl, sh, row, s, lo, hi, floor);
     cl.sync();
     if (rank == 0) {
         const int n = (int)sh.n_cand;

@@ -16,6 +16,9 @@
 #include <stdlib.h>
 #include "logits_select.cuh"
 
+#ifndef SAMPLE_CTAS
+#define SAMPLE_CTAS 3
+#endif
 namespace qmm {
 
 // What CTA 0 makes of the candidates: the answer; a sum in 64 bits is needed;
@@ -36,8 +39,10 @@ QMM_DEVINL int count_before(const double* sums, int n, double limit) {
 }
 
 template <int DT>
-__global__ void __launch_bounds__(kRowThreads, 4) sample_kernel(const SampleArgs a) {
-    __shared__ SelectShared sh;
+__global__ void __launch_bounds__(kRowThreads, SAMPLE_CTAS) sample_kernel(const SampleArgs a) {
+    extern __shared__ uint4 memory[];
+    SelectShared& sh = *reinterpret_cast<SelectShared*>(memory + kRing * kRowThreads);
+    const Ring ring = reinterpret_cast<Ring>(memory);
     cg::cluster_group cl = cg::this_cluster();
     cl.barrier_arrive();  // waited for before the first access to another CTA
     if (threadIdx.x == 0) sh.n_cand = 0;
@@ -66,15 +71,16 @@ __global__ void __launch_bounds__(kRowThreads, 4) sample_kernel(const SampleArgs
 
     // one pass over memory
     LaneSum acc;
-    const float top = sum ? stream_slice<DT, true>(row, s, c, acc) : stream_slice<DT, false>(row, s, c, acc);
-    const WarpStat stat = warp_stat(top, acc);
+    const LaneTop top =
+        sum ? stream_slice<DT, true, true>(row, s, c, acc) : stream_slice<DT, false, true>(row, s, c, acc);
+    const WarpStat stat = warp_stat(top.first, acc);
     const bool select = k_on || p_on;  // a bound from maxima
     const int want = k_on ? k : kRowThreads;
     const int lanes = lanes_to_group(warps, want);
     const bool listed = select ? 2 * want <= C * kRowThreads || want <= kRowThreads : m_on;
     cl.barrier_wait();
     all_gather(cl, sh.stats, g, stat);
-    if (select && listed) publish_maxima(cl, sh, g, lanes, top);
+    if (select && listed) publish_maxima(cl, sh, g, lanes, top.first);
     cl.sync();
     float mx;
     double total;
@@ -204,7 +210,7 @@ __global__ void __launch_bounds__(kRowThreads, 4) sample_kernel(const SampleArgs
                 }
                 // the row's sum in 64 bits, then again
                 double mass = 0.0;
-                for_vectors_slow<DT>(row, s, [&](int v, const uint4& q) {
+                for_vectors_slow<DT>(row, s, ring, [&](int v, const uint4& q) {
                     float x[Elem<DT>::kVec];
                     decode<DT>(q, x);
 #pragma unroll
@@ -241,8 +247,8 @@ __global__ void __launch_bounds__(kRowThreads, 4) sample_kernel(const SampleArgs
     // the general way: borders by search, masses and place in 64 bits
     if (select && !bordered) {
         unsigned long long from = (unsigned long long)(kKeyNegInf + 1) << 32;
-        if (k_on) from = border_key<DT, false>(cl, sh, row, s, g, warps, weight, from, (double)k);
-        if (p_on) from = border_key<DT, true>(cl, sh, row, s, g, warps, weight, from, p);
+        if (k_on) from = border_key<DT, false>(cl, sh, row, s, g, warps, ring, weight, from, (double)k);
+        if (p_on) from = border_key<DT, true>(cl, sh, row, s, g, warps, ring, weight, from, p);
         if (from > border) border = from;
     }
     const uint32_t border32 = (uint32_t)(border >> 32);
@@ -256,7 +262,7 @@ __global__ void __launch_bounds__(kRowThreads, 4) sample_kernel(const SampleArgs
         }
     };
     double mass = 0.0;
-    for_vectors_slow<DT>(row, s, [&](int v, const uint4& q) {
+    for_vectors_slow<DT>(row, s, ring, [&](int v, const uint4& q) {
         double w[Elem<DT>::kVec];
         kept(v, q, w);
 #pragma unroll
@@ -289,9 +295,9 @@ int row_cluster(long long rows, long long V, int elem_bytes, int ctas) {
 
 int launch_sample(const qmm::SampleArgs& a, long long rows, int dtype, cudaStream_t st) {
     const int C = row_cluster(rows, a.V, dtype == QMM_F32 ? 4 : 2, 4 * 148);
-    if (dtype == QMM_BF16) return launch_rows(qmm::sample_kernel<0>, qmm::kRowThreads, rows, C, 0, st, "sample launch", a);
-    if (dtype == QMM_F16) return launch_rows(qmm::sample_kernel<1>, qmm::kRowThreads, rows, C, 0, st, "sample launch", a);
-    return launch_rows(qmm::sample_kernel<2>, qmm::kRowThreads, rows, C, 0, st, "sample launch", a);
+    if (dtype == QMM_BF16) return launch_rows(qmm::sample_kernel<0>, qmm::kRowThreads, rows, C, qmm::kSelectSmem, st, "sample launch", a);
+    if (dtype == QMM_F16) return launch_rows(qmm::sample_kernel<1>, qmm::kRowThreads, rows, C, qmm::kSelectSmem, st, "sample launch", a);
+    return launch_rows(qmm::sample_kernel<2>, qmm::kRowThreads, rows, C, qmm::kSelectSmem, st, "sample launch", a);
 }
 
 }  // namespace qmm_host

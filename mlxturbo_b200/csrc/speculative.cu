@@ -58,7 +58,8 @@ __global__ void __launch_bounds__(kRowThreads, 4) spec_stats_kernel(const SpecAr
     const bool greedy = !(T > 0.0);
     const Scale c(greedy ? 1.0 : 1.0 / T);
     LaneSum acc;
-    const float top = greedy ? stream_slice<DT, false>(row, s, c, acc) : stream_slice<DT, true>(row, s, c, acc);
+    const float top = greedy ? stream_slice<DT, false, false>(row, s, c, acc).first
+                             : stream_slice<DT, true, false>(row, s, c, acc).first;
     const WarpStat stat = warp_stat(top, acc);
     cl.barrier_wait();
     all_gather(cl, stats, g, stat);
@@ -69,7 +70,7 @@ __global__ void __launch_bounds__(kRowThreads, 4) spec_stats_kernel(const SpecAr
     if (greedy) {
         int first = 0x7FFFFFFF;
         if (stat.top == mx) {  // the warp's share again
-            for_vectors_slow<DT>(row, s, [&](int v, const uint4& q) {
+            for_vectors_rare<DT>(row, s, [&](int v, const uint4& q) {
                 float x[Elem<DT>::kVec];
                 decode<DT>(q, x);
 #pragma unroll
@@ -133,7 +134,7 @@ struct Dist {
     QMM_DEVINL bool dead() const { return st.mx == -CUDART_INF_F; }  // masked throughout
 };
 
-// Ids of a vector of p's row in q's row (whose start may lie otherwise).
+// Ids of a vector of p's row in q's row, whose start may lie otherwise.
 template <int DT>
 QMM_DEVINL void paired(const Row<DT>& p, const Row<DT>& q, int v, float (&y)[Elem<DT>::kVec]) {
     if (p.shift == q.shift) {
@@ -147,20 +148,71 @@ QMM_DEVINL void paired(const Row<DT>& p, const Row<DT>& q, int v, float (&y)[Ele
     }
 }
 
+// f(vector index, p's elements, q's) over the warp's slice of p's row; q's are
+// read where BOTH, with the next vectors of either on their way (q's row lies
+// alike: its vectors are whole where p's are).
+template <int DT, typename F>
+QMM_DEVINL void for_pairs(const Row<DT>& p, const Row<DT>& q, const Slice& s, Ring ring, bool both, F&& f) {
+    constexpr int N = Elem<DT>::kVec;
+    if (!both || p.shift != q.shift) {
+        for_vectors_slow<DT>(p, s, ring, [&](int v, const uint4& u) {
+            float x[N], y[N];
+            decode<DT>(u, x);
+            if (both) paired<DT>(p, q, v, y);
+            f(v, x, y);
+        });
+        return;
+    }
+    const int t = threadIdx.x;
+    int v = s.begin + s.lane;
+    constexpr int kAhead = kRing / 2 - 1;  // pairs
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+        if (v + 32 * i < s.end) {
+            async_copy16(&ring[2 * i][t], p.base + 16LL * (v + 32 * i));
+            async_copy16(&ring[2 * i + 1][t], q.base + 16LL * (v + 32 * i));
+        }
+        async_commit();
+    }
+    auto ends = [&](int at) {
+        float x[N], y[N];
+        decode<DT>(p.load(at), x);
+        decode<DT>(q.load(at), y);
+        f(at, x, y);
+    };
+    if (s.lane == 0 && s.head >= 0) ends(s.head);
+    int slot = 0;
+#pragma unroll 1
+    for (; v < s.end; v += 32) {
+        async_wait<kAhead - 1>();
+        float x[N], y[N];
+        decode<DT>(ring[2 * slot][t], x);
+        decode<DT>(ring[2 * slot + 1][t], y);
+        const int free = slot == 0 ? kAhead : slot - 1, ahead = v + 32 * kAhead;
+        if (ahead < s.end) {
+            async_copy16(&ring[2 * free][t], p.base + 16LL * ahead);
+            async_copy16(&ring[2 * free + 1][t], q.base + 16LL * ahead);
+        }
+        async_commit();
+        slot = slot == kAhead ? 0 : slot + 1;
+        f(v, x, y);
+    }
+    async_wait<0>();
+    if (s.lane == 0 && s.tail >= 0) ends(s.tail);
+}
+
 // The sums of both rows (BOTH false: of p's) in 64 bits, by the whole cluster.
 struct TwoSums {
     double p, q;
 };
 
 template <int DT, bool BOTH>
-QMM_DEVINL void exact_sums(cg::cluster_group& cl, TwoSums* slots, Dist<DT>& p, Dist<DT>& q, int g, int warps) {
+QMM_DEVINL void exact_sums(cg::cluster_group& cl, TwoSums* slots, Ring ring, Dist<DT>& p, Dist<DT>& q, int g,
+                           int warps) {
     constexpr int N = Elem<DT>::kVec;
     TwoSums mass{0.0, 0.0};
     const Slice s = warp_slice<DT>(p.row, g, warps);
-    for_vectors_slow<DT>(p.row, s, [&](int v, const uint4& u) {
-        float x[N], y[N];
-        decode<DT>(u, x);
-        if (BOTH) paired<DT>(p.row, q.row, v, y);
+    for_pairs<DT>(p.row, q.row, s, ring, BOTH, [&](int v, const float (&x)[N], const float (&y)[N]) {
 #pragma unroll
         for (int j = 0; j < N; ++j) {
             const int id = p.row.first(v) + j;
@@ -192,6 +244,8 @@ __global__ void __launch_bounds__(kRowThreads, 2) spec_decide_kernel(const SpecA
     __shared__ int sure_flag;
     __shared__ FindShared find;
     __shared__ double table[32];
+    __shared__ uint4 ring_memory[kRing][kRowThreads];
+    const Ring ring = ring_memory;
     fill_table(table);
     constexpr int N = Elem<DT>::kVec;
     cg::cluster_group cl = cg::this_cluster();
@@ -233,7 +287,7 @@ __global__ void __launch_bounds__(kRowThreads, 2) spec_decide_kernel(const SpecA
         state = __shfl_sync(~0u, state, at);
         if (state == kOpen) {
             Dist<DT> p(a, b, taken, table), q(a, b, a.n + 1 + taken, table);
-            exact_sums<DT, true>(cl, sums, p, q, g, warps);
+            exact_sums<DT, true>(cl, sums, ring, p, q, g, warps);
             const int d = (int)ids[taken];
             state = (double)u[taken] * q.prob(d, q.row.at(d)) < p.prob(d, p.row.at(d)) ? kStands : kFails;
         }
@@ -258,28 +312,25 @@ __global__ void __launch_bounds__(kRowThreads, 2) spec_decide_kernel(const SpecA
         const bool minus = drafted && tries < 2 && !q.dead();
         if (tries == 0 && !(p.st.sum > 0.0 && q.st.sum > 0.0)) continue;  // a sum is missing
         if (tries == 1) {
-            if (minus) exact_sums<DT, true>(cl, sums, p, q, g, warps);
-            else exact_sums<DT, false>(cl, sums, p, q, g, warps);
+            if (minus) exact_sums<DT, true>(cl, sums, ring, p, q, g, warps);
+            else exact_sums<DT, false>(cl, sums, ring, p, q, g, warps);
         }
-        auto weights = [&](int v, const uint4& w, double (&out)[N]) {
-            float x[N], y[N];
-            double minus_w[N];
+        auto weigh = [&](int v, const float (&x)[N], const float (&y)[N], double (&out)[N]) {
+            double other[N];
             const int first = p.row.first(v);
-            if (minus) paired<DT>(p.row, q.row, v, y);
-            decode<DT>(w, x);
             p.probs(first, x, out);
-            if (minus) q.probs(first, y, minus_w);
+            if (minus) q.probs(first, y, other);
 #pragma unroll
             for (int j = 0; j < N; ++j) {
-                if (minus) out[j] = fmax(out[j] - minus_w[j], 0.0);
+                if (minus) out[j] = fmax(out[j] - other[j], 0.0);
                 if (first + j < 0 || first + j >= a.V) out[j] = 0.0;
             }
         };
         double mass = 0.0;
         if (exact || p.greedy || q.greedy) {
-            for_vectors_slow<DT>(p.row, s, [&](int v, const uint4& w) {
+            for_pairs<DT>(p.row, q.row, s, ring, minus, [&](int v, const float (&x)[N], const float (&y)[N]) {
                 double out[N];
-                weights(v, w, out);
+                weigh(v, x, y, out);
 #pragma unroll
                 for (int j = 0; j < N; ++j) mass += out[j];
             });
@@ -287,29 +338,14 @@ __global__ void __launch_bounds__(kRowThreads, 2) spec_decide_kernel(const SpecA
             const Scale cp(p.exact.inv_t), cq(q.exact.inv_t);
             const float ep = ceilf(p.st.mx * cp.c), eq = ceilf(q.st.mx * cq.c);
             const float fp = (float)(cp.against(ep, p.st.mx) / p.st.sum), fq = (float)(cq.against(eq, q.st.mx) / q.st.sum);
-            for_batches<DT>(p.row, s, [&](uint4* w, int v, auto n_) {
-                constexpr int n = decltype(n_)::value;
-                uint4 other[n];
-                const bool even = p.row.shift == q.row.shift;
-                if (minus && even) {
+            for_pairs<DT>(p.row, q.row, s, ring, minus, [&](int v, const float (&x)[N], const float (&y)[N]) {
+                float w[N];
 #pragma unroll
-                    for (int i = 0; i < n; ++i) other[i] = q.row.load(v + 32 * i);
+                for (int j = 0; j < N; ++j) {
+                    w[j] = fp * ex2(fmaf(x[j], cp.c, -ep));
+                    if (minus) w[j] = fmaxf(w[j] - fq * ex2(fmaf(y[j], cq.c, -eq)), 0.0f);
                 }
-#pragma unroll
-                for (int i = 0; i < n; ++i) {
-                    float x[N], y[N];
-                    decode<DT>(w[i], x);
-                    if (minus) {
-                        if (even) decode<DT>(other[i], y);
-                        else paired<DT>(p.row, q.row, v + 32 * i, y);
-                    }
-#pragma unroll
-                    for (int j = 0; j < N; ++j) {
-                        x[j] = fp * ex2(fmaf(x[j], cp.c, -ep));
-                        if (minus) x[j] = fmaxf(x[j] - fq * ex2(fmaf(y[j], cq.c, -eq)), 0.0f);
-                    }
-                    mass += (double)tree_sum<N>(x);
-                }
+                mass += (double)tree_sum<N>(w);
             });
         }
         double* const places = slots[tries & 1];
@@ -322,7 +358,13 @@ __global__ void __launch_bounds__(kRowThreads, 2) spec_decide_kernel(const SpecA
         const Place at = locate(places, warps, target);
         if (at.g >= 0 && rank == at.g / kRowWarps) {
             const Found f =
-                find_in_slice<DT>(p.row, warp_slice<DT>(p.row, at.g, warps), at.base, target, find, weights);
+                find_in_slice<DT>(p.row, warp_slice<DT>(p.row, at.g, warps), at.base, target, find,
+                                              [&](int v, const uint4& w, double (&out)[N]) {
+                                                  float x[N], y[N];
+                                                  decode<DT>(w, x);
+                                                  if (minus) paired<DT>(p.row, q.row, v, y);
+                                                  weigh(v, x, y, out);
+                                              });
             token = f.id;
             const bool sure = slack == 0.0 || (f.id >= 0 && f.before + slack <= target && f.after - slack > target);
             if (threadIdx.x < C) *cl.map_shared_rank(&sure_flag, threadIdx.x) = sure;

@@ -14,8 +14,10 @@
 namespace qmm {
 
 template <int DT, bool LSE>
-__global__ void __launch_bounds__(kRowThreads, 4) topk_kernel(const TopkArgs a) {
-    __shared__ SelectShared sh;
+__global__ void __launch_bounds__(kRowThreads, 3) topk_kernel(const TopkArgs a) {
+    extern __shared__ uint4 memory[];
+    SelectShared& sh = *reinterpret_cast<SelectShared*>(memory + kRing * kRowThreads);
+    const Ring ring = reinterpret_cast<Ring>(memory);
     cg::cluster_group cl = cg::this_cluster();
     cl.barrier_arrive();  // waited for before the first access to another CTA
     if (threadIdx.x == 0) sh.n_cand = 0;
@@ -28,13 +30,13 @@ __global__ void __launch_bounds__(kRowThreads, 4) topk_kernel(const TopkArgs a) 
     const Scale c(a.inv_t);
 
     LaneSum acc;
-    const float top = stream_slice<DT, LSE>(row, s, c, acc);
+    const LaneTop top = stream_slice<DT, LSE, true>(row, s, c, acc);
     const bool listed = a.k <= C * kRowThreads;
     const int lanes = lanes_to_group(warps, a.k);
-    const WarpStat stat = warp_stat(top, acc);
+    const WarpStat stat = warp_stat(top.first, acc);
     cl.barrier_wait();
     if (LSE) all_gather(cl, sh.stats, g, stat);
-    if (listed) publish_maxima(cl, sh, g, lanes, top);
+    if (listed) publish_maxima(cl, sh, g, lanes, top.first);
     cl.sync();
     float mx = 0.0f;
     double total = 0.0;
@@ -43,7 +45,7 @@ __global__ void __launch_bounds__(kRowThreads, 4) topk_kernel(const TopkArgs a) 
     const Weight64 weight(sh.table, mx, a.inv_t);
     if (LSE && fabsf(mx) != CUDART_INF_F && !(c.fast(mx, 1.0 / a.inv_t) && total >= 0.5 && total < CUDART_INF)) {
         double mass = 0.0;  // a NaN among the logits, or none above a mask's lowest value
-        for_vectors_slow<DT>(row, s, [&](int, const uint4& q) {
+        for_vectors_slow<DT>(row, s, ring, [&](int, const uint4& q) {
             float x[Elem<DT>::kVec];
             decode<DT>(q, x);
 #pragma unroll
@@ -69,25 +71,13 @@ __global__ void __launch_bounds__(kRowThreads, 4) topk_kernel(const TopkArgs a) 
     }
     if (n > kCand) {  // the border, then the k tokens from it on
         // the search takes logits up to its maximum: infinite ones too
-        const unsigned long long border = border_key<DT, false>(cl, sh, row, s, g, warps,
+        const unsigned long long border = border_key<DT, false>(cl, sh, row, s, g, warps, ring,
                                                                 Weight64(sh.table, CUDART_INF_F, 1.0),
                                                                 (unsigned long long)kKeyNegInf << 32, (double)a.k);
         cl.sync();
         if (threadIdx.x == 0) sh.n_cand = 0;
         cl.sync();
-        uint32_t* count = cl.map_shared_rank(&sh.n_cand, 0);
-        unsigned long long* list = cl.map_shared_rank(sh.cand, 0);
-        for_vectors_slow<DT>(row, s, [&](int v, const uint4& q) {
-            float x[Elem<DT>::kVec];
-            decode<DT>(q, x);
-#pragma unroll
-            for (int j = 0; j < Elem<DT>::kVec; ++j) {
-                const int id = row.first(v) + j;
-                if (id < 0 || id >= row.V || row_key(x[j], id) < border) continue;
-                const uint32_t at = atomicAdd(count, 1u);
-                if (at < kCand) list[at] = row_key(x[j], id);
-            }
-        });
+        append_slice<DT>(cl, sh, row, s, 0, 0xFFFFFFFFu, border);
         cl.sync();
         n = (uint32_t)a.k;
     }
@@ -95,8 +85,9 @@ __global__ void __launch_bounds__(kRowThreads, 4) topk_kernel(const TopkArgs a) 
     sort_candidates(sh.cand, (int)n);
     for (int i = threadIdx.x; i < a.k; i += kRowThreads) {
         const int id = key_id(sh.cand[i]);
-        const float x = row.at(id);  // the bits of memory: -0 stays -0
-        store_elem<DT>(a.values, r * a.k + i, x == x ? x : -CUDART_INF_F);
+        float x = key32_value((uint32_t)(sh.cand[i] >> 32));
+        if (x == 0.0f) x = row.at(id);  // -0 has the key of +0
+        store_elem<DT>(a.values, r * a.k + i, x);
         a.ids[r * a.k + i] = id;
     }
 }
@@ -108,8 +99,8 @@ namespace qmm_host {
 template <int DT>
 static int topk_dt(const qmm::TopkArgs& a, long long rows, cudaStream_t st) {
     const int C = row_cluster(rows, a.V, qmm::Elem<DT>::kBytes, 4 * 148);
-    if (a.lse) return launch_rows(qmm::topk_kernel<DT, true>, qmm::kRowThreads, rows, C, 0, st, "topk launch", a);
-    return launch_rows(qmm::topk_kernel<DT, false>, qmm::kRowThreads, rows, C, 0, st, "topk launch", a);
+    if (a.lse) return launch_rows(qmm::topk_kernel<DT, true>, qmm::kRowThreads, rows, C, qmm::kSelectSmem, st, "topk launch", a);
+    return launch_rows(qmm::topk_kernel<DT, false>, qmm::kRowThreads, rows, C, qmm::kSelectSmem, st, "topk launch", a);
 }
 
 int launch_topk(const qmm::TopkArgs& a, long long rows, int dtype, cudaStream_t st) {
