@@ -576,12 +576,13 @@ QMM_DEVINL Place locate(const double* slots, int n, double target) {
     return p;
 }
 
-// Within slice `s` of another warp: the first id at which base + the running sum
+// Within the vectors [from, to): the first id at which base + the running sum
 // of weights passes `target`, with the sums just before and after it; the last
-// id of any weight if none does.  By a whole CTA (one warp takes 10 us for the
-// 500 vectors of a slice): its warps sum an eighth each, one walks through the
-// eighth that holds the place.  weights(v, vector, w) fills a vector's weights
-// in 64 bits, 0 for elements outside the row.
+// id of any weight if none does.  By a whole CTA: each thread sums a few
+// neighbouring vectors, and the one whose sum holds the place goes through its
+// own again.  weights(v, vector, w) fills a vector's weights in 64 bits, 0 for
+// elements outside the row; its code stands here once, for both turns: what
+// runs once a call costs its fetching.
 struct Found {
     int id;
     double before, after;
@@ -590,93 +591,80 @@ struct Found {
 struct FindShared {
     double sums[kRowWarps];
     Found found;
+    int last;  // thread with the last weight
 };
 
 template <int DT, typename W>
-QMM_DEVINL Found find_in_slice(const Row<DT>& row, const Slice& s, double base, double target, FindShared& sh,
-                               W&& weights) {
+QMM_DEVINL Found find_place(const Row<DT>& row, int from, int to, double base, double target, Ring ring,
+                            FindShared& sh, W&& weights) {
     constexpr int N = Elem<DT>::kVec;
-    const int from = s.head >= 0 ? s.head : s.begin, to = s.tail >= 0 ? s.tail + 1 : s.end;
-    const int warp = threadIdx.x >> 5, per = (to - from + kRowWarps - 1) / kRowWarps;
-    const int first = min(from + per * warp, to), last = min(first + per, to);
-    double mass = 0.0;
-    for (int v = first + s.lane; v < last; v += 128) {
-        uint4 u[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (v + 32 * i < last) u[i] = row.load(v + 32 * i);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            if (v + 32 * i >= last) break;
+    const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
+    const int per = (to - from + kRowThreads - 1) / kRowThreads;
+    const int first = min(from + per * t, to), end = min(first + per, to);
+    __syncthreads();
+    if (t == 0) {
+        sh.found = Found{-1, 0.0, 0.0};
+        sh.last = -1;
+    }
+    // a thread's vectors, all at once
+    for (int i = 0; i < kRing && first + i < end; ++i) {
+        if (row.whole(first + i)) async_copy16(&ring[i][t], row.base + 16LL * (first + i));
+        else ring[i][t] = row.load(first + i);
+    }
+    async_commit();
+    async_wait<0>();
+    double mass = 0.0, run = 0.0;
+    bool done = false;
+    for (int turn = 0; turn < 2; ++turn) {
+        Found f{-1, 0.0, 0.0};
+#pragma unroll 1
+        for (int v = first; v < end; ++v) {
             double w[N];
-            weights(v + 32 * i, u[i], w);
+            const int i = v - first;
+            weights(v, i < kRing ? ring[i][t] : row.load(v), w);
 #pragma unroll
-            for (int j = 0; j < N; ++j) mass += w[j];
-        }
-    }
-    mass = warp_sum(mass);
-    __syncthreads();
-    if (s.lane == 0) sh.sums[warp] = mass;
-    __syncthreads();
-    int hit = -1;
-    double start = 0.0, run = base;
-    for (int i = 0; i < kRowWarps; ++i) {
-        const double x = sh.sums[i];
-        if (x > 0.0) {
-            hit = i;
-            start = run;
-            if (run + x > target) break;
-        }
-        run += x;
-    }
-    if (warp == max(hit, 0)) {
-        run = start;
-        uint4 next = make_uint4(0, 0, 0, 0);
-        if (first + s.lane < last) next = row.load(first + s.lane);
-        for (int v0 = first; v0 < last; v0 += 32) {
-            const int v = v0 + s.lane;
-            const uint4 u = next;
-            if (v + 32 < last) next = row.load(v + 32);
-            double w[N], mine = 0.0;
-#pragma unroll
-            for (int j = 0; j < N; ++j) w[j] = 0.0;
-            if (v < last) weights(v, u, w);
-#pragma unroll
-            for (int j = 0; j < N; ++j) mine += w[j];
-            double incl = mine;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const double y = __shfl_up_sync(~0u, incl, o);
-                if (s.lane >= o) incl += y;
-            }
-            const unsigned hits = __ballot_sync(~0u, mine > 0.0 && run + incl > target);
-            const unsigned any = __ballot_sync(~0u, mine > 0.0);
-            if (any) {
-                // the first lane that passes, else the last with a weight (kept for the end)
-                const int src = hits ? __ffs(hits) - 1 : 31 - __clz(any);
-                double sum = run + incl - mine;
-                Found f{-1, 0.0, 0.0};
-                bool done = false;
-#pragma unroll
-                for (int j = 0; j < N; ++j) {
-                    if (w[j] > 0.0 && !done) {
-                        f.id = row.first(v) + j;
-                        f.before = sum;
-                        f.after = sum + w[j];
-                        sum += w[j];
-                        done = sum > target;
-                    }
+            for (int j = 0; j < N; ++j) {
+                if (turn == 0) {
+                    mass += w[j];
+                } else if (w[j] > 0.0 && !done) {
+                    f.id = row.first(v) + j;
+                    f.before = run;
+                    run += w[j];
+                    f.after = run;
+                    done = run > target;
                 }
-                if (s.lane == src) sh.found = f;
-                __syncwarp();
             }
-            if (hits) break;
-            run += __shfl_sync(~0u, incl, 31);
         }
+        if (turn == 1) {
+            sh.found = f;
+            break;
+        }
+        double incl = mass;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const double y = __shfl_up_sync(~0u, incl, o);
+            if (lane >= o) incl += y;
+        }
+        if (lane == 31) sh.sums[warp] = incl;
+        __syncthreads();
+        run = base + incl - mass;
+        for (int i = 0; i < warp; ++i) run += sh.sums[i];
+        // the first thread that passes, or the last with a weight
+        const bool passes = mass > 0.0 && run + mass > target;
+        const int hit = __syncthreads_or(passes);
+        if (mass > 0.0) atomicMax(&sh.last, hit ? (passes ? kRowThreads - t : -1) : t);
+        __syncthreads();
+        if (sh.last != (hit ? kRowThreads - t : t)) break;
     }
     __syncthreads();
-    if (hit < 0) return Found{-1, 0.0, 0.0};
     return sh.found;
+}
+
+template <int DT, typename W>
+QMM_DEVINL Found find_in_slice(const Row<DT>& row, const Slice& s, double base, double target, Ring ring,
+                               FindShared& sh, W&& weights) {
+    return find_place<DT>(row, s.head >= 0 ? s.head : s.begin, s.tail >= 0 ? s.tail + 1 : s.end, base, target, ring,
+                          sh, weights);
 }
 
 }  // namespace qmm

@@ -229,7 +229,7 @@ __global__ void __launch_bounds__(kRowThreads, SAMPLE_CTAS) sample_kernel(const 
         const double target = u * total, slack = 2.0 * kFastEps * total;
         const Place at = locate(sh.slots[0], warps, target);
         if (rank == at.g / kRowWarps) {
-            const Found f = find_in_slice<DT>(row, warp_slice<DT>(row, at.g, warps), at.base, target, sh.find,
+            const Found f = find_in_slice<DT>(row, warp_slice<DT>(row, at.g, warps), at.base, target, ring, sh.find,
                                               [&](int, const uint4& q, double (&w)[Elem<DT>::kVec]) {
                 float x[Elem<DT>::kVec];
                 decode<DT>(q, x);
@@ -245,6 +245,32 @@ __global__ void __launch_bounds__(kRowThreads, SAMPLE_CTAS) sample_kernel(const 
     }
 
     // the general way: borders by search, masses and place in 64 bits
+    const int per = (row.nv + warps - 1) / warps;
+    if (p_on && !k_on && !bordered && per * Elem<DT>::kVec <= kBinTokens) {
+        unsigned long long from;
+        if (border_by_bins<DT>(cl, sh, row, s, g, warps, ring, weight, p, total, bound, sh.slots[0], from)) {
+            if (from >= border) {  // min-p keeps them all: CTA 0 has each warp's mass
+                if (rank != 0) return;
+                const double target = u * slots_sum(sh.slots[0], warps);
+                const Place at = locate(sh.slots[0], warps, target);
+                const uint32_t from32 = (uint32_t)(from >> 32);
+                const Found f = find_in_slice<DT>(row, warp_slice<DT>(row, at.g, warps), at.base, target, ring, sh.find,
+                                                  [&](int v, const uint4& q, double (&w)[Elem<DT>::kVec]) {
+                    float x[Elem<DT>::kVec];
+                    decode<DT>(q, x);
+#pragma unroll
+                    for (int j = 0; j < Elem<DT>::kVec; ++j) {
+                        const uint32_t k32 = key32(x[j]);
+                        const bool out = k32 < from32 || (k32 == from32 && row_key(x[j], row.first(v) + j) < from);
+                        w[j] = out ? 0.0 : weight(x[j]);
+                    }
+                });
+                if (threadIdx.x == 0) a.ids[r] = f.id;
+                return;
+            }
+            bordered = true;
+        }
+    }
     if (select && !bordered) {
         unsigned long long from = (unsigned long long)(kKeyNegInf + 1) << 32;
         if (k_on) from = border_key<DT, false>(cl, sh, row, s, g, warps, ring, weight, from, (double)k);
@@ -274,7 +300,7 @@ __global__ void __launch_bounds__(kRowThreads, SAMPLE_CTAS) sample_kernel(const 
     const double target = u * slots_sum(sh.slots[0], warps);
     const Place at = locate(sh.slots[0], warps, target);
     if (rank == at.g / kRowWarps) {
-        const Found f = find_in_slice<DT>(row, warp_slice<DT>(row, at.g, warps), at.base, target, sh.find, kept);
+        const Found f = find_in_slice<DT>(row, warp_slice<DT>(row, at.g, warps), at.base, target, ring, sh.find, kept);
         if (threadIdx.x == 0) a.ids[r] = f.id;
     }
 }

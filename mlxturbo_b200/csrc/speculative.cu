@@ -201,24 +201,25 @@ QMM_DEVINL void for_pairs(const Row<DT>& p, const Row<DT>& q, const Slice& s, Ri
     if (s.lane == 0 && s.tail >= 0) ends(s.tail);
 }
 
-// The sums of both rows (BOTH false: of p's) in 64 bits, by the whole cluster.
+// The sums of both rows (both false: of p's) in 64 bits, by the whole cluster.
 struct TwoSums {
     double p, q;
 };
 
-template <int DT, bool BOTH>
-QMM_DEVINL void exact_sums(cg::cluster_group& cl, TwoSums* slots, Ring ring, Dist<DT>& p, Dist<DT>& q, int g,
-                           int warps) {
+// Not inlined: it hardly runs, and what a call does run stays short.
+template <int DT>
+__device__ __noinline__ void exact_sums(cg::cluster_group& cl, TwoSums* slots, Ring ring, Dist<DT>& p, Dist<DT>& q, int g,
+                                        int warps, bool both) {
     constexpr int N = Elem<DT>::kVec;
     TwoSums mass{0.0, 0.0};
     const Slice s = warp_slice<DT>(p.row, g, warps);
-    for_pairs<DT>(p.row, q.row, s, ring, BOTH, [&](int v, const float (&x)[N], const float (&y)[N]) {
+    for_pairs<DT>(p.row, q.row, s, ring, both, [&](int v, const float (&x)[N], const float (&y)[N]) {
 #pragma unroll
         for (int j = 0; j < N; ++j) {
             const int id = p.row.first(v) + j;
             const bool in = id >= 0 && id < p.row.V;
             mass.p += in ? p.exact(x[j]) : 0.0;
-            if (BOTH) mass.q += in ? q.exact(y[j]) : 0.0;
+            if (both) mass.q += in ? q.exact(y[j]) : 0.0;
         }
     });
     mass.p = warp_sum(mass.p);
@@ -234,7 +235,7 @@ QMM_DEVINL void exact_sums(cg::cluster_group& cl, TwoSums* slots, Ring ring, Dis
     sp = warp_sum(sp);
     sq = warp_sum(sq);
     if (!p.greedy && !p.dead()) p.st.sum = sp;
-    if (BOTH && !q.greedy && !q.dead()) q.st.sum = sq;
+    if (both && !q.greedy && !q.dead()) q.st.sum = sq;
 }
 
 template <int DT>
@@ -287,7 +288,7 @@ __global__ void __launch_bounds__(kRowThreads, 2) spec_decide_kernel(const SpecA
         state = __shfl_sync(~0u, state, at);
         if (state == kOpen) {
             Dist<DT> p(a, b, taken, table), q(a, b, a.n + 1 + taken, table);
-            exact_sums<DT, true>(cl, sums, ring, p, q, g, warps);
+            exact_sums<DT>(cl, sums, ring, p, q, g, warps, true);
             const int d = (int)ids[taken];
             state = (double)u[taken] * q.prob(d, q.row.at(d)) < p.prob(d, p.row.at(d)) ? kStands : kFails;
         }
@@ -312,8 +313,7 @@ __global__ void __launch_bounds__(kRowThreads, 2) spec_decide_kernel(const SpecA
         const bool minus = drafted && tries < 2 && !q.dead();
         if (tries == 0 && !(p.st.sum > 0.0 && q.st.sum > 0.0)) continue;  // a sum is missing
         if (tries == 1) {
-            if (minus) exact_sums<DT, true>(cl, sums, ring, p, q, g, warps);
-            else exact_sums<DT, false>(cl, sums, ring, p, q, g, warps);
+            exact_sums<DT>(cl, sums, ring, p, q, g, warps, minus);
         }
         auto weigh = [&](int v, const float (&x)[N], const float (&y)[N], double (&out)[N]) {
             double other[N];
@@ -358,7 +358,7 @@ __global__ void __launch_bounds__(kRowThreads, 2) spec_decide_kernel(const SpecA
         const Place at = locate(places, warps, target);
         if (at.g >= 0 && rank == at.g / kRowWarps) {
             const Found f =
-                find_in_slice<DT>(p.row, warp_slice<DT>(p.row, at.g, warps), at.base, target, find,
+                find_in_slice<DT>(p.row, warp_slice<DT>(p.row, at.g, warps), at.base, target, ring, find,
                                               [&](int v, const uint4& w, double (&out)[N]) {
                                                   float x[N], y[N];
                                                   decode<DT>(w, x);
