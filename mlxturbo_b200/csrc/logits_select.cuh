@@ -10,7 +10,15 @@ namespace qmm {
 constexpr int kBins = 512;
 
 // A cluster's candidates are in its CTA 0.
-struct SelectShared {
+struct DrawShared {  // of a draw without filters
+    double slots[2][kMaxRowWarps];
+    WarpStat stats[kMaxRowWarps];
+    FindShared find;
+    double table[32];  // of Weight64
+    int verdict;
+};
+
+struct SelectShared : DrawShared {
     union {
         struct {
             union {
@@ -26,20 +34,15 @@ struct SelectShared {
         uint32_t bins[kRowWarps][2][kBins];  // of each warp: masses in two limbs
     };
     unsigned long long bin_sum[kBins];
-    double slots[2][kMaxRowWarps];
-    WarpStat stats[kMaxRowWarps];
     uint32_t found[kMaxRowWarps];
     uint32_t hist[256];
     uint32_t n_cand, sel_bin, sel_above;
-    unsigned long long bin_above;
+    unsigned long long bin_above, best;
     double scan[kRowWarps];
-    FindShared find;
-    double table[32];  // of Weight64
-    unsigned long long best;
-    int verdict;
 };
 
 constexpr size_t kSelectSmem = sizeof(SelectShared) + kRing * kRowThreads * sizeof(uint4);
+constexpr size_t kDrawSmem = sizeof(DrawShared) + kRing * kRowThreads * sizeof(uint4);
 
 // The largest 16-bit prefix b such that at least k of the n maxima have
 // key32 >> 16 >= b; 0 if there are fewer than k.  One CTA, all threads.

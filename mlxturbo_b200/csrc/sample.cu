@@ -16,9 +16,6 @@
 #include <stdlib.h>
 #include "logits_select.cuh"
 
-#ifndef SAMPLE_CTAS
-#define SAMPLE_CTAS 3
-#endif
 namespace qmm {
 
 // What CTA 0 makes of the candidates: the answer; a sum in 64 bits is needed;
@@ -38,14 +35,16 @@ QMM_DEVINL int count_before(const double* sums, int n, double limit) {
     return lo;
 }
 
-template <int DT>
-__global__ void __launch_bounds__(kRowThreads, SAMPLE_CTAS) sample_kernel(const SampleArgs a) {
+// FILTERS false: no row has a filter or is greedy, by the call's numbers.  That
+// kernel does without the selection's memory and registers: a fourth CTA to an SM.
+template <int DT, bool FILTERS>
+__global__ void __launch_bounds__(kRowThreads, FILTERS ? 3 : 4) sample_kernel(const SampleArgs a) {
     extern __shared__ uint4 memory[];
     SelectShared& sh = *reinterpret_cast<SelectShared*>(memory + kRing * kRowThreads);
     const Ring ring = reinterpret_cast<Ring>(memory);
     cg::cluster_group cl = cg::this_cluster();
     cl.barrier_arrive();  // waited for before the first access to another CTA
-    if (threadIdx.x == 0) sh.n_cand = 0;
+    if (FILTERS && threadIdx.x == 0) sh.n_cand = 0;
     fill_table(sh.table);
     const int C = (int)cl.num_blocks(), rank = (int)cl.block_rank(), warps = C * kRowWarps;
     const int g = rank * kRowWarps + (threadIdx.x >> 5);
@@ -54,16 +53,15 @@ __global__ void __launch_bounds__(kRowThreads, SAMPLE_CTAS) sample_kernel(const 
     const Slice s = warp_slice<DT>(row, g, warps);
 
     double T = a.t_rows ? (double)a.t_rows[r] : a.t;
-    const bool greedy = !(T > 0.0);
-    int k = a.k_rows ? a.k_rows[r] : a.k;
-    double p = a.p_rows ? (double)a.p_rows[r] : a.p;
-    double mp = a.m_rows ? (double)a.m_rows[r] : a.m;
-    if (greedy) {
+    int k = FILTERS && a.k_rows ? a.k_rows[r] : a.k;
+    const double p = FILTERS && a.p_rows ? (double)a.p_rows[r] : a.p;
+    double mp = FILTERS && a.m_rows ? (double)a.m_rows[r] : a.m;
+    if (!(T > 0.0)) {  // greedy
         T = 1.0;
         k = 1;
     }
-    const bool k_on = k >= 1 && k < a.V, p_on = p < 1.0 && !(k_on && k == 1);
-    const bool m_on = mp > 0.0 && !(k_on && k == 1);
+    const bool k_on = FILTERS && k >= 1 && k < a.V, p_on = FILTERS && p < 1.0 && !(k_on && k == 1);
+    const bool m_on = FILTERS && mp > 0.0 && !(k_on && k == 1);
     if (mp > 1.0) mp = 1.0;
     const double inv_t = 1.0 / T, u = (double)a.u[r];
     const bool sum = !k_on && (p_on || !m_on);
@@ -72,7 +70,7 @@ __global__ void __launch_bounds__(kRowThreads, SAMPLE_CTAS) sample_kernel(const 
     // one pass over memory
     LaneSum acc;
     const LaneTop top =
-        sum ? stream_slice<DT, true, true>(row, s, c, acc) : stream_slice<DT, false, true>(row, s, c, acc);
+        sum ? stream_slice<DT, true, FILTERS>(row, s, c, acc) : stream_slice<DT, false, true>(row, s, c, acc);
     const WarpStat stat = warp_stat(top.first, acc);
     const bool select = k_on || p_on;  // a bound from maxima
     const int want = k_on ? k : kRowThreads;
@@ -319,11 +317,21 @@ int row_cluster(long long rows, long long V, int elem_bytes, int ctas) {
     return C;
 }
 
+template <int DT>
+static int sample_dt(const qmm::SampleArgs& a, long long rows, cudaStream_t st) {
+    const bool filters = a.t_rows || a.k_rows || a.p_rows || a.m_rows || a.t == 0.0 || a.k || a.p < 1.0 || a.m > 0.0;
+    if (filters)
+        return launch_rows(qmm::sample_kernel<DT, true>, qmm::kRowThreads, rows,
+                           row_cluster(rows, a.V, qmm::Elem<DT>::kBytes, 4 * 148), qmm::kSelectSmem, st,
+                           "sample launch", a);
+    return launch_rows(qmm::sample_kernel<DT, false>, qmm::kRowThreads, rows,
+                       row_cluster(rows, a.V, qmm::Elem<DT>::kBytes, 4 * 148), qmm::kDrawSmem, st, "sample launch", a);
+}
+
 int launch_sample(const qmm::SampleArgs& a, long long rows, int dtype, cudaStream_t st) {
-    const int C = row_cluster(rows, a.V, dtype == QMM_F32 ? 4 : 2, 4 * 148);
-    if (dtype == QMM_BF16) return launch_rows(qmm::sample_kernel<0>, qmm::kRowThreads, rows, C, qmm::kSelectSmem, st, "sample launch", a);
-    if (dtype == QMM_F16) return launch_rows(qmm::sample_kernel<1>, qmm::kRowThreads, rows, C, qmm::kSelectSmem, st, "sample launch", a);
-    return launch_rows(qmm::sample_kernel<2>, qmm::kRowThreads, rows, C, qmm::kSelectSmem, st, "sample launch", a);
+    if (dtype == QMM_BF16) return sample_dt<0>(a, rows, st);
+    if (dtype == QMM_F16) return sample_dt<1>(a, rows, st);
+    return sample_dt<2>(a, rows, st);
 }
 
 }  // namespace qmm_host
