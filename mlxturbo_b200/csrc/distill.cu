@@ -41,22 +41,53 @@ struct DistillShared {
     int twice;     // an id is listed more than once
 };
 
-// The ids of the list, by one warp.
+// The ids of the list, by one warp; four loads of a lane at a time, as below.
 QMM_DEVINL void list_ids(const DistillArgs& a, DistillShared& sh, long long r) {
-    for (int j = threadIdx.x & 31; j < a.k; j += 32) {
-        const long long at = r * a.k + j;
-        const long long id = a.ti_bytes == 8 ? static_cast<const long long*>(a.ti)[at]
-                                             : (long long)static_cast<const int*>(a.ti)[at];
-        sh.id[j] = id >= 0 && id < a.V ? (int)id : -1;
+    for (int j0 = threadIdx.x & 31; j0 < a.k; j0 += 128) {
+        long long id[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const long long at = r * a.k + min(j0 + 32 * i, a.k - 1);
+            id[i] = a.ti_bytes == 8 ? __ldg(static_cast<const long long*>(a.ti) + at)
+                                    : (long long)__ldg(static_cast<const int*>(a.ti) + at);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (j0 + 32 * i < a.k) sh.id[j0 + 32 * i] = id[i] >= 0 && id[i] < a.V ? (int)id[i] : -1;
     }
     __syncwarp();
 }
 
 // The rest of it, by one warp: log p and the student's logits; entries of one
 // id share a slot whose owner is the first of them; the sums.
-template <int DT>
+template <int DT, bool TAIL>
 QMM_DEVINL void list_sums(const DistillArgs& a, DistillShared& sh, const Row<DT>& row, long long r) {
     const int lane = threadIdx.x & 31;
+    double top = -CUDART_INF;
+    float best = -CUDART_INF_F;
+    for (int j0 = lane; j0 < a.k; j0 += 128) {
+        float t[4], x[4];
+        int id[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int j = min(j0 + 32 * i, a.k - 1);
+            const long long at = r * a.k + j;
+            id[i] = sh.id[j];
+            t[i] = a.tv_dtype == 2 ? __ldg(static_cast<const float*>(a.tv) + at)
+                   : a.tv_dtype == 1 ? Half<true>::to_f32(__ldg(static_cast<const uint16_t*>(a.tv) + at))
+                                     : Half<false>::to_f32(__ldg(static_cast<const uint16_t*>(a.tv) + at));
+            x[i] = id[i] >= 0 ? row.at(id[i]) : 0.0f;
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (j0 + 32 * i >= a.k) break;
+            const double l = id[i] >= 0 ? (double)t[i] * a.inv_t : -CUDART_INF;
+            sh.x[j0 + 32 * i] = x[i];
+            sh.logp[j0 + 32 * i] = l;
+            top = fmax(top, l);  // a NaN shows in the sums
+            if (id[i] >= 0) best = fmaxf(best, x[i]);
+        }
+    }
     int size = 2;
     while (size < 2 * a.k) size <<= 1;
     for (int i = lane; i < size; i += 32) {
@@ -64,38 +95,26 @@ QMM_DEVINL void list_sums(const DistillArgs& a, DistillShared& sh, const Row<DT>
         sh.owner[i] = kMaxList;
     }
     __syncwarp();
-    double top = -CUDART_INF;
-    float best = -CUDART_INF_F;
     bool twice = false;
     for (int j = lane; j < a.k; j += 32) {
-        const long long at = r * a.k + j;
         const int id = sh.id[j];
-        const float t = a.tv_dtype == 2 ? elem_f32<2>(a.tv, at) : a.tv_dtype == 1 ? elem_f32<1>(a.tv, at)
-                                                                                 : elem_f32<0>(a.tv, at);
-        const float x = id >= 0 ? row.at(id) : 0.0f;
-        sh.x[j] = x;
-        const double l = id >= 0 ? (double)t * a.inv_t : -CUDART_INF;
-        sh.logp[j] = l;
-        top = fmax(top, l);  // a NaN shows in the sums
-        if (id >= 0) {
-            best = fmaxf(best, x);
-            int h = (int)((uint32_t)id * 2654435761u >> 16) & (size - 1);
-            for (;;) {
-                const int was = atomicCAS(&sh.table[h], -1, id);
-                twice |= was == id;
-                if (was == -1 || was == id) break;
-                h = (h + 1) & (size - 1);
-            }
-            sh.slot[j] = h;
-            atomicMin(&sh.owner[h], j);
+        if (id < 0) continue;
+        int h = (int)((uint32_t)id * 2654435761u >> 16) & (size - 1);
+        for (;;) {
+            const int was = atomicCAS(&sh.table[h], -1, id);
+            twice |= was == id;
+            if (was == -1 || was == id) break;
+            h = (h + 1) & (size - 1);
         }
+        sh.slot[j] = h;
+        atomicMin(&sh.owner[h], j);
     }
     __syncwarp();
 #pragma unroll
     for (int o = 16; o >= 1; o >>= 1) top = fmax(top, __shfl_xor_sync(~0u, top, o));
     best = warp_max(best);
     double norm = 0.0;
-    if (a.tlse) {
+    if (TAIL) {
         norm = (double)a.tlse[r];
     } else if (top != -CUDART_INF) {  // else nothing is listed
         double sum = 0.0;
@@ -109,11 +128,11 @@ QMM_DEVINL void list_sums(const DistillArgs& a, DistillShared& sh, const Row<DT>
         mass += p;
         if (sh.id[j] < 0) continue;
         if (p != 0.0) cross += p * (lp - (double)sh.x[j] * a.inv_t);
-        if (sh.owner[sh.slot[j]] == j) part += exp(((double)sh.x[j] - (double)best) * a.inv_t);
+        if (TAIL && sh.owner[sh.slot[j]] == j) part += exp(((double)sh.x[j] - (double)best) * a.inv_t);
     }
     mass = warp_sum(mass);
     cross = warp_sum(cross);
-    part = warp_sum(part);
+    if (TAIL) part = warp_sum(part);
     twice = __any_sync(~0u, twice);
     if (lane == 0) {
         sh.mass = mass;
@@ -156,7 +175,7 @@ QMM_DEVINL bool out_of_range(float ref) { return fabsf(ref) > kFastMax && fabsf(
 
 // TAIL: the teacher's log-sum-exp is given.  MODE kBackward needs no cluster.
 template <int DT, bool TAIL, int MODE>
-__global__ void __launch_bounds__(kDistillThreads, MODE == kLossGrad ? 3 : 4)
+__global__ void __launch_bounds__(kDistillThreads, 4)
     distill_kernel(const DistillArgs a, int C) {
     __shared__ DistillShared sh;
     extern __shared__ uint32_t marks[];  // TAIL: a byte to a vector of this CTA
@@ -186,7 +205,7 @@ __global__ void __launch_bounds__(kDistillThreads, MODE == kLossGrad ? 3 : 4)
         sum = st.w;
         if (!reader && weight != 0.0f) {
             list_ids(a, sh, r);
-            list_sums<DT>(a, sh, row, r);
+            list_sums<DT, TAIL>(a, sh, row, r);
         }
     } else {
         if (!reader) list_ids(a, sh, r);
@@ -214,7 +233,7 @@ __global__ void __launch_bounds__(kDistillThreads, MODE == kLossGrad ? 3 : 4)
             });
             stat = warp_stat(top.first, acc);
         } else {
-            list_sums<DT>(a, sh, row, r);
+            list_sums<DT, TAIL>(a, sh, row, r);
         }
         cl.barrier_wait();
         if (reader) all_gather(cl, sh.stats, g, stat);
@@ -244,19 +263,17 @@ __global__ void __launch_bounds__(kDistillThreads, MODE == kLossGrad ? 3 : 4)
         if (MODE == kLoss && (rank != 0 || reader)) return;
         // the list's part of the sum
         const double mass = sh.mass;
-        double rest = 0.0, log_other = 0.0;
+        double rest = 0.0;
         mx = ref;
         sum = s_ref;
         if (TAIL) {
             mx = fmaxf(ref, sh.best);
-            const double lift = ref == -CUDART_INF_F ? 0.0 : exp(((double)ref - (double)mx) * a.inv_t);
-            const double listed =
-                sh.best == -CUDART_INF_F ? 0.0 : sh.part * exp(((double)sh.best - (double)mx) * a.inv_t);
-            sum = s_ref * lift + listed;
+            // one of the two is 1; the other to some digits of 32 bits
+            const float lift = ref == -CUDART_INF_F ? 0.0f : expf((float)(((double)ref - (double)mx) * a.inv_t));
+            const float down = sh.best == -CUDART_INF_F ? 0.0f : expf((float)(((double)sh.best - (double)mx) * a.inv_t));
+            sum = s_ref * (double)lift + sh.part * (double)down;
             rest = mass < 1.0 ? 1.0 - mass : mass >= 1.0 ? 0.0 : mass;
-            log_other = ref == -CUDART_INF_F ? -CUDART_INF
-                                             : ((double)ref - (double)mx) * a.inv_t + log(s_ref) - log(sum);
-            others = lift / sum - (s_ref > 0.0 ? rest / s_ref : 0.0);
+            others = (double)lift / sum - (s_ref > 0.0 ? rest / s_ref : 0.0);
             if (ref == -CUDART_INF_F) others = 0.0;  // no token that is not listed has any probability
         } else {
             others = mass == 0.0 ? 0.0 : 1.0 / sum;
@@ -264,7 +281,12 @@ __global__ void __launch_bounds__(kDistillThreads, MODE == kLossGrad ? 3 : 4)
         if (rank == 0 && threadIdx.x == kRowThreads) {
             double loss = sh.cross;
             if (mass != 0.0) loss += mass * ((double)mx * a.inv_t + log(sum));
-            if (TAIL && rest != 0.0) loss += rest * (log(rest) - log_other);
+            if (TAIL && rest != 0.0) {
+                const double log_other = ref == -CUDART_INF_F
+                                             ? -CUDART_INF
+                                             : ((double)ref - (double)mx) * a.inv_t + log(s_ref) - log(sum);
+                loss += rest * (log(rest) - log_other);
+            }
             a.loss[r] = none ? 0.0f : (float)loss;
             if (MODE == kLoss && a.stats) a.stats[r] = make_float4(ref, (float)others, mx, (float)sum);
         }

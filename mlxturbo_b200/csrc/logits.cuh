@@ -237,8 +237,10 @@ constexpr double kFastMinT = 1e-6, kFastMaxT = 1e6;
 struct Scale {
     float c;
     QMM_DEVINL explicit Scale(double inv_t) : c((float)(inv_t * 1.4426950408889634)) {}
-    // what turns a sum against E into one against the weight of mx
-    QMM_DEVINL double against(float e, float mx) const { return exp2((double)e - (double)mx * (double)c); }
+    // what turns a sum against E = ceil(mx c) into one against the weight of mx
+    QMM_DEVINL double against(float e, float mx) const {
+        return (double)exp2f((float)((double)e - (double)mx * (double)c));
+    }
     QMM_DEVINL bool fast(float mx, double T) const {
         return fabsf(mx) <= kFastMax && T >= kFastMinT && T <= kFastMaxT;
     }
