@@ -673,8 +673,9 @@ QMM_DEVINL Found find_in_slice(const Row<DT>& row, const Slice& s, double base, 
 
 namespace qmm_host {
 
-// CTAs to a row: so many that a lane holds at most 64 vectors, and more, down to
-// 2 vectors to a lane, until the call has `ctas` of them.
+// CTAs to a row: so many that a lane holds at most 64 vectors; more, down to 8
+// vectors to a lane, until the call has `ctas` of them, and down to 2 until it
+// has one for every SM.
 int row_cluster(long long rows, long long V, int elem_bytes, int ctas);
 
 // Launch `kernel` over rows * C CTAs in clusters of C.

@@ -21,6 +21,7 @@
 #include <ATen/cuda/CUDAContext.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
+#include <torch/csrc/autograd/custom_function.h>
 #include <torch/library.h>
 #include <torch/types.h>
 
@@ -575,6 +576,55 @@ at::Tensor distill_backward(const at::Tensor& logits, const at::Tensor& tv, cons
     return grad;
 }
 
+// The differentiable loss: below autograd it is the loss alone; where the logits
+// ask for a gradient, the loss with what its backward pass takes.
+at::Tensor distill(const at::Tensor& logits, const at::Tensor& tv, const at::Tensor& ti,
+                   const std::optional<at::Tensor>& lse, double t) {
+    return std::get<0>(distill_loss(logits, tv, ti, lse, t, false));
+}
+
+// The operators as the dispatcher has them, so that modes below autograd see the calls.
+template <typename F>
+auto registered(const char* name) {
+    return c10::Dispatcher::singleton().findSchemaOrThrow(name, "").typed<F>();
+}
+
+struct DistillFunction : torch::autograd::Function<DistillFunction> {
+    static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& logits, const at::Tensor& tv,
+                              const at::Tensor& ti, const std::optional<at::Tensor>& lse, double t) {
+        at::AutoDispatchBelowADInplaceOrView below;
+        at::Tensor loss, stats;
+        static const auto op = registered<decltype(distill_loss)>("mlxturbo_b200::distill_loss");
+        std::tie(loss, stats) = op.call(logits, tv, ti, lse, t, true);
+        ctx->save_for_backward({logits, tv, ti, lse.has_value() ? *lse : at::Tensor(), stats});
+        ctx->saved_data["t"] = t;
+        return loss;
+    }
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                   torch::autograd::variable_list grads) {
+        const auto saved = ctx->get_saved_variables();
+        if (at::GradMode::is_enabled() && grads[0].requires_grad())
+            fail(Err::kNotImplemented, "the distillation loss has no second derivative");
+        at::AutoDispatchBelowADInplaceOrView below;
+        const std::optional<at::Tensor> lse = saved[3].defined() ? std::optional<at::Tensor>(saved[3]) : std::nullopt;
+        static const auto op = registered<decltype(distill_backward)>("mlxturbo_b200::distill_backward");
+        return {op.call(saved[0], saved[1], saved[2], lse, ctx->saved_data["t"].toDouble(), saved[4], grads[0]),
+                at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()};
+    }
+};
+
+at::Tensor distill_autograd(const at::Tensor& logits, const at::Tensor& tv, const at::Tensor& ti,
+                            const std::optional<at::Tensor>& lse, double t) {
+    if (at::GradMode::is_enabled()) {
+        if (tv.requires_grad() || (lse.has_value() && lse->requires_grad()))
+            fail(Err::kNotImplemented, "the distillation loss has no gradient for the teacher's side; detach it");
+        if (logits.requires_grad()) return DistillFunction::apply(logits, tv, ti, lse, t);
+    }
+    at::AutoDispatchBelowADInplaceOrView below;
+    static const auto op = registered<decltype(distill)>("mlxturbo_b200::distill");
+    return op.call(logits, tv, ti, lse, t);
+}
+
 // grad: a new tensor, or (out) one given, which may be the logits themselves.
 at::Tensor run_distill_loss_grad(const at::Tensor& logits, const at::Tensor& tv, const at::Tensor& ti,
                                  const std::optional<at::Tensor>& weight, const std::optional<at::Tensor>& lse,
@@ -662,6 +712,8 @@ TORCH_LIBRARY(mlxturbo_b200, m) {
           "-> (Tensor, Tensor)");
     m.def("distill_loss(Tensor logits, Tensor teacher_values, Tensor teacher_ids, Tensor? teacher_logsumexp, "
           "float temperature, bool stats) -> (Tensor, Tensor)");
+    m.def("distill(Tensor logits, Tensor teacher_values, Tensor teacher_ids, Tensor? teacher_logsumexp, "
+          "float temperature) -> Tensor");
     m.def("distill_backward(Tensor logits, Tensor teacher_values, Tensor teacher_ids, Tensor? teacher_logsumexp, "
           "float temperature, Tensor stats, Tensor grad_loss) -> Tensor");
     m.def("distill_loss_grad(Tensor logits, Tensor teacher_values, Tensor teacher_ids, Tensor? row_weight, "
@@ -685,6 +737,7 @@ void logits_impl(torch::Library& m) {
     m.impl("sample", &sample);
     m.impl("topk", &topk);
     m.impl("speculative_sample", &speculative_sample);
+    m.impl("distill", &distill);
     m.impl("distill_loss", &distill_loss);
     m.impl("distill_backward", &distill_backward);
     m.impl("distill_loss_grad", &distill_loss_grad);
@@ -704,3 +757,5 @@ TORCH_LIBRARY_IMPL(mlxturbo_b200, CPU, m) {
     mx_impl(m);
     logits_impl(m);
 }
+
+TORCH_LIBRARY_IMPL(mlxturbo_b200, Autograd, m) { m.impl("distill", &distill_autograd); }

@@ -551,8 +551,7 @@ class _LogitsOps:
         self.sample = ops.sample.default
         self.topk = ops.topk.default
         self.speculative = ops.speculative_sample.default
-        self.distill = ops.distill_loss.default
-        self.distill_backward = ops.distill_backward.default
+        self.distill = ops.distill.default
         self.distill_grad = ops.distill_loss_grad.default
         self.distill_grad_out = ops.distill_loss_grad_out.default
 
@@ -631,23 +630,6 @@ def speculative_sample(logits: torch.Tensor, draft_logits: torch.Tensor, draft_i
                                      *_rows_or_one(draft_temperature, 0.0))
 
 
-class _DistillLoss(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, teacher_values, teacher_ids, teacher_logsumexp, temperature):
-        loss, stats = _logits_ops().distill(logits, teacher_values, teacher_ids, teacher_logsumexp, temperature, True)
-        ctx.save_for_backward(logits, teacher_values, teacher_ids, teacher_logsumexp, stats)
-        ctx.temperature = temperature
-        return loss
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, grad_loss):
-        logits, teacher_values, teacher_ids, teacher_logsumexp, stats = ctx.saved_tensors
-        grad = _logits_ops().distill_backward(logits, teacher_values, teacher_ids, teacher_logsumexp,
-                                              ctx.temperature, stats, grad_loss)
-        return grad, None, None, None, None
-
-
 def _no_teacher_grad(*tensors) -> None:
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
         raise NotImplementedError("the distillation loss has no gradient for the teacher's side; detach it")
@@ -669,10 +651,7 @@ def distill_loss(logits: torch.Tensor, teacher_values: torch.Tensor, teacher_ids
     gradient is 0 is 0, whatever its logits; the loss is not multiplied by
     temperature squared.
     """
-    _no_teacher_grad(teacher_values, teacher_logsumexp)
-    if torch.is_grad_enabled() and logits.requires_grad:
-        return _DistillLoss.apply(logits, teacher_values, teacher_ids, teacher_logsumexp, temperature)
-    return _logits_ops().distill(logits, teacher_values, teacher_ids, teacher_logsumexp, temperature, False)[0]
+    return _logits_ops().distill(logits, teacher_values, teacher_ids, teacher_logsumexp, temperature)
 
 
 def distill_loss_and_grad(logits: torch.Tensor, teacher_values: torch.Tensor, teacher_ids: torch.Tensor,
