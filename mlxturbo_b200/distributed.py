@@ -27,7 +27,7 @@ verify or prefill projection runs as an independent replica per GPU.
 The local matmul defaults to ``ops.quantized_matmul``.  Expert compute and
 the combine default to the CUDA kernels.  There is no CPU path: tests of the
 partitioning logic on CPU (``gloo``) pass their own ``matmul`` /
-``expert_fn`` / ``combine_fn``.
+``expert_fn`` / ``combine_fn`` / ``sampler``.
 """
 
 from __future__ import annotations
@@ -188,8 +188,8 @@ class ColumnShardedLMHead(_ShardedBase):
         Each rank takes the top k of its own slice, so only M*P*k (value, id)
         pairs cross the interconnect instead of the M*N logits, then every rank
         merges the P*k candidates.  Equal values keep the lowest token id, as a
-        single-device ``argmax`` does (for k = 1 exactly; for k > 1 a tie at a
-        shard's k-th value may keep either id).  k=1 is greedy sampling.
+        single-device ``argmax`` does (for k > ``ops.TOPK_MAX``, and on the CPU, a
+        tie at a shard's k-th value may keep either id).  k=1 is greedy sampling.
         """
         lead = x.shape[:-1]
         local = self.forward(x, gather=False).reshape(-1, self.shard_rows)  # [M, N/P]
@@ -198,6 +198,9 @@ class ColumnShardedLMHead(_ShardedBase):
         kk = min(k, local.shape[1])
         if kk == 1:  # first occurrence of the maximum, like argmax on one device
             vals, idx = local.float().max(dim=-1, keepdim=True)
+        elif local.is_cuda and kk <= ops.TOPK_MAX:
+            vals, idx = ops.topk(local, kk)
+            vals = vals.float()
         else:  # (ties at a shard's k-th value may keep either id)
             vals, idx = torch.topk(local.float(), kk, dim=-1, sorted=True)
         idx = idx.to(torch.int64) + rank * self.shard_rows
@@ -241,6 +244,22 @@ class ColumnShardedLMHead(_ShardedBase):
             dist.all_gather_into_tensor(keys, key.contiguous(), group=self.group)
             key = ops.max_keys(keys.view(world, -1), dim=0)
         return ops.argmax_from_keys(key).reshape(lead)
+
+    def _all_logits(self, x):
+        return self.forward(x, gather=_group_rank_world(self.group)[1] > 1)
+
+    def sample(self, x, u, *, sampler=None, **settings):
+        """Sampled next-token ids [...] from the uniform numbers u [...] (``ops.sample`` and its settings).
+
+        A filter or a sum needs the whole row, so the logits are gathered; every
+        rank that is given the same u draws the same ids.
+        """
+        return (sampler or ops.sample)(self._all_logits(x), u, **settings)
+
+    def distill_loss(self, x, teacher_values, teacher_ids, *, loss=None, **settings):
+        """Divergence [...] of this head's logits from a teacher's top logits (``ops.distill_loss``): what
+        quantisation costs, with ``topk`` of the unquantised model's logits as the lists."""
+        return (loss or ops.distill_loss)(self._all_logits(x), teacher_values, teacher_ids, **settings)
 
 
 def _default_expert_fn(glu, x_rows: torch.Tensor, local_ids: torch.Tensor) -> torch.Tensor:
