@@ -192,12 +192,18 @@ struct Weight64 {
     double c, b, inv_t;
     float mx, least, far;  // below `least` nothing is left; below `far` the result is made in two steps
 
-    QMM_DEVINL Weight64(const double* table_, float mx_, double inv_t_)
+    // inv_t = 1 / T
+    QMM_DEVINL Weight64(const double* table_, float mx_, double T, double inv_t_)
         : table(table_), c(inv_t_ * 1.4426950408889634), b(-(double)mx_ * c), inv_t(inv_t_), mx(mx_),
-          least((float)((double)mx_ - 1080.0 / c)), far((float)((double)mx_ - 900.0 / c)) {}
+          least(mx_ - 748.6f * (float)T), far(mx_ - 623.8f * (float)T) {}  // 1080 and 900 powers of two
 
     QMM_DEVINL double operator()(float x) const {
-        const double t = fma((double)x, c, b);
+        const double w = power(fma((double)x, c, b), x < far);
+        return x == mx ? 1.0 : x > least ? w : 0.0;
+    }
+
+    // 2^t for -1080 < t < 1000; small: t < -800 or so
+    QMM_DEVINL double power(double t, bool small) const {
         const double magic = 6755399441055744.0 / 32.0;  // 1.5 * 2^52 / 32: sums are whole 32nds
         const double k = t + magic;
         const double r = t - (k - magic);
@@ -208,12 +214,9 @@ struct Weight64 {
         p = fma(r, p, 2.4022650695910072e-1);
         p = fma(r, p, 6.931471805599453e-1);
         p = fma(r, p, 1.0) * table[n & 31];
-        const bool small = x < far;
         const int up = (n >> 5) + (small ? 300 : 0);
-        double w = __hiloint2double(__double2hiint(p) + (up << 20), __double2loint(p));
-        w *= small ? 4.909093465297727e-91 : 1.0;  // 2^-300
-        w = x > least ? w : 0.0;
-        return x == mx ? 1.0 : w;
+        const double w = __hiloint2double(__double2hiint(p) + (up << 20), __double2loint(p));
+        return w * (small ? 4.909093465297727e-91 : 1.0);  // 2^-300
     }
 };
 
@@ -252,8 +255,9 @@ struct LaneSum {
     double s = 0.0;
 };
 
-template <int N>
-QMM_DEVINL float tree_sum(float (&e)[N]) {
+// In a tree: one long chain of 64-bit additions outlasts the weights themselves.
+template <typename T, int N>
+QMM_DEVINL T tree_sum(T (&e)[N]) {
 #pragma unroll
     for (int h = N / 2; h >= 1; h /= 2)
 #pragma unroll
@@ -446,7 +450,7 @@ QMM_DEVINL LaneTop stream_slice(const Row<DT>& row, const Slice& s, const Scale&
             decode<DT>(u[i], e);
 #pragma unroll
             for (int j = 0; j < N; ++j) e[j] = ex2(fmaf(e[j], c.c, -acc.e));
-            sum += tree_sum<N>(e);
+            sum += tree_sum(e);
         }
         acc.s += (double)sum;
     });
@@ -624,11 +628,13 @@ QMM_DEVINL Found find_place(const Row<DT>& row, int from, int to, double base, d
             double w[N];
             const int i = v - first;
             weights(v, i < kRing ? ring[i][t] : row.load(v), w);
+            if (turn == 0) {
+                mass += tree_sum(w);
+                continue;
+            }
 #pragma unroll
             for (int j = 0; j < N; ++j) {
-                if (turn == 0) {
-                    mass += w[j];
-                } else if (w[j] > 0.0 && !done) {
+                if (w[j] > 0.0 && !done) {
                     f.id = row.first(v) + j;
                     f.before = run;
                     run += w[j];

@@ -38,6 +38,7 @@ struct TopkArgs {
 
 struct RowStat {
     double sum;  // NaN: only a sum in 64 bits will do
+    double inv_t;
     float mx;
     int arg;  // lowest id of the maximum, of greedy rows
 };

@@ -88,7 +88,7 @@ __global__ void __launch_bounds__(kRowThreads, FILTERS ? 3 : 4) sample_kernel(co
         return;
     }
     const bool fast = sum && c.fast(mx, T) && total >= 0.5 && total < CUDART_INF;  // else 64 bits
-    const Weight64 weight(sh.table, mx, inv_t);
+    const Weight64 weight(sh.table, mx, T, inv_t);
 
     // smallest key that min-p keeps; masked tokens have none
     uint32_t kmin = kKeyNegInf + 1;
@@ -210,9 +210,11 @@ __global__ void __launch_bounds__(kRowThreads, FILTERS ? 3 : 4) sample_kernel(co
                 double mass = 0.0;
                 for_vectors_slow<DT>(row, s, ring, [&](int v, const uint4& q) {
                     float x[Elem<DT>::kVec];
+                    double w[Elem<DT>::kVec];
                     decode<DT>(q, x);
 #pragma unroll
-                    for (int j = 0; j < Elem<DT>::kVec; ++j) mass += weight(x[j]);
+                    for (int j = 0; j < Elem<DT>::kVec; ++j) w[j] = weight(x[j]);
+                    mass += tree_sum(w);
                 });
                 all_gather(cl, sh.slots[1], g, warp_sum(mass));
                 cl.sync();
@@ -289,8 +291,7 @@ __global__ void __launch_bounds__(kRowThreads, FILTERS ? 3 : 4) sample_kernel(co
     for_vectors_slow<DT>(row, s, ring, [&](int v, const uint4& q) {
         double w[Elem<DT>::kVec];
         kept(v, q, w);
-#pragma unroll
-        for (int j = 0; j < Elem<DT>::kVec; ++j) mass += w[j];
+        mass += tree_sum(w);
     });
     cl.sync();
     all_gather(cl, sh.slots[0], g, warp_sum(mass));

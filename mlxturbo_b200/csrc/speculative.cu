@@ -88,6 +88,7 @@ __global__ void __launch_bounds__(kRowThreads, 4) spec_stats_kernel(const SpecAr
         st.mx = mx;
         st.arg = -1;
         st.sum = 1.0;
+        st.inv_t = greedy ? 1.0 : 1.0 / T;
         if (greedy) {
             int first = 0x7FFFFFFF;
             for (int w = s.lane; w < warps; w += 32) first = min(first, args[w]);
@@ -108,9 +109,10 @@ struct Dist {
     Weight64 exact;
 
     QMM_DEVINL Dist(const SpecArgs& a, long long b, int i, const double* table)
-        : row(spec_row<DT>(a, b, i)), st(a.stats[b * (2 * a.n + 1) + i]),
-          greedy(!(spec_temperature(a, b, i > a.n) > 0.0)),
-          exact(table, st.mx, greedy ? 1.0 : 1.0 / spec_temperature(a, b, i > a.n)) {
+        : Dist(a, b, i, table, spec_temperature(a, b, i > a.n)) {}
+    QMM_DEVINL Dist(const SpecArgs& a, long long b, int i, const double* table, double T)
+        : row(spec_row<DT>(a, b, i)), st(a.stats[b * (2 * a.n + 1) + i]), greedy(!(T > 0.0)),
+          exact(table, st.mx, T, st.inv_t) {
         if (dead()) st.sum = 1.0;
     }
     QMM_DEVINL double weight(int id, float x) const {
@@ -213,14 +215,16 @@ __device__ __noinline__ void exact_sums(cg::cluster_group& cl, TwoSums* slots, R
     constexpr int N = Elem<DT>::kVec;
     TwoSums mass{0.0, 0.0};
     const Slice s = warp_slice<DT>(p.row, g, warps);
-    for_pairs<DT>(p.row, q.row, s, ring, both, [&](int v, const float (&x)[N], const float (&y)[N]) {
+    const Weight64 wp = p.exact, wq = q.exact;  // in registers
+    for_pairs<DT>(p.row, q.row, s, ring, both, [&](int, const float (&x)[N], const float (&y)[N]) {
+        double w[N];  // past the ends -infinity: nothing
 #pragma unroll
-        for (int j = 0; j < N; ++j) {
-            const int id = p.row.first(v) + j;
-            const bool in = id >= 0 && id < p.row.V;
-            mass.p += in ? p.exact(x[j]) : 0.0;
-            if (both) mass.q += in ? q.exact(y[j]) : 0.0;
-        }
+        for (int j = 0; j < N; ++j) w[j] = wp(x[j]);
+        mass.p += tree_sum(w);
+        if (!both) return;
+#pragma unroll
+        for (int j = 0; j < N; ++j) w[j] = wq(y[j]);
+        mass.q += tree_sum(w);
     });
     mass.p = warp_sum(mass.p);
     mass.q = warp_sum(mass.q);
@@ -331,8 +335,7 @@ __global__ void __launch_bounds__(kRowThreads, 2) spec_decide_kernel(const SpecA
             for_pairs<DT>(p.row, q.row, s, ring, minus, [&](int v, const float (&x)[N], const float (&y)[N]) {
                 double out[N];
                 weigh(v, x, y, out);
-#pragma unroll
-                for (int j = 0; j < N; ++j) mass += out[j];
+                mass += tree_sum(out);
             });
         } else {
             const Scale cp(p.exact.inv_t), cq(q.exact.inv_t);
@@ -345,7 +348,7 @@ __global__ void __launch_bounds__(kRowThreads, 2) spec_decide_kernel(const SpecA
                     w[j] = fp * ex2(fmaf(x[j], cp.c, -ep));
                     if (minus) w[j] = fmaxf(w[j] - fq * ex2(fmaf(y[j], cq.c, -eq)), 0.0f);
                 }
-                mass += (double)tree_sum<N>(w);
+                mass += (double)tree_sum(w);
             });
         }
         double* const places = slots[tries & 1];

@@ -42,14 +42,16 @@ __global__ void __launch_bounds__(kRowThreads, 3) topk_kernel(const TopkArgs a) 
     double total = 0.0;
     if (LSE) row_stat(sh.stats, warps, c, mx, total, nullptr);
     const uint32_t bound = listed ? kth_bound(sh, warps * (32 / lanes), a.k) : 0;
-    const Weight64 weight(sh.table, mx, a.inv_t);
+    const Weight64 weight(sh.table, mx, 1.0 / a.inv_t, a.inv_t);
     if (LSE && fabsf(mx) != CUDART_INF_F && !(c.fast(mx, 1.0 / a.inv_t) && total >= 0.5 && total < CUDART_INF)) {
         double mass = 0.0;  // a NaN among the logits, or none above a mask's lowest value
         for_vectors_slow<DT>(row, s, ring, [&](int, const uint4& q) {
             float x[Elem<DT>::kVec];
+            double w[Elem<DT>::kVec];
             decode<DT>(q, x);
 #pragma unroll
-            for (int j = 0; j < Elem<DT>::kVec; ++j) mass += weight(x[j]);
+            for (int j = 0; j < Elem<DT>::kVec; ++j) w[j] = weight(x[j]);
+            mass += tree_sum(w);
         });
         all_gather(cl, sh.slots[1], g, warp_sum(mass));
         cl.sync();
@@ -72,7 +74,7 @@ __global__ void __launch_bounds__(kRowThreads, 3) topk_kernel(const TopkArgs a) 
     if (n > kCand) {  // the border, then the k tokens from it on
         // the search takes logits up to its maximum: infinite ones too
         const unsigned long long border = border_key<DT, false>(cl, sh, row, s, g, warps, ring,
-                                                                Weight64(sh.table, CUDART_INF_F, 1.0),
+                                                                Weight64(sh.table, CUDART_INF_F, 1.0, 1.0),
                                                                 (unsigned long long)kKeyNegInf << 32, (double)a.k);
         cl.sync();
         if (threadIdx.x == 0) sh.n_cand = 0;
