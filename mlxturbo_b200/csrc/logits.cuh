@@ -183,27 +183,26 @@ QMM_DEVINL float ex2(float a) {
 
 // In 64 bits: 2^t, t = (x - max) log2(e) / T, as a table's 2^(j/32) times the
 // Taylor polynomial of 2^r, |r| <= 1/64 (the term left out is below 3e-15),
-// with the whole part added to the exponent: 12 operations of the 64-bit pipe
+// with the whole part added to the exponent: 10 operations of the 64-bit pipe
 // and no branch, so the elements of a vector overlap (with exp() and its
-// branches a vector of 8 took 3.4 us of a warp's time).  The largest logit
-// weighs 1 even where it is infinite; NaN weighs nothing.
+// branches a vector of 8 took 3.4 us of a warp's time).  That pipe takes a cycle
+// of an SM to 32 elements, so a pass over a row costs four times what reading
+// 16-bit logits does; summing all rows of a call this way took 200 us for 512
+// rows of 248320, against 180 with fast sums and 64 bits for the open rows only.
+// The largest logit weighs 1 even where it is infinite; below 2^-1000, and for
+// NaN, there is no weight.
 struct Weight64 {
     const double* table;  // 2^(j/32), j = 0 .. 31, in shared memory
     double c, b, inv_t;
-    float mx, least, far;  // below `least` nothing is left; below `far` the result is made in two steps
+    float mx, least;
 
     // inv_t = 1 / T
     QMM_DEVINL Weight64(const double* table_, float mx_, double T, double inv_t_)
         : table(table_), c(inv_t_ * 1.4426950408889634), b(-(double)mx_ * c), inv_t(inv_t_), mx(mx_),
-          least(mx_ - 748.6f * (float)T), far(mx_ - 623.8f * (float)T) {}  // 1080 and 900 powers of two
+          least(mx_ - 693.0f * (float)T) {}  // 1000 ln2
 
     QMM_DEVINL double operator()(float x) const {
-        const double w = power(fma((double)x, c, b), x < far);
-        return x == mx ? 1.0 : x > least ? w : 0.0;
-    }
-
-    // 2^t for -1080 < t < 1000; small: t < -800 or so
-    QMM_DEVINL double power(double t, bool small) const {
+        const double t = fma((double)x, c, b);
         const double magic = 6755399441055744.0 / 32.0;  // 1.5 * 2^52 / 32: sums are whole 32nds
         const double k = t + magic;
         const double r = t - (k - magic);
@@ -214,9 +213,8 @@ struct Weight64 {
         p = fma(r, p, 2.4022650695910072e-1);
         p = fma(r, p, 6.931471805599453e-1);
         p = fma(r, p, 1.0) * table[n & 31];
-        const int up = (n >> 5) + (small ? 300 : 0);
-        const double w = __hiloint2double(__double2hiint(p) + (up << 20), __double2loint(p));
-        return w * (small ? 4.909093465297727e-91 : 1.0);  // 2^-300
+        const double w = __hiloint2double(__double2hiint(p) + ((n >> 5) << 20), __double2loint(p));
+        return x == mx ? 1.0 : x > least ? w : 0.0;
     }
 };
 
@@ -357,10 +355,10 @@ QMM_DEVINL void for_vectors_rare(const Row<DT>& row, const Slice& s, F&& f) {
 }
 
 // The same for passes whose arithmetic in 64 bits needs the registers: vectors
-// one at a time, the next seven on their way into shared memory (cp.async, each
+// one at a time, the next three on their way into shared memory (cp.async, each
 // thread's own slots, so nothing has to be synchronised).  With one load ahead
 // instead, a pass of 30 vectors to a lane took 30 us under a busy memory.
-constexpr int kRing = 8;
+constexpr int kRing = 4;
 using Ring = uint4 (*)[kRowThreads];  // [kRing][kRowThreads] in shared memory
 
 QMM_DEVINL void async_copy16(uint4* to, const void* from) {
@@ -492,9 +490,12 @@ struct alignas(16) WarpStat {
     float top, e;
 };
 
-QMM_DEVINL WarpStat warp_stat(float top, const LaneSum& acc) {
+QMM_DEVINL WarpStat warp_stat(float top, const LaneSum& acc, bool sum = true) {
     WarpStat w;
     w.top = warp_max(top);
+    w.e = 0.0f;
+    w.s = 0.0;
+    if (!sum) return w;
     w.e = warp_max(acc.e);
     w.s = warp_sum(acc.s * (double)ex2(acc.e - w.e));
     return w;
@@ -504,14 +505,16 @@ QMM_DEVINL WarpStat warp_stat(float top, const LaneSum& acc) {
 // maximum (NaN where 32 bits do not do), and each warp's part of it into
 // `slots` (by warp 0; null: not wanted).  Alike in every warp.
 template <typename S>
-QMM_DEVINL void row_stat(const WarpStat* stats, int warps, const S& c, float& mx, double& total, double* slots) {
+QMM_DEVINL void row_stat(const WarpStat* stats, int warps, const S& c, float& mx, double& total, double* slots,
+                         bool sum = true) {
     const int lane = threadIdx.x & 31;
     mx = -CUDART_INF_F;
     for (int i = lane; i < warps; i += 32) mx = fmaxf(mx, stats[i].top);
     mx = warp_max(mx);
+    total = 0.0;
+    if (!sum) return;
     const float e = ceilf(mx * c.c);
     const double back = c.against(e, mx);
-    total = 0.0;
     for (int i = lane; i < warps; i += 32) {
         const double x = stats[i].s * (double)ex2(stats[i].e - e) * back;
         if (slots && threadIdx.x < 32) slots[i] = x;

@@ -121,22 +121,34 @@ QMM_DEVINL void publish_maxima(cg::cluster_group& cl, SelectShared& sh, int g, i
 }
 
 // key32 of a bound that at least k of the n maxima reach (0: fewer than k are
-// there).  All threads of a CTA.
-constexpr int kWarpSearch = 256;
-QMM_DEVINL uint32_t kth_bound(SelectShared& sh, int n, int k) {
-    if (n > kWarpSearch) return kth_prefix(sh, n, k) << 16;
+// there).  Up to 256 maxima by each warp on its own, else by the CTA together.
+template <int PER>
+QMM_DEVINL uint32_t kth_of_warp(const float* maxima, int n, int k) {
     const int lane = threadIdx.x & 31;
-    uint32_t key[kWarpSearch / 32];
+    uint32_t key[PER], most = 0, least = 0xFFFFu;
 #pragma unroll
-    for (int i = 0; i < kWarpSearch / 32; ++i) key[i] = i * 32 + lane < n ? key32(sh.maxima[i * 32 + lane]) >> 16 : 0;
-    uint32_t b = 0;  // bit by bit: the largest prefix that k keys reach
-    for (uint32_t bit = 0x8000u; bit; bit >>= 1) {
+    for (int i = 0; i < PER; ++i) {
+        key[i] = i * 32 + lane < n ? key32(maxima[i * 32 + lane]) >> 16 : 0;
+        most = max(most, key[i]);
+        least = min(least, key[i]);
+    }
+    // bit by bit, below the bits that all keys share: the largest prefix that k keys reach
+    const uint32_t all = __reduce_max_sync(~0u, most), differ = all ^ __reduce_min_sync(~0u, least);
+    uint32_t bit = differ ? 0x80000000u >> __clz(differ) : 0, b = bit ? all & ~(2 * bit - 1) : all;
+    for (; bit; bit >>= 1) {
         int reach = 0;
 #pragma unroll
-        for (int i = 0; i < kWarpSearch / 32; ++i) reach += __popc(__ballot_sync(~0u, key[i] >= (b | bit)));
+        for (int i = 0; i < PER; ++i) reach += __popc(__ballot_sync(~0u, key[i] >= (b | bit)));
         if (reach >= k) b |= bit;
     }
     return b << 16;
+}
+
+QMM_DEVINL uint32_t kth_bound(SelectShared& sh, int n, int k) {
+    if (n < k) return 0;
+    if (n <= 128) return kth_of_warp<4>(sh.maxima, n, k);
+    if (n <= 256) return kth_of_warp<8>(sh.maxima, n, k);
+    return kth_prefix(sh, n, k) << 16;
 }
 
 // The tokens of K vectors to a lane that `take` wants to CTA 0's list, in any

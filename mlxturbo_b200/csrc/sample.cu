@@ -13,7 +13,6 @@
 // a bound on their error; only a row whose decision lies within that bound of
 // a border takes a second pass in 64 bits.
 
-#include <stdlib.h>
 #include "logits_select.cuh"
 
 namespace qmm {
@@ -71,7 +70,7 @@ __global__ void __launch_bounds__(kRowThreads, FILTERS ? 3 : 4) sample_kernel(co
     LaneSum acc;
     const LaneTop top =
         sum ? stream_slice<DT, true, FILTERS>(row, s, c, acc) : stream_slice<DT, false, true>(row, s, c, acc);
-    const WarpStat stat = warp_stat(top.first, acc);
+    const WarpStat stat = warp_stat(top.first, acc, sum);
     const bool select = k_on || p_on;  // a bound from maxima
     const int want = k_on ? k : kRowThreads;
     const int lanes = lanes_to_group(warps, want);
@@ -82,7 +81,7 @@ __global__ void __launch_bounds__(kRowThreads, FILTERS ? 3 : 4) sample_kernel(co
     cl.sync();
     float mx;
     double total;
-    row_stat(sh.stats, warps, c, mx, total, sh.slots[0]);
+    row_stat(sh.stats, warps, c, mx, total, sh.slots[0], sum);
     if (mx == -CUDART_INF_F) {  // nothing to draw from
         if (rank == 0 && threadIdx.x == 0) a.ids[r] = -1;
         return;

@@ -14,7 +14,7 @@
 namespace qmm {
 
 template <int DT, bool LSE>
-__global__ void __launch_bounds__(kRowThreads, 3) topk_kernel(const TopkArgs a) {
+__global__ void __launch_bounds__(kRowThreads, 4) topk_kernel(const TopkArgs a) {
     extern __shared__ uint4 memory[];
     SelectShared& sh = *reinterpret_cast<SelectShared*>(memory + kRing * kRowThreads);
     const Ring ring = reinterpret_cast<Ring>(memory);
@@ -33,7 +33,7 @@ __global__ void __launch_bounds__(kRowThreads, 3) topk_kernel(const TopkArgs a) 
     const LaneTop top = stream_slice<DT, LSE, true>(row, s, c, acc);
     const bool listed = a.k <= C * kRowThreads;
     const int lanes = lanes_to_group(warps, a.k);
-    const WarpStat stat = warp_stat(top.first, acc);
+    const WarpStat stat = warp_stat(top.first, acc, LSE);
     cl.barrier_wait();
     if (LSE) all_gather(cl, sh.stats, g, stat);
     if (listed) publish_maxima(cl, sh, g, lanes, top.first);
