@@ -28,11 +28,6 @@ namespace qmm {
 constexpr int kDistillThreads = kRowThreads + 32;
 
 struct DistillShared {
-    double logp[kMaxList];
-    float x[kMaxList];   // the student's logits of the list
-    int id[kMaxList];    // or -1
-    int slot[kMaxList];  // place in the table of distinct ids
-    int table[2 * kMaxList], owner[2 * kMaxList];
     WarpStat stats[kMaxRowWarps];
     double mass;   // sum p
     double cross;  // sum p (log p - l / tau)
@@ -41,8 +36,28 @@ struct DistillShared {
     int twice;     // an id is listed more than once
 };
 
+// The list, in dynamic shared memory.
+struct List {
+    double* logp;
+    float* x;   // the student's logits
+    int* id;    // or -1
+    int* slot;  // place in the table of distinct ids
+    int *table, *owner;
+    int size;  // of the table
+
+    static __host__ __device__ int table_size(int k) {
+        int n = 2;
+        while (n < 2 * k) n <<= 1;
+        return n;
+    }
+    static __host__ __device__ size_t bytes(int k) { return (size_t)k * 20 + (size_t)table_size(k) * 8; }
+    QMM_DEVINL List(void* memory, int k)
+        : logp(static_cast<double*>(memory)), x(reinterpret_cast<float*>(logp + k)), id(reinterpret_cast<int*>(x + k)),
+          slot(id + k), table(slot + k), owner(table + table_size(k)), size(table_size(k)) {}
+};
+
 // The ids of the list, by one warp; four loads of a lane at a time, as below.
-QMM_DEVINL void list_ids(const DistillArgs& a, DistillShared& sh, long long r) {
+QMM_DEVINL void list_ids(const DistillArgs& a, const List& li, long long r) {
     for (int j0 = threadIdx.x & 31; j0 < a.k; j0 += 128) {
         long long id[4];
 #pragma unroll
@@ -53,7 +68,7 @@ QMM_DEVINL void list_ids(const DistillArgs& a, DistillShared& sh, long long r) {
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-            if (j0 + 32 * i < a.k) sh.id[j0 + 32 * i] = id[i] >= 0 && id[i] < a.V ? (int)id[i] : -1;
+            if (j0 + 32 * i < a.k) li.id[j0 + 32 * i] = id[i] >= 0 && id[i] < a.V ? (int)id[i] : -1;
     }
     __syncwarp();
 }
@@ -61,7 +76,7 @@ QMM_DEVINL void list_ids(const DistillArgs& a, DistillShared& sh, long long r) {
 // The rest of it, by one warp: log p and the student's logits; entries of one
 // id share a slot whose owner is the first of them; the sums.
 template <int DT, bool TAIL>
-QMM_DEVINL void list_sums(const DistillArgs& a, DistillShared& sh, const Row<DT>& row, long long r) {
+QMM_DEVINL void list_sums(const DistillArgs& a, DistillShared& sh, const List& li, const Row<DT>& row, long long r) {
     const int lane = threadIdx.x & 31;
     double top = -CUDART_INF;
     float best = -CUDART_INF_F;
@@ -72,7 +87,7 @@ QMM_DEVINL void list_sums(const DistillArgs& a, DistillShared& sh, const Row<DT>
         for (int i = 0; i < 4; ++i) {
             const int j = min(j0 + 32 * i, a.k - 1);
             const long long at = r * a.k + j;
-            id[i] = sh.id[j];
+            id[i] = li.id[j];
             t[i] = a.tv_dtype == 2 ? __ldg(static_cast<const float*>(a.tv) + at)
                    : a.tv_dtype == 1 ? Half<true>::to_f32(__ldg(static_cast<const uint16_t*>(a.tv) + at))
                                      : Half<false>::to_f32(__ldg(static_cast<const uint16_t*>(a.tv) + at));
@@ -82,32 +97,30 @@ QMM_DEVINL void list_sums(const DistillArgs& a, DistillShared& sh, const Row<DT>
         for (int i = 0; i < 4; ++i) {
             if (j0 + 32 * i >= a.k) break;
             const double l = id[i] >= 0 ? (double)t[i] * a.inv_t : -CUDART_INF;
-            sh.x[j0 + 32 * i] = x[i];
-            sh.logp[j0 + 32 * i] = l;
+            li.x[j0 + 32 * i] = x[i];
+            li.logp[j0 + 32 * i] = l;
             top = fmax(top, l);  // a NaN shows in the sums
             if (id[i] >= 0) best = fmaxf(best, x[i]);
         }
     }
-    int size = 2;
-    while (size < 2 * a.k) size <<= 1;
-    for (int i = lane; i < size; i += 32) {
-        sh.table[i] = -1;
-        sh.owner[i] = kMaxList;
+    for (int i = lane; i < li.size; i += 32) {
+        li.table[i] = -1;
+        li.owner[i] = kMaxList;
     }
     __syncwarp();
     bool twice = false;
     for (int j = lane; j < a.k; j += 32) {
-        const int id = sh.id[j];
+        const int id = li.id[j];
         if (id < 0) continue;
-        int h = (int)((uint32_t)id * 2654435761u >> 16) & (size - 1);
+        int h = (int)((uint32_t)id * 2654435761u >> 16) & (li.size - 1);
         for (;;) {
-            const int was = atomicCAS(&sh.table[h], -1, id);
+            const int was = atomicCAS(&li.table[h], -1, id);
             twice |= was == id;
             if (was == -1 || was == id) break;
-            h = (h + 1) & (size - 1);
+            h = (h + 1) & (li.size - 1);
         }
-        sh.slot[j] = h;
-        atomicMin(&sh.owner[h], j);
+        li.slot[j] = h;
+        atomicMin(&li.owner[h], j);
     }
     __syncwarp();
 #pragma unroll
@@ -118,17 +131,17 @@ QMM_DEVINL void list_sums(const DistillArgs& a, DistillShared& sh, const Row<DT>
         norm = (double)a.tlse[r];
     } else if (top != -CUDART_INF) {  // else nothing is listed
         double sum = 0.0;
-        for (int j = lane; j < a.k; j += 32) sum += exp(sh.logp[j] - top);
+        for (int j = lane; j < a.k; j += 32) sum += exp(li.logp[j] - top);
         norm = top + log(warp_sum(sum));
     }
     double mass = 0.0, cross = 0.0, part = 0.0;
     for (int j = lane; j < a.k; j += 32) {
-        const double lp = sh.logp[j] - norm, p = exp(lp);
-        sh.logp[j] = lp;
+        const double lp = li.logp[j] - norm, p = exp(lp);
+        li.logp[j] = lp;
         mass += p;
-        if (sh.id[j] < 0) continue;
-        if (p != 0.0) cross += p * (lp - (double)sh.x[j] * a.inv_t);
-        if (TAIL && sh.owner[sh.slot[j]] == j) part += exp(((double)sh.x[j] - (double)best) * a.inv_t);
+        if (li.id[j] < 0) continue;
+        if (p != 0.0) cross += p * (lp - (double)li.x[j] * a.inv_t);
+        if (TAIL && li.owner[li.slot[j]] == j) part += exp(((double)li.x[j] - (double)best) * a.inv_t);
     }
     mass = warp_sum(mass);
     cross = warp_sum(cross);
@@ -175,10 +188,14 @@ QMM_DEVINL bool out_of_range(float ref) { return fabsf(ref) > kFastMax && fabsf(
 
 // TAIL: the teacher's log-sum-exp is given.  MODE kBackward needs no cluster.
 template <int DT, bool TAIL, int MODE>
-__global__ void __launch_bounds__(kDistillThreads, 4)
+__global__ void __launch_bounds__(kDistillThreads, MODE == kBackward ? 3 : 4)
     distill_kernel(const DistillArgs a, int C) {
     __shared__ DistillShared sh;
-    extern __shared__ uint32_t marks[];  // TAIL: a byte to a vector of this CTA
+    extern __shared__ uint4 memory[];
+    const StreamRing ring = reinterpret_cast<StreamRing>(memory);  // of the passes that write
+    const List li(memory + (MODE == kLoss ? 0 : kStream * kRowThreads), a.k);
+    // TAIL: a byte to a vector of this CTA
+    uint32_t* const marks = reinterpret_cast<uint32_t*>(li.owner + li.size);
     constexpr int N = Elem<DT>::kVec;
     cg::cluster_group cl = cg::this_cluster();
     if (MODE != kBackward) cl.barrier_arrive();
@@ -204,18 +221,18 @@ __global__ void __launch_bounds__(kDistillThreads, 4)
         mx = st.z;
         sum = st.w;
         if (!reader && weight != 0.0f) {
-            list_ids(a, sh, r);
-            list_sums<DT, TAIL>(a, sh, row, r);
+            list_ids(a, li, r);
+            list_sums<DT, TAIL>(a, sh, li, row, r);
         }
     } else {
-        if (!reader) list_ids(a, sh, r);
+        if (!reader) list_ids(a, li, r);
         if (TAIL) {
             for (int i = threadIdx.x; i < (per * kRowWarps + 3) / 4; i += kDistillThreads) marks[i] = 0;
             __syncthreads();
             if (!reader) {
                 for (int j = s.lane; j < a.k; j += 32) {
-                    const int at = sh.id[j] + row.shift, v = at / N - cta_begin;
-                    if (sh.id[j] >= 0 && v >= 0 && v < per * kRowWarps)
+                    const int at = li.id[j] + row.shift, v = at / N - cta_begin;
+                    if (li.id[j] >= 0 && v >= 0 && v < per * kRowWarps)
                         atomicOr(&marks[v / 4], 1u << (8 * (v & 3) + at % N));
                 }
             }
@@ -225,15 +242,18 @@ __global__ void __launch_bounds__(kDistillThreads, 4)
         WarpStat stat{};
         if (reader) {
             LaneSum acc;
-            const LaneTop top = stream_slice<DT, true, false>(row, s, c, acc, [&](int v, uint4& u) {
+            auto unlisted = [&](int v, uint4& u) {
                 if (TAIL) {
                     const uint32_t m = mark[v - cta_begin];
                     if (m) take_out<DT>(u, m);
                 }
-            });
+            };
+            LaneTop top;
+            if constexpr (MODE == kLoss) top = stream_slice<DT, true, false>(row, s, c, acc, unlisted);
+            else top = stream_slice<DT, true, false>(row, s, c, acc, unlisted, ring);
             stat = warp_stat(top.first, acc);
         } else {
-            list_sums<DT, TAIL>(a, sh, row, r);
+            list_sums<DT, TAIL>(a, sh, li, row, r);
         }
         cl.barrier_wait();
         if (reader) all_gather(cl, sh.stats, g, stat);
@@ -331,23 +351,23 @@ __global__ void __launch_bounds__(kDistillThreads, 4)
 #pragma unroll
                 for (int j = 0; j < N; ++j) x[j] = scaled * ex2(fmaf(x[j], c.c, -e));
                 store(v, x);
-            });
+            }, ring);
         }
     }
     if (weight == 0.0f) return;
     __syncthreads();  // the listed tokens' values after the others' formula has been written in their place
     const bool empty = !TAIL && sh.mass == 0.0;
     for (int j = threadIdx.x; j < a.k; j += kDistillThreads) {
-        const int id = sh.id[j];
-        if (id < 0 || sh.owner[sh.slot[j]] != j) continue;
+        const int id = li.id[j];
+        if (id < 0 || li.owner[li.slot[j]] != j) continue;
         const int v = (id + row.shift) / N;
         if (v < cta_begin || v >= cta_end) continue;
-        double p = exp(sh.logp[j]);
+        double p = exp(li.logp[j]);
         if (sh.twice) {
             for (int i = j + 1; i < a.k; ++i)
-                if (sh.id[i] == id) p += exp(sh.logp[i]);
+                if (li.id[i] == id) p += exp(li.logp[i]);
         }
-        const double q = empty ? 0.0 : exp(((double)sh.x[j] - (double)mx) * a.inv_t) / sum;
+        const double q = empty ? 0.0 : exp(((double)li.x[j] - (double)mx) * a.inv_t) / sum;
         store_elem<DT>(out, id, (float)(scale * (q - p)));
     }
 }
@@ -358,21 +378,23 @@ namespace qmm_host {
 
 template <int DT, bool TAIL, int MODE>
 static int distill_launch(const qmm::DistillArgs& a, long long rows, cudaStream_t st) {
-    const int C = row_cluster(rows, a.V, qmm::Elem<DT>::kBytes, 3 * 148);
+    const int C = row_cluster(rows, a.V, qmm::Elem<DT>::kBytes, (MODE == qmm::kBackward ? 3 : 4) * 148);
+    size_t smem = qmm::List::bytes(a.k);
+    if (MODE != qmm::kLoss) smem += qmm::kStream * qmm::kRowThreads * sizeof(uint4);
     if (MODE == qmm::kBackward)  // CTAs on their own
-        return launch_rows(qmm::distill_kernel<DT, TAIL, MODE>, qmm::kDistillThreads, rows * C, 1, 0, st, "distill launch",
-                           a, C);
-    size_t smem = 0;
+        return launch_rows(qmm::distill_kernel<DT, TAIL, MODE>, qmm::kDistillThreads, rows * C, 1, smem, st,
+                           "distill launch", a, C);
     if (TAIL) {
         const long long vecs = (a.V + 2LL * qmm::Elem<DT>::kVec - 2) / qmm::Elem<DT>::kVec;  // any start of a row
         const int warps = C * qmm::kRowWarps;
-        smem = (size_t)(((vecs + warps - 1) / warps) * qmm::kRowWarps + 3) / 4 * 4;
-        if (smem + sizeof(qmm::DistillShared) > 48 * 1024) {
+        smem += (size_t)(((vecs + warps - 1) / warps) * qmm::kRowWarps + 3) / 4 * 4;
+        if (smem > 200 * 1024) {
             set_error("distill: V=%d is too long for teacher_logsumexp", a.V);
             return QMM_EUNSUPPORTED;
         }
     }
-    return launch_rows(qmm::distill_kernel<DT, TAIL, MODE>, qmm::kDistillThreads, rows, C, smem, st, "distill launch", a, C);
+    return launch_rows(qmm::distill_kernel<DT, TAIL, MODE>, qmm::kDistillThreads, rows, C, smem, st, "distill launch", a,
+                       C);
 }
 
 template <int DT, bool TAIL>

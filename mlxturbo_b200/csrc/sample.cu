@@ -60,7 +60,7 @@ __global__ void __launch_bounds__(kRowThreads, FILTERS ? 3 : 4) sample_kernel(co
         k = 1;
     }
     const bool k_on = FILTERS && k >= 1 && k < a.V, p_on = FILTERS && p < 1.0 && !(k_on && k == 1);
-    const bool m_on = FILTERS && mp > 0.0 && !(k_on && k == 1);
+    const bool m_on = FILTERS && mp > 1e-300 && !(k_on && k == 1);  // no weight is below that
     if (mp > 1.0) mp = 1.0;
     const double inv_t = 1.0 / T, u = (double)a.u[r];
     const bool sum = !k_on && (p_on || !m_on);
@@ -310,7 +310,8 @@ namespace qmm_host {
 int row_cluster(long long rows, long long V, int elem_bytes, int ctas) {
     const long long vecs = (V * elem_bytes + 15) / 16, lanes = qmm::kRowThreads;
     int C = 1;
-    while (C < 8 && vecs > 2 * C * lanes && (vecs > 64 * C * lanes || rows * C < 148 || (rows * C < ctas && vecs > 8 * C * lanes)))
+    while (C < 8 && vecs > 2 * C * lanes &&
+           (vecs > 64 * C * lanes || rows * C * 2 <= 148 || (rows * C * 2 <= ctas && vecs > 8 * C * lanes)))
         C *= 2;
     // clusters of 16 find room on fewer SMs: for calls that fit at once
     if (C == 8 && rows * 16 <= 148 && vecs > 16 * lanes) C = 16;
@@ -322,7 +323,7 @@ static int sample_dt(const qmm::SampleArgs& a, long long rows, cudaStream_t st) 
     const bool filters = a.t_rows || a.k_rows || a.p_rows || a.m_rows || a.t == 0.0 || a.k || a.p < 1.0 || a.m > 0.0;
     if (filters)
         return launch_rows(qmm::sample_kernel<DT, true>, qmm::kRowThreads, rows,
-                           row_cluster(rows, a.V, qmm::Elem<DT>::kBytes, 4 * 148), qmm::kSelectSmem, st,
+                           row_cluster(rows, a.V, qmm::Elem<DT>::kBytes, 8 * 148), qmm::kSelectSmem, st,
                            "sample launch", a);
     return launch_rows(qmm::sample_kernel<DT, false>, qmm::kRowThreads, rows,
                        row_cluster(rows, a.V, qmm::Elem<DT>::kBytes, 4 * 148), qmm::kDrawSmem, st, "sample launch", a);
