@@ -215,28 +215,73 @@ QMM_DEVINL uint32_t append(cg::cluster_group& cl, SelectShared& sh, const Row<DT
     });
 }
 
-// The same over the whole slice.
+// The same over the whole slice.  A lane keeps up to four tokens until the end,
+// so that a warp reserves its places once (a round trip to CTA 0 is 1 us, and
+// hits come in most turns of the loop); where a lane meets more, vector by vector.
+template <int DT, typename F>
+QMM_DEVINL uint32_t append_slice(cg::cluster_group& cl, SelectShared& sh, const Row<DT>& row, const Slice& s,
+                                 F&& take) {
+    constexpr int N = Elem<DT>::kVec, kKeep = 4;
+    const int first = s.head >= 0 ? s.head : s.begin, last = s.tail >= 0 ? s.tail + 1 : s.end;
+    auto each = [&](auto&& f) {
+        for (int v0 = first; v0 < last; v0 += 128) {
+            uint4 u[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int v = v0 + 32 * i + s.lane;
+                u[i] = v < last ? row.load(v) : make_uint4(0, 0, 0, 0);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) f(v0 + 32 * i + s.lane, u[i]);
+        }
+    };
+    unsigned long long key[kKeep] = {};
+    uint32_t mine = 0;
+    each([&](int v, const uint4& u) {
+        if (v >= last) return;
+        float x[N];
+        decode<DT>(u, x);
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            const int id = row.first(v) + j;
+            if (id < 0 || id >= row.V || !take(id, x[j])) continue;
+#pragma unroll
+            for (int i = 0; i < kKeep; ++i)
+                if (mine == (uint32_t)i) key[i] = row_key(x[j], id);
+            ++mine;
+        }
+    });
+    uint32_t found = 0;
+    if (__any_sync(~0u, mine > kKeep)) {
+        each([&](int v, const uint4& u) { found += append_if<DT>(cl, sh, row, v < last ? v : -1, u, take); });
+        return found;
+    }
+    uint32_t incl = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t y = __shfl_up_sync(~0u, incl, o);
+        if (s.lane >= o) incl += y;
+    }
+    found = __shfl_sync(~0u, incl, 31);
+    if (!found) return 0;
+    uint32_t at = 0;
+    if (s.lane == 0) at = atomicAdd(cl.map_shared_rank(&sh.n_cand, 0), found);
+    at = __shfl_sync(~0u, at, 0) + incl - mine;
+    unsigned long long* list = cl.map_shared_rank(sh.cand, 0);
+#pragma unroll
+    for (int i = 0; i < kKeep; ++i)
+        if ((uint32_t)i < mine && at + i < kCand) list[at + i] = key[i];
+    return found;
+}
+
+// Those with key32 in [lo, hi) and key >= floor.
 template <int DT>
 QMM_DEVINL uint32_t append_slice(cg::cluster_group& cl, SelectShared& sh, const Row<DT>& row, const Slice& s,
                                  uint32_t lo, uint32_t hi, unsigned long long floor) {
-    const int first = s.head >= 0 ? s.head : s.begin, last = s.tail >= 0 ? s.tail + 1 : s.end;
-    uint32_t found = 0;
-    for (int v0 = first; v0 < last; v0 += 128) {
-        uint4 u[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int v = v0 + 32 * i + s.lane;
-            u[i] = v < last ? row.load(v) : make_uint4(0, 0, 0, 0);
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int v = v0 + 32 * i + s.lane;
-            const int at[1] = {v < last ? v : -1};
-            const uint4 one[1] = {u[i]};
-            found += append<DT, 1>(cl, sh, row, at, one, lo, hi, floor);
-        }
-    }
-    return found;
+    return append_slice<DT>(cl, sh, row, s, [&](int id, float x) {
+        const uint32_t k = key32(x);
+        return k >= lo && k < hi && row_key(x, id) >= floor;
+    });
 }
 
 // Candidates: every token with key32 >= bound.  A lane reads its two vectors
@@ -678,45 +723,93 @@ QMM_DEVINL bool border_by_bins(cg::cluster_group& cl, SelectShared& sh, const Ro
     cl.sync();  // bins and sums are read; the list takes their place
     if (s.lane == 0) *cl.map_shared_rank(slots + g, 0) = top + (double)kept * unit;
     if (rank == 0 && t < warps) sh.bin_sum[t] = 0;
-    const int first = s.head >= 0 ? s.head : s.begin, last = s.tail >= 0 ? s.tail + 1 : s.end;
-    for (int v0 = first; v0 < last; v0 += 128) {
-        uint4 u[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int v = v0 + 32 * i + s.lane;
-            u[i] = v < last ? row.load(v) : make_uint4(0, 0, 0, 0);
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int v = v0 + 32 * i + s.lane;
-            append_if<DT>(cl, sh, row, v < last ? v : -1, u[i],
-                          [&](int, float x) { return x < edge && bin_of(x) == bin; });
-        }
-    }
+    append_slice<DT>(cl, sh, row, s, [&](int, float x) { return x < edge && bin_of(x) == bin; });
     cl.sync();
     if (rank == 0) {
-        const int n = (int)sh.n_cand;
-        const bool ok = n > 0 && n <= kCand;
+        int n = (int)sh.n_cand;
+        bool ok = n > 0 && n <= kCand;
         if (ok) {
-            sort_candidates(sh.cand, n);
-            for (int i = t; i < n; i += kRowThreads) sh.w[i] = weight(key32_value((uint32_t)(sh.cand[i] >> 32)));
-            __syncthreads();
-            // the kept ones of the list go to their warps
             const int per = (row.nv + warps - 1) / warps;
-            scan_weights(sh, n);
-            int b = 0, e = n - 1;  // the token at which the target is reached
-            while (b < e) {
-                const int m = (b + e) / 2;
-                if (above + sh.w[m] >= target) e = m;
-                else b = m + 1;
+            double start = above;
+            // a token that is kept goes to its warp's sum, in units
+            auto keep = [&](unsigned long long key) {
+                const double w = weight(key32_value((uint32_t)(key >> 32)));
+                atomicAdd(&sh.bin_sum[(key_id(key) + row.shift) / N / per], (unsigned long long)(w * per_unit));
+            };
+            if (n > kRowThreads) {
+                // the bin once more in 256: sorting 1000 tokens takes 10 us, this 2
+                uint32_t* const fine = reinterpret_cast<uint32_t*>(sh.w);  // two limbs
+                unsigned long long* const part = reinterpret_cast<unsigned long long*>(fine + 512);
+                constexpr uint32_t kPart = kCand - 256;  // what is left of sh.w
+                auto fine_of = [&](unsigned long long key) {
+                    const float d = (edge - key32_value((uint32_t)(key >> 32))) * scale - (float)bin;
+                    return min(max((int)(d * 256.0f), 0), 255);
+                };
+                fine[t] = fine[256 + t] = 0;
+                if (t == 0) sh.sel_above = 0;
+                __syncthreads();
+                for (int i = t; i < n; i += kRowThreads) {
+                    const int f = fine_of(sh.cand[i]);
+                    const double k = fma(weight(key32_value((uint32_t)(sh.cand[i] >> 32))), per_unit, kBinMagic);
+                    const uint32_t lo = (uint32_t)__double2loint(k), hi = (uint32_t)__double2hiint(k);
+                    atomicAdd(&fine[f], lo & 0xFFFFFu);
+                    atomicAdd(&fine[256 + f], __funnelshift_r(lo, hi, 20) & 0x1FFFFFu);
+                }
+                __syncthreads();
+                const unsigned long long mine = ((unsigned long long)fine[256 + t] << 20) + fine[t];
+                unsigned long long sum = mine;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const unsigned long long y = __shfl_up_sync(~0u, sum, o);
+                    if (s.lane >= o) sum += y;
+                }
+                if (s.lane == 31) parts[warp] = sum;
+                if (t == 0) {
+                    sh.sel_bin = 255;
+                    sh.bin_above = 0;
+                }
+                __syncthreads();
+                for (int i = 0; i < warp; ++i) sum += parts[i];
+                // (the last one in any case: rounding may leave the target past the end)
+                const bool here = above + (double)(sum - mine) * unit < target &&
+                                  (above + (double)sum * unit >= target || t == 255);
+                if (here) {
+                    sh.sel_bin = (uint32_t)t;
+                    sh.bin_above = sum - mine;
+                }
+                __syncthreads();
+                const int f = (int)sh.sel_bin;
+                start = above + (double)sh.bin_above * unit;
+                for (int i = t; i < n; i += kRowThreads) {
+                    const int at = fine_of(sh.cand[i]);
+                    if (at < f) keep(sh.cand[i]);
+                    if (at != f) continue;
+                    const uint32_t to = atomicAdd(&sh.sel_above, 1u);
+                    if (to < kPart) part[to] = sh.cand[i];
+                }
+                __syncthreads();
+                ok = sh.sel_above <= kPart;  // else one value's tokens nearly all
+                n = ok ? (int)sh.sel_above : 0;
+                for (int i = t; i < n; i += kRowThreads) sh.cand[i] = part[i];
+                __syncthreads();
             }
-            for (int i = t; i <= b; i += kRowThreads) {
-                const double w = weight(key32_value((uint32_t)(sh.cand[i] >> 32)));
-                atomicAdd(&sh.bin_sum[(key_id(sh.cand[i]) + row.shift) / N / per], (unsigned long long)(w * per_unit));
+            if (ok) {
+                sort_candidates(sh.cand, n);
+                for (int i = t; i < n; i += kRowThreads)
+                    sh.w[i] = weight(key32_value((uint32_t)(sh.cand[i] >> 32)));
+                __syncthreads();
+                scan_weights(sh, n);
+                int b = 0, e = n - 1;  // the token at which the target is reached
+                while (b < e) {
+                    const int m = (b + e) / 2;
+                    if (start + sh.w[m] >= target) e = m;
+                    else b = m + 1;
+                }
+                for (int i = t; i <= b; i += kRowThreads) keep(sh.cand[i]);
+                __syncthreads();
+                if (t < warps) slots[t] += (double)sh.bin_sum[t] * unit;
+                if (t < C) *cl.map_shared_rank(&sh.best, t) = sh.cand[b];
             }
-            __syncthreads();
-            if (t < warps) slots[t] += (double)sh.bin_sum[t] * unit;
-            if (t < C) *cl.map_shared_rank(&sh.best, t) = sh.cand[b];
         }
         if (t < C) *cl.map_shared_rank(&sh.verdict, t) = ok;
     }

@@ -21,6 +21,9 @@ namespace qmm {
 // the border, but more kept tokens than it draws from itself; not enough of them.
 enum { kDone, kNeedSum, kBorder, kGeneral };
 constexpr int kDrawHere = 2 * kRowThreads;
+// What a row with top-p alone lists first: enough where the model is sure of
+// itself, and about 180 tokens, which a CTA sorts in one turn.
+constexpr int kNucleus = 128;
 
 // How many of the first n running sums stand before `limit`: the tokens whose
 // mass before them (the sum of the one above) is below it.  The first always is.
@@ -72,7 +75,7 @@ __global__ void __launch_bounds__(kRowThreads, FILTERS ? 3 : 4) sample_kernel(co
         sum ? stream_slice<DT, true, FILTERS>(row, s, c, acc) : stream_slice<DT, false, true>(row, s, c, acc);
     const WarpStat stat = warp_stat(top.first, acc, sum);
     const bool select = k_on || p_on;  // a bound from maxima
-    const int want = k_on ? k : kRowThreads;
+    const int want = k_on ? k : kNucleus;
     const int lanes = lanes_to_group(warps, want);
     const bool listed = select ? 2 * want <= C * kRowThreads || want <= kRowThreads : m_on;
     cl.barrier_wait();
