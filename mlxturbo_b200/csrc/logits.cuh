@@ -416,8 +416,7 @@ QMM_DEVINL void for_vectors_rare(const Row<DT>& row, const Slice& s, F&& f) {
 
 // The same for passes whose arithmetic in 64 bits needs the registers: vectors
 // one at a time, the next three on their way into shared memory (cp.async, each
-// thread's own slots, so nothing has to be synchronised).  With one load ahead
-// instead, a pass of 30 vectors to a lane took 30 us under a busy memory.
+// thread's own slots, so nothing has to be synchronised).
 constexpr int kRing = 4;
 using Ring = uint4 (*)[kRowThreads];  // [kRing][kRowThreads] in shared memory
 

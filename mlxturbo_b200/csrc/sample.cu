@@ -12,6 +12,15 @@
 // needed (top-p without top-k, no filter at all) a 32-bit pass gives them with
 // a bound on their error; only a row whose decision lies within that bound of
 // a border takes a second pass in 64 bits.
+//
+// One reading of memory bounds it from below, and a chain of steps beside that:
+// a row's cluster reads (2 us of the 12 of a single row of 248320), exchanges
+// maxima, collects the candidates, and CTA 0 sorts and draws.  With top-k no
+// exponential is taken but of the candidates.  Measured on a B200, V 248320: one
+// row, top-k 20 and top-p 0.95, 12 us; 65 rows of 50021 with settings of their
+// own 16 us; 128 rows with top-p 0.95, half of them open, 160 us (floor 9.7: the
+// open rows' pass in 64 bits and the steps after it); 512 rows of fp32 without a
+// filter 180 us (floor 78: 129 where the model is sure, the rest second passes).
 
 #include "logits_select.cuh"
 
