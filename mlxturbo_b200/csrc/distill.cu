@@ -384,7 +384,8 @@ namespace qmm_host {
 
 template <int DT, bool TAIL, int MODE>
 static int distill_launch(const qmm::DistillArgs& a, long long rows, cudaStream_t st) {
-    const int C = row_cluster(rows, a.V, qmm::Elem<DT>::kBytes, (MODE == qmm::kBackward ? 3 : 4) * 148);
+    const int C = row_cluster(rows, a.V, qmm::Elem<DT>::kBytes, (MODE == qmm::kBackward ? 3 : 4) * 148,
+                              MODE == qmm::kLoss ? 128 : 64);
     size_t smem = qmm::List::bytes(a.k);
     if (MODE != qmm::kLoss) smem += qmm::kStream * qmm::kRowThreads * sizeof(uint4);
     if (MODE == qmm::kBackward)  // CTAs on their own

@@ -732,31 +732,42 @@ QMM_DEVINL Found find_in_slice(const Row<DT>& row, const Slice& s, double base, 
 
 namespace qmm_host {
 
-// CTAs to a row: so many that a lane holds at most 64 vectors; more, down to 8
-// vectors to a lane, while the call has no more than `ctas` of them (what runs
+// CTAs to a row: so many that a lane holds at most `most` vectors; more, down to
+// 8 vectors to a lane, while the call has no more than `ctas` of them (what runs
 // at once, or several times that where a row's work is uneven), and down to 2
 // while there is one to an SM at most.
-int row_cluster(long long rows, long long V, int elem_bytes, int ctas);
+int row_cluster(long long rows, long long V, int elem_bytes, int ctas, int most = 64);
 
-// Launch `kernel` over rows * C CTAs in clusters of C.
-template <typename... P, typename... A>
-int launch_rows(void (*kernel)(P...), int threads, long long rows, int C, size_t smem, cudaStream_t st, const char* what,
-                A... args) {
+bool pdl_enabled();                                                   // tma.cuh
+int ensure_smem_limit(const void* func, int bytes, const char* what);  // tma.cuh
+
+// Launch `kernel` over rows * C CTAs in clusters of C.  AFTER: it may start while
+// the stream's previous kernel runs, and waits for it itself.
+template <bool AFTER = false, typename... P, typename... A>
+int launch_rows(void (*kernel)(P...), int threads, long long rows, int C, size_t smem, cudaStream_t st,
+                const char* what, A... args) {
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)(rows * C));
     cfg.blockDim = dim3((unsigned)threads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
-    cudaLaunchAttribute at{};
-    at.id = cudaLaunchAttributeClusterDimension;
-    at.val.clusterDim.x = (unsigned)C;
-    at.val.clusterDim.y = at.val.clusterDim.z = 1;
-    cfg.attrs = &at;
+    cudaLaunchAttribute at[2]{};
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = (unsigned)C;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    cfg.attrs = at;
     cfg.numAttrs = 1;
+    if (AFTER && pdl_enabled()) {
+        at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        at[1].val.programmaticStreamSerializationAllowed = 1;
+        cfg.numAttrs = 2;
+    }
     cudaError_t e = cudaSuccess;
     if (C > 8) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-    if (e == cudaSuccess && smem > 16 * 1024)
-        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e == cudaSuccess && smem > 16 * 1024) {  // beside the kernel's static memory
+        const int rc = ensure_smem_limit(reinterpret_cast<const void*>(kernel), (int)smem, what);
+        if (rc) return rc;
+    }
     if (e == cudaSuccess) e = cudaLaunchKernelEx(&cfg, kernel, args...);
     return cuda_status(e, what);
 }

@@ -319,11 +319,11 @@ __global__ void __launch_bounds__(kRowThreads, FILTERS ? 3 : 4) sample_kernel(co
 
 namespace qmm_host {
 
-int row_cluster(long long rows, long long V, int elem_bytes, int ctas) {
+int row_cluster(long long rows, long long V, int elem_bytes, int ctas, int most) {
     const long long vecs = (V * elem_bytes + 15) / 16, lanes = qmm::kRowThreads;
     int C = 1;
     while (C < 8 && vecs > 2 * C * lanes &&
-           (vecs > 64 * C * lanes || rows * C * 2 <= 148 || (rows * C * 2 <= ctas && vecs > 8 * C * lanes)))
+           (vecs > most * C * lanes || rows * C * 2 <= 148 || (rows * C * 2 <= ctas && vecs > 8 * C * lanes)))
         C *= 2;
     // clusters of 16 find room on fewer SMs: for calls that fit at once
     if (C == 8 && rows * 16 <= 148 && vecs > 16 * lanes) C = 16;

@@ -19,6 +19,7 @@
 // 139 us (44 and 95; a sequence whose draw is made again takes 90 of these).
 
 #include "logits.cuh"
+#include "tma.cuh"
 
 namespace qmm {
 
@@ -40,6 +41,7 @@ __global__ void __launch_bounds__(kRowThreads, 4) spec_stats_kernel(const SpecAr
     __shared__ int args[kMaxRowWarps];
     cg::cluster_group cl = cg::this_cluster();
     cl.barrier_arrive();
+    pdl_launch_dependents();  // the second kernel's start beside this one's end
     const int C = (int)cl.num_blocks(), rank = (int)cl.block_rank(), warps = C * kRowWarps;
     const int g = rank * kRowWarps + (threadIdx.x >> 5);
     const long long at = blockIdx.x / C;
@@ -260,6 +262,7 @@ __global__ void __launch_bounds__(kRowThreads, 2) spec_decide_kernel(const SpecA
     constexpr int N = Elem<DT>::kVec;
     cg::cluster_group cl = cg::this_cluster();
     cl.sync();  // every CTA is there before its memory is written
+    pdl_wait();  // the sums; nothing of global memory is read before
     const int C = (int)cl.num_blocks(), rank = (int)cl.block_rank(), warps = C * kRowWarps;
     const int g = rank * kRowWarps + (threadIdx.x >> 5), lane = threadIdx.x & 31;
     const long long b = blockIdx.x / C;
@@ -403,10 +406,11 @@ template <int DT>
 static int speculative_dt(const qmm::SpecArgs& a, cudaStream_t st) {
     const long long rows = (long long)a.B * (2 * a.n + 1);
     const int bytes = qmm::Elem<DT>::kBytes;
-    const int rc = launch_rows(qmm::spec_stats_kernel<DT>, qmm::kRowThreads, rows, row_cluster(rows, a.V, bytes, 4 * 148), 0, st,
-                               "speculative sums launch", a);
+    const int rc = launch_rows(qmm::spec_stats_kernel<DT>, qmm::kRowThreads, rows,
+                               row_cluster(rows, a.V, bytes, 4 * 148, 128), 0, st, "speculative sums launch", a);
     if (rc) return rc;
-    return launch_rows(qmm::spec_decide_kernel<DT>, qmm::kRowThreads, a.B, row_cluster(a.B, a.V, bytes, 4 * 148), 0, st, "speculative launch", a);
+    return launch_rows<true>(qmm::spec_decide_kernel<DT>, qmm::kRowThreads, a.B, row_cluster(a.B, a.V, bytes, 4 * 148),
+                             0, st, "speculative launch", a);
 }
 
 int launch_speculative(const qmm::SpecArgs& a, int dtype, cudaStream_t st) {

@@ -105,7 +105,11 @@ namespace qmm_host {
 
 template <int DT>
 static int topk_dt(const qmm::TopkArgs& a, long long rows, cudaStream_t st) {
-    const int C = row_cluster(rows, a.V, qmm::Elem<DT>::kBytes, 4 * 148);
+    // One CTA holds a long row's maxima as well as two (2011 rows of 248320, k 64: 248 us against 274), if they
+    // are twice k.
+    int C = row_cluster(rows, a.V, qmm::Elem<DT>::kBytes, 4 * 148, 128);
+    while (C < 8 && C * qmm::kRowThreads < 2 * a.k && (long long)a.V * qmm::Elem<DT>::kBytes > 32LL * C * qmm::kRowThreads)
+        C *= 2;
     if (a.lse) return launch_rows(qmm::topk_kernel<DT, true>, qmm::kRowThreads, rows, C, qmm::kSelectSmem, st, "topk launch", a);
     return launch_rows(qmm::topk_kernel<DT, false>, qmm::kRowThreads, rows, C, qmm::kSelectSmem, st, "topk launch", a);
 }
