@@ -333,10 +333,15 @@ int row_cluster(long long rows, long long V, int elem_bytes, int ctas, int most)
 template <int DT>
 static int sample_dt(const qmm::SampleArgs& a, long long rows, cudaStream_t st) {
     const bool filters = a.t_rows || a.k_rows || a.p_rows || a.m_rows || a.t == 0.0 || a.k || a.p < 1.0 || a.m > 0.0;
-    if (filters)
-        return launch_rows(qmm::sample_kernel<DT, true>, qmm::kRowThreads, rows,
-                           row_cluster(rows, a.V, qmm::Elem<DT>::kBytes, 8 * 148), qmm::kSelectSmem, st,
+    if (filters) {
+        int C = row_cluster(rows, a.V, qmm::Elem<DT>::kBytes, 8 * 148);
+        // up to k = 1024, maxima enough for a list of candidates: beyond that the border is searched, pass by pass
+        while (C < 8 && a.k <= 1024 && C * qmm::kRowThreads < 2 * a.k &&
+               (long long)a.V * qmm::Elem<DT>::kBytes > 32LL * C * qmm::kRowThreads)
+            C *= 2;
+        return launch_rows(qmm::sample_kernel<DT, true>, qmm::kRowThreads, rows, C, qmm::kSelectSmem, st,
                            "sample launch", a);
+    }
     return launch_rows(qmm::sample_kernel<DT, false>, qmm::kRowThreads, rows,
                        row_cluster(rows, a.V, qmm::Elem<DT>::kBytes, 4 * 148), qmm::kDrawSmem, st, "sample launch", a);
 }
