@@ -534,7 +534,7 @@ QMM_DEVINL void all_gather(cg::cluster_group& cl, T* slots, int g, const T& valu
 }
 
 // What a warp knows of a row after its pass: the maximum, and the sum of
-// weights against 2^e.
+// weights against 2^e (without sums, e is the lowest of its lanes' maxima).
 struct alignas(16) WarpStat {
     double s;
     float top, e;
@@ -543,9 +543,11 @@ struct alignas(16) WarpStat {
 QMM_DEVINL WarpStat warp_stat(float top, const LaneSum& acc, bool sum = true) {
     WarpStat w;
     w.top = warp_max(top);
-    w.e = 0.0f;
     w.s = 0.0;
-    if (!sum) return w;
+    if (!sum) {
+        w.e = -warp_max(top == -CUDART_INF_F ? top : -top);
+        return w;
+    }
     w.e = warp_max(acc.e);
     w.s = warp_sum(acc.s * (double)ex2(acc.e - w.e));
     return w;

@@ -86,6 +86,8 @@ __global__ void __launch_bounds__(kRowThreads, FILTERS ? 3 : 4) sample_kernel(co
     const bool select = k_on || p_on;  // a bound from maxima
     const int want = k_on ? k : kNucleus;
     const int lanes = lanes_to_group(warps, want);
+    // Beyond, the bins: 16 rows of 248320, k 1000, on 16 CTAs each, listed 60 us, by bins 123; 300 rows of 50000
+    // on 8 CTAs for the list's sake 323, by bins on 2 CTAs 199.
     const bool listed = select ? 2 * want <= C * kRowThreads || want <= kRowThreads : m_on;
     cl.barrier_wait();
     all_gather(cl, sh.stats, g, stat);
@@ -255,11 +257,25 @@ __global__ void __launch_bounds__(kRowThreads, FILTERS ? 3 : 4) sample_kernel(co
         if (sh.verdict == kDone) return;
     }
 
-    // the general way: borders by search, masses and place in 64 bits
+    // the general way: borders by bins or search, masses and place in 64 bits
     const int per = (row.nv + warps - 1) / warps;
-    if (p_on && !k_on && !bordered && per * Elem<DT>::kVec <= kBinTokens) {
-        unsigned long long from;
-        if (border_by_bins<DT>(cl, sh, row, s, g, warps, ring, weight, p, total, bound, sh.slots[0], from)) {
+    const unsigned long long bottom = (unsigned long long)(kKeyNegInf + 1) << 32;
+    unsigned long long from = bottom;
+    if (k_on && !bordered) {
+        float low = CUDART_INF_F;
+        for (int i = s.lane; i < warps; i += 32) low = fminf(low, sh.stats[i].e);
+        low = -warp_max(-low);
+        if (!kth_by_bins<DT>(cl, sh, row, s, mx, low, k, from))
+            from = border_key<DT, false>(cl, sh, row, s, g, warps, ring, weight, bottom, (double)k);
+    }
+    if (p_on && !bordered && per * Elem<DT>::kVec <= kBinTokens) {
+        // without top-k down to where what is left, V tokens at most, is half of what top-p leaves out
+        const float edge = k_on ? mx : key32_value(bound);
+        const double deep = k_on ? ((double)mx - (double)key32_value((uint32_t)(from >> 32))) * inv_t * 1.001
+                                 : log(2.0 * row.V * weight(edge) / ((1.0 - p) * total));
+        unsigned long long found;
+        if (border_by_bins<DT>(cl, sh, row, s, g, warps, ring, weight, p, edge, deep, from, sh.slots[0], found)) {
+            from = found;
             if (from >= border) {  // min-p keeps them all: CTA 0 has each warp's mass
                 if (rank != 0) return;
                 const double target = u * slots_sum(sh.slots[0], warps);
@@ -283,8 +299,6 @@ __global__ void __launch_bounds__(kRowThreads, FILTERS ? 3 : 4) sample_kernel(co
         }
     }
     if (select && !bordered) {
-        unsigned long long from = (unsigned long long)(kKeyNegInf + 1) << 32;
-        if (k_on) from = border_key<DT, false>(cl, sh, row, s, g, warps, ring, weight, from, (double)k);
         if (p_on) from = border_key<DT, true>(cl, sh, row, s, g, warps, ring, weight, from, p);
         if (from > border) border = from;
     }
@@ -335,10 +349,9 @@ static int sample_dt(const qmm::SampleArgs& a, long long rows, cudaStream_t st) 
     const bool filters = a.t_rows || a.k_rows || a.p_rows || a.m_rows || a.t == 0.0 || a.k || a.p < 1.0 || a.m > 0.0;
     if (filters) {
         int C = row_cluster(rows, a.V, qmm::Elem<DT>::kBytes, 8 * 148);
-        // up to k = 1024, maxima enough for a list of candidates: beyond that the border is searched, pass by pass
-        while (C < 8 && a.k <= 1024 && C * qmm::kRowThreads < 2 * a.k &&
-               (long long)a.V * qmm::Elem<DT>::kBytes > 32LL * C * qmm::kRowThreads)
-            C *= 2;
+        // a row that may need top-p's bins: no more tokens to a warp than they take
+        const bool bins = (a.p_rows || a.p < 1.0) && (a.k_rows || a.k == 0 || a.k > qmm::kRowThreads);
+        while (bins && C < 8 && a.V > C * qmm::kRowWarps * (qmm::kBinTokens - 32)) C *= 2;
         return launch_rows(qmm::sample_kernel<DT, true>, qmm::kRowThreads, rows, C, qmm::kSelectSmem, st,
                            "sample launch", a);
     }

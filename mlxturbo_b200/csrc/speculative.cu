@@ -15,7 +15,7 @@
 //
 // The first launch is bound by memory and the exponential unit (both near 65%),
 // the second by its chain: tests, a pass over two rows in L2, the exchange, the
-// place.  B200, V 248320: one sequence of 4 drafted tokens 27 us, 48 of up to 3
+// place.  B200, V 248320: one sequence of 4 drafted tokens 24 us, 48 of up to 3
 // 139 us (44 and 95; a sequence whose draw is made again takes 90 of these).
 
 #include "logits.cuh"

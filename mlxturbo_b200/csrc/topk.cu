@@ -10,9 +10,9 @@
 // border key and collect above it.
 //
 // Bound by memory and, with the log-sum-exp, by the exponential unit (eight of
-// them to 16 bytes: 111 of 268 us); what keeps it from its floor is the tail of
+// them to 16 bytes: 111 of 245 us); what keeps it from its floor is the tail of
 // a row, 10 us in which its CTAs read nothing.  B200, V 248320: 2011 rows, k 64,
-// with log-sum-exp 268 us (floor 153); 5 rows, k 20, 10 us.
+// with log-sum-exp 245 us (floor 153); 5 rows, k 20, 10 us.
 
 #include "logits_select.cuh"
 

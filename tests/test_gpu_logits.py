@@ -548,19 +548,25 @@ def test_open_rows_of_a_batch(ops, rows, dtype):
     x[::3] -= 0.0
     x[1::4] = (x[1::4] * 2).round() / 2  # few distinct values: hundreds of equal tokens
     u = uniform(91, rows)
-    for T, p in ((1.0, 0.95), (1.7, 0.8), (0.8, 0.999), (1.0, 1.0)):
-        got = ops.sample(x, u, temperature=T, top_p=p)
+    for T, p, k in ((1.0, 0.95, 0), (1.7, 0.8, 0), (0.8, 0.999, 0), (1.0, 1.0, 0), (1.0, 0.9, 300), (2.0, 0.97, 2000),
+                    (1.3, 1.0, 5000), (2.0, 0.5, V // 3)):
+        got = ops.sample(x, u, temperature=T, top_p=p, top_k=k)
+        if k:  # a number a row goes to the same tokens
+            ks = torch.full((rows,), k, device="cuda")
+            assert torch.equal(got, ops.sample(x, u, temperature=T, top_p=p, top_k=ks))
         l = x.double()
         w = torch.exp((l - l.amax(-1, keepdim=True)) / T)
-        if p < 1:
+        if p < 1 or k:
             order = l.sort(dim=-1, descending=True, stable=True).indices
             ws = w.gather(-1, order)
+            if k:
+                ws[:, k:] = 0.0
             cum = ws.cumsum(-1)
-            keep = torch.zeros_like(w, dtype=torch.bool).scatter_(-1, order, cum - ws < p * cum[:, -1:])
+            keep = torch.zeros_like(w, dtype=torch.bool).scatter_(-1, order, (ws > 0) & (cum - ws < p * cum[:, -1:]))
             w = torch.where(keep, w, 0.0)
         cum = w.cumsum(-1)
         want = (cum > u.double()[:, None] * cum[:, -1:]).to(torch.int8).argmax(-1)
-        assert torch.equal(got, want), (T, p)
+        assert torch.equal(got, want), (T, p, k)
 
 
 def test_second_derivative_is_refused(ops):
