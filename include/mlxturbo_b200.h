@@ -470,7 +470,8 @@ QMM_API int qmm_copy_kernel(void* dst, const void* src, size_t bytes, void* stre
  * any start that is a multiple of an element, rows `row_stride` elements apart,
  * at most 2^30 logits a row and 2^26 rows).  The order of a row's tokens is
  * (logit descending, id ascending), -0 equals +0, and but for the distillation
- * a NaN counts as -infinity.
+ * a NaN counts as -infinity.  A temperature given as a number lies in
+ * [1e-6, 1e6], or is 0 where an entry says so.
  */
 
 /*
@@ -482,8 +483,9 @@ QMM_API int qmm_copy_kernel(void* dst, const void* src, size_t bytes, void* stre
  * always; 1: all); and those with w_i >= min_p (0: all).  ids[r] is the first
  * id, in the order of ids, at which the kept weights add up to more than u
  * times their sum.  Temperature 0: the lowest id of the largest logit.  A
- * logit of -infinity is never drawn; a row of nothing else gives -1.  The ids
- * are those of 64-bit arithmetic, the same in every call.
+ * logit of -infinity is never drawn, nor one that weighs less than 2^-1000; a
+ * row of nothing but -infinity gives -1.  The ids are those of 64-bit
+ * arithmetic, the same in every call.
  * Each setting is one number, or (pointer not null) one a row; a row's
  * temperature <= 0 or NaN is 0, top_k <= 0 all, top_p >= 1 or NaN all and <= 0
  * the first token, min_p <= 0 or NaN all and >= 1 the largest.
@@ -531,6 +533,8 @@ QMM_API int qmm_speculative_sample(const void* logits, int64_t seq_stride, int64
  * listed values over `temperature`, or with teacher_logsumexp [rows] (of the
  * teacher's row over the same temperature) exp(value / temperature -
  * logsumexp), the rest of 1 being the class of all tokens not listed.
+ * (teacher_logsumexp goes with rows of up to 4 million logits at least;
+ * QMM_EUNSUPPORTED where their marks pass what shared memory holds.)
  * loss [rows] = KL(p || softmax(logits / temperature)).  A row with nothing
  * listed, or whose logsumexp is -infinity, has loss 0 and gradient 0.
  * Gradients are with respect to the logits, in their dtype, times row_weight /

@@ -101,6 +101,13 @@ def test_distill_arguments(which):
         refused(distill(which, **b), _lib.QMM_EUNSUPPORTED, b"distill")
 
 
+def test_rows_too_long_for_the_marks_of_a_list():
+    """teacher_logsumexp needs a byte of shared memory to 16 bytes of a CTA's part of a row."""
+    V = 1 << 24
+    rc = _lib.load().qmm_distill_loss(P, V, 2, V, _lib.QMM_F32, P, 0, P, 8, P, 5, 1.0, P, None, None)
+    refused(rc, _lib.QMM_EUNSUPPORTED, b"too long")
+
+
 def test_all_cpu_arguments_are_refused():
     from mlxturbo_b200 import ops
 
