@@ -23,6 +23,7 @@
 // filter 180 us (floor 78: 129 where the model is sure, the rest second passes).
 
 #include "logits_select.cuh"
+#include "search.cuh"
 
 namespace qmm {
 
@@ -107,12 +108,7 @@ __global__ void __launch_bounds__(kRowThreads, FILTERS ? 3 : 4) sample_kernel(co
     uint32_t kmin = kKeyNegInf + 1;
     if (m_on) {
         const float guess = (float)((double)mx + T * log(mp));
-        uint32_t b = guess == guess && key32(guess) > kmin ? key32(guess) : kmin;
-        const uint32_t top_key = key32(mx);
-        if (b > top_key) b = top_key;
-        while (b > kmin && weight(key32_value(b - 1)) >= mp) --b;
-        while (b < top_key && weight(key32_value(b)) < mp) ++b;
-        kmin = b;
+        kmin = lowest_kept(kmin, key32(mx), key32(guess), [&](uint32_t b) { return weight(key32_value(b)) >= mp; });
     }
     // Top-k without top-p: tokens below min-p play no part.
     uint32_t bound = kmin;

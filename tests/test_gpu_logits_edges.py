@@ -1,0 +1,56 @@
+"""Rows of logits where a border, a list or a sum lies at the edge of what 32 or 64 bits tell apart."""
+
+import math
+
+import pytest
+import torch
+
+import _logits as R
+
+pytestmark = pytest.mark.gpu
+
+DTYPES = [torch.bfloat16, torch.float16, torch.float32]
+
+
+@pytest.fixture
+def ops():
+    from mlxturbo_b200 import ops
+
+    return ops
+
+
+def uniform(seed, *shape):
+    return torch.rand(shape, generator=torch.Generator().manual_seed(seed)).cuda()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("V", [3, 4099, 70001])
+def test_min_p_border_around_zero(ops, V, dtype):
+    """A largest logit of 0, or a border there: keys of 32 bits are dense around it, weights alike."""
+    g = torch.Generator().manual_seed(V)
+    x = -0.01 - torch.rand((8, V), generator=g) * 6
+    for at in (-4.0, -5.0):  # no logit where its last bit decides
+        x[(x - at).abs() < 0.05] = -4.5
+    x[0] = 0.0
+    x[1, ::3] = 0.0  # equal largest ones
+    x[2, V // 2] = -0.0
+    x[3, V - 1], x[3, 1] = 0.0, -1e-20 if dtype == torch.float32 else -0.5  # weighs 1 in 64 bits too
+    x[4, 0] = 1e-20 if dtype == torch.float32 else 1e-7
+    x[5, 1] = 5.0
+    x[6, 1], x[6, 2] = 4.0, 0.25
+    x[7] = torch.finfo(dtype).min
+    x, u = x.to(dtype).cuda(), uniform(1, 8)
+    T = torch.tensor([1.0, 0.5, 2.0, 1.0, 1e-6, 3e38, math.inf, 1e30]).cuda()
+    for s in (dict(min_p=1.0), dict(min_p=math.exp(-5.0)), dict(temperature=0.5, min_p=math.exp(-8.0)),
+              dict(top_k=2, min_p=1.0), dict(top_p=0.5, min_p=1.0), dict(temperature=T, min_p=1.0),
+              dict(temperature=T, min_p=torch.full((8,), 3.0).cuda())):
+        got = ops.sample(x, u, **s)
+        t = s.get("temperature", 1.0)
+        m = s["min_p"]
+        # Exponentials in 64 bits agree to a few roundings: with |t| = |x - max| log2(e) / T below 8 here, c, the offset
+        # and the difference are off by 2^-53 each of at most 8, t so by 2^-48, the weight by ln 2 times that and the
+        # polynomial's 3e-15: below 2^-47.  A weight that near to min_p (fp16 has -1.0 = 4 - 5) may fall to either side.
+        wants = [[R.sample(x[r], u[r], float(t[r]) if torch.is_tensor(t) else t, s.get("top_k", 0), s.get("top_p", 1.0),
+                           (float(m[r]) if torch.is_tensor(m) else m) * (1 + side * 2.0 ** -47)) for side in (-1, 1)]
+                 for r in range(8)]
+        assert all(i in w for i, w in zip(got.tolist(), wants)), (s, got.tolist(), wants)
