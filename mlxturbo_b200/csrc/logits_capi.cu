@@ -30,7 +30,8 @@ int check_rows(const char* what, int64_t rows, int64_t V, int64_t stride, int dt
 }
 
 // Logits start at any element; other arrays at theirs.
-bool misaligned(const void* p, int bytes) { return !p || (uintptr_t)p % bytes; }
+bool askew(const void* p, int bytes) { return (uintptr_t)p % bytes; }  // null, an array that is not given, is not
+bool misaligned(const void* p, int bytes) { return !p || askew(p, bytes); }
 
 int check_temperature(const char* what, double t, bool zero) {
     if (zero && t == 0.0) return QMM_OK;
@@ -65,7 +66,7 @@ int distill_args(const char* what, qmm::DistillArgs& d, const void* logits, int6
         return QMM_EUNSUPPORTED;
     }
     if (rows && (misaligned(logits, elem_bytes(dtype)) || misaligned(teacher_values, elem_bytes(teacher_dtype)) ||
-                 misaligned(teacher_ids, id_bytes)))
+                 misaligned(teacher_ids, id_bytes) || askew(teacher_logsumexp, 4)))
         return null_error(what);
     d.logits = logits;
     d.stride = row_stride;
@@ -105,7 +106,9 @@ int qmm_sample(const void* logits, int64_t row_stride, int64_t rows, int64_t V, 
         return QMM_EINVAL;
     }
     if (rows == 0) return QMM_OK;
-    if (misaligned(logits, elem_bytes(dtype)) || misaligned(u, 4) || misaligned(ids, 8)) return null_error("sample");
+    if (misaligned(logits, elem_bytes(dtype)) || misaligned(u, 4) || misaligned(ids, 8) ||
+        askew(temperature_rows, 4) || askew(top_k_rows, 4) || askew(top_p_rows, 4) || askew(min_p_rows, 4))
+        return null_error("sample");
     qmm::SampleArgs a{};
     a.logits = logits;
     a.stride = row_stride;
@@ -139,7 +142,8 @@ int qmm_topk(const void* logits, int64_t row_stride, int64_t rows, int64_t V, in
         return QMM_EUNSUPPORTED;
     }
     if (rows == 0) return QMM_OK;
-    if (misaligned(logits, elem_bytes(dtype)) || misaligned(values, elem_bytes(dtype)) || misaligned(ids, 8))
+    if (misaligned(logits, elem_bytes(dtype)) || misaligned(values, elem_bytes(dtype)) || misaligned(ids, 8) ||
+        askew(logsumexp, 4))
         return null_error("topk");
     qmm::TopkArgs a{};
     a.logits = logits;
@@ -179,6 +183,7 @@ int qmm_speculative_sample(const void* logits, int64_t seq_stride, int64_t row_s
     if (!draft_temperature_rows && (rc = check_temperature("speculative_sample", draft_temperature, true))) return rc;
     if (B == 0) return QMM_OK;
     if (misaligned(logits, elem_bytes(dtype)) || misaligned(u, 4) || misaligned(tokens, 8) || misaligned(accepted, 8) ||
+        askew(temperature_rows, 4) || askew(draft_temperature_rows, 4) ||
         (n && (misaligned(draft_logits, elem_bytes(dtype)) || misaligned(draft_ids, 8))))
         return null_error("speculative_sample");
     const size_t need = speculative_workspace(B, n);
@@ -219,7 +224,7 @@ int qmm_distill_loss(const void* logits, int64_t row_stride, int64_t rows, int64
     int rc = distill_args("distill_loss", d, logits, row_stride, rows, V, dtype, teacher_values, teacher_dtype,
                           teacher_ids, id_bytes, teacher_logsumexp, k, temperature);
     if (rc || rows == 0) return rc;
-    if (misaligned(loss, 4) || (uintptr_t)stats % 16) return null_error("distill_loss");
+    if (misaligned(loss, 4) || askew(stats, 16)) return null_error("distill_loss");
     d.loss = loss;
     d.stats = static_cast<float4*>(stats);
     fire("distill_loss");
@@ -235,7 +240,8 @@ int qmm_distill_loss_grad(const void* logits, int64_t row_stride, int64_t rows, 
     int rc = distill_args("distill_loss_grad", d, logits, row_stride, rows, V, dtype, teacher_values, teacher_dtype,
                           teacher_ids, id_bytes, teacher_logsumexp, k, temperature);
     if (rc || rows == 0) return rc;
-    if (misaligned(loss, 4) || misaligned(grad, elem_bytes(dtype))) return null_error("distill_loss_grad");
+    if (misaligned(loss, 4) || misaligned(grad, elem_bytes(dtype)) || askew(row_weight, 4))
+        return null_error("distill_loss_grad");
     if (grad_stride < V || (grad == logits && grad_stride != row_stride)) {
         set_error("distill_loss_grad: gradient rows %lld apart for V=%lld, logits %lld", (long long)grad_stride,
                   (long long)V, (long long)row_stride);
