@@ -516,7 +516,7 @@ QMM_API int qmm_topk(const void* logits, int64_t row_stride, int64_t rows, int64
  * are the standing tokens, the drawn one (-1 if every logit there is
  * -infinity), then -1; accepted [B] counts the standing ones.
  * `workspace` (16-byte aligned) needs no clearing and is not shared by
- * concurrent calls.
+ * concurrent calls.  n <= 2^16, and B (2 n + 1) <= 2^26 rows.
  */
 QMM_API size_t qmm_speculative_sample_workspace_size(int64_t B, int64_t n);
 QMM_API int qmm_speculative_sample(const void* logits, int64_t seq_stride, int64_t row_stride,

@@ -11,6 +11,7 @@ namespace {
 
 constexpr int64_t kMaxVocab = 1LL << 30;  // ids and vector counts are ints
 constexpr int64_t kMaxRows = 1LL << 26;   // rows * 16 CTAs in one grid
+constexpr int64_t kMaxDraft = 1LL << 16;  // a warp looks through a sequence's ids before each of its rows
 
 int check_rows(const char* what, int64_t rows, int64_t V, int64_t stride, int dtype) {
     if (dtype != QMM_BF16 && dtype != QMM_F16 && dtype != QMM_F32) {
@@ -175,8 +176,9 @@ int qmm_speculative_sample(const void* logits, int64_t seq_stride, int64_t row_s
         set_error("speculative_sample: bad shape n=%lld or a negative stride", (long long)n);
         return QMM_EINVAL;
     }
-    if (n > kMaxRows || B * (2 * n + 1) > kMaxRows) {
-        set_error("speculative_sample: B=%lld n=%lld exceed the limit of 2^26 rows", (long long)B, (long long)n);
+    if (n > kMaxDraft || B * (2 * n + 1) > kMaxRows) {
+        set_error("speculative_sample: B=%lld n=%lld exceed the limits of 2^16 drafted tokens and 2^26 rows",
+                  (long long)B, (long long)n);
         return QMM_EUNSUPPORTED;
     }
     if (!temperature_rows && (rc = check_temperature("speculative_sample", temperature, true))) return rc;

@@ -51,11 +51,11 @@ __global__ void __launch_bounds__(kRowThreads, 4) spec_stats_kernel(const SpecAr
     // rows that come after the end of the draft are not looked at
     const int pos = draft ? i - a.n - 1 : i, need = draft ? pos + 1 : pos;
     bool skip = false;
-    for (int j = 0; j < need; ++j) {
+    for (int j = threadIdx.x & 31; j < need; j += 32) {
         const int64_t d = a.ids[b * a.n + j];
         skip |= d < 0 || d >= a.V;
     }
-    if (skip) {
+    if (__any_sync(~0u, skip)) {
         cl.barrier_wait();
         return;
     }

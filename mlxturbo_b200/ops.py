@@ -612,8 +612,8 @@ def speculative_sample(logits: torch.Tensor, draft_logits: torch.Tensor, draft_i
                        temperature=1.0, draft_temperature=None) -> tuple[torch.Tensor, torch.Tensor]:
     """Which drafted tokens stand, and the token after them: (tokens [..., n + 1], accepted [...]), int64.
 
-    logits [..., n + 1, V] are the model's at the n drafted positions and the
-    one after, draft_logits [..., n, V] what draft_ids [..., n] were drawn
+    logits [..., n + 1, V] are the model's at the n <= 65536 drafted positions
+    and the one after, draft_logits [..., n, V] what draft_ids [..., n] were drawn
     from; an id outside [0, V) (-1) ends a shorter draft.  With
     p = softmax(logits / temperature) and q = softmax(draft_logits /
     draft_temperature) (default: temperature), token i stands while

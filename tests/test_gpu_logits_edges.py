@@ -54,3 +54,23 @@ def test_min_p_border_around_zero(ops, V, dtype):
                            (float(m[r]) if torch.is_tensor(m) else m) * (1 + side * 2.0 ** -47)) for side in (-1, 1)]
                  for r in range(8)]
         assert all(i in w for i, w in zip(got.tolist(), wants)), (s, got.tolist(), wants)
+
+
+@pytest.mark.parametrize("B,n", [(2, 33), (3, 1500)])
+def test_speculative_long_drafts(ops, B, n):
+    """More positions than a warp has lanes, a draft that ends behind them, one that ends there."""
+    V = 8
+    g = torch.Generator().manual_seed(n)
+    logits = torch.randn((B, n + 1, V), generator=g).cuda()
+    draft = logits[:, :n].clone()  # every token stands ...
+    ids = torch.randint(0, V, (B, n), generator=g).cuda()
+    u = uniform(2, B, n + 1)
+    ids[0, n - 1] = -1
+    draft[1, n - 1] = -20.0
+    draft[1, n - 1, ids[1, n - 1]] = 20.0  # ... but this one, nearly always
+    u[1, n - 1] = 0.999
+    tokens, accepted = ops.speculative_sample(logits, draft, ids, u)
+    for b in range(B):
+        want, j = R.speculative(logits[b], draft[b], ids[b], u[b])
+        assert tokens[b].tolist() == want and int(accepted[b]) == j
+    assert accepted.tolist()[:2] == [n - 1, n - 1]

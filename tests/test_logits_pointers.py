@@ -1,5 +1,5 @@
-"""Arrays that a call may leave out are refused where they are given and misaligned, without a GPU: the kernels read
-them in whole elements (the pointers stand for nothing)."""
+"""Refusals of the operators on rows of logits, without a GPU (the pointers stand for nothing): arrays that a call may
+leave out, given and misaligned, which the kernels read in whole elements, and drafts too long to be looked through."""
 
 import ctypes
 
@@ -42,3 +42,11 @@ def backward(lse=None):
 def test_misaligned_arrays(call, name):
     assert call(**{name: ODD}) == _lib.QMM_EINVAL
     assert b"misaligned" in _lib.load().qmm_last_error()
+
+
+def test_longest_draft():
+    """Each row's warp looks through the ids before it: lengths whose square would take minutes are refused."""
+    lib = _lib.load()
+    rc = lib.qmm_speculative_sample(P, 1 << 20, 4, P, 1 << 20, 4, 1, (1 << 16) + 1, 4, 0, P, P, None, 1.0, None, 1.0, P, P,
+                                    P, ctypes.c_size_t(1 << 40), None)
+    assert rc == _lib.QMM_EUNSUPPORTED and b"drafted" in lib.qmm_last_error()
