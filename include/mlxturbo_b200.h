@@ -529,10 +529,11 @@ QMM_API int qmm_speculative_sample(const void* logits, int64_t seq_stride, int64
 /*
  * Divergence from a teacher's top logits.  teacher_values [rows, k] (k <= 512)
  * and teacher_ids [rows, k] (int32 or int64 by id_bytes; an id outside [0, V)
- * is an empty place, an id listed twice adds up).  p are the softmax of the
- * listed values over `temperature`, or with teacher_logsumexp [rows] (of the
- * teacher's row over the same temperature) exp(value / temperature -
- * logsumexp), the rest of 1 being the class of all tokens not listed.
+ * is an empty place; the p of an id listed twice is the sum over its entries,
+ * in the loss as in the gradient).  p are the softmax of the listed values over
+ * `temperature`, or with teacher_logsumexp [rows] (of the teacher's row over
+ * the same temperature) exp(value / temperature - logsumexp), the rest of 1
+ * being the class of all tokens not listed.
  * (teacher_logsumexp goes with rows of up to 4 million logits at least;
  * QMM_EUNSUPPORTED where their marks pass what shared memory holds.)
  * loss [rows] = KL(p || softmax(logits / temperature)).  A row with nothing

@@ -11,6 +11,8 @@
 //   dloss/dl_i = (q_i - p_i) / tau                     listed tokens
 //              = e_i (1 / Z  [ - rest / O ]) / tau     the others, e_i / Z = q_i
 //
+// j counts distinct ids: p_j is the sum over the entries that name the id.
+//
 // O is summed on its own (a bit to an element marks the listed ones), not as a
 // difference: it may be a billionth of Z.  Its weights are taken against the
 // largest logit that is not listed, so neither O nor rest / O leaves the range
@@ -36,7 +38,7 @@ constexpr int kDistillThreads = kRowThreads + 32;
 struct DistillShared {
     WarpStat stats[kMaxRowWarps];
     double mass;   // sum p
-    double cross;  // sum p (log p - l / tau)
+    double cross;  // sum p (log p - l / tau), for the loss
     double part;   // sum over distinct listed tokens of exp((l - best) / tau)
     float best;    // largest listed logit
     int twice;     // an id is listed more than once
@@ -80,8 +82,8 @@ QMM_DEVINL void list_ids(const DistillArgs& a, const List& li, long long r) {
 }
 
 // The rest of it, by one warp: log p and the student's logits; entries of one
-// id share a slot whose owner is the first of them; the sums.
-template <int DT, bool TAIL>
+// id share a slot whose owner is the first of them; the sums (LOSS: the loss' too).
+template <int DT, bool TAIL, bool LOSS>
 QMM_DEVINL void list_sums(const DistillArgs& a, DistillShared& sh, const List& li, const Row<DT>& row, long long r) {
     const int lane = threadIdx.x & 31;
     double top = -CUDART_INF;
@@ -129,6 +131,7 @@ QMM_DEVINL void list_sums(const DistillArgs& a, DistillShared& sh, const List& l
         atomicMin(&li.owner[h], j);
     }
     __syncwarp();
+    twice = __any_sync(~0u, twice);
 #pragma unroll
     for (int o = 16; o >= 1; o >>= 1) top = fmax(top, __shfl_xor_sync(~0u, top, o));
     best = warp_max(best);
@@ -146,13 +149,23 @@ QMM_DEVINL void list_sums(const DistillArgs& a, DistillShared& sh, const List& l
         li.logp[j] = lp;
         mass += p;
         if (li.id[j] < 0) continue;
-        if (p != 0.0) cross += p * (lp - (double)li.x[j] * a.inv_t);
+        if (LOSS && !twice && p != 0.0) cross += p * (lp - (double)li.x[j] * a.inv_t);
         if (TAIL && li.owner[li.slot[j]] == j) part += exp(((double)li.x[j] - (double)best) * a.inv_t);
+    }
+    if (LOSS && twice) {  // an id's entries added up before the logarithm
+        __syncwarp();
+        for (int j = lane; j < a.k; j += 32) {
+            const int id = li.id[j];
+            if (id < 0 || li.owner[li.slot[j]] != j) continue;
+            double p = exp(li.logp[j]);
+            for (int i = j + 1; i < a.k; ++i)
+                if (li.id[i] == id) p += exp(li.logp[i]);
+            if (p != 0.0) cross += p * (log(p) - (double)li.x[j] * a.inv_t);
+        }
     }
     mass = warp_sum(mass);
     cross = warp_sum(cross);
     if (TAIL) part = warp_sum(part);
-    twice = __any_sync(~0u, twice);
     if (lane == 0) {
         sh.mass = mass;
         sh.cross = cross;
@@ -228,7 +241,7 @@ __global__ void __launch_bounds__(kDistillThreads, MODE == kBackward ? 3 : 4)
         sum = st.w;
         if (!reader && weight != 0.0f) {
             list_ids(a, li, r);
-            list_sums<DT, TAIL>(a, sh, li, row, r);
+            list_sums<DT, TAIL, false>(a, sh, li, row, r);
         }
     } else {
         if (!reader) list_ids(a, li, r);
@@ -259,7 +272,7 @@ __global__ void __launch_bounds__(kDistillThreads, MODE == kBackward ? 3 : 4)
             else top = stream_slice<DT, true, false>(row, s, c, acc, unlisted, ring);
             stat = warp_stat(top.first, acc);
         } else {
-            list_sums<DT, TAIL>(a, sh, li, row, r);
+            list_sums<DT, TAIL, true>(a, sh, li, row, r);
         }
         cl.barrier_wait();
         if (reader) all_gather(cl, sh.stats, g, stat);

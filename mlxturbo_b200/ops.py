@@ -640,9 +640,9 @@ def distill_loss(logits: torch.Tensor, teacher_values: torch.Tensor, teacher_ids
     """KL divergence (float32 [...]) of each row's softmax(logits / temperature) from a teacher's top logits.
 
     logits are [..., V]; teacher_values and teacher_ids [..., k], k <= 512, as
-    ``topk`` gives them.  An id outside [0, V) is an empty place; an id listed
-    twice adds up.  The teacher's probabilities are those of the listed values,
-    renormalised; with ``teacher_logsumexp`` [...] (``topk`` with logsumexp=True
+    ``topk`` gives them.  An id outside [0, V) is an empty place; the entries of
+    an id listed twice add up to one probability.  The teacher's probabilities
+    are those of the listed values, renormalised; with ``teacher_logsumexp`` [...] (``topk`` with logsumexp=True
     and the same temperature) they are taken as they are, and the rest of the
     teacher's mass is compared with the model's on all tokens not listed.  A row
     with nothing listed, or whose teacher_logsumexp is -inf, has loss 0.

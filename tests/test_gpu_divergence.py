@@ -1,0 +1,92 @@
+"""Divergence from a teacher's list and its gradient for every kind of list, against 64 bits.
+
+Tolerances: the sums of weights are off by REL of themselves (the derivation stands in test_gpu_logits.py), so a
+logarithm by REL, for the listed tokens and for the rest's class; the loss is rounded to 32 bits.  Sums over the list
+are 64-bit ones."""
+
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from _divergence import divergence
+
+pytestmark = pytest.mark.gpu
+
+DTYPES = [torch.bfloat16, torch.float16, torch.float32]
+REL = 1e-5
+
+
+@pytest.fixture
+def ops():
+    from mlxturbo_b200 import ops
+
+    return ops
+
+
+def check(ops, x, tv, ti, T=1.0, lse=None, weight=None):
+    """Loss and gradient of all calls against 64 bits."""
+    rows = x.shape[0]
+    w = torch.ones(rows, device="cuda") if weight is None else weight
+    kw = dict(temperature=T, teacher_logsumexp=lse)
+    leaf = x.detach().clone().requires_grad_()
+    loss = ops.distill_loss(leaf, tv, ti, **kw)
+    (grad,) = torch.autograd.grad(loss, leaf, w)
+    loss1, grad1 = ops.distill_loss_and_grad(x, tv, ti, weight, **kw)
+    assert torch.equal(ops.distill_loss(x, tv, ti, **kw), loss.detach()) and torch.equal(loss.detach(), loss1)
+    fin = torch.finfo(x.dtype)
+    for r in range(rows):
+        want, g, size = divergence(x[r], tv[r], ti[r], T, None if lse is None else float(lse[r]), float(w[r]))
+        got = float(loss1[r])
+        assert got == want or abs(got - want) <= 2 * REL + 2 ** -23 * abs(want) < math.inf, (r, got, want)
+        bound = fin.eps / 2 * np.abs(g) + 2.01 * REL * size + fin.smallest_normal * fin.eps / 2
+        for d in (grad, grad1):
+            err = np.abs(d[r].double().cpu().numpy() - g)
+            assert (err <= bound).all(), (r, float((err / bound).max()))
+    return loss1
+
+
+def student(rows, V, dtype, seed):
+    g = torch.Generator().manual_seed(seed)
+    teacher = torch.randn((rows, V), generator=g) * 3
+    x = teacher + 0.5 * torch.randn((rows, V), generator=g)
+    return x.to(dtype).cuda(), teacher.to(dtype).cuda()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("tail", [False, True])
+@pytest.mark.parametrize("V,k", [(40, 12), (3001, 12), (3001, 130)])
+def test_repeated_ids(ops, V, k, tail, dtype):
+    """Ids listed twice and more, beside empty places, empty lists, values of -inf and any order of the list."""
+    x, teacher = student(9, V, dtype, V + k)
+    tv, ti, lse = ops.topk(teacher, min(k, V), logsumexp=True)
+    ti[0, 3:] = -1
+    ti[1] = -1
+    ti[2, 5:] = ti[2, 4]
+    ti[3] = ti[3, 0]
+    tv[2:5] -= math.log(k) + 1  # as often as k times the same id: its mass stays below 1
+    ti[4, 1::2] = ti[4, ::2]
+    tv[5, 2:7] = -torch.inf
+    tv[6] = -torch.inf
+    ti[7], tv[7] = ti[7].flip(0), tv[7].flip(0)
+    ti[8, 1], ti[8, 2], ti[8, 5] = V, 2 ** 40, ti[8, 0]
+    tv[8] -= 1
+    if tail:
+        lse[6] = -torch.inf  # nothing of the teacher's row is left
+    weight = torch.tensor([1.0, 1.0, 1.0, 0.5, -2.0, 1.0, 1.0, 0.0, 1.0]).cuda()
+    loss = check(ops, x, tv, ti, 1.0, lse if tail else None, weight)
+    check(ops, x, tv.float(), ti.clamp(-1, V).int(), 2.0, lse if tail else None)
+    assert float(loss[6]) == 0.0 and (loss >= -2 * REL).all()  # a divergence
+
+
+def test_an_id_in_equal_parts(ops):
+    """However an id's probability is cut into entries, the divergence is the same: none here."""
+    x = torch.full((3, 500), -40.0, device="cuda")
+    x[:, 7] = 10.0
+    ti = torch.tensor([[7, 7, 7, 7], [7, 7, -1, -1], [7, -1, -1, -1]]).cuda()
+    tv = torch.zeros((3, 4), device="cuda")
+    lse = torch.tensor([4.0, 2.0, 1.0]).log().cuda()
+    for kw in (dict(), dict(teacher_logsumexp=lse)):
+        loss, grad = ops.distill_loss_and_grad(x, tv, ti, **kw)
+        assert loss.abs().max() <= 2 * REL and grad.abs().max() <= 2 * REL
