@@ -533,7 +533,9 @@ QMM_API int qmm_speculative_sample(const void* logits, int64_t seq_stride, int64
  * in the loss as in the gradient).  p are the softmax of the listed values over
  * `temperature`, or with teacher_logsumexp [rows] (of the teacher's row over
  * the same temperature) exp(value / temperature - logsumexp), the rest of 1
- * being the class of all tokens not listed.
+ * being the class of all tokens not listed.  Where these all lie more than 700
+ * temperatures below the row's largest logit (a list of all that is not
+ * masked), a rest up to 2^-17 + 2^-23 |logsumexp|, its rounding, is none.
  * (teacher_logsumexp goes with rows of up to 4 million logits at least;
  * QMM_EUNSUPPORTED where their marks pass what shared memory holds.)
  * loss [rows] = KL(p || softmax(logits / temperature)).  A row with nothing

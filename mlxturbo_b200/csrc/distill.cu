@@ -32,6 +32,10 @@
 
 namespace qmm {
 
+// Temperatures below the largest logit at which a token has no weight, whatever
+// their number: exp(-700) is 1e-304.
+constexpr double kNoWeight = -700.0;
+
 // A CTA: eight warps read logits, a ninth works through the list meanwhile.
 constexpr int kDistillThreads = kRowThreads + 32;
 
@@ -227,8 +231,9 @@ __global__ void __launch_bounds__(kDistillThreads, MODE == kBackward ? 3 : 4)
     const int cta_end = cta_begin + per * kRowWarps;
     const Slice s = warp_slice<DT>(row, g, warps);
     const Scale c(a.inv_t);
+    const float tlse = TAIL ? a.tlse[r] : 0.0f;
     // a teacher's row that is masked throughout carries no loss
-    const bool none = TAIL && a.tlse[r] == -CUDART_INF_F;
+    const bool none = TAIL && tlse == -CUDART_INF_F;
     const float weight = none ? 0.0f : a.weight ? a.weight[r] : 1.0f;
 
     float ref, mx;       // the others' reference; the row's maximum
@@ -312,6 +317,11 @@ __global__ void __launch_bounds__(kDistillThreads, MODE == kBackward ? 3 : 4)
             const float down = sh.best == -CUDART_INF_F ? 0.0f : expf((float)(((double)sh.best - (double)mx) * a.inv_t));
             sum = s_ref * (double)lift + sh.part * (double)down;
             rest = mass < 1.0 ? 1.0 - mass : mass >= 1.0 ? 0.0 : mass;
+            // A list of all that is not masked leaves a rest of rounding alone: of the log-sum-exp's 32 bits and of
+            // the fast sums it may come from.
+            if (((double)ref - (double)mx) * a.inv_t < kNoWeight &&
+                rest <= 2.0 * kFastEps + fabs((double)tlse) * (1.0 / 8388608.0))
+                rest = 0.0;
             others = (double)lift / sum - (s_ref > 0.0 ? rest / s_ref : 0.0);
             if (ref == -CUDART_INF_F) others = 0.0;  // no token that is not listed has any probability
         } else {

@@ -644,8 +644,10 @@ def distill_loss(logits: torch.Tensor, teacher_values: torch.Tensor, teacher_ids
     an id listed twice add up to one probability.  The teacher's probabilities
     are those of the listed values, renormalised; with ``teacher_logsumexp`` [...] (``topk`` with logsumexp=True
     and the same temperature) they are taken as they are, and the rest of the
-    teacher's mass is compared with the model's on all tokens not listed.  A row
-    with nothing listed, or whose teacher_logsumexp is -inf, has loss 0.
+    teacher's mass is compared with the model's on all tokens not listed (where
+    these are all masked, a rest up to 2^-17 + 2^-23 |teacher_logsumexp|, its
+    rounding, is none, and a larger one an infinite loss).  A row with nothing
+    listed, or whose teacher_logsumexp is -inf, has loss 0.
 
     Differentiable in the logits.  The gradient of a row whose incoming
     gradient is 0 is 0, whatever its logits; the loss is not multiplied by

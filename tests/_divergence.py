@@ -26,6 +26,8 @@ def divergence(row, tv, ti, T=1.0, lse=None, weight=1.0):
         listed = np.zeros(V, bool)
         listed[ids] = True
         rest, other = max(0.0, 1.0 - p.sum()), q[~listed].sum()
+        if (x[~listed] - x.max() < -700).all() and rest <= 2.0 ** -17 + 2.0 ** -23 * abs(lse):
+            rest = 0.0  # the rounding of the log-sum-exp: nothing is left but masked tokens
         if rest > 0:
             with np.errstate(divide="ignore"):
                 loss += float(rest * (np.log(rest) - np.log(other)))

@@ -90,3 +90,32 @@ def test_an_id_in_equal_parts(ops):
     for kw in (dict(), dict(teacher_logsumexp=lse)):
         loss, grad = ops.distill_loss_and_grad(x, tv, ti, **kw)
         assert loss.abs().max() <= 2 * REL and grad.abs().max() <= 2 * REL
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("mask", [None, "lowest", "inf"])
+@pytest.mark.parametrize("V,k,T", [(40, 40, 1.0), (9, 9, 2.5), (300, 30, 0.7)])
+def test_lists_of_all_that_is_left(ops, V, k, T, mask, dtype):
+    """Small vocabularies and constrained answers: a list of all tokens that have any probability.  What the given
+    log-sum-exp's rounding leaves of 1 is no rest; a rest beyond that stays an infinite loss."""
+    rows = 64
+    x, teacher = student(rows, V, dtype, V)
+    if mask is None:
+        k = V
+    else:
+        allowed = torch.zeros((rows, V), dtype=torch.bool, device="cuda")
+        allowed.scatter_(1, uniform_ids(rows, V, k).cuda(), True)
+        low = torch.finfo(dtype).min if mask == "lowest" else -torch.inf
+        x, teacher = x.masked_fill(~allowed, low), teacher.masked_fill(~allowed, low)
+    tv, ti, lse = ops.topk(teacher, k, logsumexp=True, temperature=T)
+    for given in (lse, torch.logsumexp(teacher.float() / T, -1)):
+        loss = check(ops, x, tv, ti, T, given)
+        assert loss.isfinite().all() and (loss >= -2 * REL).all()
+    if mask != "lowest":
+        loss, grad = ops.distill_loss_and_grad(x, tv, ti, temperature=T, teacher_logsumexp=lse + 0.1)
+        assert (loss == torch.inf).all() and grad.isfinite().all()
+
+
+def uniform_ids(rows, V, k):
+    g = torch.Generator().manual_seed(rows + V)
+    return torch.stack([torch.randperm(V, generator=g)[:k] for _ in range(rows)])
