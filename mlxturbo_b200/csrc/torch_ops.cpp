@@ -589,6 +589,22 @@ auto registered(const char* name) {
     return c10::Dispatcher::singleton().findSchemaOrThrow(name, "").typed<F>();
 }
 
+bool has_tangent(const at::Tensor& t) { return t.defined() && t._fw_grad(0).defined(); }
+
+// The gradient where a graph of it is asked for (create_graph): what differentiates it again is told.
+struct DistillGradient : torch::autograd::Function<DistillGradient> {
+    static at::Tensor forward(torch::autograd::AutogradContext*, const at::Tensor& logits, const at::Tensor& tv,
+                              const at::Tensor& ti, const std::optional<at::Tensor>& lse, double t,
+                              const at::Tensor& stats, const at::Tensor& grad_loss) {
+        at::AutoDispatchBelowADInplaceOrView below;
+        static const auto op = registered<decltype(distill_backward)>("mlxturbo_b200::distill_backward");
+        return op.call(logits, tv, ti, lse, t, stats, grad_loss);
+    }
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext*, torch::autograd::variable_list) {
+        fail(Err::kNotImplemented, "the distillation loss has no second derivative");
+    }
+};
+
 struct DistillFunction : torch::autograd::Function<DistillFunction> {
     static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& logits, const at::Tensor& tv,
                               const at::Tensor& ti, const std::optional<at::Tensor>& lse, double t) {
@@ -603,18 +619,26 @@ struct DistillFunction : torch::autograd::Function<DistillFunction> {
     static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
                                                    torch::autograd::variable_list grads) {
         const auto saved = ctx->get_saved_variables();
-        if (at::GradMode::is_enabled() && grads[0].requires_grad())
+        if ((at::GradMode::is_enabled() && grads[0].requires_grad()) || has_tangent(grads[0]))
             fail(Err::kNotImplemented, "the distillation loss has no second derivative");
-        at::AutoDispatchBelowADInplaceOrView below;
         const std::optional<at::Tensor> lse = saved[3].defined() ? std::optional<at::Tensor>(saved[3]) : std::nullopt;
-        static const auto op = registered<decltype(distill_backward)>("mlxturbo_b200::distill_backward");
-        return {op.call(saved[0], saved[1], saved[2], lse, ctx->saved_data["t"].toDouble(), saved[4], grads[0]),
-                at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()};
+        const double t = ctx->saved_data["t"].toDouble();
+        at::Tensor grad;
+        if (at::GradMode::is_enabled()) {
+            grad = DistillGradient::apply(saved[0], saved[1], saved[2], lse, t, saved[4], grads[0]);
+        } else {
+            at::AutoDispatchBelowADInplaceOrView below;
+            static const auto op = registered<decltype(distill_backward)>("mlxturbo_b200::distill_backward");
+            grad = op.call(saved[0], saved[1], saved[2], lse, t, saved[4], grads[0]);
+        }
+        return {grad, at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()};
     }
 };
 
 at::Tensor distill_autograd(const at::Tensor& logits, const at::Tensor& tv, const at::Tensor& ti,
                             const std::optional<at::Tensor>& lse, double t) {
+    if (has_tangent(logits) || has_tangent(tv) || (lse.has_value() && has_tangent(*lse)))
+        fail(Err::kNotImplemented, "the distillation loss has no forward-mode derivative");
     if (at::GradMode::is_enabled()) {
         if (tv.requires_grad() || (lse.has_value() && lse->requires_grad()))
             fail(Err::kNotImplemented, "the distillation loss has no gradient for the teacher's side; detach it");

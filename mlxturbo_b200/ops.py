@@ -24,6 +24,7 @@ from __future__ import annotations
 import math
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -600,6 +601,7 @@ TOPK_MAX = 1024
 def topk(logits: torch.Tensor, k: int, *, logsumexp: bool = False, temperature: float = 1.0):
     """(values, ids) of the k <= 1024 largest logits of each row [..., V], in the order of (value
     descending, id ascending): values [..., k] in the logits' dtype, ids int64.  A NaN counts as -inf.
+    Outside autograd: neither the values nor the log-sum-exp carry a gradient.
 
     With ``logsumexp`` also the float32 [...] logarithm of the sum of
     exp(logits / temperature): a teacher's side of ``distill_loss``.
@@ -630,6 +632,12 @@ def speculative_sample(logits: torch.Tensor, draft_logits: torch.Tensor, draft_i
                                      *_rows_or_one(draft_temperature, 0.0))
 
 
+def _no_tangent(*tensors) -> None:
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None
+                                              for t in tensors):
+        raise NotImplementedError("the distillation loss has no forward-mode derivative")
+
+
 def _no_teacher_grad(*tensors) -> None:
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
         raise NotImplementedError("the distillation loss has no gradient for the teacher's side; detach it")
@@ -649,9 +657,10 @@ def distill_loss(logits: torch.Tensor, teacher_values: torch.Tensor, teacher_ids
     rounding, is none, and a larger one an infinite loss).  A row with nothing
     listed, or whose teacher_logsumexp is -inf, has loss 0.
 
-    Differentiable in the logits.  The gradient of a row whose incoming
-    gradient is 0 is 0, whatever its logits; the loss is not multiplied by
-    temperature squared.
+    Differentiable in the logits, once and in reverse mode (anything else
+    raises NotImplementedError).  The gradient of a row whose incoming gradient
+    is 0 is 0, whatever its logits; the loss is not multiplied by temperature
+    squared.
     """
     return _logits_ops().distill(logits, teacher_values, teacher_ids, teacher_logsumexp, temperature)
 
@@ -667,6 +676,7 @@ def distill_loss_and_grad(logits: torch.Tensor, teacher_values: torch.Tensor, te
     are read once and never kept; ``out`` may be the logits themselves.
     Outside autograd: logits that require a gradient are refused.
     """
+    _no_tangent(logits, teacher_values, teacher_logsumexp, row_weight)
     _no_teacher_grad(teacher_values, teacher_logsumexp, row_weight)
     if torch.is_grad_enabled() and logits.requires_grad:
         raise NotImplementedError("distill_loss_and_grad is outside autograd: detach the logits, or use distill_loss")
