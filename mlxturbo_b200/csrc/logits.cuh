@@ -710,7 +710,8 @@ QMM_DEVINL Found find_place(const Row<DT>& row, int from, int to, double base, d
         }
         if (lane == 31) sh.sums[warp] = incl;
         __syncthreads();
-        run = base + incl - mass;
+        run = __shfl_up_sync(~0u, incl, 1);  // not incl - mass, which loses what is small beside mass
+        run = base + (lane == 0 ? 0.0 : run);
         for (int i = 0; i < warp; ++i) run += sh.sums[i];
         // the first thread that passes, or the last with a weight
         const bool passes = mass > 0.0 && run + mass > target;

@@ -31,6 +31,7 @@ namespace qmm {
 // the border, but more kept tokens than it draws from itself; not enough of them.
 enum { kDone, kNeedSum, kBorder, kGeneral };
 constexpr int kDrawHere = 2 * kRowThreads;
+static_assert(kDrawHere <= kBins, "their weights lie in bin_sum");
 // What a row with top-p alone lists first: enough where the model is sure of
 // itself, and about 180 tokens, which a CTA sorts in one turn.
 constexpr int kNucleus = 128;
@@ -133,6 +134,9 @@ __global__ void __launch_bounds__(kRowThreads, FILTERS ? 3 : 4) sample_kernel(co
             if (rank != 0 && sure) return;
             bool sorted = false;
             double eps = k_on ? 0.0 : fast ? kFastEps : 1.0;
+            // Of the tokens that are drawn from: a difference of the running sums in sh.w would be 0 for one below
+            // 2^-53 of them, which u = 0 may ask for.
+            double* const own = reinterpret_cast<double*>(sh.bin_sum);
             for (;;) {
                 if (rank == 0) {
                     int verdict = kDone;
@@ -146,8 +150,11 @@ __global__ void __launch_bounds__(kRowThreads, FILTERS ? 3 : 4) sample_kernel(co
                     int kept = (int)n;
                     if (verdict == kDone && !sorted) {
                         sort_candidates(sh.cand, (int)n);
-                        for (int i = threadIdx.x; i < (int)n; i += kRowThreads)
-                            sh.w[i] = weight(key32_value((uint32_t)(sh.cand[i] >> 32)));
+                        for (int i = threadIdx.x; i < (int)n; i += kRowThreads) {
+                            const double w = weight(key32_value((uint32_t)(sh.cand[i] >> 32)));
+                            sh.w[i] = w;
+                            if (i < kDrawHere) own[i] = w;
+                        }
                         __syncthreads();
                         scan_weights(sh, (int)n);
                         sorted = true;
@@ -180,14 +187,10 @@ __global__ void __launch_bounds__(kRowThreads, FILTERS ? 3 : 4) sample_kernel(co
                         unsigned long long best = ~0ull;
                         for (int j = threadIdx.x; j < kept; j += kRowThreads) {
                             const int id = key_id(sh.cand[j]);
-                            double run = 0.0, prev = 0.0;
-                            const double own = sh.w[j] - (j ? sh.w[j - 1] : 0.0);
-                            for (int i = 0; i < kept; ++i) {
-                                const double cum = sh.w[i];
-                                if (key_id(sh.cand[i]) <= id) run += cum - prev;
-                                prev = cum;
-                            }
-                            if (own > 0.0) {
+                            double run = 0.0;
+                            for (int i = 0; i < kept; ++i)
+                                if (key_id(sh.cand[i]) <= id) run += own[i];
+                            if (own[j] > 0.0) {
                                 // past the target: the smallest id; if none is, the largest id of all
                                 const unsigned long long code =
                                     run > target ? (unsigned long long)id : (1ull << 40) + (0xFFFFFFFFu - (uint32_t)id);

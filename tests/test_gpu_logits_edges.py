@@ -74,3 +74,24 @@ def test_speculative_long_drafts(ops, B, n):
         want, j = R.speculative(logits[b], draft[b], ids[b], u[b])
         assert tokens[b].tolist() == want and int(accepted[b]) == j
     assert accepted.tolist()[:2] == [n - 1, n - 1]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("V", [40, 5003, 120001])
+def test_numbers_near_zero(ops, V, dtype):
+    """u = 0, or far below 2^-53, asks for tokens that weigh nothing beside the sum: the first id that is kept."""
+    g = torch.Generator().manual_seed(V)
+    x = torch.randn((12, V), generator=g) * 3
+    for r in range(12):
+        x[r, torch.randperm(V, generator=g)[:5]] = 60.0 - r
+    x[6:, :4] = torch.tensor([-9.0, 12.0, 9.0, 20.0])
+    x = x.to(dtype).cuda()
+    u = torch.tensor([0.0, 0.0, 1e-30, 1e-38, 1e-20, 1e-12] * 2).cuda()
+    for s in (dict(top_k=2), dict(top_k=6), dict(temperature=0.5, top_k=30), dict(temperature=0.3, top_k=20, top_p=0.999),
+              dict(top_k=39, min_p=1e-30), dict(temperature=0.7, top_k=300), dict(min_p=1e-25), dict(min_p=1e-9),
+              dict(temperature=0.6), dict(temperature=2.0)):
+        if s.get("top_k", 0) >= V:
+            continue
+        want = [R.sample(x[r], u[r], s.get("temperature", 1.0), s.get("top_k", 0), s.get("top_p", 1.0), s.get("min_p", 0.0))
+                for r in range(12)]
+        assert ops.sample(x, u, **s).tolist() == want, s
