@@ -611,8 +611,11 @@ QMM_DEVINL unsigned long long border_key(cg::cluster_group& cl, SelectShared& sh
 // of tokens are kept.  One pass weighs every token in 64 bits.  Those below
 // `bound` (all but some hundreds) go into bins of equal depth, as whole numbers
 // of 2^-40 of the weight there; each warp has bins of its own, in two limbs of
-// 20 bits, so that 32-bit adds do for fewer than 4096 tokens to a warp, and the
-// sums are exact whatever their order.  The bins reach down to where what is
+// 20 bits, so that 32-bit adds do for fewer than 4096 tokens to a warp, and a
+// sum of whole numbers is the same in any order.  A token is off by half such a
+// unit, so a bin's sums, a mass above a bin and a part of the whole by half a
+// unit for each token: a border or a draw nearer than that is made in 64 bits
+// (one row in 10^4 or fewer).  The bins reach down to where what is
 // left, V tokens at most, is half of what top-p leaves out.  The tokens of the
 // bin that holds the border, less than a hundredth of them, go to CTA 0's
 // list.  What lies above it of each warp is kept for the draw, so no token is
@@ -705,22 +708,26 @@ QMM_DEVINL bool kth_by_bins(cg::cluster_group& cl, SelectShared& sh, const Row<D
     return sh.verdict != 0;
 }
 
-// Border of the part `p` of the mass of the tokens with keys >= floor.  Tokens
-// from `edge` on are summed beside the bins, which reach `deep` temperatures
-// below it.  Returns false where bins do not give it: it lies above the edge, in
-// the last bin, or in one with more tokens than the list holds (equal ones).
-// Else `border` is it, and slots[g] in CTA 0 (only) the mass of warp g's tokens
-// from it on; slots is a shared array for all warps.
+// Border of the part `p` of the mass of the tokens with keys >= floor, `tokens` of
+// them at most.  Tokens from `edge` on are summed beside the bins, which reach
+// `deep` temperatures below it.  Returns false where bins do not give it: it lies
+// above the edge, in the last bin, in one with more tokens than the list holds
+// (equal ones), or nearer to a token's end than their sums are.  Else `border` is
+// it, and slots[g] in CTA 0 (only) the mass of warp g's tokens from it on; slots
+// is a shared array for all warps.  Sums of them, and parts of their whole, are
+// off by `slack` together at most.
 template <int DT>
 QMM_DEVINL bool border_by_bins(cg::cluster_group& cl, SelectShared& sh, const Row<DT>& row, const Slice& s, int g,
                                int warps, Ring ring, const Weight64& weight, double p, float edge, double deep,
-                               unsigned long long floor, double* slots, unsigned long long& border) {
+                               unsigned long long floor, int tokens, double* slots, unsigned long long& border,
+                               double& slack) {
     constexpr int N = Elem<DT>::kVec;
     const int rank = (int)cl.block_rank(), warp = threadIdx.x >> 5, t = threadIdx.x, C = (int)cl.num_blocks();
     const double w_edge = weight(edge);
     if (!(w_edge > 1e-250) || !(deep > 0.0) || !(deep < 1e3)) return false;
     const float scale = (float)((kBins - 1) * weight.inv_t / deep);
     const double unit = exp2(ceil(log2(w_edge)) - 40.0), per_unit = 1.0 / unit;
+    slack = (double)tokens * unit;  // half a unit a token on either side of a comparison
     const float floor_value = key32_value((uint32_t)(floor >> 32));
     auto counts = [&](int id, float x) {
         return x > floor_value || (x == floor_value && row_key(x, id) >= floor);
@@ -821,7 +828,7 @@ QMM_DEVINL bool border_by_bins(cg::cluster_group& cl, SelectShared& sh, const Ro
             // a token that is kept goes to its warp's sum, in units
             auto keep = [&](unsigned long long key) {
                 const double w = weight(key32_value((uint32_t)(key >> 32)));
-                atomicAdd(&sh.bin_sum[(key_id(key) + row.shift) / N / per], (unsigned long long)(w * per_unit));
+                atomicAdd(&sh.bin_sum[(key_id(key) + row.shift) / N / per], (unsigned long long)(w * per_unit + 0.5));
             };
             if (n > kRowThreads) {
                 // the bin once more in 256: sorting 1000 tokens takes 10 us, this 2
@@ -892,6 +899,7 @@ QMM_DEVINL bool border_by_bins(cg::cluster_group& cl, SelectShared& sh, const Ro
                     if (start + sh.w[m] >= target) e = m;
                     else b = m + 1;
                 }
+                ok = start + (b > 0 ? sh.w[b - 1] : 0.0) + slack < target && start + sh.w[b] - slack >= target;
                 for (int i = t; i <= b; i += kRowThreads) keep(sh.cand[i]);
                 __syncthreads();
                 if (t < warps) slots[t] += (double)sh.bin_sum[t] * unit;

@@ -273,15 +273,14 @@ __global__ void __launch_bounds__(kRowThreads, FILTERS ? 3 : 4) sample_kernel(co
         const double deep = k_on ? ((double)mx - (double)key32_value((uint32_t)(from >> 32))) * inv_t * 1.001
                                  : log(2.0 * row.V * weight(edge) / ((1.0 - p) * total));
         unsigned long long found;
-        if (border_by_bins<DT>(cl, sh, row, s, g, warps, ring, weight, p, edge, deep, from, sh.slots[0], found)) {
+        double slack;
+        if (border_by_bins<DT>(cl, sh, row, s, g, warps, ring, weight, p, edge, deep, from, k_on ? k : row.V,
+                               sh.slots[0], found, slack)) {
             from = found;
             if (from >= border) {  // min-p keeps them all: CTA 0 has each warp's mass
                 if (rank != 0) return;
-                const double target = u * slots_sum(sh.slots[0], warps);
-                const Place at = locate(sh.slots[0], warps, target);
                 const uint32_t from32 = (uint32_t)(from >> 32);
-                const Found f = find_in_slice<DT>(row, warp_slice<DT>(row, at.g, warps), at.base, target, ring, sh.find,
-                                                  [&](int v, const uint4& q, double (&w)[Elem<DT>::kVec]) {
+                auto from_on = [&](int v, const uint4& q, double (&w)[Elem<DT>::kVec]) {
                     float x[Elem<DT>::kVec];
                     decode<DT>(q, x);
 #pragma unroll
@@ -290,9 +289,30 @@ __global__ void __launch_bounds__(kRowThreads, FILTERS ? 3 : 4) sample_kernel(co
                         const bool out = k32 < from32 || (k32 == from32 && row_key(x[j], row.first(v) + j) < from);
                         w[j] = out ? 0.0 : weight(x[j]);
                     }
-                });
-                if (threadIdx.x == 0) a.ids[r] = f.id;
-                return;
+                };
+#pragma unroll 1
+                for (;; slack = 0.0) {
+                    const double target = u * slots_sum(sh.slots[0], warps);
+                    const Place at = locate(sh.slots[0], warps, target);
+                    const Found f = find_in_slice<DT>(row, warp_slice<DT>(row, at.g, warps), at.base, target, ring,
+                                                      sh.find, from_on);
+                    if (slack == 0.0 || (f.id >= 0 && f.before + slack <= target && f.after - slack > target)) {
+                        if (threadIdx.x == 0) a.ids[r] = f.id;
+                        return;
+                    }
+                    // the masses in 64 bits, by this CTA alone: the others have left
+                    for (int i = threadIdx.x >> 5; i < warps; i += kRowWarps) {
+                        double mass = 0.0;
+                        for_vectors_slow<DT>(row, warp_slice<DT>(row, i, warps), ring, [&](int v, const uint4& q) {
+                            double w[Elem<DT>::kVec];
+                            from_on(v, q, w);
+                            mass += tree_sum(w);
+                        });
+                        mass = warp_sum(mass);
+                        if (s.lane == 0) sh.slots[0][i] = mass;
+                    }
+                    __syncthreads();
+                }
             }
             bordered = true;
         }

@@ -95,3 +95,71 @@ def test_numbers_near_zero(ops, V, dtype):
         want = [R.sample(x[r], u[r], s.get("temperature", 1.0), s.get("top_k", 0), s.get("top_p", 1.0), s.get("min_p", 0.0))
                 for r in range(12)]
         assert ops.sample(x, u, **s).tolist() == want, s
+
+
+def _far_tokens(V, seed, first):
+    """A row of five tokens that weigh 1, 4000 that weigh 1e-10 each, and id 3 with logit `first`; k and top-p keep
+    most of the 4000."""
+    g = torch.Generator().manual_seed(seed)
+    x = torch.full((V,), -60.0)
+    at = V // 2 + torch.randperm(V // 2, generator=g)[:4005]
+    x[at] = -23.5 + torch.rand(4005, generator=g)
+    x[at[:5]] = 0.0
+    x[3] = first
+    return x
+
+
+def test_draws_finer_than_the_bins(ops):
+    """Masses that bins hold in whole parts of 2^-40: a draw that falls between a token's weight and its rounding."""
+    V, k, p = 120001, 4500, 1 - 1e-9
+    unit = 2.0 ** -40
+    rows, u = [], []
+    for i in range(40):
+        first = -22.6 - i / 400
+        x = _far_tokens(V, i, first)
+        own = math.exp(float(x[3]))
+        whole = round(own / unit)
+        l = R.values(x)
+        w = R.weights(l, 1.0)[R.order(l)[:k]]
+        mass = w.cumsum()
+        total = mass[int((mass - w < p * mass[-1]).sum()) - 1]
+        rows.append(x)
+        u.append((own + whole * unit) / 2 / total)  # between the weight and the whole number
+    x, u = torch.stack(rows).cuda(), torch.tensor(u, dtype=torch.float32).cuda()
+    want = [R.sample(x[r], u[r], 1.0, k, p) for r in range(40)]
+    assert 5 < sum(i == 3 for i in want) < 35  # either side
+    assert ops.sample(x, u, top_k=k, top_p=p).tolist() == want
+
+
+def test_borders_finer_than_the_bins(ops):
+    """A border of top-p that falls within the rounding of the thousands of masses above it: id 3 is kept or not."""
+    V, k = 120001, 4500
+    u = torch.zeros(24, device="cuda")
+    seen = set()
+    for seed in range(12):
+        x = _far_tokens(V, seed, -23.3)
+        l = R.values(x)
+        o = R.order(l)[:k]
+        mass = R.weights(l, 1.0)[o].cumsum()
+        before = mass[o.tolist().index(3) - 1]
+        for side in (-1, 1):
+            p = float((before + side * 2.0 ** -40) / mass[-1])
+            want = R.sample(x, 0.0, 1.0, k, p)
+            seen.add(want == 3)
+            got = ops.sample(x.cuda().expand(24, -1), u, top_k=k, top_p=p)
+            assert got.tolist() == [want] * 24, (seed, side)
+    assert seen == {True, False}
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_first_and_last_draws_of_open_rows(ops, dtype):
+    """u = 0 and the last number below 1 where bins hold the masses, with and without min-p."""
+    V = 60013
+    g = torch.Generator().manual_seed(1)
+    x = (torch.randn((16, V), generator=g) * 1.8).to(dtype).cuda()
+    u = torch.tensor([0.0, 1e-30, 1e-9, 1 - 2 ** -24] * 4).cuda()
+    for s in (dict(top_p=0.95), dict(top_p=0.5, temperature=1.5), dict(top_k=3000, top_p=0.9), dict(top_k=20000),
+              dict(top_p=0.9, min_p=1e-4)):
+        want = [R.sample(x[r], u[r], s.get("temperature", 1.0), s.get("top_k", 0), s.get("top_p", 1.0), s.get("min_p", 0.0))
+                for r in range(16)]
+        assert ops.sample(x, u, **s).tolist() == want, s
