@@ -504,8 +504,9 @@ QMM_DEVINL unsigned long long border_key(cg::cluster_group& cl, SelectShared& sh
         }
         const double got = above + (MASS ? tm : (double)tn);
         if (round == 0 && MASS) target = fmax(want * __shfl_sync(~0u, got, 0), 1e-300);
-        const unsigned reached = __ballot_sync(~0u, got >= target) & 0xFFu;
-        if (!(reached & 1u)) return floor;  // not even all of them: the first round
+        unsigned reached = __ballot_sync(~0u, got >= target) & 0xFFu;
+        if (round == 0 && !(reached & 1u)) return floor;  // not even all of them
+        reached |= 1u;  // lo was found to reach it: sums cut otherwise may fall short of that by their last bits
         const int at = 31 - __clz(reached), nxt = at < 7 ? at + 1 : 7;
         const uint32_t n_at = __shfl_sync(~0u, tn, at), n_next = __shfl_sync(~0u, tn, nxt);
         const double got_next = __shfl_sync(~0u, got, nxt);

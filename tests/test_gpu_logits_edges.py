@@ -2,6 +2,7 @@
 
 import math
 
+import numpy as np
 import pytest
 import torch
 
@@ -163,3 +164,27 @@ def test_first_and_last_draws_of_open_rows(ops, dtype):
         want = [R.sample(x[r], u[r], s.get("temperature", 1.0), s.get("top_k", 0), s.get("top_p", 1.0), s.get("min_p", 0.0))
                 for r in range(16)]
         assert ops.sample(x, u, **s).tolist() == want, s
+
+
+def test_border_searched_at_a_token_s_end(ops):
+    """top-p whose target is the mass up to a token to the last bits, where the border is searched by passes (a
+    vocabulary of 262144): the passes cut their sums in different ways, and none may lose the border."""
+    V, rows = 262144, 12
+    u = torch.full((rows,), 0.5, device="cuda")
+    for seed in range(10):
+        x = (torch.randn(V, generator=torch.Generator().manual_seed(seed)) * 1.5).cuda()
+        l = R.values(x)
+        w, o = R.weights(l, 1.0), R.order(l)
+        mass = w[o].cumsum()
+        rank = np.empty(V, np.int64)
+        rank[o] = np.arange(V)
+        for depth in (3.5, 5.5, 8.0):  # where the first pass cuts
+            n = int((l >= np.float32(l.max()) - np.float32(depth)).sum())
+            want = set()
+            for kept in (n - 1, n, n + 1):  # which of them: the last bits
+                cum = (w * (rank < kept)).cumsum()
+                want.add(int((cum > 0.5 * cum[-1]).argmax()))
+            for bits in range(-40, 41):
+                p = float(mass[n - 1] / mass[-1]) * (1 + bits * 2.0 ** -52)
+                got = ops.sample(x.expand(rows, -1), u, top_p=p)
+                assert set(got.tolist()) <= want, (seed, depth, bits)
