@@ -3,6 +3,7 @@
 #pragma once
 
 #include "logits.cuh"
+#include "search.cuh"
 
 namespace qmm {
 
@@ -527,10 +528,10 @@ QMM_DEVINL unsigned long long border_key(cg::cluster_group& cl, SelectShared& sh
     if (inside > kInRange) {
         // one logit's value, more often than the list is long: the first of them by id.  Equal weights: a count.
         const double w = weight(key32_value(lo));
-        double need = MASS ? ceil((target - above) / w) : target - above;
-        if (MASS) {  // the quotient's rounding
-            while (need > 1.0 && above + (need - 1.0) * w >= target) need -= 1.0;
-            while (above + need * w < target && need < (double)inside) need += 1.0;
+        double need = target - above;
+        if (MASS) {  // a quotient rounds, and is no number where w is 0
+            const double guess = fmin(fmax(ceil(need / w), 1.0), (double)inside);
+            need = (double)lowest_kept(1, inside, (uint32_t)guess, [&](uint32_t n) { return above + n * w >= target; });
         }
         unsigned long long a = (unsigned long long)lo << 32, b = (unsigned long long)(lo + 1) << 32;
         if (floor > a) a = floor;

@@ -23,7 +23,6 @@
 // filter 180 us (floor 78: 129 where the model is sure, the rest second passes).
 
 #include "logits_select.cuh"
-#include "search.cuh"
 
 namespace qmm {
 

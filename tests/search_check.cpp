@@ -77,6 +77,49 @@ static void borders(bool walk) {
     }
 }
 
+// How many equal weights w above a mass reach a target, of `inside` of them.  `walk`: one by one from the quotient.
+static uint32_t count(double above, double w, double target, uint32_t inside, bool walk) {
+    long calls = 0;
+    auto reach = [&](uint32_t n) { return ++calls, above + n * w >= target; };
+    const double guess = std::fmin(std::fmax(std::ceil((target - above) / w), 1.0), (double)inside);
+    uint32_t n = (uint32_t)guess;
+    if (walk) {
+        while (n > 1 && reach(n - 1)) --n;
+        while (n < inside && !reach(n)) ++n;
+    } else {
+        n = qmm::lowest_kept(1, inside, n, reach);
+    }
+    if (calls > g_most) g_most = calls;
+    if (calls > 66 || n < 1 || n > inside || (n < inside && !reach(n)) || (n > 1 && reach(n - 1))) {
+        ++g_bad;
+        std::printf("above %.17g w %g target %.17g inside %u: %u after %ld\n", above, w, target, inside, n, calls);
+    }
+    return n;
+}
+
+static void counts(bool walk) {
+    // weights below the last bit of the mass above them: any of a whole range of counts gives the same sum
+    count(1.0, 1e-22, 1.0 + std::ldexp(1.0, -51), 100000000, walk);
+    count(1.0, 1e-25, 1.0 + std::ldexp(1.0, -52), 1u << 30, walk);
+    count(3.0, 1e-300, 3.5, 1u << 30, walk);
+    count(3.0, 0.0, 3.0, 1000, walk);  // no quotient
+    count(3.0, 0.0, 3.5, 1000, walk);
+    count(0.0, 0.5, 1e300, 1000, walk);
+    std::mt19937 rng(2);
+    std::uniform_real_distribution<double> u(0.0, 1.0);
+    for (int i = 0; i < 20000; ++i) {
+        const uint32_t inside = 1 + rng() % 5000;
+        const double w = std::exp(-30.0 * u(rng)), above = u(rng) * 10, target = above + w * inside * u(rng) * 1.01;
+        const uint32_t got = count(above, w, target, inside, walk);
+        uint32_t first = 1;
+        while (i % 20 == 0 && first < inside && !(above + first * w >= target)) ++first;
+        if (i % 20 == 0 && got != first) {
+            ++g_bad;
+            std::printf("count %u, not %u\n", got, first);
+        }
+    }
+}
+
 // Every border and every guess of a short range, at the ends of the keys too.
 static void every_border() {
     for (uint32_t base : {0u, 1000u, 0xFFFFFFFFu - 40u})
@@ -102,6 +145,7 @@ static void every_border() {
 int main(int argc, char** argv) {
     const bool walk = argc > 1 && argv[1][0] == 'w';
     borders(walk);
+    counts(walk);
     if (!walk) every_border();
     std::printf("%d %ld\n", g_bad, g_most);
     return 0;

@@ -28,7 +28,8 @@ def check(tmp_path_factory):
 
 def test_borders(check):
     """min-p's border where a largest logit of 0, min_p = 1 or a huge temperature puts 1e9 keys between it and where
-    its formula says, and in ordinary rows."""
+    its formula says, and in ordinary rows; the number of equal weights that a mass takes, down to weights that the
+    sum does not feel."""
     (bad, most), lines = check()
     assert bad == 0, lines[:5]
     assert most <= 66
@@ -38,3 +39,4 @@ def test_walking_key_by_key_does_not_end(check):
     """What the bound is for: from the formula's guess the same borders are more than a million keys away."""
     (bad, most), lines = check("walk")
     assert bad > 0 and most >= 1000000 and any(line.startswith("max 0 T 1 min-p 1:") for line in lines)
+    assert any(line.startswith("above 1 w 1e-22") for line in lines)
