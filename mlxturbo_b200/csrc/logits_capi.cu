@@ -244,7 +244,7 @@ int qmm_distill_loss_grad(const void* logits, int64_t row_stride, int64_t rows, 
     if (rc || rows == 0) return rc;
     if (misaligned(loss, 4) || misaligned(grad, elem_bytes(dtype)) || askew(row_weight, 4))
         return null_error("distill_loss_grad");
-    if (grad_stride < V || (grad == logits && grad_stride != row_stride)) {
+    if (grad_stride < V || (grad == logits && grad_stride != row_stride && rows > 1)) {
         set_error("distill_loss_grad: gradient rows %lld apart for V=%lld, logits %lld", (long long)grad_stride,
                   (long long)V, (long long)row_stride);
         return QMM_EINVAL;

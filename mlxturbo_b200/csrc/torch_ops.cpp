@@ -668,7 +668,8 @@ at::Tensor run_distill_loss_grad(const at::Tensor& logits, const at::Tensor& tv,
             fail(Err::kValue, "%s: out must be contiguous, of the logits' shape %s and dtype", what,
                  dims(logits.sizes()).c_str());
         // over the logits, or clear of everything that is read
-        const bool same = grad.data_ptr() == l.data_ptr() && l.stride(0) == l.size(1);
+        // (the stride of a single row says nothing)
+        const bool same = grad.data_ptr() == l.data_ptr() && (l.stride(0) == l.size(1) || l.size(0) == 1);
         auto touches = [&](const at::Tensor& x, int64_t bytes) {
             const char *a = static_cast<const char*>(grad.data_ptr()), *b = static_cast<const char*>(x.data_ptr());
             return a < b + bytes && b < a + grad.numel() * grad.element_size();

@@ -119,3 +119,19 @@ def test_lists_of_all_that_is_left(ops, V, k, T, mask, dtype):
 def uniform_ids(rows, V, k):
     g = torch.Generator().manual_seed(rows + V)
     return torch.stack([torch.randperm(V, generator=g)[:k] for _ in range(rows)])
+
+
+@pytest.mark.parametrize("rows,first", [(1, 0), (1, 3), (0, 0)])
+def test_last_chunk_in_place(ops, rows, first):
+    """A chunk of one row of a wider buffer is contiguous whatever its row stride, and may hold its own gradient."""
+    V = 700
+    buf = torch.randn((4, V + 20), generator=torch.Generator().manual_seed(1)).cuda()
+    x = buf[first:first + rows, :V]
+    assert x.is_contiguous()
+    keep = buf.clone()
+    tv, ti = ops.topk(keep[first:first + rows, :V].contiguous() * 0.9, 6)
+    loss, grad = ops.distill_loss_and_grad(keep[first:first + rows, :V], tv, ti)
+    again, out = ops.distill_loss_and_grad(x, tv, ti, out=x)
+    assert out is x and torch.equal(loss, again)
+    keep[first:first + rows, :V] = grad
+    assert torch.equal(buf, keep)
