@@ -190,6 +190,8 @@ class ColumnShardedLMHead(_ShardedBase):
         merges the P*k candidates.  Equal values keep the lowest token id, as a
         single-device ``argmax`` does (for k > ``ops.TOPK_MAX``, and on the CPU, a
         tie at a shard's k-th value may keep either id).  k=1 is greedy sampling.
+        A NaN is the largest value where ``torch`` picks (k = 1, k >
+        ``ops.TOPK_MAX``, on the CPU) and counts as -inf in ``ops.topk``.
         """
         lead = x.shape[:-1]
         local = self.forward(x, gather=False).reshape(-1, self.shard_rows)  # [M, N/P]
@@ -198,10 +200,11 @@ class ColumnShardedLMHead(_ShardedBase):
         kk = min(k, local.shape[1])
         if kk == 1:  # first occurrence of the maximum, like argmax on one device
             vals, idx = local.float().max(dim=-1, keepdim=True)
-        elif local.is_cuda and kk <= ops.TOPK_MAX:
+        elif (local.is_cuda and 1 < kk <= ops.TOPK_MAX and local.dtype in ops.LOGITS_DTYPES
+              and not (local.requires_grad and torch.is_grad_enabled())):
             vals, idx = ops.topk(local, kk)
             vals = vals.float()
-        else:  # (ties at a shard's k-th value may keep either id)
+        else:  # (ties at a shard's k-th value may keep either id); with a gradient, or a matmul's other types
             vals, idx = torch.topk(local.float(), kk, dim=-1, sorted=True)
         idx = idx.to(torch.int64) + rank * self.shard_rows
         if world > 1:

@@ -596,6 +596,7 @@ def sample(logits: torch.Tensor, u: torch.Tensor, *, temperature=1.0, top_k=0, t
 
 
 TOPK_MAX = 1024
+LOGITS_DTYPES = (torch.bfloat16, torch.float16, torch.float32)  # of rows of logits
 
 
 def topk(logits: torch.Tensor, k: int, *, logsumexp: bool = False, temperature: float = 1.0):
