@@ -16,7 +16,8 @@
 // O is summed on its own (a bit to an element marks the listed ones), not as a
 // difference: it may be a billionth of Z.  Its weights are taken against the
 // largest logit that is not listed, so neither O nor rest / O leaves the range
-// of 32 bits.
+// of 32 bits.  A gradient below 2^-126 may come out as 0: the
+// exponentials have no smaller values.
 //
 // Bound by memory: the loss reads the logits once, the gradient reads and
 // writes them once.  Loss and gradient in one call are one launch, a cluster to
@@ -205,9 +206,11 @@ QMM_DEVINL uint4 encode(const float (&x)[Elem<DT>::kVec]) {
     }
 }
 
-// A finite reference that the fast weights do not take: rows masked throughout
-// with a type's lowest value.
-QMM_DEVINL bool out_of_range(float ref) { return fabsf(ref) > kFastMax && fabsf(ref) < CUDART_INF_F; }
+// A finite reference that the fast weights do not take, its E's rounding being
+// above a half: rows masked throughout with a type's lowest value.
+QMM_DEVINL bool out_of_range(float ref, const Scale& c) {
+    return fabsf(ref * c.c) > 16777216.0f && fabsf(ref) < CUDART_INF_F;
+}
 
 // TAIL: the teacher's log-sum-exp is given.  MODE kBackward needs no cluster.
 template <int DT, bool TAIL, int MODE>
@@ -285,7 +288,7 @@ __global__ void __launch_bounds__(kDistillThreads, MODE == kBackward ? 3 : 4)
         double s_ref;
         row_stat(sh.stats, warps, c, ref, s_ref, nullptr);
         if (ref == -CUDART_INF_F) s_ref = 0.0;
-        if (out_of_range(ref)) {
+        if (out_of_range(ref, c)) {
             double share = 0.0;
             if (reader) {
                 for_vectors_rare<DT>(row, s, [&](int v, uint4 u) {
@@ -363,7 +366,7 @@ __global__ void __launch_bounds__(kDistillThreads, MODE == kBackward ? 3 : 4)
             for (int v = s.begin + s.lane; v < s.end; v += 32) store(v, zero);
             if (s.lane == 0 && s.head >= 0) store(s.head, zero);
             if (s.lane == 0 && s.tail >= 0) store(s.tail, zero);
-        } else if (out_of_range(ref)) {
+        } else if (out_of_range(ref, c)) {
             for_vectors_rare<DT>(row, s, [&](int v, const uint4& u) {
                 float x[N];
                 decode<DT>(u, x);

@@ -229,9 +229,10 @@ QMM_DEVINL void fill_table(double* table) {
 // log2(V) + 2 <= 30: 1.9e-6; ex2.approx 2^-22; five roundings within a batch of
 // 4 vectors, 3.0e-7; batches are added in 64 bits.  Together 2.5e-6 < 2^-18.
 constexpr double kFastEps = 1.0 / 262144.0;
-// It stands for finite maxima up to kFastMax and these temperatures: exponents
-// stay finite.  Beyond, or where a NaN or an infinity enters, a sum comes out as
-// NaN or outside [0.5, inf) and is made in 64 bits.
+// It stands for finite maxima up to kFastMax and these temperatures.  Beyond, or
+// where a NaN or an infinity enters, a sum comes out as NaN or outside
+// [0.5, inf) and is made in 64 bits; so it does where E is so large (2^31 and
+// more) that its own rounding leaves the exponent's range.
 constexpr float kFastMax = 1e29f;
 constexpr double kFastMinT = 1e-6, kFastMaxT = 1e6;
 
@@ -252,6 +253,11 @@ struct LaneSum {
     float e = -3e38f;
     double s = 0.0;
 };
+
+// Such a sum against a larger reference, `by` the factor between them.  Tokens
+// that are all masked with a huge number have a sum of any value, infinity among
+// them, against their own E; by 0 it is nothing.  A NaN stays.
+QMM_DEVINL double rescaled(double s, float by) { return by > 0.0f || s != s ? s * (double)by : 0.0; }
 
 // In a tree: one long chain of 64-bit additions outlasts the weights themselves.
 template <typename T, int N>
@@ -488,7 +494,7 @@ QMM_DEVINL LaneTop stream_slice(const Row<DT>& row, const Slice& s, const Scale&
         const float t = bm * c.c;
         if (t > acc.e + 16.0f) {  // weights stay below 2^17
             const float e = ceilf(t);
-            acc.s *= (double)ex2(acc.e - e);
+            acc.s = rescaled(acc.s, ex2(acc.e - e));
             acc.e = e;
         }
         float sum = 0.0f;
@@ -549,7 +555,7 @@ QMM_DEVINL WarpStat warp_stat(float top, const LaneSum& acc, bool sum = true) {
         return w;
     }
     w.e = warp_max(acc.e);
-    w.s = warp_sum(acc.s * (double)ex2(acc.e - w.e));
+    w.s = warp_sum(rescaled(acc.s, ex2(acc.e - w.e)));
     return w;
 }
 
@@ -568,7 +574,7 @@ QMM_DEVINL void row_stat(const WarpStat* stats, int warps, const S& c, float& mx
     const float e = ceilf(mx * c.c);
     const double back = c.against(e, mx);
     for (int i = lane; i < warps; i += 32) {
-        const double x = stats[i].s * (double)ex2(stats[i].e - e) * back;
+        const double x = rescaled(stats[i].s, ex2(stats[i].e - e)) * back;
         if (slots && threadIdx.x < 32) slots[i] = x;
         total += x;
     }

@@ -16,8 +16,8 @@ def divergence(row, tv, ti, T=1.0, lse=None, weight=1.0):
     norm = lse if lse is not None else t.max() + np.log(np.exp(t - t.max()).sum())
     p = np.zeros(V)
     np.add.at(p, ids, np.exp(t - norm))
-    x = l / T
-    logq = x - (x.max() + np.log(np.exp(x - x.max()).sum()))
+    x = (l - l.max()) / T if l.max() > -np.inf else l
+    logq = x - np.log(np.exp(x).sum())
     q = np.exp(logq)
     seen = p > 0
     loss = float((p[seen] * (np.log(p[seen]) - logq[seen])).sum())
@@ -26,7 +26,7 @@ def divergence(row, tv, ti, T=1.0, lse=None, weight=1.0):
         listed = np.zeros(V, bool)
         listed[ids] = True
         rest, other = max(0.0, 1.0 - p.sum()), q[~listed].sum()
-        if (x[~listed] - x.max() < -700).all() and rest <= 2.0 ** -17 + 2.0 ** -23 * abs(lse):
+        if (x[~listed] < -700).all() and rest <= 2.0 ** -17 + 2.0 ** -23 * abs(lse):
             rest = 0.0  # the rounding of the log-sum-exp: nothing is left but masked tokens
         if rest > 0:
             with np.errstate(divide="ignore"):

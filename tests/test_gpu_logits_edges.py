@@ -188,3 +188,32 @@ def test_border_searched_at_a_token_s_end(ops):
                 p = float(mass[n - 1] / mass[-1]) * (1 + bits * 2.0 ** -52)
                 got = ops.sample(x.expand(rows, -1), u, top_p=p)
                 assert set(got.tolist()) <= want, (seed, depth, bits)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_masks_of_any_size(ops, dtype):
+    """Stretches of a row that a mask fills with one huge number, at every temperature."""
+    V = 70003
+    g = torch.Generator().manual_seed(5)
+    x = torch.randn((6, V), generator=g) * 2
+    hide = torch.rand((6, V), generator=g) < 0.7
+    hide[:, 50:V // 2] = True
+    u = uniform(6, 6)
+    for size in (1e4, 1e9, 1e10, 3e20, 1e30, 2.9e38, 3.3e38):
+        if size > torch.finfo(dtype).max:
+            continue
+        y = x.masked_fill(hide, -size).to(dtype).cuda()
+        ids = y[:, :2].argmax(-1)[:, None]
+        for T in (0.3, 1.0, 2.0, 4.0):
+            for s in (dict(), dict(top_p=0.9), dict(top_k=300, top_p=0.9)):
+                want = [R.sample(y[r], u[r], T, s.get("top_k", 0), s.get("top_p", 1.0)) for r in range(6)]
+                assert ops.sample(y, u, temperature=T, **s).tolist() == want, (size, T, s)
+            lse = ops.topk(y, 3, logsumexp=True, temperature=T)[2]
+            for r in range(6):
+                want = R.logsumexp(y[r], T)
+                assert abs(float(lse[r]) - want) <= 1e-5 + 2 ** -24 * abs(want)
+            tokens, accepted = ops.speculative_sample(y.view(3, 2, V), y.view(3, 2, V)[:, 1:], ids[::2], u.view(3, 2),
+                                                      temperature=T)
+            for b in range(3):
+                want, j = R.speculative(y[2 * b:2 * b + 2], y[2 * b + 1:2 * b + 2], ids[2 * b], u[2 * b:2 * b + 2], T)
+                assert tokens[b].tolist() == want and int(accepted[b]) == j
