@@ -155,7 +155,9 @@ QMM_DEVINL void list_sums(const DistillArgs& a, DistillShared& sh, const List& l
         mass += p;
         if (li.id[j] < 0) continue;
         if (LOSS && !twice && p != 0.0) cross += p * (lp - (double)li.x[j] * a.inv_t);
-        if (TAIL && li.owner[li.slot[j]] == j) part += exp(((double)li.x[j] - (double)best) * a.inv_t);
+        // (where the list holds nothing but masked tokens, best is -infinity as they are)
+        if (TAIL && li.owner[li.slot[j]] == j && li.x[j] != -CUDART_INF_F)
+            part += exp(((double)li.x[j] - (double)best) * a.inv_t);
     }
     if (LOSS && twice) {  // an id's entries added up before the logarithm
         __syncwarp();

@@ -156,3 +156,23 @@ def test_masks_of_any_size(ops, V, tail, dtype):
             y, t = x.masked_fill(hide, low), teacher.masked_fill(hide, low)
             tv, ti, lse = ops.topk(t, 8, logsumexp=True, temperature=T)
             check(ops, y, tv, ti, T, lse if tail else None)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("tail", [False, True])
+@pytest.mark.parametrize("V", [2, 500, 40001])
+def test_lists_of_masked_tokens(ops, V, tail, dtype):
+    """All listed tokens masked in the model's row: an infinite loss with a finite gradient, or a loss of what is left
+    where the teacher gives them nothing either."""
+    x, teacher = student(5, V, dtype, V)
+    k = min(V - 1, 6)
+    tv, ti, lse = ops.topk(teacher, k, logsumexp=True)
+    x.scatter_(1, ti, -torch.inf)
+    x[3].scatter_(0, ti[3, :1], 1.0)  # all but one
+    ti[1, 1:], tv[1, :1] = -1, -torch.inf
+    ti[2] = -1
+    tv[4] = -torch.inf
+    loss = check(ops, x, tv, ti, 1.0, lse if tail else None)
+    assert float(loss[0]) == math.inf
+    for r in (1, 2, 4):
+        assert float(loss[r]) < 1e-4 or (tail and V == 2)
