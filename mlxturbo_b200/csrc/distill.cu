@@ -16,8 +16,10 @@
 // O is summed on its own (a bit to an element marks the listed ones), not as a
 // difference: it may be a billionth of Z.  Its weights are taken against the
 // largest logit that is not listed, so neither O nor rest / O leaves the range
-// of 32 bits.  A gradient below 2^-126 may come out as 0: the
-// exponentials have no smaller values.
+// of 32 bits.  The loss, too, is made of differences to the largest listed
+// logit: of logits near a type's limit 64 bits would keep no digit.  A gradient
+// below 2^-126 times its row's weight / tau may come out as 0: the exponentials
+// have no smaller values.
 //
 // Bound by memory: the loss reads the logits once, the gradient reads and
 // writes them once.  Loss and gradient in one call are one launch, a cluster to
@@ -43,9 +45,12 @@ constexpr int kDistillThreads = kRowThreads + 32;
 struct DistillShared {
     WarpStat stats[kMaxRowWarps];
     double mass;   // sum p
-    double cross;  // sum p (log p - l / tau), for the loss
+    double cross;  // sum p (log p - (l - base) / tau), for the loss
     double part;   // sum over distinct listed tokens of exp((l - best) / tau)
     float best;    // largest listed logit
+
+    // what the loss' logits are counted from
+    QMM_DEVINL static double base(float best) { return fabsf(best) < CUDART_INF_F ? (double)best : 0.0; }
     int twice;     // an id is listed more than once
 };
 
@@ -148,13 +153,14 @@ QMM_DEVINL void list_sums(const DistillArgs& a, DistillShared& sh, const List& l
         for (int j = lane; j < a.k; j += 32) sum += exp(li.logp[j] - top);
         norm = top + log(warp_sum(sum));
     }
+    const double base = DistillShared::base(best);
     double mass = 0.0, cross = 0.0, part = 0.0;
     for (int j = lane; j < a.k; j += 32) {
         const double lp = li.logp[j] - norm, p = exp(lp);
         li.logp[j] = lp;
         mass += p;
         if (li.id[j] < 0) continue;
-        if (LOSS && !twice && p != 0.0) cross += p * (lp - (double)li.x[j] * a.inv_t);
+        if (LOSS && !twice && p != 0.0) cross += p * (lp - ((double)li.x[j] - base) * a.inv_t);
         // (where the list holds nothing but masked tokens, best is -infinity as they are)
         if (TAIL && li.owner[li.slot[j]] == j && li.x[j] != -CUDART_INF_F)
             part += exp(((double)li.x[j] - (double)best) * a.inv_t);
@@ -167,7 +173,7 @@ QMM_DEVINL void list_sums(const DistillArgs& a, DistillShared& sh, const List& l
             double p = exp(li.logp[j]);
             for (int i = j + 1; i < a.k; ++i)
                 if (li.id[i] == id) p += exp(li.logp[i]);
-            if (p != 0.0) cross += p * (log(p) - (double)li.x[j] * a.inv_t);
+            if (p != 0.0) cross += p * (log(p) - ((double)li.x[j] - base) * a.inv_t);
         }
     }
     mass = warp_sum(mass);
@@ -334,7 +340,7 @@ __global__ void __launch_bounds__(kDistillThreads, MODE == kBackward ? 3 : 4)
         }
         if (rank == 0 && threadIdx.x == kRowThreads) {
             double loss = sh.cross;
-            if (mass != 0.0) loss += mass * ((double)mx * a.inv_t + log(sum));
+            if (mass != 0.0) loss += mass * (((double)mx - DistillShared::base(sh.best)) * a.inv_t + log(sum));
             if (TAIL && rest != 0.0) {
                 const double log_other = ref == -CUDART_INF_F
                                              ? -CUDART_INF

@@ -176,3 +176,30 @@ def test_lists_of_masked_tokens(ops, V, tail, dtype):
     assert float(loss[0]) == math.inf
     for r in (1, 2, 4):
         assert float(loss[r]) < 1e-4 or (tail and V == 2)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("tail", [False, True])
+@pytest.mark.parametrize("V", [3000, 70003])
+def test_rows_of_huge_logits(ops, V, tail, dtype):
+    """Rows masked throughout with a huge number, their list among them, and rows whose live logits are all that
+    large: 64 bits of l / T itself would hold none of the differences."""
+    x, teacher = student(4, V, dtype, V)
+    k = 8
+    for size in (1e4, 1e9, 1e10, 3e20, 1e30, 2.9e38, 3.3e38):
+        if size > torch.finfo(dtype).max:
+            continue
+        low = -torch.tensor(size, dtype=dtype).item()
+        for T in (0.3, 1.0, 2.0, 4.0):
+            tv, ti, lse = ops.topk(teacher, k, logsumexp=True, temperature=T)
+            lse += 0.5  # the tokens not listed have a share
+            y = x.clone()
+            y[0] = low
+            y[1] = -low
+            y[2, ::2] = low
+            y[2, 1::2] = low * (1 + 2 ** -6)
+            y[2].scatter_(0, ti[2], low)
+            y[3] = -low
+            y[3, V // 3:V // 2] = 0.0
+            y[3].scatter_(0, ti[3], -low)
+            check(ops, y, tv, ti, T, lse if tail else None)
