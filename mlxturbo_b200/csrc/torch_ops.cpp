@@ -450,8 +450,10 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> topk(const at::Tensor& logits, in
     const int dt = mx_dtype_code(logits.scalar_type());
     c10::cuda::CUDAGuard guard(logits.device());
     const at::Tensor l = logits_rows("topk", logits);
+    if (k < 1 || k > l.size(1))  // before anything of that size is allocated
+        fail(Err::kValue, "topk: k=%lld is not in [1, V=%lld]", (long long)k, (long long)l.size(1));
     std::vector<int64_t> shape(logits.sizes().begin(), logits.sizes().end());
-    shape.back() = k < 0 ? 0 : k;
+    shape.back() = k;
     at::Tensor values = empty_like_device(shape, l.scalar_type(), l), ids = empty_like_device(shape, at::kLong, l);
     shape.pop_back();
     at::Tensor sums = lse ? empty_like_device(shape, at::kFloat, l) : at::Tensor();

@@ -203,3 +203,34 @@ def test_rows_of_huge_logits(ops, V, tail, dtype):
             y[3, V // 3:V // 2] = 0.0
             y[3].scatter_(0, ti[3], -low)
             check(ops, y, tv, ti, T, lse if tail else None)
+
+
+@pytest.mark.parametrize("tail", [False, True])
+def test_captured_loss_and_backward_pass(ops, tail):
+    """Loss and gradient through autograd in one captured graph, replayed on other logits, lists and weights."""
+    rows, V, k = 7, 5001, 9
+    first, second = (student(rows, V, torch.bfloat16, s) for s in (1, 2))
+    lists = [ops.topk(t, k, logsumexp=True) for _, t in (first, second)]
+    weights = [torch.rand(rows, generator=torch.Generator().manual_seed(s)).cuda() for s in (3, 4)]
+
+    def step(x, tv, ti, lse, w):
+        loss = ops.distill_loss(x, tv, ti, teacher_logsumexp=lse if tail else None)
+        return loss.detach(), torch.autograd.grad(loss, x, w)[0]
+
+    leaf = first[0].clone().requires_grad_()
+    tv, ti, lse, w = (t.clone() for t in (*lists[0], weights[0]))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(leaf, tv, ti, lse, w)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        loss, grad = step(leaf, tv, ti, lse, w)
+    for (x, _), (v, i, s), wt in zip((second, first), lists[::-1], weights[::-1]):
+        leaf.detach().copy_(x)
+        for a, b in zip((tv, ti, lse, w), (v, i, s, wt)):
+            a.copy_(b)
+        graph.replay()
+        want = step(x.clone().requires_grad_(), v, i, s, wt)
+        assert torch.equal(loss, want[0]) and torch.equal(grad, want[1])

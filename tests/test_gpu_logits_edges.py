@@ -217,3 +217,13 @@ def test_masks_of_any_size(ops, dtype):
             for b in range(3):
                 want, j = R.speculative(y[2 * b:2 * b + 2], y[2 * b + 1:2 * b + 2], ids[2 * b], u[2 * b:2 * b + 2], T)
                 assert tokens[b].tolist() == want and int(accepted[b]) == j
+
+
+def test_topk_of_more_than_a_row(ops):
+    """Refused before outputs of that size are asked for."""
+    x = torch.randn((3, 50), device="cuda")
+    before = torch.cuda.memory_allocated()
+    for k in (51, 2 ** 31, 2 ** 40, 2 ** 62):
+        with pytest.raises(ValueError, match="not in"):
+            ops.topk(x, k, logsumexp=True)
+    assert torch.cuda.memory_allocated() == before
