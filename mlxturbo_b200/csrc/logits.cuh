@@ -225,9 +225,9 @@ QMM_DEVINL void fill_table(double* table) {
 // Fast weights: 2^(x c - E) with c = log2(e) / T in 32 bits and a whole number
 // E, so one multiply-add, and every change of reference is exact.
 // Bound of the relative error of a fast sum: the exponent's rounding and c's
-// own, |a| ln2 (2^-24 + 2^-25) with a weighted mean of |a| of at most about
-// log2(V) + 2 <= 30: 1.9e-6; ex2.approx 2^-22; five roundings within a batch of
-// 4 vectors, 3.0e-7; batches are added in 64 bits.  Together 2.5e-6 < 2^-18.
+// own, |a| ln2 (2^-24 + 2^-24) with a weighted mean of |a| of at most about
+// log2(V) + 2 <= 30: 2.5e-6; ex2.approx 2^-22; five roundings within a batch of
+// 4 vectors, 3.0e-7; batches are added in 64 bits.  Together 3.1e-6 < 2^-18.
 constexpr double kFastEps = 1.0 / 262144.0;
 // It stands for finite maxima up to kFastMax and these temperatures.  Beyond, or
 // where a NaN or an infinity enters, a sum comes out as NaN or outside

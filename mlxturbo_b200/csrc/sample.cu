@@ -18,9 +18,10 @@
 // maxima, collects the candidates, and CTA 0 sorts and draws.  With top-k no
 // exponential is taken but of the candidates.  Measured on a B200, V 248320: one
 // row, top-k 20 and top-p 0.95, 12 us; 65 rows of 50021 with settings of their
-// own 16 us; 128 rows with top-p 0.95, half of them open, 160 us (floor 9.7: the
-// open rows' pass in 64 bits and the steps after it); 512 rows of fp32 without a
-// filter 180 us (floor 78: 129 where the model is sure, the rest second passes).
+// own 17 us; 128 rows with top-p 0.95, half of them open, 160 to 178 us (floor
+// 9.7: no unit is busy, the 64-bit pipe at 5%; a cluster's other CTAs wait at
+// barriers for the one that lists and sorts); 512 rows of fp32 without a filter
+// 180 us (floor 78: 129 where the model is sure, the rest second passes).
 
 #include "logits_select.cuh"
 

@@ -16,7 +16,9 @@
 // The first launch is bound by memory and the exponential unit (both near 65%),
 // the second by its chain: tests, a pass over two rows in L2, the exchange, the
 // place.  B200, V 248320: one sequence of 4 drafted tokens 24 us, 48 of up to 3
-// 139 us (44 and 95; a sequence whose draw is made again takes 90 of these).
+// 117 to 147 us (44 and the draws; a sequence whose draw is made again takes 90
+// of these).  Where the model's rows and the draft's start differently, as with
+// an odd V, the draft's are read element by element: 201 us at V 248321.
 
 #include "logits.cuh"
 #include "tma.cuh"
