@@ -26,10 +26,11 @@
 // a row, which reads the row twice; of the second reading L2 has a third, since
 // the rows at work (296 of 497 KB) are more than it holds, and fewer rows at
 // work, by more CTAs to a row, cost more in their steps than they save (2048 rows
-// of 248320 by 2, 4, 8 CTAs: 464, 500, 767 us of the device's time).  B200, V 248320, bf16: loss of 333
-// rows 43 to 45 us (floor 25), of 1024 96 us (78); backward of 1024 rows 161 us,
-// 96% of the copy rate; both of 2048 rows in one launch 485 to 490 us through the
-// public call (floor 311 with one reading, 466 with two).
+// of 248320 by 2, 4, 8 CTAs: 464, 500, 767 us of the device's time).  B200,
+// V 248320, bf16: loss of 333 rows 43 to 45 us (floor 25), of 1024 96 us (78);
+// backward of 1024 rows 161 us, 96% of the copy rate; both of 2048 rows in one
+// launch 485 to 490 us through the public call (floor 311 with one reading, 466
+// with two).
 
 #include "logits.cuh"
 

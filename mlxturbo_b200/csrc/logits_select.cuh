@@ -617,11 +617,12 @@ QMM_DEVINL unsigned long long border_key(cg::cluster_group& cl, SelectShared& sh
 // sum of whole numbers is the same in any order.  A token is off by half such a
 // unit, so a bin's sums, a mass above a bin and a part of the whole by half a
 // unit for each token: a border or a draw nearer than that is made in 64 bits
-// (one row in 10^4 or fewer).  The bins reach down to where what is
-// left, V tokens at most, is half of what top-p leaves out.  The tokens of the
-// bin that holds the border, less than a hundredth of them, go to CTA 0's
-// list.  What lies above it of each warp is kept for the draw, so no token is
-// weighed twice.  (128 rows of 248320 at top-p 0.95, half of them open: 411 us
+// (V units are 2^-21 of the weight at the edge for V 248320, kept tokens weigh
+// a hundredth of it and more: by estimate one row in 10^4 or fewer).  The bins
+// reach down to where what is left, V tokens at most, is half of what top-p
+// leaves out.  The tokens of the bin that holds the border, less than a
+// hundredth of them, go to CTA 0's list.  What lies above it of each warp is
+// kept for the draw, so no token is weighed twice.  (128 rows of 248320 at top-p 0.95, half of them open: 411 us
 // with border_key's rounds.)
 
 constexpr double kBinMagic = 4503599627370496.0;  // 2^52: a sum with it is a whole number
